@@ -29,6 +29,7 @@ EXPORTS = (
     "fsvd_exchange_region_export", "fsvd_exchange_region_import", "fsvd_exchange_region_release",
     "fsvd_exchange_create", "fsvd_exchange_destroy", "fsvd_exchange_set_trace", "fsvd_tp_workspace_bytes",
     "fsvd_tp_decode_layer", "fsvd_prompt_create", "fsvd_prompt_run",
+    "fsvd_rope_qk", "fsvd_kv8_workspace_bytes", "fsvd_kv8_append", "fsvd_kv8_load", "fsvd_flash_decode_kv8", "fsvd_sample",
 )
 
 
@@ -50,6 +51,11 @@ LAYER_FIELDS = (
 
 class FsvdLayer(C.Structure):
     _fields_ = [(name, C.c_void_p) for name in LAYER_FIELDS]
+
+
+class FsvdKv8(C.Structure):
+    _fields_ = [("k8", C.c_void_p), ("v8", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("B", C.c_int), ("Hk", C.c_int), ("S_max", C.c_int), ("Dh", C.c_int), ("block", C.c_int)]
 
 
 class FsvdError(RuntimeError):
@@ -130,6 +136,14 @@ def load() -> C.CDLL:
     lib.fsvd_tp_workspace_bytes.restype = sz
     lib.fsvd_tp_decode_layer.argtypes = [
         C.POINTER(FsvdDims), C.POINTER(FsvdLayer), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    fp, ll = C.c_float, C.c_longlong
+    lib.fsvd_rope_qk.argtypes = [vp, ll, vp, ll, vp, vp, ip, ip, fp, vp, vp] + [ip] * 5 + [vp]
+    lib.fsvd_kv8_workspace_bytes.argtypes = [ip] * 5
+    lib.fsvd_kv8_workspace_bytes.restype = sz
+    lib.fsvd_kv8_append.argtypes = [C.POINTER(FsvdKv8), vp, vp, ll, ll, vp, vp, vp, ll, ll, vp, vp, ip, ip, fp, ip, ip, vp, sz, vp]
+    lib.fsvd_kv8_load.argtypes = [C.POINTER(FsvdKv8), ip, ip, vp, ip, vp, vp, vp]
+    lib.fsvd_flash_decode_kv8.argtypes = [C.POINTER(FsvdKv8), vp, vp, ip, vp, ip, fp, vp, sz, vp]
+    lib.fsvd_sample.argtypes = [vp, ll, ip, vp, vp, vp, vp, vp, fp, ip, fp, fp, vp, vp, ip, ip, vp]
     for name in EXPORTS:
         fn = getattr(lib, name)
         if fn.restype is C.c_int and name not in ("fsvd_version",):

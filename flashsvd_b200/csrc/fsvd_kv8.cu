@@ -1,0 +1,685 @@
+// Rotary positions and the 8-bit key / value cache: rotation, append, read-back and single-query attention
+// (fsvd_rope_qk, fsvd_kv8_append, fsvd_kv8_load, fsvd_flash_decode_kv8 of include/flashsvd_b200.h).
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "../../include/flashsvd_b200.h"
+#include "fsvd_rope.cuh"
+#include "fsvd_stage.h"
+#include "fsvd_tile.h"
+
+namespace fsvd_kv8_impl {
+
+using fsvd::DS_CACHE_FULL;
+using fsvd::DS_OK;
+using fsvd::SyncState;
+using fsvd_rope::Rotary;
+
+static int fail(int code, const char* fmt, ...) {
+  char msg[256];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(msg, sizeof(msg), fmt, ap);
+  va_end(ap);
+  fsvd_tile_set_error(code, msg);
+  return code;
+}
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static int sm_count() {
+  static std::atomic<int> cache[16];
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) return n;
+  if (dev >= 0 && dev < 16 && (n = cache[dev].load()) > 0) return n;
+  n = 148;
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  if (dev >= 0 && dev < 16) cache[dev].store(n);
+  return n;
+}
+
+// Every kernel of this file may start while the one before it in the stream is still draining, and waits for it
+// (griddepcontrol) before it touches memory.
+__device__ __forceinline__ void pdl_begin() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... Params, typename... Args>
+static int launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, void* stream, Args... args) {
+  // Above the 48 KB that a kernel has by itself the limit is raised at every such launch: a setting of the current
+  // device, so nothing is remembered.
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return fail(FSVD_ERR_CUDA, "shared memory of %zu bytes: %s", smem, cudaGetErrorString(e));
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+  if (e != cudaSuccess) return fail(FSVD_ERR_CUDA, "kernel launch failed: %s", cudaGetErrorString(e));
+  fsvd_tile_count_launch();
+  return 0;
+}
+
+constexpr int kThreads = 256;
+
+// ------------------------------------------------------------------------------------------ rotary positions
+struct RopeArgs {
+  const void *q, *k;
+  void *q_out, *k_out;
+  long long q_stride, k_stride;
+  const int* positions;
+  Rotary rot;
+  int T, H, Hk, Dh, tokens, heads;   // tokens and heads of a CTA
+};
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void rotate_row(const T* in, T* out, int u, int R, int interleaved, const float (&c)[8],
+                                           const float (&s)[8]) {
+  float a[8], b[8];
+  fsvd_rope::load_unit<WIDE>(in, u, R, interleaved, a, b);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float x = a[i], y = b[i];
+    if (8 * u + i < (R >> 1)) {   // (the others are copied: an infinity times a sine of zero is no number)
+      a[i] = x * c[i] - y * s[i];
+      b[i] = y * c[i] + x * s[i];
+    }
+  }
+  fsvd_rope::store_unit<WIDE>(out, u, R, interleaved, a, b);
+}
+
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kThreads) rope_kernel(const RopeArgs a) {
+  extern __shared__ float2 table[];   // [tokens][R / 2] cosine, sine
+  const int half = a.rot.R >> 1, tid = threadIdx.x;
+  const int t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.T - t0);
+  pdl_begin();
+  for (int i = tid; i < nt * half; i += kThreads) {
+    double c, s;
+    const int t = i / half;
+    fsvd_rope::angle(a.positions[t0 + t], a.rot.inv_freq[i - t * half], a.rot.scale, c, s);
+    table[i] = make_float2((float)c, (float)s);
+  }
+  __syncthreads();
+  const int U = a.Dh / 16, u = tid % U, per = kThreads / U;
+  const int h0 = blockIdx.y * a.heads, h1 = min(h0 + a.heads, a.H + a.Hk);
+  if (tid >= per * U) return;
+  for (int t = 0; t < nt; ++t) {
+    float c[8], s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int p = 8 * u + i;
+      const float2 cs = p < half ? table[t * half + p] : make_float2(1.0f, 0.0f);
+      c[i] = cs.x;
+      s[i] = cs.y;
+    }
+    const size_t tt = t0 + t;
+    for (int h = h0 + tid / U; h < h1; h += per) {
+      if (h < a.H)
+        rotate_row<T, WIDE>(reinterpret_cast<const T*>(a.q) + tt * a.q_stride + (size_t)h * a.Dh,
+                            reinterpret_cast<T*>(a.q_out) + (tt * a.H + h) * a.Dh, u, a.rot.R, a.rot.interleaved, c, s);
+      else
+        rotate_row<T, WIDE>(reinterpret_cast<const T*>(a.k) + tt * a.k_stride + (size_t)(h - a.H) * a.Dh,
+                            reinterpret_cast<T*>(a.k_out) + (tt * a.Hk + h - a.H) * a.Dh, u, a.rot.R, a.rot.interleaved, c, s);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ append
+struct AppendArgs {
+  fsvd_kv8 c;
+  const __nv_bfloat16 *k, *v, *q;
+  __nv_bfloat16* q_out;
+  long long kv_batch, kv_token, q_batch, q_token;
+  const int *seqlens, *new_lens;
+  int* status;
+  Rotary rot;       // R = 0: no rotation
+  int H, L, groups; // groups: head groups of a (sequence, block)
+  int nblk;         // blocks that L tokens can touch
+};
+
+// Exponent of the scale for a largest magnitude: the smallest e >= -60 with amax <= 448 2^e (448 = 1.75 * 2^8).
+__device__ __forceinline__ int scale_exponent(float amax) {
+  const uint32_t b = __float_as_uint(amax);
+  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return max(e, -60);
+}
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Two numbers as e4m3 codes; what is not finite becomes NaN.
+__device__ __forceinline__ uint32_t code2(float x, float y) {
+  uint32_t r = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+  if (!isfinite(x)) r = (r & 0xff00u) | 0x7fu;
+  if (!isfinite(y)) r = (r & 0x00ffu) | 0x7f00u;
+  return r;
+}
+__device__ __forceinline__ float2 decode2(uint32_t codes) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// x c - y s for bf16 x, y and (c, s) given as sums of two fp32 numbers each: the error of the result is that of its
+// last rounding, so that a rotated key falls on the same side of a rounding border as in 64 bits.  (Products of a bf16
+// and an fp32 number do not fit 24 bits: their rounding errors are carried along.)
+__device__ __forceinline__ float turn(float x, float y, float ch, float cl, float sh, float sl) {
+  const float p = x * ch, pe = fmaf(x, ch, -p);
+  const float q = y * sh, qe = fmaf(y, sh, -q);
+  const float d = p - q, z = d - p, de = (p - (d - z)) - (q + z);
+  return d + (de + (pe - qe) + (x * cl - y * sl));
+}
+
+template <int DH, int BLOCK>
+__device__ __forceinline__ int unit_offset(int u, int R, int interleaved, int which) {
+  const bool split = !interleaved && 16 * u < R;
+  return split ? 8 * u + (which ? (R >> 1) : 0) : 16 * u + 8 * which;
+}
+
+// One CTA per (sequence, block of the cache, group of kv heads): a tile of at most BLOCK tokens x DH of a head sits in
+// registers (bf16) between the maximum and the rounding, so that each input is read once and each code written once.
+template <int DH, int BLOCK, bool WIDE>
+__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
+  constexpr int U = DH / 16, ROWS = kThreads / U, NIT = (BLOCK + ROWS - 1) / ROWS;
+  extern __shared__ float4 tab[];   // [tokens][R / 2] cosine and sine as (c_hi, c_lo, s_hi, s_lo)
+  __shared__ float red[2][2][kThreads / 32];
+  const int tid = threadIdx.x, u = tid % U, r0 = tid / U;
+  int idx = blockIdx.x;
+  const int grp = idx % a.groups;
+  idx /= a.groups;
+  const int j = idx % a.nblk, b = idx / a.nblk;
+  pdl_begin();
+  const int start = max(a.seqlens[b], 0);
+  const int count = a.new_lens ? min(max(a.new_lens[b], 0), a.L) : a.L;
+  const long long end_ll = (long long)start + count;
+  const int end = (int)min(end_ll, (long long)a.c.S_max);
+  if (end_ll > a.c.S_max && j == 0 && grp == 0 && tid == 0) atomicCAS(a.status, (int)DS_OK, (int)DS_CACHE_FULL);
+  const int blk = start / BLOCK + j;
+  const long long blk0 = (long long)blk * BLOCK;
+  if (blk0 >= end_ll) return;
+  const int lo = (int)max((long long)start, blk0), hi = (int)min((long long)end, blk0 + BLOCK);
+  // (queries of tokens beyond the cache are rotated too: their range is not cut at the capacity)
+  const int nq = (int)(min(end_ll, blk0 + BLOCK) - lo), n = max(0, hi - lo);
+  const int R = a.rot.R, half = R >> 1, inter = a.rot.interleaved;
+  if (R) {
+    for (int i = tid; i < nq * half; i += kThreads) {
+      const int t = i / half;
+      double c, s;
+      fsvd_rope::angle(lo + t, a.rot.inv_freq[i - t * half], a.rot.scale, c, s);
+      const float ch = (float)c, sh = (float)s;
+      tab[i] = make_float4(ch, (float)(c - (double)ch), sh, (float)(s - (double)sh));
+    }
+    __syncthreads();
+  }
+  const int Hk = a.c.Hk, nb = (a.c.S_max + BLOCK - 1) / BLOCK;
+  const int hk0 = (int)((long long)Hk * grp / a.groups), hk1 = (int)((long long)Hk * (grp + 1) / a.groups);
+  const bool held = start > blk0;   // the block holds tokens already
+  int parity = 0;
+  for (int hk = hk0; hk < hk1 && n > 0; ++hk, parity ^= 1) {
+    uint32_t kreg[NIT][8], vreg[NIT][8];   // packed pairs (a, b)
+    float kmax = 0.0f, vmax = 0.0f;
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+      const int t = r0 + it * ROWS;
+      if (t < n) {
+        const size_t off = (size_t)b * a.kv_batch + (size_t)(lo - start + t) * a.kv_token + (size_t)hk * DH;
+        float x[8], y[8];
+        fsvd_rope::load_unit<WIDE>(a.v + off, u, R, inter, x, y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          vreg[it][i] = fsvd_rope::pack2(x[i], y[i]);
+          if (isfinite(x[i])) vmax = fmaxf(vmax, fabsf(x[i]));
+          if (isfinite(y[i])) vmax = fmaxf(vmax, fabsf(y[i]));
+        }
+        fsvd_rope::load_unit<WIDE>(a.k + off, u, R, inter, x, y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int p = 8 * u + i;
+          if (p < half) {
+            const float4 cs = tab[t * half + p];
+            const float x0 = x[i], y0 = y[i];
+            x[i] = turn(x0, y0, cs.x, cs.y, cs.z, cs.w);
+            y[i] = turn(y0, -x0, cs.x, cs.y, cs.z, cs.w);
+          }
+          kreg[it][i] = fsvd_rope::pack2(x[i], y[i]);
+          x[i] = __uint_as_float(kreg[it][i] << 16);
+          y[i] = __uint_as_float(kreg[it][i] & 0xffff0000u);
+          if (isfinite(x[i])) kmax = fmaxf(kmax, fabsf(x[i]));
+          if (isfinite(y[i])) kmax = fmaxf(kmax, fabsf(y[i]));
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) {
+      kmax = fmaxf(kmax, __shfl_xor_sync(0xffffffffu, kmax, x));
+      vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, x));
+    }
+    if ((tid & 31) == 0) {
+      red[parity][0][tid >> 5] = kmax;
+      red[parity][1][tid >> 5] = vmax;
+    }
+    const size_t si = ((size_t)b * Hk + hk) * nb + blk;
+    const float kold = held ? a.c.k_scale[si] : 0.0f, vold = held ? a.c.v_scale[si] : 0.0f;
+    __syncthreads();   // (two halves of `red` in turn: the next head writes the other one)
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      kmax = fmaxf(kmax, red[parity][0][w]);
+      vmax = fmaxf(vmax, red[parity][1][w]);
+    }
+    const int ke = scale_exponent(kmax), ve = scale_exponent(vmax);
+    const float ks = fmaxf(kold, two_to(ke)), vs = fmaxf(vold, two_to(ve));
+    const size_t base = (((size_t)b * Hk + hk) * a.c.S_max + (size_t)blk0) * DH;
+    uint8_t* kc = reinterpret_cast<uint8_t*>(a.c.k8) + base;
+    uint8_t* vc = reinterpret_cast<uint8_t*>(a.c.v8) + base;
+    if (held) {   // a larger scale: round what the block holds once more
+      const int old_bytes = (int)(start - blk0) * DH;
+      for (int which = 0; which < 2; ++which) {
+        const float was = which ? vold : kold, now = which ? vs : ks;
+        if (!(now > was)) continue;
+        uint32_t* w = reinterpret_cast<uint32_t*>(which ? vc : kc);
+        const float f = was / now;
+        for (int i = tid; i < old_bytes / 4; i += kThreads) {
+          const uint32_t x = w[i];
+          const float2 p = decode2(x & 0xffffu), q = decode2(x >> 16);
+          w[i] = code2(p.x * f, p.y * f) | (code2(q.x * f, q.y * f) << 16);
+        }
+      }
+    }
+    const float ki = 1.0f / ks, vi = 1.0f / vs;
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+      const int t = r0 + it * ROWS;
+      if (t < n) {
+        const size_t row = (size_t)(lo - blk0 + t) * DH;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+          uint8_t* dst = (which ? vc : kc) + row;
+          const float inv = which ? vi : ki;
+          uint32_t cd[8];   // codes of the pairs: low byte a, high byte b
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t w = which ? vreg[it][i] : kreg[it][i];
+            float x = __uint_as_float(w << 16) * inv, y = __uint_as_float(w & 0xffff0000u) * inv;
+            if (inv <= 0x1p-120f) {   // 256 * 2^120 is no 32-bit number any more
+              x = fabsf(x) > 240.0f && isfinite(x) ? copysignf(240.0f, x) : x;
+              y = fabsf(y) > 240.0f && isfinite(y) ? copysignf(240.0f, y) : y;
+            }
+            cd[i] = code2(x, y);
+          }
+          if constexpr (WIDE) {
+            const bool split = !inter && 16 * u < R;
+            uint2 first, second;
+            const uint32_t a03 = __byte_perm(__byte_perm(cd[0], cd[1], 0x0040), __byte_perm(cd[2], cd[3], 0x0040), 0x5410);
+            const uint32_t a47 = __byte_perm(__byte_perm(cd[4], cd[5], 0x0040), __byte_perm(cd[6], cd[7], 0x0040), 0x5410);
+            const uint32_t b03 = __byte_perm(__byte_perm(cd[0], cd[1], 0x0051), __byte_perm(cd[2], cd[3], 0x0051), 0x5410);
+            const uint32_t b47 = __byte_perm(__byte_perm(cd[4], cd[5], 0x0051), __byte_perm(cd[6], cd[7], 0x0051), 0x5410);
+            first = split ? make_uint2(a03, a47) : make_uint2(cd[0] | (cd[1] << 16), cd[2] | (cd[3] << 16));
+            second = split ? make_uint2(b03, b47) : make_uint2(cd[4] | (cd[5] << 16), cd[6] | (cd[7] << 16));
+            *reinterpret_cast<uint2*>(dst + (split ? 8 * u : 16 * u)) = first;
+            *reinterpret_cast<uint2*>(dst + (split ? 8 * u + half : 16 * u + 8)) = second;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int2 at = fsvd_rope::pair_at(8 * u + i, R, inter);
+              dst[at.x] = (uint8_t)(cd[i] & 0xffu);
+              dst[at.y] = (uint8_t)(cd[i] >> 8);
+            }
+          }
+        }
+      }
+    }
+    if (tid == 0) {
+      a.c.k_scale[si] = ks;
+      a.c.v_scale[si] = vs;
+    }
+  }
+  if (!a.q) return;
+  const int h0 = (int)((long long)a.H * grp / a.groups), h1 = (int)((long long)a.H * (grp + 1) / a.groups);
+  for (int i = r0; i < nq * (h1 - h0); i += ROWS) {
+    const int t = i / (h1 - h0), h = h0 + i - t * (h1 - h0);
+    const size_t tok = (size_t)(lo - start + t);
+    float x[8], y[8];
+    fsvd_rope::load_unit<WIDE>(a.q + (size_t)b * a.q_batch + tok * a.q_token + (size_t)h * DH, u, R, inter, x, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int p = 8 * u + e;
+      if (p < half) {
+        const float4 cs = tab[t * half + p];
+        const float x0 = x[e], y0 = y[e];
+        x[e] = x0 * cs.x - y0 * cs.z;
+        y[e] = y0 * cs.x + x0 * cs.z;
+      }
+    }
+    fsvd_rope::store_unit<WIDE>(a.q_out + (((size_t)b * a.L + tok) * a.H + h) * DH, u, R, inter, x, y);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ read-back
+struct LoadArgs {
+  fsvd_kv8 c;
+  int start, length, seqlen_add;
+  const int* seqlens;
+  __nv_bfloat16 *k_out, *v_out;
+};
+
+__global__ void __launch_bounds__(kThreads) load_kernel(const LoadArgs a) {
+  pdl_begin();
+  const int DH = a.c.Dh, V = DH / 16, nb = (a.c.S_max + a.c.block - 1) / a.c.block;
+  const size_t rows = (size_t)a.c.B * a.c.Hk * a.length, total = rows * V;
+  for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < 2 * total; i += (size_t)gridDim.x * kThreads) {
+    const bool second = i >= total;
+    const size_t at = second ? i - total : i, row = at / V, bh = row / a.length;
+    const int c = (int)(at - row * V), t = a.start + (int)(row - bh * a.length);
+    uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+    if (!a.seqlens || t < a.seqlens[bh / a.c.Hk] + a.seqlen_add) {
+      const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(second ? a.c.v8 : a.c.k8) +
+                                                      (bh * a.c.S_max + t) * DH + 16 * c);
+      const float s = (second ? a.c.v_scale : a.c.k_scale)[bh * nb + t / a.c.block];
+      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+      uint32_t o[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 p = decode2(x[e] & 0xffffu), q = decode2(x[e] >> 16);
+        o[2 * e] = fsvd_rope::pack2(p.x * s, p.y * s);
+        o[2 * e + 1] = fsvd_rope::pack2(q.x * s, q.y * s);
+      }
+      lo = make_uint4(o[0], o[1], o[2], o[3]);
+      hi = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+    uint4* out = reinterpret_cast<uint4*>((second ? a.v_out : a.k_out) + row * DH + 16 * c);
+    out[0] = lo;
+    out[1] = hi;
+  }
+}
+
+// ------------------------------------------------------------------------------------------ attention
+constexpr int kAttnThreads = 128;
+constexpr int kMaxSplits = 64;
+constexpr int kMaxGroup = 16;
+
+struct AttnArgs {
+  fsvd_kv8 c;
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  const int* seqlens;
+  float* part;       // [B, Hk, splits, G, DH + 2]
+  int* counters;     // [B, Hk], zero between launches
+  int H, seqlen_add, splits;
+  float scale;
+};
+
+// One CTA per (sequence, kv head, split of the keys), a warp per key in turn; the last CTA of a (sequence, kv head)
+// merges the splits in their order.
+template <int DH>
+__global__ void __launch_bounds__(kAttnThreads) attn_kernel(const AttnArgs a) {
+  constexpr int W = kAttnThreads / 32, D = DH / 32;
+  extern __shared__ float sh[];   // per warp and head of the group: DH sums, maximum, sum
+  __shared__ int last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = a.H / a.c.Hk, rec = DH + 2, BLOCK = a.c.block, nb = (a.c.S_max + BLOCK - 1) / BLOCK;
+  const int split = blockIdx.x % a.splits, bh = blockIdx.x / a.splits, b = bh / a.c.Hk, hk = bh % a.c.Hk;
+  pdl_begin();
+  const int n = (int)min(max((long long)a.seqlens[b] + a.seqlen_add, 0ll), (long long)a.c.S_max);
+  const int per = (n + a.splits - 1) / a.splits, j0 = min(n, split * per), j1 = min(n, j0 + per);
+  const uint8_t* kc = reinterpret_cast<const uint8_t*>(a.c.k8) + (size_t)bh * a.c.S_max * DH;
+  const uint8_t* vc = reinterpret_cast<const uint8_t*>(a.c.v8) + (size_t)bh * a.c.S_max * DH;
+  const float* ksc = a.c.k_scale + (size_t)bh * nb;
+  const float* vsc = a.c.v_scale + (size_t)bh * nb;
+  for (int g = 0; g < G; ++g) {
+    const __nv_bfloat16* q = a.q + ((size_t)b * a.H + (size_t)hk * G + g) * DH + lane * D;
+    float qf[D], o[D], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D; ++e) {
+      qf[e] = __bfloat162float(q[e]) * a.scale;
+      o[e] = 0.0f;
+    }
+    for (int t = j0 + warp; t < j1; t += W) {
+      float kf[D], vf[D], s = 0.0f;
+#pragma unroll
+      for (int e = 0; e < D; e += 2) {
+        const float2 x = decode2(*reinterpret_cast<const uint16_t*>(kc + (size_t)t * DH + lane * D + e));
+        const float2 y = decode2(*reinterpret_cast<const uint16_t*>(vc + (size_t)t * DH + lane * D + e));
+        kf[e] = x.x; kf[e + 1] = x.y; vf[e] = y.x; vf[e + 1] = y.y;
+      }
+#pragma unroll
+      for (int e = 0; e < D; ++e) s += qf[e] * kf[e];
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+      s *= ksc[t / BLOCK];
+      const float mn = fmaxf(m, s), corr = expf(m - mn), p = expf(s - mn), pv = p * vsc[t / BLOCK];
+      m = mn;
+      l = l * corr + p;
+#pragma unroll
+      for (int e = 0; e < D; ++e) o[e] = o[e] * corr + pv * vf[e];
+    }
+    float* r = sh + (size_t)(warp * G + g) * rec;
+#pragma unroll
+    for (int e = 0; e < D; ++e) r[lane * D + e] = o[e];
+    if (lane == 0) {
+      r[DH] = m;
+      r[DH + 1] = l;
+    }
+  }
+  __syncthreads();
+  // sums of `count` records that lie `stride` floats apart, rounded to the output when it is the last step
+  auto merge = [&](const float* src, size_t stride, int count, float* dst, __nv_bfloat16* out) {
+    for (int i = tid; i < G * DH; i += kAttnThreads) {
+      const int g = i / DH, d = i - g * DH;
+      float mm = -INFINITY, l = 0.0f, o = 0.0f;
+      for (int w = 0; w < count; ++w) mm = fmaxf(mm, src[w * stride + (size_t)g * rec + DH]);
+      for (int w = 0; w < count; ++w) {
+        const float* r = src + w * stride + (size_t)g * rec;
+        const float f = r[DH] == -INFINITY ? 0.0f : expf(r[DH] - mm);
+        if (r[DH + 1] != 0.0f) {
+          l += f * r[DH + 1];
+          o += f * r[d];
+        }
+      }
+      if (out) out[(size_t)g * DH + d] = __float2bfloat16_rn(l != 0.0f ? o / l : 0.0f);
+      else {
+        dst[(size_t)g * rec + d] = o;
+        if (d == 0) {
+          dst[(size_t)g * rec + DH] = mm;
+          dst[(size_t)g * rec + DH + 1] = l;
+        }
+      }
+    }
+  };
+  __nv_bfloat16* out = a.out + ((size_t)b * a.H + (size_t)hk * G) * DH;
+  if (a.splits == 1) {
+    merge(sh, (size_t)G * rec, W, nullptr, out);
+    return;
+  }
+  float* part = a.part + (size_t)bh * a.splits * G * rec;
+  merge(sh, (size_t)G * rec, W, part + (size_t)split * G * rec, nullptr);
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) last = atomicAdd(a.counters + bh, 1) == a.splits - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  merge(part, (size_t)G * rec, a.splits, nullptr, out);
+  if (tid == 0) a.counters[bh] = 0;
+}
+
+// ------------------------------------------------------------------------------------------ host
+static int check_cache(const fsvd_kv8* c) {
+  if (!c || !c->k8 || !c->v8 || !c->k_scale || !c->v_scale) return fail(FSVD_ERR_ARG, "null cache");
+  if (c->B < 1 || c->Hk < 1 || c->S_max < 1) return fail(FSVD_ERR_ARG, "bad cache sizes B=%d Hk=%d S_max=%d", c->B, c->Hk, c->S_max);
+  if (c->Dh != 64 && c->Dh != 128) return fail(FSVD_ERR_UNSUPPORTED, "head_dim %d unsupported (64, 128)", c->Dh);
+  if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128)
+    return fail(FSVD_ERR_UNSUPPORTED, "block of %d tokens unsupported (16, 32, 64, 128)", c->block);
+  if ((long long)c->B * c->Hk > (1 << 22)) return fail(FSVD_ERR_UNSUPPORTED, "B * Hk = %lld is beyond 2^22", (long long)c->B * c->Hk);
+  if (c->S_max > (1 << 30)) return fail(FSVD_ERR_UNSUPPORTED, "S_max = %d is beyond 2^30", c->S_max);
+  if (!aligned16(c->k8) || !aligned16(c->v8)) return fail(FSVD_ERR_ALIGN, "the cache must be 16-byte aligned");
+  return 0;
+}
+static int check_rotary(const double* inv_freq, int R, int Dh) {
+  if (!inv_freq) return 0;
+  if (R < 2 || R > Dh || R % 2) return fail(FSVD_ERR_ARG, "rotary_dim %d must be even, 2..%d", R, Dh);
+  return 0;
+}
+
+struct Kv8Ws {
+  size_t counters, part, total;
+};
+static Kv8Ws ws_layout(long long B, long long H, long long Hk, long long Dh) {
+  Kv8Ws w;
+  w.counters = 256;   // behind the status word (fsvd_workspace_status)
+  w.part = w.counters + (size_t)((B * Hk * 4 + 255) / 256 * 256);
+  w.total = w.part + (size_t)B * H * kMaxSplits * (Dh + 2) * 4;
+  return w;
+}
+
+template <int DH, int BLOCK>
+static int launch_append(const AppendArgs& a, size_t smem, unsigned grid, void* stream) {
+  if (a.rot.R % 16 == 0) return launch(append_kernel<DH, BLOCK, true>, dim3(grid), kThreads, smem, stream, a);
+  return launch(append_kernel<DH, BLOCK, false>, dim3(grid), kThreads, smem, stream, a);
+}
+template <int DH>
+static int launch_append(const AppendArgs& a, size_t smem, unsigned grid, void* stream) {
+  switch (a.c.block) {
+    case 16: return launch_append<DH, 16>(a, smem, grid, stream);
+    case 32: return launch_append<DH, 32>(a, smem, grid, stream);
+    case 64: return launch_append<DH, 64>(a, smem, grid, stream);
+    default: return launch_append<DH, 128>(a, smem, grid, stream);
+  }
+}
+
+}  // namespace fsvd_kv8_impl
+
+using namespace fsvd_kv8_impl;
+
+extern "C" {
+
+int fsvd_rope_qk(const void* q, long long q_stride, const void* k, long long k_stride, const int* positions,
+                 const double* inv_freq, int rotary_dim, int interleaved, float rope_scale, void* q_out, void* k_out, int T,
+                 int H, int Hk, int Dh, int dtype, void* stream) {
+  if (!q || !positions || !inv_freq || !q_out || (k != nullptr) != (k_out != nullptr)) return fail(FSVD_ERR_ARG, "null argument");
+  if (dtype != FSVD_DTYPE_BF16 && dtype != FSVD_DTYPE_F32) return fail(FSVD_ERR_ARG, "bad dtype %d", dtype);
+  if (T < 0 || H < 1 || (k && Hk < 1)) return fail(FSVD_ERR_ARG, "bad sizes T=%d H=%d Hk=%d", T, H, Hk);
+  if (Dh < 16 || Dh > 256 || Dh % 16) return fail(FSVD_ERR_UNSUPPORTED, "head_dim %d unsupported (multiples of 16 up to 256)", Dh);
+  if (int e = check_rotary(inv_freq, rotary_dim, Dh)) return e;
+  const int es = dtype == FSVD_DTYPE_F32 ? 4 : 2;
+  if (!k) Hk = 0;
+  if (q_stride < 0 || k_stride < 0) return fail(FSVD_ERR_ARG, "negative stride");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(q_out) || !aligned16(k_out) || q_stride * es % 16 || (k && k_stride * es % 16))
+    return fail(FSVD_ERR_ALIGN, "rows must start on 16-byte boundaries");
+  if (T == 0) return 0;
+  RopeArgs a;
+  a.q = q; a.k = k; a.q_out = q_out; a.k_out = k_out;
+  a.q_stride = q_stride; a.k_stride = k_stride; a.positions = positions;
+  a.rot = Rotary{inv_freq, rotary_dim, interleaved != 0, rope_scale};
+  a.T = T; a.H = H; a.Hk = Hk; a.Dh = Dh;
+  a.tokens = std::min(16, T);
+  a.heads = H + Hk;
+  const dim3 grid((T + a.tokens - 1) / a.tokens, (H + Hk + a.heads - 1) / a.heads);
+  const size_t smem = (size_t)a.tokens * (rotary_dim / 2) * sizeof(float2);
+  const bool wide = rotary_dim % 16 == 0;
+  if (dtype == FSVD_DTYPE_F32)
+    return wide ? launch(rope_kernel<float, true>, grid, kThreads, smem, stream, a)
+                : launch(rope_kernel<float, false>, grid, kThreads, smem, stream, a);
+  return wide ? launch(rope_kernel<__nv_bfloat16, true>, grid, kThreads, smem, stream, a)
+              : launch(rope_kernel<__nv_bfloat16, false>, grid, kThreads, smem, stream, a);
+}
+
+size_t fsvd_kv8_workspace_bytes(int B, int H, int Hk, int Dh, int S_max) {
+  if (B < 1 || H < 1 || Hk < 1 || (Dh != 64 && Dh != 128) || S_max < 1) return 0;
+  return ws_layout(B, H, Hk, Dh).total;
+}
+
+int fsvd_kv8_append(const fsvd_kv8* cache, const void* k, const void* v, long long kv_batch_stride, long long kv_token_stride,
+                    const int* cache_seqlens, const int* new_lens, const void* q, long long q_batch_stride,
+                    long long q_token_stride, void* q_out, const double* inv_freq, int rotary_dim, int interleaved,
+                    float rope_scale, int H, int L, void* ws, size_t ws_bytes, void* stream) {
+  if (int e = check_cache(cache)) return e;
+  if (!k || !v || !cache_seqlens || (q != nullptr) != (q_out != nullptr)) return fail(FSVD_ERR_ARG, "null argument");
+  if (q && !inv_freq) return fail(FSVD_ERR_ARG, "queries are passed to be rotated: inv_freq is missing");
+  if (int e = check_rotary(inv_freq, rotary_dim, cache->Dh)) return e;
+  if (L < 0 || (q && H < 1)) return fail(FSVD_ERR_ARG, "bad sizes L=%d H=%d", L, H);
+  if (kv_batch_stride < 0 || kv_token_stride < 0 || q_batch_stride < 0 || q_token_stride < 0) return fail(FSVD_ERR_ARG, "negative stride");
+  if (!aligned16(k) || !aligned16(v) || !aligned16(q) || !aligned16(q_out) || kv_batch_stride % 8 || kv_token_stride % 8 ||
+      (q && (q_batch_stride % 8 || q_token_stride % 8)))
+    return fail(FSVD_ERR_ALIGN, "rows must start on 16-byte boundaries");
+  if (!ws || ws_bytes < 256) return fail(FSVD_ERR_WORKSPACE, "no workspace");
+  if (!aligned16(ws)) return fail(FSVD_ERR_ALIGN, "workspace is not 16-byte aligned");
+  if (L == 0) return 0;
+  AppendArgs a;
+  a.c = *cache;
+  a.k = reinterpret_cast<const __nv_bfloat16*>(k);
+  a.v = reinterpret_cast<const __nv_bfloat16*>(v);
+  a.q = reinterpret_cast<const __nv_bfloat16*>(q);
+  a.q_out = reinterpret_cast<__nv_bfloat16*>(q_out);
+  a.kv_batch = kv_batch_stride; a.kv_token = kv_token_stride; a.q_batch = q_batch_stride; a.q_token = q_token_stride;
+  a.seqlens = cache_seqlens; a.new_lens = new_lens;
+  a.status = &reinterpret_cast<SyncState*>(ws)->status;
+  a.rot = Rotary{inv_freq, inv_freq ? rotary_dim : 0, interleaved != 0, rope_scale};
+  a.H = q ? H : 0; a.L = L;
+  const int BLOCK = cache->block;
+  a.nblk = (int)(((long long)L + BLOCK - 2) / BLOCK + 1);
+  a.groups = cache->Hk;
+  const long long grid = (long long)cache->B * a.nblk * a.groups;
+  if (grid > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many tokens for one call");
+  const size_t smem = (size_t)std::min(BLOCK, L) * (a.rot.R / 2) * sizeof(float4);
+  return cache->Dh == 64 ? launch_append<64>(a, smem, (unsigned)grid, stream) : launch_append<128>(a, smem, (unsigned)grid, stream);
+}
+
+int fsvd_kv8_load(const fsvd_kv8* cache, int start, int length, const int* cache_seqlens, int seqlen_add, void* k_out,
+                  void* v_out, void* stream) {
+  if (int e = check_cache(cache)) return e;
+  if (!k_out || !v_out) return fail(FSVD_ERR_ARG, "null argument");
+  if (start < 0 || length < 0 || (long long)start + length > cache->S_max)
+    return fail(FSVD_ERR_ARG, "positions %d + %d are outside the cache (%d)", start, length, cache->S_max);
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail(FSVD_ERR_ALIGN, "outputs must be 16-byte aligned");
+  if (length == 0) return 0;
+  LoadArgs a = {*cache, start, length, seqlen_add, cache_seqlens, reinterpret_cast<__nv_bfloat16*>(k_out),
+                reinterpret_cast<__nv_bfloat16*>(v_out)};
+  const long long items = 2ll * cache->B * cache->Hk * length * (cache->Dh / 16);
+  const long long grid = std::min<long long>((items + kThreads - 1) / kThreads, 16ll * sm_count());
+  return launch(load_kernel, dim3((unsigned)grid), kThreads, 0, stream, a);
+}
+
+int fsvd_flash_decode_kv8(const fsvd_kv8* cache, const void* q, const int* cache_seqlens, int seqlen_add, void* out, int H,
+                          float scale, void* ws, size_t ws_bytes, void* stream) {
+  if (int e = check_cache(cache)) return e;
+  if (!q || !cache_seqlens || !out) return fail(FSVD_ERR_ARG, "null argument");
+  if (H < 1 || H % cache->Hk) return fail(FSVD_ERR_ARG, "H=%d not a multiple of Hk=%d", H, cache->Hk);
+  const int G = H / cache->Hk;
+  if (G > kMaxGroup) return fail(FSVD_ERR_UNSUPPORTED, "H/Hk=%d unsupported (1..%d)", G, kMaxGroup);
+  if (!aligned16(q) || !aligned16(out)) return fail(FSVD_ERR_ALIGN, "q and out must be 16-byte aligned");
+  const Kv8Ws L = ws_layout(cache->B, H, cache->Hk, cache->Dh);
+  if (!ws) return fail(FSVD_ERR_WORKSPACE, "null workspace");
+  if (!aligned16(ws)) return fail(FSVD_ERR_ALIGN, "workspace is not 16-byte aligned");
+  if (ws_bytes < L.total) return fail(FSVD_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", ws_bytes, L.total);
+  AttnArgs a;
+  a.c = *cache;
+  a.q = reinterpret_cast<const __nv_bfloat16*>(q);
+  a.out = reinterpret_cast<__nv_bfloat16*>(out);
+  a.seqlens = cache_seqlens;
+  a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + L.part);
+  a.counters = reinterpret_cast<int*>(reinterpret_cast<char*>(ws) + L.counters);
+  a.H = H; a.seqlen_add = seqlen_add;
+  a.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)cache->Dh);
+  const long long heads = (long long)cache->B * cache->Hk;
+  a.splits = (int)std::max(1ll, std::min({4ll * sm_count() / heads, (long long)(cache->S_max + 127) / 128, (long long)kMaxSplits}));
+  const size_t smem = (size_t)(kAttnThreads / 32) * G * (cache->Dh + 2) * sizeof(float);
+  const dim3 grid((unsigned)(heads * a.splits));
+  return cache->Dh == 64 ? launch(attn_kernel<64>, grid, kAttnThreads, smem, stream, a)
+                         : launch(attn_kernel<128>, grid, kAttnThreads, smem, stream, a);
+}
+
+}  // extern "C"

@@ -1,0 +1,110 @@
+// Rotary positions: the arithmetic that fsvd_rope_qk and fsvd_kv8_append share.
+//
+// A head of Dh dimensions is Dh / 2 pairs: pair p < R / 2 turns by position * inv_freq[p] and is made of dimensions
+// (p, p + R / 2), or (2 p, 2 p + 1) when interleaved; the pairs behind them, (R + 2 j, R + 2 j + 1), stay.  A thread
+// owns a unit of eight consecutive pairs of a row: it reads all 16 numbers before it writes any, so that a row can be
+// rotated in place.  When R is a multiple of 16 a unit is two 16-byte vectors (WIDE); else 16 single numbers.
+#pragma once
+#include <cuda_bf16.h>
+#include <stdint.h>
+
+namespace fsvd_rope {
+
+struct Rotary {
+  const double* inv_freq;   // [R / 2], radians per position
+  int R, interleaved;
+  float scale;
+};
+
+// Sine and cosine of position * f, f in radians per position.  The angle is formed and reduced in 64 bits: in 32, a
+// position of 10^5 leaves the fastest pair 0.004 radians off.
+__device__ __forceinline__ void angle(int position, double f, float scale, double& c, double& s) {
+  const double turns = (double)position * (f * 0.15915494309189533577);   // 1 / (2 pi)
+  sincospi(2.0 * (turns - rint(turns)), &s, &c);
+  c *= (double)scale;
+  s *= (double)scale;
+}
+
+// Offsets of the two numbers of pair p within the row.
+__device__ __forceinline__ int2 pair_at(int p, int R, int interleaved) {
+  const int half = R >> 1;
+  if (p >= half || interleaved) return make_int2(2 * p, 2 * p + 1);   // (behind the rotated part: R + 2 (p - R / 2))
+  return make_int2(p, p + half);
+}
+
+__device__ __forceinline__ void widen(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) { widen(*reinterpret_cast<const uint4*>(p), f); }
+__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack2(f[0], f[1]), pack2(f[2], f[3]), pack2(f[4], f[5]), pack2(f[6], f[7]));
+}
+__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+__device__ __forceinline__ float num(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float num(float x) { return x; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+__device__ __forceinline__ void put(float* p, float x) { *p = x; }
+
+// The eight pairs of unit u as (a[i], b[i]).
+template <bool WIDE, typename T>
+__device__ __forceinline__ void load_unit(const T* row, int u, int R, int interleaved, float (&a)[8], float (&b)[8]) {
+  if constexpr (WIDE) {
+    const bool split = !interleaved && 16 * u < R;   // (16 u = twice the first pair)
+    float x[8], y[8];
+    load8(row + (split ? 8 * u : 16 * u), x);
+    load8(row + (split ? 8 * u + (R >> 1) : 16 * u + 8), y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float lo = i < 4 ? x[(2 * i) & 7] : y[(2 * i) & 7], hi = i < 4 ? x[(2 * i + 1) & 7] : y[(2 * i + 1) & 7];
+      a[i] = split ? x[i] : lo;
+      b[i] = split ? y[i] : hi;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int2 at = pair_at(8 * u + i, R, interleaved);
+      a[i] = num(row[at.x]);
+      b[i] = num(row[at.y]);
+    }
+  }
+}
+template <bool WIDE, typename T>
+__device__ __forceinline__ void store_unit(T* row, int u, int R, int interleaved, const float (&a)[8], const float (&b)[8]) {
+  if constexpr (WIDE) {
+    const bool split = !interleaved && 16 * u < R;
+    float x[8], y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float lo = (i & 1) ? b[i >> 1] : a[i >> 1], hi = (i & 1) ? b[4 + (i >> 1)] : a[4 + (i >> 1)];
+      x[i] = split ? a[i] : lo;
+      y[i] = split ? b[i] : hi;
+    }
+    store8(row + (split ? 8 * u : 16 * u), x);
+    store8(row + (split ? 8 * u + (R >> 1) : 16 * u + 8), y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int2 at = pair_at(8 * u + i, R, interleaved);
+      put(row + at.x, a[i]);
+      put(row + at.y, b[i]);
+    }
+  }
+}
+
+}  // namespace fsvd_rope

@@ -291,3 +291,226 @@ def tp_decode_layer(dims: FsvdDims, layer: FsvdLayer, cos, sin, cache_seqlens, x
         C.byref(dims), C.byref(layer), _ptr(cos), _ptr(sin), _ptr(cache_seqlens), _ptr(x_in), _ptr(x_norm_in),
         _ptr(x_out), _ptr(next_norm_w), _ptr(x_norm_out), exchange, ws.ptr, ws.nbytes, _stream()))
     return x_out
+
+
+# ---- operators for callers that drive the layers themselves: rotary positions, the 8-bit cache, the next token
+def _raw_stream(device: torch.device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class _SameDevice:
+    """Makes the device of the tensors current for the launch (nothing to do when it is)."""
+
+    __slots__ = ("index", "was")
+
+    def __init__(self, device: torch.device):
+        self.index, self.was = device.index, None
+
+    def __enter__(self):
+        now = torch.cuda.current_device()
+        if now != self.index:
+            self.was = now
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.was is not None:
+            torch.cuda.set_device(self.was)
+
+
+def _want(name: str, t, dtype, device, shape=None, strided: bool = False):
+    """Checks one tensor argument; with `strided` only the last two dimensions have to be contiguous."""
+    if not torch.is_tensor(t) or not t.is_cuda:
+        raise ValueError(f"{name}: flashsvd_b200 ops need CUDA tensors (there is no CPU path)")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on {device}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if strided:
+        if t.numel() and (t.stride(-1) != 1 and t.shape[-1] > 1 or t.stride(-2) != t.shape[-1] and t.shape[-2] > 1):
+            raise ValueError(f"{name}: heads and dimensions must be contiguous")
+    elif not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t
+
+
+def rope_qk(q, k, positions, inv_freq, *, interleaved=False, scale=1.0, q_out=None, k_out=None):
+    """Rotates q[T, H, Dh] and k[T, Hk, Dh] (or None) at positions[T] (int32); returns (q_out, k_out).
+
+    Dimensions [0, 2 * len(inv_freq)) of a head take part: pair i turns by ``position * inv_freq[i]`` (float64, formed
+    in 64 bits), pairs are (i, i + len(inv_freq)), or (2i, 2i + 1) with ``interleaved``; cos and sin are multiplied by
+    ``scale``; the other dimensions are copied.  bfloat16 or float32; tokens may be strided (slices of a packed
+    projection).  q_out / k_out may be q / k themselves when those are contiguous."""
+    if q.ndim != 3:
+        raise ValueError(f"q must be [T, H, Dh], got {tuple(q.shape)}")
+    T, H, Dh = q.shape
+    dtype, dev = q.dtype, q.device
+    code = _dtype_code(dtype)
+    _want("q", q, dtype, dev, strided=True)
+    _want("positions", positions, torch.int32, dev, (T,))
+    if inv_freq.ndim != 1:
+        raise ValueError("inv_freq must be a vector")
+    _want("inv_freq", inv_freq, torch.float64, dev)
+    Hk = 0
+    if k is not None:
+        if k.ndim != 3:
+            raise ValueError(f"k must be [T, Hk, Dh], got {tuple(k.shape)}")
+        Hk = k.shape[1]
+        _want("k", k, dtype, dev, (T, Hk, Dh), strided=True)
+        k_out = torch.empty((T, Hk, Dh), dtype=dtype, device=dev) if k_out is None else _want("k_out", k_out, dtype, dev, k.shape)
+    elif k_out is not None:
+        raise ValueError("k_out without k")
+    q_out = torch.empty((T, H, Dh), dtype=dtype, device=dev) if q_out is None else _want("q_out", q_out, dtype, dev, q.shape)
+    if T == 0:
+        return q_out, k_out
+    with _SameDevice(dev):
+        check(_lib.load().fsvd_rope_qk(
+            q.data_ptr(), q.stride(0) if T > 1 else 0, None if k is None else k.data_ptr(), 0 if k is None or T < 2 else k.stride(0),
+            positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(interleaved), float(scale), q_out.data_ptr(),
+            None if k is None else k_out.data_ptr(), T, H, Hk, Dh, code, _raw_stream(dev)))
+    return q_out, k_out
+
+
+def make_kv8_workspace(batch, num_heads, num_kv_heads, head_dim, max_len, device) -> Workspace:
+    """Scratch of ``kv8_append`` and ``flash_decode_kv8`` for these sizes; launches that share one must be ordered."""
+    n = int(_lib.load().fsvd_kv8_workspace_bytes(int(batch), int(num_heads), int(num_kv_heads), int(head_dim), int(max_len)))
+    if n == 0:
+        raise ValueError(f"no 8-bit cache of these sizes: batch {batch}, heads {num_heads}/{num_kv_heads}, head_dim {head_dim}, "
+                         f"max_len {max_len}")
+    return Workspace(torch.zeros(n, dtype=torch.uint8, device=device), n)
+
+
+def _ws_of(ws: Workspace, dev) -> Workspace:
+    if ws.buf.device != dev:
+        raise ValueError(f"the workspace is on {ws.buf.device}, the call's tensors on {dev}")
+    return ws
+
+
+def kv8_append(k, v, cache, cache_seqlens, ws: Workspace, *, new_lens=None, q=None, rotary=None, q_out=None):
+    """Quantises k / v [B, L, Hk, Dh] into ``cache`` (kv8.KV8Cache) at positions cache_seqlens[b] .. + L - 1
+    (+ new_lens[b] - 1 with ``new_lens``); with ``rotary`` (kv8.Rotary) the keys, and q [B, L, H, Dh] when given, are
+    rotated at their positions first.  Returns the rotated q (rows past new_lens[b] are not written) or None.
+
+    cache_seqlens (int32 [B]) is not advanced.  A token that does not fit the cache is dropped and sets the workspace
+    status, as in ``qkv_rope_append``.  Batch and tokens may be strided."""
+    st, dev = cache.struct, cache.device
+    if k.ndim != 4:
+        raise ValueError(f"k must be [B, L, {st.Hk}, {st.Dh}], got {tuple(k.shape)}")
+    B, L = k.shape[0], k.shape[1]
+    _want("k", k, torch.bfloat16, dev, (st.B, L, st.Hk, st.Dh), strided=True)
+    _want("v", v, torch.bfloat16, dev, k.shape, strided=True)
+    if v.stride() != k.stride():
+        v = v.contiguous()
+        k = k.contiguous()
+    _want("cache_seqlens", cache_seqlens, torch.int32, dev, (B,))
+    if new_lens is not None:
+        _want("new_lens", new_lens, torch.int32, dev, (B,))
+    H, qs = 0, (0, 0)
+    if rotary is not None:
+        if rotary.inv_freq.ndim != 1:
+            raise ValueError("inv_freq must be a vector")
+        _want("inv_freq", rotary.inv_freq, torch.float64, dev)
+    if q is not None:
+        if rotary is None:
+            raise ValueError("q is passed to be rotated: rotary is missing")
+        if q.ndim != 4:
+            raise ValueError(f"q must be [B, L, H, Dh], got {tuple(q.shape)}")
+        H = q.shape[2]
+        _want("q", q, torch.bfloat16, dev, (B, L, H, st.Dh), strided=True)
+        qs = (q.stride(0), q.stride(1))
+        if q_out is None:
+            q_out = torch.empty((B, L, H, st.Dh), dtype=torch.bfloat16, device=dev)
+        else:
+            _want("q_out", q_out, torch.bfloat16, dev, q.shape)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    _ws_of(ws, dev)
+    if L == 0:
+        return q_out
+    with _SameDevice(dev):
+        check(_lib.load().fsvd_kv8_append(
+            cache.ref, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), cache_seqlens.data_ptr(),
+            None if new_lens is None else new_lens.data_ptr(), None if q is None else q.data_ptr(), *qs,
+            None if q is None else q_out.data_ptr(), None if rotary is None else rotary.inv_freq.data_ptr(),
+            0 if rotary is None else 2 * rotary.inv_freq.shape[0], 0 if rotary is None else int(rotary.interleaved),
+            1.0 if rotary is None else float(rotary.scale), H, L, ws.ptr, ws.nbytes, _raw_stream(dev)))
+    return q_out
+
+
+def kv8_load(cache, start, length, *, cache_seqlens=None, seqlen_add=0, k_out=None, v_out=None):
+    """Positions [start, start + length) of the cache as bfloat16 numbers: (k, v), each [B, Hk, length, Dh].  With
+    ``cache_seqlens`` rows from cache_seqlens[b] + seqlen_add on are zeros."""
+    st, dev = cache.struct, cache.device
+    start, length = int(start), int(length)
+    if start < 0 or length < 0 or start + length > st.S_max:
+        raise ValueError(f"positions {start} + {length} are outside the cache ({st.S_max})")
+    shape = (st.B, st.Hk, length, st.Dh)
+    if cache_seqlens is not None:
+        _want("cache_seqlens", cache_seqlens, torch.int32, dev, (st.B,))
+    k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if k_out is None else _want("k_out", k_out, torch.bfloat16, dev, shape)
+    v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if v_out is None else _want("v_out", v_out, torch.bfloat16, dev, shape)
+    if length == 0:
+        return k_out, v_out
+    with _SameDevice(dev):
+        check(_lib.load().fsvd_kv8_load(cache.ref, start, length, None if cache_seqlens is None else cache_seqlens.data_ptr(),
+                                        int(seqlen_add), k_out.data_ptr(), v_out.data_ptr(), _raw_stream(dev)))
+    return k_out, v_out
+
+
+def flash_decode_kv8(q, cache, cache_seqlens, ws: Workspace, *, seqlen_add=0, scale=0.0, out=None):
+    """``flash_decode`` over an 8-bit cache: q[B, H, Dh] bfloat16 against positions [0, cache_seqlens[b] + seqlen_add),
+    scale <= 0 selects 1/sqrt(Dh); a sequence without positions gives zeros."""
+    st, dev = cache.struct, cache.device
+    if q.ndim != 3:
+        raise ValueError(f"q must be [B, H, Dh], got {tuple(q.shape)}")
+    H = q.shape[1]
+    _want("q", q, torch.bfloat16, dev, (st.B, H, st.Dh))
+    _want("cache_seqlens", cache_seqlens, torch.int32, dev, (st.B,))
+    out = torch.empty_like(q) if out is None else _want("out", out, torch.bfloat16, dev, q.shape)
+    _ws_of(ws, dev)
+    with _SameDevice(dev):
+        check(_lib.load().fsvd_flash_decode_kv8(cache.ref, q.data_ptr(), cache_seqlens.data_ptr(), int(seqlen_add), out.data_ptr(),
+                                                H, float(scale), ws.ptr, ws.nbytes, _raw_stream(dev)))
+    return out
+
+
+def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, probs_out=None):
+    """One token per row of logits[B, V] (float32 or bfloat16; rows may be strided) from uniforms[B] (float32 in [0, 1)):
+    (tokens int32 [B], probs float32 [B]).
+
+    Weights are exp((logit - max) / temperature).  In descending order of the logits (lower index first among equals)
+    the first ``top_k`` stay (0: all), of those the ones whose preceding mass is at most ``top_p`` of it (1: all), of
+    those the ones with weight >= ``min_p`` (0: all).  The token is the first one in index order whose running mass
+    exceeds uniforms[b] of the kept mass; probs is its share.  temperature <= 0 takes the largest logit.  Each setting
+    is a number or a tensor with one value per row (float32; top_k int32)."""
+    if logits.ndim != 2:
+        raise ValueError(f"logits must be [B, V], got {tuple(logits.shape)}")
+    B, V = logits.shape
+    dev = logits.device
+    code = _dtype_code(logits.dtype)
+    if not logits.is_cuda:
+        raise ValueError("logits: flashsvd_b200 ops need CUDA tensors (there is no CPU path)")
+    if V < 1:
+        raise ValueError("logits of an empty vocabulary")
+    if V > 1 and logits.stride(1) != 1:
+        raise ValueError("logits: a row must be contiguous")
+    _want("uniforms", uniforms, torch.float32, dev, (B,))
+    ptrs, values = [], []
+    for name, x, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
+        if torch.is_tensor(x):
+            ptrs.append(_want(name, x, dtype, dev, (B,)).data_ptr())
+            values.append(0)
+        else:
+            ptrs.append(None)
+            values.append(int(x) if dtype == torch.int32 else float(x))
+    out = torch.empty(B, dtype=torch.int32, device=dev) if out is None else _want("out", out, torch.int32, dev, (B,))
+    probs_out = torch.empty(B, dtype=torch.float32, device=dev) if probs_out is None else _want("probs_out", probs_out, torch.float32, dev, (B,))
+    if B == 0:
+        return out, probs_out
+    with _SameDevice(dev):
+        check(_lib.load().fsvd_sample(
+            logits.data_ptr(), logits.stride(0) if B > 1 else V, code, uniforms.data_ptr(), *ptrs, *values, out.data_ptr(),
+            probs_out.data_ptr(), B, V, _raw_stream(dev)))
+    return out, probs_out

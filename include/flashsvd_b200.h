@@ -339,6 +339,73 @@ int fsvd_tp_decode_layer(const fsvd_dims* dims, const fsvd_layer* layer, const v
                          const void* x_norm_in, void* x_out, const void* next_norm_w, void* x_norm_out,
                          fsvd_exchange* ex, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- Operators for callers that drive the layers themselves ---------------------------------
+ * Rotary positions, a key / value cache held in 8 bits, and the choice of the next token.  No
+ * counterpart in the reference, whose cache is dense in the model dtype
+ * (runtime/cache/attn_dense_kv.py:7-15) and whose sampler runs on sorted probabilities in PyTorch
+ * (scripts/demo_support/api.py:192-209).  Row strides are in elements; the last two dimensions of
+ * q, k and v are contiguous.  All pointers are 16-byte aligned, strides multiples of 16 bytes.
+ *
+ * Rotary: dimensions [0, rotary_dim) of a head turn by position * inv_freq[i] (double, radians per
+ * position, device memory, rotary_dim / 2 entries), pair i = dimensions (i, i + rotary_dim / 2), or
+ * (2 i, 2 i + 1) when interleaved; cos and sin are multiplied by rope_scale.  The angle is formed in
+ * 64 bits, so that far positions keep their phase.  rotary_dim is even, 2..Dh.
+ *
+ * q_out / k_out [T, H|Hk, Dh] (contiguous) may be the inputs when those are contiguous.  k and k_out
+ * may both be NULL.  dtype bf16 or f32, Dh a multiple of 8 up to 256. */
+int fsvd_rope_qk(const void* q, long long q_stride, const void* k, long long k_stride, const int* positions,
+                 const double* inv_freq, int rotary_dim, int interleaved, float rope_scale, void* q_out, void* k_out,
+                 int T, int H, int Hk, int Dh, int dtype, void* stream);
+
+/* 8-bit cache: k8 / v8 [B, Hk, S_max, Dh] e4m3 codes, k_scale / v_scale [B, Hk, ceil(S_max / block)]
+ * fp32; the number that a code stands for is code * scale.  block is 16, 32, 64 or 128, Dh 64 or 128;
+ * activations are bf16. */
+typedef struct fsvd_kv8 {
+  void* k8;
+  void* v8;
+  float* k_scale;
+  float* v_scale;
+  int B, Hk, S_max, Dh, block;
+} fsvd_kv8;
+/* Scratch of fsvd_kv8_append and fsvd_flash_decode_kv8 for H query heads: status word (read with
+ * fsvd_workspace_status), arrival counters, partial results of the key splits.  Zero it once
+ * (fsvd_workspace_init).  Launches that share one must be ordered on the device. */
+size_t fsvd_kv8_workspace_bytes(int B, int H, int Hk, int Dh, int S_max);
+/* New tokens k / v [B, L, Hk, Dh] (batch and token strides given) go to positions cache_seqlens[b] ..
+ * + new_lens[b] - 1 (new_lens NULL: L each).  With inv_freq the keys, and q [B, L, H, Dh] -> q_out when
+ * q is given, are rotated at their positions first (a key is rounded to bf16 before it is quantised).
+ * A block's scale is the smallest power of two >= 2^-60 for which its largest finite magnitude fits
+ * 448 * scale; codes are rounded to nearest even (down where a code times 2^120 would pass the 32-bit range).  When a later token needs a larger scale, the codes
+ * that the block already holds are rounded again to the new one.  Values that are not finite are stored as
+ * NaN and take no part in the scale.  Scales of blocks that hold tokens must be positive and finite.
+ * cache_seqlens is not advanced.  A token at a position >= S_max is dropped and sets status 4. */
+int fsvd_kv8_append(const fsvd_kv8* cache, const void* k, const void* v, long long kv_batch_stride, long long kv_token_stride,
+                    const int* cache_seqlens, const int* new_lens, const void* q, long long q_batch_stride,
+                    long long q_token_stride, void* q_out, const double* inv_freq, int rotary_dim, int interleaved,
+                    float rope_scale, int H, int L, void* ws, size_t ws_bytes, void* stream);
+/* Positions [start, start + length) as bf16 numbers, k_out / v_out [B, Hk, length, Dh].  With
+ * cache_seqlens, rows from cache_seqlens[b] + seqlen_add on are zeros. */
+int fsvd_kv8_load(const fsvd_kv8* cache, int start, int length, const int* cache_seqlens, int seqlen_add, void* k_out,
+                  void* v_out, void* stream);
+/* As fsvd_flash_decode over an 8-bit cache: q and out [B, H, Dh] bf16, H / Hk any whole number up to
+ * 16; a sequence of length 0 gives zeros. */
+int fsvd_flash_decode_kv8(const fsvd_kv8* cache, const void* q, const int* cache_seqlens, int seqlen_add, void* out, int H,
+                          float scale, void* ws, size_t ws_bytes, void* stream);
+
+/* One token per row of logits[B, V] (dtype f32 or bf16, rows row_stride elements apart).  Weights are
+ * exp((l - max) / temperature).  The vocabulary is ordered by logit, descending, lower index first; the
+ * tokens kept are a prefix of it: the first top_k (0 or >= V: all), of those the ones whose preceding
+ * mass is at most top_p times the mass of all of them (>= 1: all), of those the ones with weight >=
+ * min_p (<= 0: all); at least one.  The token is the first kept one in index order whose running mass
+ * exceeds uniforms[b] times the kept mass; probs (may be NULL) gets its share of that mass.  A
+ * temperature <= 0 (or NaN) takes the largest logit, an infinite one counts as the largest finite number.  NaN counts as -infinity; a row without anything above
+ * -infinity gives token 0 with share 0.  temperature, top_k, top_p, min_p: one value per row in
+ * device memory, or NULL and the value for all rows.  Masses are integer sums of weights in fixed point:
+ * the result does not depend on the order of additions. */
+int fsvd_sample(const void* logits, long long row_stride, int dtype, const float* uniforms, const float* temperature,
+                const int* top_k, const float* top_p, const float* min_p, float temperature_all, int top_k_all,
+                float top_p_all, float min_p_all, int* tokens, float* probs, int B, int V, void* stream);
+
 /* Kernel launches enqueued by this library since load (for launch accounting). */
 long long fsvd_launch_count(void);
 
