@@ -74,6 +74,8 @@ static Settings current_settings() {
   return g_set;
 }
 
+long long fsvd_tile_wait_limit() { return current_settings().wait_limit; }
+
 struct DevProps {
   int device = -1, sms = 0, smem_optin = 0;
 };

@@ -13,6 +13,7 @@
 #include <atomic>
 
 #include "../../include/flashsvd_b200.h"
+#include "fsvd_kv8_attn.cuh"
 #include "fsvd_rope.cuh"
 #include "fsvd_stage.h"
 #include "fsvd_tile.h"
@@ -53,7 +54,7 @@ __device__ __forceinline__ void pdl_begin() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 template <typename... Params, typename... Args>
-static int launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, void* stream, Args... args) {
+static int launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, void* stream, const Args&... args) {
   // Above the 48 KB that a kernel has by itself the limit is raised at every such launch: a setting of the current
   // device, so nothing is remembered.
   if (smem > 48 * 1024) {
@@ -70,7 +71,7 @@ static int launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) return fail(FSVD_ERR_CUDA, "kernel launch failed: %s", cudaGetErrorString(e));
   fsvd_tile_count_launch();
   return 0;
@@ -406,116 +407,6 @@ __global__ void __launch_bounds__(kThreads) load_kernel(const LoadArgs a) {
   }
 }
 
-// ------------------------------------------------------------------------------------------ attention
-constexpr int kAttnThreads = 128;
-constexpr int kMaxSplits = 64;
-constexpr int kMaxGroup = 16;
-
-struct AttnArgs {
-  fsvd_kv8 c;
-  const __nv_bfloat16* q;
-  __nv_bfloat16* out;
-  const int* seqlens;
-  float* part;       // [B, Hk, splits, G, DH + 2]
-  int* counters;     // [B, Hk], zero between launches
-  int H, seqlen_add, splits;
-  float scale;
-};
-
-// One CTA per (sequence, kv head, split of the keys), a warp per key in turn; the last CTA of a (sequence, kv head)
-// merges the splits in their order.
-template <int DH>
-__global__ void __launch_bounds__(kAttnThreads) attn_kernel(const AttnArgs a) {
-  constexpr int W = kAttnThreads / 32, D = DH / 32;
-  extern __shared__ float sh[];   // per warp and head of the group: DH sums, maximum, sum
-  __shared__ int last;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int G = a.H / a.c.Hk, rec = DH + 2, BLOCK = a.c.block, nb = (a.c.S_max + BLOCK - 1) / BLOCK;
-  const int split = blockIdx.x % a.splits, bh = blockIdx.x / a.splits, b = bh / a.c.Hk, hk = bh % a.c.Hk;
-  pdl_begin();
-  const int n = (int)min(max((long long)a.seqlens[b] + a.seqlen_add, 0ll), (long long)a.c.S_max);
-  const int per = (n + a.splits - 1) / a.splits, j0 = min(n, split * per), j1 = min(n, j0 + per);
-  const uint8_t* kc = reinterpret_cast<const uint8_t*>(a.c.k8) + (size_t)bh * a.c.S_max * DH;
-  const uint8_t* vc = reinterpret_cast<const uint8_t*>(a.c.v8) + (size_t)bh * a.c.S_max * DH;
-  const float* ksc = a.c.k_scale + (size_t)bh * nb;
-  const float* vsc = a.c.v_scale + (size_t)bh * nb;
-  for (int g = 0; g < G; ++g) {
-    const __nv_bfloat16* q = a.q + ((size_t)b * a.H + (size_t)hk * G + g) * DH + lane * D;
-    float qf[D], o[D], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < D; ++e) {
-      qf[e] = __bfloat162float(q[e]) * a.scale;
-      o[e] = 0.0f;
-    }
-    for (int t = j0 + warp; t < j1; t += W) {
-      float kf[D], vf[D], s = 0.0f;
-#pragma unroll
-      for (int e = 0; e < D; e += 2) {
-        const float2 x = decode2(*reinterpret_cast<const uint16_t*>(kc + (size_t)t * DH + lane * D + e));
-        const float2 y = decode2(*reinterpret_cast<const uint16_t*>(vc + (size_t)t * DH + lane * D + e));
-        kf[e] = x.x; kf[e + 1] = x.y; vf[e] = y.x; vf[e + 1] = y.y;
-      }
-#pragma unroll
-      for (int e = 0; e < D; ++e) s += qf[e] * kf[e];
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= ksc[t / BLOCK];
-      const float mn = fmaxf(m, s), corr = expf(m - mn), p = expf(s - mn), pv = p * vsc[t / BLOCK];
-      m = mn;
-      l = l * corr + p;
-#pragma unroll
-      for (int e = 0; e < D; ++e) o[e] = o[e] * corr + pv * vf[e];
-    }
-    float* r = sh + (size_t)(warp * G + g) * rec;
-#pragma unroll
-    for (int e = 0; e < D; ++e) r[lane * D + e] = o[e];
-    if (lane == 0) {
-      r[DH] = m;
-      r[DH + 1] = l;
-    }
-  }
-  __syncthreads();
-  // sums of `count` records that lie `stride` floats apart, rounded to the output when it is the last step
-  auto merge = [&](const float* src, size_t stride, int count, float* dst, __nv_bfloat16* out) {
-    for (int i = tid; i < G * DH; i += kAttnThreads) {
-      const int g = i / DH, d = i - g * DH;
-      float mm = -INFINITY, l = 0.0f, o = 0.0f;
-      for (int w = 0; w < count; ++w) mm = fmaxf(mm, src[w * stride + (size_t)g * rec + DH]);
-      for (int w = 0; w < count; ++w) {
-        const float* r = src + w * stride + (size_t)g * rec;
-        const float f = r[DH] == -INFINITY ? 0.0f : expf(r[DH] - mm);
-        if (r[DH + 1] != 0.0f) {
-          l += f * r[DH + 1];
-          o += f * r[d];
-        }
-      }
-      if (out) out[(size_t)g * DH + d] = __float2bfloat16_rn(l != 0.0f ? o / l : 0.0f);
-      else {
-        dst[(size_t)g * rec + d] = o;
-        if (d == 0) {
-          dst[(size_t)g * rec + DH] = mm;
-          dst[(size_t)g * rec + DH + 1] = l;
-        }
-      }
-    }
-  };
-  __nv_bfloat16* out = a.out + ((size_t)b * a.H + (size_t)hk * G) * DH;
-  if (a.splits == 1) {
-    merge(sh, (size_t)G * rec, W, nullptr, out);
-    return;
-  }
-  float* part = a.part + (size_t)bh * a.splits * G * rec;
-  merge(sh, (size_t)G * rec, W, part + (size_t)split * G * rec, nullptr);
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) last = atomicAdd(a.counters + bh, 1) == a.splits - 1;
-  __syncthreads();
-  if (!last) return;
-  __threadfence();
-  merge(part, (size_t)G * rec, a.splits, nullptr, out);
-  if (tid == 0) a.counters[bh] = 0;
-}
-
 // ------------------------------------------------------------------------------------------ host
 static int check_cache(const fsvd_kv8* c) {
   if (!c || !c->k8 || !c->v8 || !c->k_scale || !c->v_scale) return fail(FSVD_ERR_ARG, "null cache");
@@ -534,6 +425,8 @@ static int check_rotary(const double* inv_freq, int R, int Dh) {
   return 0;
 }
 
+constexpr int kMaxCtas = 3;   // attention CTAs of an SM, at most
+
 struct Kv8Ws {
   size_t counters, part, total;
 };
@@ -541,8 +434,51 @@ static Kv8Ws ws_layout(long long B, long long H, long long Hk, long long Dh) {
   Kv8Ws w;
   w.counters = 256;   // behind the status word (fsvd_workspace_status)
   w.part = w.counters + (size_t)((B * Hk * 4 + 255) / 256 * 256);
-  w.total = w.part + (size_t)B * H * kMaxSplits * (Dh + 2) * 4;
+  w.total = w.part + (size_t)kMaxCtas * sm_count() * 2 * (H / Hk) * (Dh + 2) * 4;
   return w;
+}
+
+// Descriptor of the codes: B * Hk planes of S_max rows of Dh bytes, read in boxes of kBox rows under the swizzle of a row.
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn encode_fn() {
+  static const EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<EncodeFn>(p) : nullptr;
+  }();
+  return fn;
+}
+static int encode(CUtensorMap* map, const void* codes, const fsvd_kv8& c) {
+  const EncodeFn enc = encode_fn();
+  if (!enc) return fail(FSVD_ERR_CUDA, "cuTensorMapEncodeTiled is not available in this driver");
+  const cuuint64_t dims[3] = {(cuuint64_t)c.Dh, (cuuint64_t)c.S_max, (cuuint64_t)c.B * c.Hk};
+  const cuuint64_t strides[2] = {(cuuint64_t)c.Dh, (cuuint64_t)c.S_max * c.Dh};
+  const cuuint32_t box[3] = {(cuuint32_t)c.Dh, (cuuint32_t)fsvd_kv8_attn::kBox, 1}, es[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(codes), dims, strides, box, es,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, c.Dh == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : fail(FSVD_ERR_CUDA, "cuTensorMapEncodeTiled failed with code %d", (int)r);
+}
+
+template <int DH, int GP>
+static int launch_attn(const CUtensorMap& km, const CUtensorMap& vm, const fsvd_kv8_attn::Args& a, void* stream) {
+  using S = fsvd_kv8_attn::Shape<DH, GP>;
+  static_assert(S::kCtas <= kMaxCtas);
+  const long long tiles = (long long)a.B * a.Hk * ((a.S_max + fsvd_kv8_attn::kTile - 1) / fsvd_kv8_attn::kTile);
+  const unsigned grid = (unsigned)std::min<long long>(tiles, (long long)S::kCtas * sm_count());
+  return launch(fsvd_kv8_attn::attn_kernel<DH, GP>, dim3(grid), fsvd_kv8_attn::kThreads, S::kSmem, stream, km, vm, a);
+}
+template <int DH>
+static int launch_attn(const CUtensorMap& km, const CUtensorMap& vm, const fsvd_kv8_attn::Args& a, void* stream) {
+  if (a.G == 1) return launch_attn<DH, 1>(km, vm, a, stream);
+  if (a.G == 2) return launch_attn<DH, 2>(km, vm, a, stream);
+  if (a.G <= 4) return launch_attn<DH, 4>(km, vm, a, stream);
+  if (a.G <= 8) return launch_attn<DH, 8>(km, vm, a, stream);
+  return launch_attn<DH, 16>(km, vm, a, stream);
 }
 
 template <int DH, int BLOCK>
@@ -659,27 +595,32 @@ int fsvd_flash_decode_kv8(const fsvd_kv8* cache, const void* q, const int* cache
   if (!q || !cache_seqlens || !out) return fail(FSVD_ERR_ARG, "null argument");
   if (H < 1 || H % cache->Hk) return fail(FSVD_ERR_ARG, "H=%d not a multiple of Hk=%d", H, cache->Hk);
   const int G = H / cache->Hk;
-  if (G > kMaxGroup) return fail(FSVD_ERR_UNSUPPORTED, "H/Hk=%d unsupported (1..%d)", G, kMaxGroup);
+  if (G > fsvd_kv8_attn::kMaxGroup)
+    return fail(FSVD_ERR_UNSUPPORTED, "H/Hk=%d unsupported (1..%d)", G, fsvd_kv8_attn::kMaxGroup);
   if (!aligned16(q) || !aligned16(out)) return fail(FSVD_ERR_ALIGN, "q and out must be 16-byte aligned");
   const Kv8Ws L = ws_layout(cache->B, H, cache->Hk, cache->Dh);
   if (!ws) return fail(FSVD_ERR_WORKSPACE, "null workspace");
   if (!aligned16(ws)) return fail(FSVD_ERR_ALIGN, "workspace is not 16-byte aligned");
   if (ws_bytes < L.total) return fail(FSVD_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", ws_bytes, L.total);
-  AttnArgs a;
-  a.c = *cache;
+  CUtensorMap km, vm;
+  if (int e = encode(&km, cache->k8, *cache)) return e;
+  if (int e = encode(&vm, cache->v8, *cache)) return e;
+  fsvd_kv8_attn::Args a;
+  a.k_scale = cache->k_scale;
+  a.v_scale = cache->v_scale;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q);
   a.out = reinterpret_cast<__nv_bfloat16*>(out);
   a.seqlens = cache_seqlens;
   a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + L.part);
   a.counters = reinterpret_cast<int*>(reinterpret_cast<char*>(ws) + L.counters);
-  a.H = H; a.seqlen_add = seqlen_add;
+  a.status = &reinterpret_cast<SyncState*>(ws)->status;
+  a.wait_limit = fsvd_tile_wait_limit();
+  a.B = cache->B; a.Hk = cache->Hk; a.S_max = cache->S_max;
+  a.block_log2 = cache->block == 16 ? 4 : cache->block == 32 ? 5 : cache->block == 64 ? 6 : 7;
+  a.nb = (cache->S_max + cache->block - 1) / cache->block;
+  a.G = G; a.seqlen_add = seqlen_add;
   a.scale = scale > 0.0f ? scale : 1.0f / sqrtf((float)cache->Dh);
-  const long long heads = (long long)cache->B * cache->Hk;
-  a.splits = (int)std::max(1ll, std::min({4ll * sm_count() / heads, (long long)(cache->S_max + 127) / 128, (long long)kMaxSplits}));
-  const size_t smem = (size_t)(kAttnThreads / 32) * G * (cache->Dh + 2) * sizeof(float);
-  const dim3 grid((unsigned)(heads * a.splits));
-  return cache->Dh == 64 ? launch(attn_kernel<64>, grid, kAttnThreads, smem, stream, a)
-                         : launch(attn_kernel<128>, grid, kAttnThreads, smem, stream, a);
+  return cache->Dh == 64 ? launch_attn<64>(km, vm, a, stream) : launch_attn<128>(km, vm, a, stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,545 @@
+// Single-query attention over the 8-bit cache on the tensor cores, without widening a code.
+//
+//   s_t = scale ks(t) q . k8_t,   out = sum_t softmax(s)_t vs(t) v8_t
+//
+// tcgen05.mma kind::f8f6f4 multiplies e4m3 by e4m3 exactly and adds in 32 bits, so the codes go from TMA to the tensor
+// core as they lie in memory.  What is not e4m3 is written as a sum of e4m3 numbers and takes a column of the small
+// operand each: a query row is hi + lo / 16 (a bf16 number has 8 bits, an e4m3 number 4: nothing is lost above 2^-22 of
+// the row's largest), a weight is w0 + w1 / 16 + w2 / 256 + w3 / 4096, which is good to 2^-19 of itself and 2^-26 of the
+// largest.  A tile is 128 tokens: S^T [128 tokens, 2 G] = K8 . q^T, then O^T [Dh, 4 G] = V8^T . w^T, where V8^T is the
+// tile as it lies, read along its other axis.  Scales are applied to the scores in 32 bits: the exponent of a weight is
+// s log2(e) + log2(vs), so that the weight carries its value's scale, and the denominator divides it out.
+//
+// A thread of the four softmax warps owns a token of S^T and a dimension of O^T; one more thread issues the copies, one
+// the products.  O^T is read back after every tile and summed in registers, where a new maximum rescales it.
+//
+// The tiles of all (sequence, kv head) pairs form one list that is cut into equal parts, one per CTA, whatever the
+// lengths are; a pair that more than one CTA works on is merged, in the order of its parts, by the CTA that finishes it.
+#pragma once
+#include <cuda.h>
+#include <cuda_fp8.h>
+
+#include "fsvd_tc.cuh"
+
+namespace fsvd_kv8_attn {
+
+using namespace fsvd_tile;
+
+constexpr int kTile = 128;      // tokens
+constexpr int kBox = 32;        // tokens of a TMA box: a short last tile is fetched in as many as it needs
+constexpr int kSoft = 128;      // threads of the softmax warps
+constexpr int kThreads = 192;
+constexpr int kPieces = 4;      // e4m3 numbers of a weight
+constexpr int kMaxGroup = 16;
+
+struct Args {
+  const float *k_scale, *v_scale;
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  const int* seqlens;
+  float* part;       // [CTAs][2][G][Dh + 2]: partial sums, maximum, denominator
+  int* counters;     // [B * Hk], zero between launches
+  int* status;
+  long long wait_limit;
+  int B, Hk, S_max, block_log2, nb, G, seqlen_add;
+  float scale;
+};
+
+template <int DH, int GP>
+struct Shape {
+  static constexpr int kCtas = GP <= 4 ? 3 : GP <= 8 ? 2 : 1;           // per SM
+  static constexpr int kStages = (GP <= 4 ? 2 : GP <= 8 ? 3 : 5) * (128 / DH);
+  static constexpr int kNq = 2 * GP < 16 ? 16 : 2 * GP;                 // columns of S
+  static constexpr int kNw = kPieces * GP < 16 ? 16 : kPieces * GP;     // columns of O
+  static constexpr int kCols = 2 * (kNq + kNw) <= 64 ? 64 : 2 * (kNq + kNw) <= 128 ? 128 : 256;
+  static constexpr int kHalf = kTile * DH;                              // bytes of a K or V tile
+  static constexpr int kQ = kNq * DH < 1024 ? 1024 : kNq * DH, kW = kNw * kTile;
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * 2 * kHalf + 2 * kQ + 2 * kW;
+};
+
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// e4m3 x e4m3 -> fp32, M = 128, N columns; A along its rows (K-major) or along its columns (transposed)
+__device__ __forceinline__ uint32_t idesc_f8(int N, bool a_transposed) {
+  return (1u << 4) | ((a_transposed ? 1u : 0u) << 15) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+// Operand of rows of ROW bytes (64 or 128) under the swizzle of that span; eight rows are 8 ROW bytes.  The stride
+// between spans is zero: a transposed operand of 64 rows repeats them as rows 64..127 (which nobody reads).
+template <int ROW>
+__device__ __forceinline__ uint64_t desc_f8(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(8 * ROW >> 4) << 32) | (1ull << 46) | ((ROW == 128 ? 2ull : 4ull) << 61);
+}
+// byte c of row r of such an operand
+template <int ROW>
+__device__ __forceinline__ uint32_t swizzled(int r, int c) {
+  const int x = ROW == 128 ? (r & 7) : ((r >> 1) & 3);
+  return (uint32_t)(r * ROW + (((c >> 4) ^ x) << 4) + (c & 15));
+}
+__device__ __forceinline__ void tma_box_3d(uint32_t dst, const void* tmap, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ float warp_max(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// N consecutive columns of this thread's lane.
+template <int N>
+__device__ __forceinline__ void tm_ld(uint32_t taddr, float* v);
+template <>
+__device__ __forceinline__ void tm_ld<2>(uint32_t taddr, float* v) {
+  uint32_t r[2];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x2.b32 {%0,%1}, [%2];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1])
+               : "r"(taddr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v[i] = __uint_as_float(r[i]);
+}
+template <>
+__device__ __forceinline__ void tm_ld<4>(uint32_t taddr, float* v) {
+  uint32_t r[4];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+}
+template <>
+__device__ __forceinline__ void tm_ld<8>(uint32_t taddr, float* v) {
+  uint32_t r[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+template <>
+__device__ __forceinline__ void tm_ld<16>(uint32_t taddr, float* v) {
+  uint32_t r[16];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+template <>
+__device__ __forceinline__ void tm_ld<32>(uint32_t taddr, float* v) {
+  uint32_t r[32];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(taddr) : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+template <>
+__device__ __forceinline__ void tm_ld<64>(uint32_t taddr, float* v) {
+  tm_ld<32>(taddr, v);
+  tm_ld<32>(taddr + 32, v + 32);
+}
+
+// Two fp32 numbers -> their nearest e4m3 codes (x in the low byte), and what the codes stand for.
+__device__ __forceinline__ uint32_t to_codes(float x, float y, float& dx, float& dy) {
+  const uint32_t c = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c, __NV_E4M3);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  dx = f.x;
+  dy = f.y;
+  return c;
+}
+
+// The part of the list of tiles that a CTA works on, as runs of tiles of one (sequence, kv head).
+struct Cursor {
+  const int* seqlens;
+  int add, S_max, Hk, B;
+  int b, hk, tiles, n;       // tiles of the sequence, positions of the sequence
+  int tile, left;            // next tile, tiles left for this CTA
+  __device__ __forceinline__ int positions(int i) const {
+    return (int)min(max((long long)seqlens[i] + add, 0ll), (long long)S_max);
+  }
+  __device__ __forceinline__ void enter() {
+    n = positions(b);
+    tiles = (n + kTile - 1) / kTile;
+  }
+  // tiles of the current run
+  __device__ __forceinline__ int run() const { return min(left, tiles - tile); }
+  __device__ __forceinline__ void next(int done) {
+    left -= done;
+    tile += done;
+    if (tile == tiles && left > 0) {
+      tile = 0;
+      if (++hk == Hk) {
+        hk = 0;
+        do {
+          ++b;
+          enter();
+        } while (tiles == 0);
+      }
+    }
+  }
+};
+
+template <int DH, int GP>
+__global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(const __grid_constant__ CUtensorMap kmap,
+                                                                             const __grid_constant__ CUtensorMap vmap,
+                                                                             const Args a) {
+  using S = Shape<DH, GP>;
+  extern __shared__ uint8_t raw[];
+  __shared__ __align__(8) unsigned long long kv_full[S::kStages], kv_empty[S::kStages], s_full[2], w_full[2], o_full[2], q_full[2];
+  __shared__ uint32_t tmem_slot;
+  __shared__ float qfac[2][GP], wmax[2][4][GP], red[4][GP];
+  __shared__ int start_b, start_hk, start_tile, last_sh, giveup_sh;
+  __shared__ long long total_sh, base_sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.G;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* qs = smem + S::kStages * 2 * S::kHalf;
+  uint8_t* ws = qs + 2 * S::kQ;
+  volatile int* giveup = &giveup_sh;
+
+  if (tid == 0) {
+    giveup_sh = 0;
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(smem_u32(&kv_full[i]), 1);
+      mbar_init(smem_u32(&kv_empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&s_full[i]), 1);
+      mbar_init(smem_u32(&w_full[i]), kSoft);
+      mbar_init(smem_u32(&o_full[i]), 1);
+      mbar_init(smem_u32(&q_full[i]), kSoft);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 5) tc_alloc(smem_u32(&tmem_slot), S::kCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();   // (the kernel behind this one must not take the tensor memory first)
+  pdl_wait();
+
+  // where this CTA's part of the list begins: every sequence has Hk * tiles entries
+  Cursor cur;
+  cur.seqlens = a.seqlens; cur.add = a.seqlen_add; cur.S_max = a.S_max; cur.Hk = a.Hk; cur.B = a.B;
+  if (warp == 0) {
+    long long total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      long long x = b0 + lane < a.B ? (long long)((cur.positions(b0 + lane) + kTile - 1) / kTile) * a.Hk : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+      total += x;
+    }
+    const long long per = (total + gridDim.x - 1) / gridDim.x, w0 = per * blockIdx.x;
+    long long before = 0;
+    int found = 0;
+    for (int b0 = 0; b0 < a.B && !found && w0 < total; b0 += 32) {
+      const int t = b0 + lane < a.B ? (cur.positions(b0 + lane) + kTile - 1) / kTile : 0;
+      const long long x = (long long)t * a.Hk;
+      long long inc = x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += y;
+      }
+      const bool mine = w0 >= before + inc - x && w0 < before + inc;
+      if (mine) {
+        const long long off = w0 - (before + inc - x);
+        start_b = b0 + lane;
+        start_hk = (int)(off / t);
+        start_tile = (int)(off % t);
+        base_sh = before + inc - x;   // list index of the sequence's first tile
+      }
+      found = __any_sync(0xffffffffu, mine);
+      before += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    if (lane == 0) total_sh = total;
+  }
+  __syncthreads();
+  const uint32_t tmem = tmem_slot;
+  const long long total = total_sh, per = (total + gridDim.x - 1) / gridDim.x, w0 = per * blockIdx.x;
+  cur.left = (int)max(0ll, min(per, total - w0));
+  if (cur.left > 0) {
+    cur.b = start_b; cur.hk = start_hk; cur.tile = start_tile;
+    cur.enter();
+  }
+
+  if (warp == 4) {   // ---- copies
+    if (lane == 0 && cur.left > 0) {
+      int j = 0;
+      while (cur.left > 0) {
+        const int run = cur.run(), plane = cur.b * a.Hk + cur.hk;
+        for (int t = cur.tile; t < cur.tile + run; ++t, ++j) {
+          const int st = j % S::kStages;
+          if (j >= S::kStages) wait_bar(smem_u32(&kv_empty[st]), (j / S::kStages - 1) & 1, giveup, a.status, a.wait_limit, DS_COPY_TIMEOUT);
+          if (*giveup) break;
+          const int boxes = min(kTile, cur.n - t * kTile + kBox - 1) / kBox;
+          const uint32_t dst = smem_u32(smem + st * 2 * S::kHalf), bar = smem_u32(&kv_full[st]);
+          mbar_expect_tx(bar, (uint32_t)boxes * 2 * kBox * DH);
+          for (int i = 0; i < boxes; ++i) tma_box_3d(dst + i * kBox * DH, &kmap, 0, t * kTile + i * kBox, plane, bar);
+          for (int i = 0; i < boxes; ++i) tma_box_3d(dst + S::kHalf + i * kBox * DH, &vmap, 0, t * kTile + i * kBox, plane, bar);
+        }
+        if (*giveup) break;
+        cur.next(run);
+      }
+      // nothing may be on its way to this CTA's shared memory when it ends: the releases of the last stages, and
+      // after a wait that ran out the copies into them
+      for (int i = max(0, j - S::kStages); i < j; ++i) {
+        const uint32_t full = smem_u32(&kv_full[i % S::kStages]);
+        const long long c0 = clock64();
+        while (!mbar_try_wait(full, (i / S::kStages) & 1) && clock64() - c0 < a.wait_limit) {
+        }
+        wait_bar(smem_u32(&kv_empty[i % S::kStages]), (i / S::kStages) & 1, giveup, a.status, a.wait_limit, DS_COPY_TIMEOUT);
+      }
+    }
+  } else if (warp == 5) {   // ---- products
+    if (lane == 0 && cur.left > 0) {
+      const uint32_t iq = idesc_f8(S::kNq, false), iw = idesc_f8(S::kNw, true);
+      const int n = cur.left;
+      int seg = 0, in_run = cur.run();
+      auto weigh = [&](int j) {   // O(j) = V8^T . w^T
+        const int st = j % S::kStages, buf = j & 1;
+        wait_bar(smem_u32(&w_full[buf]), (j >> 1) & 1, giveup, a.status, a.wait_limit, DS_BARRIER_TIMEOUT);
+        tc_fence_after();
+        const uint32_t v = smem_u32(smem + st * 2 * S::kHalf + S::kHalf), w = smem_u32(ws + buf * S::kW);
+#pragma unroll
+        for (int k = 0; k < kTile / 32; ++k)
+          mma_f8(tmem + 2 * S::kNq + buf * S::kNw, desc_f8<DH>(v + 32 * DH * k), desc_f8<128>(w + 32 * k), iw, k > 0);
+        tc_commit(smem_u32(&o_full[buf]));
+        tc_commit(smem_u32(&kv_empty[st]));
+      };
+      for (int j = 0; j < n; ++j) {
+        if (in_run == 0) {
+          ++seg;
+          cur.next(cur.run());
+          in_run = cur.run();
+        }
+        --in_run;
+        const int st = j % S::kStages, buf = j & 1;
+        wait_bar(smem_u32(&q_full[seg & 1]), (seg >> 1) & 1, giveup, a.status, a.wait_limit, DS_BARRIER_TIMEOUT);
+        wait_bar(smem_u32(&kv_full[st]), (j / S::kStages) & 1, giveup, a.status, a.wait_limit, DS_COPY_TIMEOUT);
+        if (*giveup) break;
+        tc_fence_after();
+        const uint32_t k8 = smem_u32(smem + st * 2 * S::kHalf), q8 = smem_u32(qs + (seg & 1) * S::kQ);
+#pragma unroll
+        for (int k = 0; k < DH / 32; ++k) mma_f8(tmem + buf * S::kNq, desc_f8<DH>(k8 + 32 * k), desc_f8<DH>(q8 + 32 * k), iq, k > 0);
+        tc_commit(smem_u32(&s_full[buf]));
+        if (j > 0) weigh(j - 1);
+      }
+      if (!*giveup) weigh(n - 1);
+    }
+  } else {   // ---- softmax
+    // the query rows of (b, hk) as hi + lo / 16, scaled to a largest magnitude in [128, 256)
+    auto build_q = [&](int b, int hk, int which) {
+      constexpr int D = DH / 32;
+      uint8_t* dst = qs + which * S::kQ;
+      for (int g = warp; g < G; g += 4) {
+        const __nv_bfloat16* row = a.q + (((size_t)b * a.Hk + hk) * G + g) * DH + lane * D;
+        float x[D], top = 0.0f;
+        bool fine = true;
+#pragma unroll
+        for (int e = 0; e < D; ++e) {
+          x[e] = __bfloat162float(row[e]);
+          top = fmaxf(top, fabsf(x[e]));
+          fine = fine && isfinite(x[e]);
+        }
+        top = warp_max(top);
+        fine = __all_sync(0xffffffffu, fine);
+        const int e2 = (int)(__float_as_uint(top) >> 23) - 127;          // top in [2^e2, 2^(e2 + 1))
+        const int up = fine ? min(max(7 - e2, -120), 120) : 0;
+        const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+        uint32_t hi = 0, lo = 0;
+#pragma unroll
+        for (int e = 0; e < D; e += 2) {
+          float h0, h1, l0, l1;
+          const float x0 = x[e] * f, x1 = x[e + 1] * f;
+          const uint32_t ch = to_codes(x0, x1, h0, h1), cl = to_codes((x0 - h0) * 16.0f, (x1 - h1) * 16.0f, l0, l1);
+          hi |= ch << (8 * e);
+          lo |= cl << (8 * e);
+        }
+        if (!fine) hi = lo = 0x7f7f7f7fu;   // a query that is not finite gives no number
+        uint8_t* p0 = dst + swizzled<DH>(g, lane * D);
+        uint8_t* p1 = dst + swizzled<DH>(GP + g, lane * D);
+        if constexpr (D == 4) {
+          *reinterpret_cast<uint32_t*>(p0) = hi;
+          *reinterpret_cast<uint32_t*>(p1) = lo;
+        } else {
+          *reinterpret_cast<uint16_t*>(p0) = (uint16_t)hi;
+          *reinterpret_cast<uint16_t*>(p1) = (uint16_t)lo;
+        }
+        if (lane == 0) qfac[which][g] = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - up) << 23);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(smem_u32(&q_full[which]));
+    };
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const bool owns = tid < DH;   // a dimension of the result
+    long long seq_base = cur.left > 0 ? base_sh : 0;
+    int j = 0, seg = 0;
+    if (cur.left > 0) {
+      build_q(cur.b, cur.hk, 0);
+      soft_sync();
+    }
+    while (cur.left > 0) {
+      const int run = cur.run(), first = cur.tile, bh = cur.b * a.Hk + cur.hk, n = cur.n, ntiles = cur.tiles, hk = cur.hk;
+      const long long list0 = seq_base + (long long)hk * ntiles;   // list index of the pair's first tile
+      const float* ksc = a.k_scale + (size_t)bh * a.nb;
+      const float* vsc = a.v_scale + (size_t)bh * a.nb;
+      float m[GP], l[GP], acc[GP], corr[GP];
+#pragma unroll
+      for (int g = 0; g < GP; ++g) {
+        m[g] = -INFINITY;
+        l[g] = acc[g] = 0.0f;
+      }
+      auto collect = [&](int jj, const float (&c)[GP]) {   // acc = acc c + O(jj)
+        const int buf = jj & 1;
+        wait_bar(smem_u32(&o_full[buf]), (jj >> 1) & 1, giveup, a.status, a.wait_limit, DS_BARRIER_TIMEOUT);
+        tc_fence_after();
+        if (warp * 32 < DH) {
+          float o[kPieces * GP];
+          tm_ld<kPieces * GP>(tmem + 2 * S::kNq + buf * S::kNw + lanes, o);
+#pragma unroll
+          for (int g = 0; g < GP; ++g)
+            acc[g] = acc[g] * c[g] + (((o[3 * GP + g] * 0.0625f + o[2 * GP + g]) * 0.0625f + o[GP + g]) * 0.0625f + o[g]);
+        }
+      };
+      float ks = 0.0f, vs = 1.0f;
+      auto scales = [&](int t) {
+        const int at = t * kTile + tid;
+        ks = at < n ? ksc[at >> a.block_log2] : 0.0f;
+        vs = at < n ? vsc[at >> a.block_log2] : 1.0f;
+      };
+      scales(first);
+      for (int i = 0; i < run; ++i, ++j) {
+        const int t = first + i, buf = j & 1;
+        const bool valid = t * kTile + tid < n;
+        const float kf = ks, lv = log2f(vs), inv = valid ? 1.0f / vs : 0.0f;
+        if (i + 1 < run) scales(t + 1);
+        wait_bar(smem_u32(&s_full[buf]), (j >> 1) & 1, giveup, a.status, a.wait_limit, DS_BARRIER_TIMEOUT);
+        tc_fence_after();
+        float s[2 * GP], e[GP];
+        tm_ld<2 * GP>(tmem + buf * S::kNq + lanes, s);
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          const float x = (s[GP + g] * 0.0625f + s[g]) * (kf * qfac[seg & 1][g]) + lv;
+          e[g] = valid ? x : -INFINITY;
+          const float top = warp_max(e[g]);
+          if (lane == 0) wmax[buf][warp][g] = top;
+        }
+        if (!valid) {   // the last tile: a row behind the end may hold anything
+          uint4* row = reinterpret_cast<uint4*>(smem + (j % S::kStages) * 2 * S::kHalf + S::kHalf + tid * DH);
+#pragma unroll
+          for (int x = 0; x < DH / 16; ++x) row[x] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        soft_sync();
+        float prev[GP];   // rescaling of the tile before, which is collected below
+        uint8_t* dst = ws + buf * S::kW;
+#pragma unroll
+        for (int g = 0; g < GP; ++g) {
+          const float top = fmaxf(fmaxf(wmax[buf][0][g], wmax[buf][1][g]), fmaxf(wmax[buf][2][g], wmax[buf][3][g]));
+          const float mn = fmaxf(m[g], top);
+          prev[g] = corr[g];
+          corr[g] = m[g] == mn ? 1.0f : exp2f(m[g] - mn);
+          m[g] = mn;
+          e[g] = valid ? exp2f(e[g] - mn) : 0.0f;
+          l[g] = l[g] * corr[g] + e[g] * inv;
+          e[g] *= 256.0f;
+        }
+#pragma unroll
+        for (int g = 0; g < GP; g += 2) {
+          float x = e[g], y = GP > 1 ? e[(g + 1) % GP] : 0.0f;
+#pragma unroll
+          for (int p = 0; p < kPieces; ++p) {
+            float dx, dy;
+            const uint32_t c = to_codes(x, y, dx, dy);
+            dst[swizzled<128>(p * GP + g, tid)] = (uint8_t)(c & 0xffu);
+            if (GP > 1) dst[swizzled<128>(p * GP + g + 1, tid)] = (uint8_t)(c >> 8);
+            x = (x - dx) * 16.0f;
+            y = (y - dy) * 16.0f;
+          }
+        }
+        tc_fence_before();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(smem_u32(&w_full[buf]));
+        if (i > 0) collect(j - 1, prev);
+      }
+      cur.next(run);
+      if (hk == a.Hk - 1 && first + run == ntiles) seq_base += (long long)a.Hk * ntiles;
+      if (cur.left > 0) build_q(cur.b, cur.hk, (seg + 1) & 1);
+      collect(j - 1, corr);
+      // denominators
+#pragma unroll
+      for (int g = 0; g < GP; ++g) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], o);
+        if (lane == 0) red[warp][g] = l[g];
+      }
+      soft_sync();
+#pragma unroll
+      for (int g = 0; g < GP; ++g) l[g] = (red[0][g] + red[1][g]) + (red[2][g] + red[3][g]);
+      __nv_bfloat16* out = a.out + (size_t)bh * G * DH + tid;
+      const int rec = DH + 2;
+      if (run == ntiles) {
+        if (owns) {
+#pragma unroll
+          for (int g = 0; g < GP; ++g)
+            if (g < G) out[g * DH] = __float2bfloat16_rn(acc[g] * (1.0f / 256.0f) / l[g]);
+        }
+      } else {
+        float* rp = a.part + ((size_t)blockIdx.x * 2 + (seg > 0)) * G * rec;
+#pragma unroll
+        for (int g = 0; g < GP; ++g)
+          if (g < G) {
+            if (owns) rp[g * rec + tid] = acc[g] * (1.0f / 256.0f);
+            if (tid == 0) *reinterpret_cast<float2*>(rp + g * rec + DH) = make_float2(m[g], l[g]);
+          }
+        __threadfence();
+        soft_sync();
+        const int c0 = (int)(list0 / per), c1 = (int)((list0 + ntiles - 1) / per);   // the CTAs of this pair
+        if (tid == 0) last_sh = atomicAdd(a.counters + bh, 1) == c1 - c0;
+        soft_sync();
+        if (last_sh) {
+          __threadfence();
+          for (int g = 0; g < G; ++g) {
+            float mm = -INFINITY, ll = 0.0f, o = 0.0f;
+            for (int c = c0; c <= c1; ++c) {
+              const float* r = a.part + (((size_t)c * 2 + (per * c < list0)) * G + g) * rec;
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(r + DH));
+              const float x = owns ? __ldcg(r + tid) : 0.0f;
+              const float mn = fmaxf(mm, ml.x), f0 = mm == mn ? 1.0f : exp2f(mm - mn), f1 = ml.x == mn ? 1.0f : exp2f(ml.x - mn);
+              mm = mn;
+              ll = ll * f0 + ml.y * f1;
+              o = o * f0 + x * f1;
+            }
+            if (owns) out[g * DH] = __float2bfloat16_rn(o / ll);
+          }
+          if (tid == 0) a.counters[bh] = 0;
+        }
+      }
+      ++seg;
+      soft_sync();   // `red`, `last_sh`
+    }
+    // sequences without positions
+    for (int i = blockIdx.x; i < a.B; i += gridDim.x)
+      if (cur.positions(i) == 0)
+        for (int x = tid; x < a.Hk * G * DH / 8; x += kSoft)
+          reinterpret_cast<uint4*>(a.out + (size_t)i * a.Hk * G * DH)[x] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 5) tc_dealloc(tmem, S::kCols);
+}
+
+}  // namespace fsvd_kv8_attn

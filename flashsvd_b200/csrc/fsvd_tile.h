@@ -14,6 +14,7 @@ void fsvd_tile_set_error(int code, const char* msg);
 void fsvd_tile_count_launch();
 void fsvd_tile_count_launches(long long n);
 long long fsvd_tile_launches();
+long long fsvd_tile_wait_limit();   // budget of a device-side wait, SM clocks
 
 // provided by fsvd_tile.cu
 size_t fsvd_tile_workspace_bytes(const fsvd_dims* dims);
