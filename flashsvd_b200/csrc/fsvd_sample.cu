@@ -2,13 +2,12 @@
 //
 // The vocabulary is ordered by logit (descending, lower index first); every filter keeps a prefix of that order, so the
 // kept set is {key > t} and the first r of {key = t} in index order, for one threshold key t.  It is found without a
-// sort: a histogram of 1024 bins over the values narrows the threshold to one bin, and a few dozen candidates are then
-// ranked directly; where a bin holds too many, bins over the integer keys inside it narrow it on.
+// sort: a histogram of 1024 bins over the values narrows the threshold to a few of them, and a hundred candidates are
+// then ranked directly; where there are more, bins over the integer keys inside narrow it on.
 //
-// Weights are integers, exp((l - max) / T) * 2^frac: their sums do not depend on the order of addition (the histograms
-// are built by atomics), and comparisons of running sums with u Z and p Z are exact in them.  A weight is good to 2^-29
-// of itself: between V boundaries of a flat row a draw lands on another token than in exact arithmetic once in
-// 2^29 / sqrt(V) rows.  (32-bit exponentials miss 64 times as often, 64-bit ones take a third of the kernel's time.)
+// Weights exp((l - max) / T) are 64-bit numbers good to 2^-34, and every sum has a fixed order, or is one of integers where
+// its terms come in any order.  32-bit weights would put a draw from a flat row of 10^5 tokens on another token than exact
+// arithmetic once in 10^4 rows.
 //
 // A row belongs to a cluster of up to eight CTAs, each with a contiguous piece of it in shared memory, so that HBM is read
 // once; sums and histograms meet through distributed shared memory.
@@ -27,15 +26,19 @@
 
 namespace fsvd_sample_impl {
 
-using fsvd_tile::cluster_sync;
 typedef unsigned long long u64;
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 1024, kWarps = kThreads / 32;
+static_assert(kWarps == 32, "a warp folds one number of every warp");
 constexpr int kBins = 1024;
-constexpr int kLimbs = 4, kLimbBits = 12;   // a weight of at most 2^46 as four numbers of 12 bits: 2^20 of them fit 32-bit sums
-constexpr int kList = 96;                   // candidates that are ranked directly
+constexpr int kFrac = 40;                   // bits behind the point of a weight as an integer (at most one; 2^20 of them fit)
+constexpr int kLimbs = 4, kLimbBits = 12;   // such an integer as four numbers of 12 bits: 2^20 of them fit 32-bit sums
+constexpr int kList = 1024;                 // candidates of a CTA that are listed
+constexpr int kRank = 192;                  // candidates of a row that are ranked directly
 constexpr int kBlock = 128;                 // elements of a warp's step: four neighbours per lane
+constexpr int kPackPiece = 256, kPackAlone = 1024;   // elements that a warp's short list holds, beside the piece and without
 constexpr int kMaxCluster = 8;
-constexpr int kMaxVocab = 1 << 22;
+constexpr int kMaxVocab = 1 << 20;          // (2^17 elements of a CTA fit a bin's 32-bit sums of 15-bit numbers)
+constexpr float kHuge = 3.402823466e38f;
 
 struct Args {
   const void* logits;
@@ -46,47 +49,43 @@ struct Args {
   int k_all;
   int* tokens;
   float* probs;
-  int V, chunk, frac;   // chunk: elements of a CTA, a multiple of kBlock
+  int V, chunk;   // chunk: elements of a CTA, a multiple of kBlock
 };
 
-// What a CTA shows to the others of its cluster.
+// What a CTA shows to the others of its cluster (each number is written once between two reads by the others).
 struct Slot {
-  u64 best, count, mass, sum, above;   // (each written once between two reads by the others)
-  float low;
-  uint32_t n, kmin, kmax, eq;
+  double count, mass, sum;
+  float top, low;
+  uint32_t first, finite, n, kmin, kmax, eq;
 };
 
 struct Shared {
   uint32_t hist[kLimbs][kBins];
   u64 total[kBins];
-  u64 warp_sum[kWarps];
-  uint32_t warp_eq[kWarps];
+  double table[64];
+  double warp_sum[kWarps], scan_d[kWarps];
   u64 scan[kWarps];
-  uint32_t list_key[kList];
-  int list_at[kList];
-  uint32_t all_key[kList];
-  int all_at[kList];
-  u64 all_w[kList];
-  uint32_t table[64];
-  Slot slot;
-  Slot red[kWarps];
-  int pick_lo, pick_hi, list_n;
+  uint32_t warp_eq[kWarps];
+  uint32_t list_key[kList], list_at[kList];
+  uint32_t all_key[kRank], all_at[kRank];
+  u64 all_w[kRank];
+  Slot slot, red[kWarps];
+  int pick, list_n;
   u64 pick_above;
-  uint32_t pick_key;
-  u64 pick_ties;
+  double pick_front;
+  uint32_t pick_key, pick_ties, pick_equal;
 };
 
-// Ascending keys for ascending numbers above -infinity; 0 for -infinity.
+// Ascending keys for ascending numbers above -infinity (the zeros share theirs); 0 for -infinity and NaN.
 __device__ __forceinline__ uint32_t key_of(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return x == -INFINITY ? 0u : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return !(x > -INFINITY) ? 0u : (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
-__device__ __forceinline__ float plain(float x) { return x > -INFINITY ? x + 0.0f : -INFINITY; }   // NaN counts as -infinity; one zero
-__device__ __forceinline__ float logit(const float* row, int i) { return plain(row[i]); }
-__device__ __forceinline__ float logit(const __nv_bfloat16* row, int i) { return plain(__bfloat162float(row[i])); }
+__device__ __forceinline__ float num(float x) { return x; }
+__device__ __forceinline__ float num(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 __device__ __forceinline__ uint32_t remote(const void* p, int rank) {
   uint32_t r;
@@ -98,9 +97,12 @@ __device__ __forceinline__ uint32_t peek(const uint32_t* p, int rank) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(remote(p, rank)) : "memory");
   return x;
 }
-__device__ __forceinline__ u64 peek(const u64* p, int rank) {
-  u64 x;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(remote(p, rank)) : "memory");
+__device__ __forceinline__ float peek(const float* p, int rank) {
+  return __uint_as_float(peek(reinterpret_cast<const uint32_t*>(p), rank));
+}
+__device__ __forceinline__ double peek(const double* p, int rank) {
+  double x;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(x) : "r"(remote(p, rank)) : "memory");
   return x;
 }
 __device__ __forceinline__ void poke(u64* p, int rank, u64 x) {
@@ -116,531 +118,798 @@ __device__ __forceinline__ int cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-template <typename F>
-__device__ __forceinline__ u64 warp_reduce(u64 x, F f) {
+template <typename N, typename F>
+__device__ __forceinline__ N warp_fold(N x, F f) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x = f(x, __shfl_xor_sync(0xffffffffu, x, o));
   return x;
 }
-__device__ __forceinline__ u64 warp_add(u64 x) {
-  return warp_reduce(x, [](u64 a, u64 b) { return a + b; });
+__device__ __forceinline__ double warp_add(double x) {
+  return warp_fold(x, [](double p, double q) { return p + q; });
+}
+__device__ __forceinline__ float warp_min(float x) {
+  return warp_fold(x, [](float p, float q) { return fminf(p, q); });
+}
+// Inclusive prefix sums over the lanes.
+template <typename N>
+__device__ __forceinline__ N warp_scan(N x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const N y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+// fp32 -> fp64 of a finite number by its bits (the conversion instruction runs at an eighth of the rate of additions; a
+// zero comes out as 2^-127, which no sum here sees)
+__device__ __forceinline__ double wide(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
 }
 
-// exp((x - max) / T) as an integer.  log2 of it is formed in 64 bits as a fixed-point number: added to 1.5 * 2^20 its
-// fraction fills the low 32 bits of the sum.  2^fraction = 2^(j / 64) (1 + q), j the top six bits, q a polynomial in the
-// other 26 (Taylor: the next term is below 2^-38).
+// exp((x - max) / T) = 2^(k / 64) 2^(r / 64) with k whole and |r| <= 1/2: a table of 64, a polynomial of degree three
+// (Taylor; the next term is below 2^-34), and k / 64 into the exponent.  For x >= cut; callers raise what is below to it and
+// drop the result, so that four weights are formed side by side without a branch (each is a chain of a dozen steps).
 struct Weigher {
-  double max, c;   // c = log2(e) / T
-  float half_max, fc2;     // for a 32-bit logarithm: halves, so that a difference of finite numbers stays finite
-  int frac;
-  const uint32_t* table;   // 2^(31 + j / 64)
-  __device__ __forceinline__ float log2f32(float x) const { return fmaf(0.5f, x, -half_max) * fc2; }   // to 2^-22 of itself
-  __device__ __forceinline__ u64 operator()(float x) const {
-    if (!(log2f32(x) > -60.0f)) return 0;
-    const double t = fma((double)x - max, c, 1572864.0);
-    const uint32_t lo = (uint32_t)__double2loint(t);
-    const int n = 0x41380000 - __double2hiint(t);   // 2^-n
-    const float z = __uint_as_float(0x3f800000u | ((lo & 0x3ffffffu) >> 3)) - 1.0f;   // 64 times the rest, in [0, 1)
-    constexpr float a1 = 0.69314718056f;   // 64 q = a1 z + a1^2 z^2 / 128 + a1^3 z^3 / (6 * 64^2) + a1^4 z^4 / (24 * 64^3)
-    const float q = z * (a1 + z * (a1 * a1 / 128.0f + z * (a1 * a1 * a1 / 24576.0f + z * (a1 * a1 * a1 * a1 / 6291456.0f))));
-    const uint32_t m = (__float_as_uint(1.0f + q) & 0x7fffffu) << 3;   // q 2^32
-    const uint32_t T = table[lo >> 26];
-    return ((u64)(T + __umulhi(T, m)) << (frac - 31)) >> n;
+  double max, c;           // c = 64 log2(e) / T
+  float cut;               // below it a weight is under 2^-60 and counts as zero; finite
+  const double* table;     // 2^(j / 64)
+  __device__ __forceinline__ double operator()(float x, int& bin, int& q) const {   // q: w = 2^(-bin / 64) (1 + q 2^-36)
+    constexpr double magic = 6755399441055744.0, a = 0.010830424696249145459;   // 1.5 * 2^52; ln(2) / 64
+    const double d = wide(x) - max, k = fma(d, c, magic);
+    const int lo = __double2loint(k);
+    const double r = fma(d, c, -(k - magic));
+    const double e = fma(r, fma(r, fma(r, a * a * a / 6.0, a * a / 2.0), a), 1.0);
+    const double w = table[lo & 63] * e;
+    bin = -lo;             // 64ths of a factor of two below the maximum
+    q = __double2loint(e + 98304.0);   // (1.5 * 2^16: the low word counts 2^-36)
+    return __hiloint2double(__double2hiint(w) + ((lo >> 6) << 20), __double2loint(w));
   }
+  __device__ __forceinline__ double operator()(float x, int& bin) const {
+    int q;
+    return (*this)(x, bin, q);   // (what nobody asks for costs nothing)
+  }
+  __device__ __forceinline__ int bin_of(float x) const { return -__double2loint(fma(wide(x) - max, c, 6755399441055744.0)); }
+  __device__ __forceinline__ double operator()(float x) const {
+    int bin;
+    return x >= cut ? (*this)(x, bin) : 0.0;
+  }
+  __device__ __forceinline__ u64 fixed(float x) const { return (u64)__double2ll_rn((*this)(x) * (double)(1ull << kFrac)); }
 };
 
+// (out of line: it is hardly ever called)
+__device__ __noinline__ double library_exp(double x) { return exp(x); }
+
 template <typename T, bool RESIDENT>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const Args a) {
-  extern __shared__ float vals[];   // RESIDENT: this CTA's piece, -infinity behind the end
+__global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
+  constexpr int kPack = RESIDENT ? kPackPiece : kPackAlone;
+  // short lists of the warps (what may still be kept, in index order): values, and places in the warp's part; then, if
+  // RESIDENT, this CTA's elements as they are in memory
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  unsigned char* piece = dynamic + kWarps * kPack * 6;
   __shared__ Shared s;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.V;
   const int rank = cluster_rank(), C = cluster_size(), b = blockIdx.x / C;
-  const int base = rank * a.chunk, len = max(0, min(a.chunk, V - base));
   const T* row = reinterpret_cast<const T*>(a.logits) + (size_t)b * a.stride;
+  // Elements are counted from the 16-byte boundary in front of the row: place i is element i - shift.
+  constexpr int kVec = 16 / sizeof(T);
+  const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+  row -= shift;
+  const int base = rank * a.chunk, i_end = min(base + a.chunk, V + shift), i_begin = max(base, shift);
+  const int len = max(0, i_end - base);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (tid < 64) s.table[tid] = (uint32_t)__double2ll_rn(exp2((double)tid / 64.0) * 2147483648.0);
+  if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const float temp = fminf(a.temperature ? a.temperature[b] : a.T_all, 3.402823466e38f);
+  const float temp = fminf(a.temperature ? a.temperature[b] : a.T_all, kHuge);
   int k = a.top_k ? a.top_k[b] : a.k_all;
   const float p = a.top_p ? a.top_p[b] : a.p_all, mp = fminf(a.min_p ? a.min_p[b] : a.m_all, 1.0f);
   if (k <= 0 || k > V) k = V;
 
-  // ---- the row into shared memory; its largest element (lowest index among equals) and its smallest finite one
-  u64 best = 0;
-  float low = INFINITY;
-  {
-    constexpr int U = 8;
-    const int padded = (len + kBlock - 1) / kBlock * kBlock;
-    for (int i0 = tid; i0 < padded; i0 += U * kThreads) {
-      float x[U];
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        const int i = i0 + e * kThreads;
-        x[e] = i < len ? logit(row, base + i) : -INFINITY;
-      }
-#pragma unroll
-      for (int e = 0; e < U; ++e) {
-        const int i = i0 + e * kThreads;
-        if (RESIDENT && i < padded) vals[i] = x[e];
-        best = max(best, ((u64)key_of(x[e]) << 32) | (uint32_t)~(base + i));
-        if (x[e] > -INFINITY) low = fminf(low, x[e]);
-      }
-    }
-  }
-  auto larger = [](u64 x, u64 y) { return x > y ? x : y; };
-  best = warp_reduce(best, larger);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-  if (lane == 0) {
-    s.red[warp].best = best;
-    s.red[warp].low = low;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kWarps; ++w) {
-      best = larger(best, s.red[w].best);
-      low = fminf(low, s.red[w].low);
-    }
-    s.slot.best = best;
-    s.slot.low = low;
-  }
-  cluster_sync();
-  best = 0;
-  low = INFINITY;
-  for (int r = 0; r < C; ++r) {
-    best = larger(best, peek(&s.slot.best, r));
-    low = fminf(low, __uint_as_float(peek(reinterpret_cast<const uint32_t*>(&s.slot.low), r)));
-  }
-  const uint32_t kbest = (uint32_t)(best >> 32);
-  if (kbest == 0u || !(temp > 0.0f) || k == 1) {
-    if (rank == 0 && tid == 0) {
-      a.tokens[b] = kbest == 0u ? 0 : (int)~(uint32_t)best;
-      if (a.probs) a.probs[b] = kbest == 0u ? 0.0f : 1.0f;
-    }
-    cluster_sync();   // (the others may still be reading this CTA's slot)
-    return;
-  }
-  // An infinite maximum: the elements that equal it share everything, the others get nothing.
-  const bool inf = value_of(kbest) == INFINITY;
-  const float top = inf ? 0.0f : value_of(kbest);
-  if (inf) low = 0.0f;
+  // ---- the row into shared memory: whole 16-byte pieces asynchronously, the ragged ends one by one
   const int nblk = (len + kBlock - 1) / kBlock, per = (nblk + kWarps - 1) / kWarps;
   const int blk0 = min(nblk, warp * per), blk1 = min(nblk, blk0 + per);
-  auto get4 = [&](int blk, float (&x)[4]) {
-    const int i = blk * kBlock + 4 * lane;
-    if constexpr (RESIDENT) {
-      const float4 v = *reinterpret_cast<const float4*>(vals + i);
-      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-    } else {
+  if constexpr (RESIDENT) {
+    T* vals = reinterpret_cast<T*>(piece);
+    for (int v = tid; v < nblk * (kBlock / kVec); v += kThreads) {
+      const int i = base + v * kVec;
+      if (i >= i_begin && i + kVec <= i_end) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(fsvd_tile::smem_u32(vals + v * kVec)), "l"(row + i) : "memory");
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = i + e < len ? logit(row, base + i + e) : -INFINITY;
+        for (int e = 0; e < kVec; ++e)
+          vals[v * kVec + e] = i + e >= i_begin && i + e < i_end ? row[i + e] : T(-INFINITY);
+      }
     }
-    if (inf) {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+  }
+  // a barrier of the cluster (a CTA by itself has a cheaper one)
+  auto meet = [&] {
+    if (C > 1) fsvd_tile::cluster_sync();
+    else __syncthreads();
+  };
+  bool inf = false;   // an infinite maximum: the elements that equal it share everything, the others get nothing
+  float* short_x = reinterpret_cast<float*>(dynamic) + warp * kPack;
+  uint16_t* short_at = reinterpret_cast<uint16_t*>(dynamic + kWarps * kPack * 4) + warp * kPack;
+  int packed = -1;   // elements in the warp's short list; -1: the warp goes through all of its part
+  auto get4 = [&](int blk, float (&x)[4]) {
+    const int v = blk * kBlock + 4 * lane;
+    if constexpr (RESIDENT && sizeof(T) == 4) {
+      const float4 f = *reinterpret_cast<const float4*>(piece + 4 * v);
+      x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
+    } else if constexpr (RESIDENT) {
+      const uint2 w = *reinterpret_cast<const uint2*>(piece + 2 * v);
+      x[0] = __uint_as_float(w.x << 16); x[1] = __uint_as_float(w.x & 0xffff0000u);
+      x[2] = __uint_as_float(w.y << 16); x[3] = __uint_as_float(w.y & 0xffff0000u);
+    } else {
+      const int i = base + v;
+      if (i >= i_begin && i + 4 <= i_end) {
+        if constexpr (sizeof(T) == 4) {
+          const float4 f = __ldg(reinterpret_cast<const float4*>(row + i));
+          x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
+        } else {
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(row + i));
+          x[0] = __uint_as_float(w.x << 16); x[1] = __uint_as_float(w.x & 0xffff0000u);
+          x[2] = __uint_as_float(w.y << 16); x[3] = __uint_as_float(w.y & 0xffff0000u);
+        }
+      } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = x[e] == INFINITY ? 0.0f : -INFINITY;
+        for (int e = 0; e < 4; ++e) x[e] = i + e >= i_begin && i + e < i_end ? num(row[i + e]) : -INFINITY;
+      }
     }
   };
+  // fn(block, its four elements of this lane) for the blocks [first, end): from memory two blocks are under way.
+  auto each = [&](int first, int end, auto fn) {
+    if (packed >= 0) {
+      for (int blk = 0; blk * kBlock < packed; ++blk) {
+        const float4 f = *reinterpret_cast<const float4*>(short_x + blk * kBlock + 4 * lane);
+        const float x[4] = {f.x, f.y, f.z, f.w};
+        fn(blk, x);
+      }
+      return;
+    }
+    auto call = [&](int blk, float (&x)[4]) {
+      if (inf) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = x[e] == INFINITY ? 0.0f : -INFINITY;
+      }
+      fn(blk, x);
+    };
+    if constexpr (RESIDENT) {
+      for (int blk = first; blk < end; ++blk) {
+        float x[4];
+        get4(blk, x);
+        call(blk, x);
+      }
+    } else {
+      constexpr int D = 2;
+      float ahead[D][4], x[4];
+#pragma unroll
+      for (int d = 0; d < D; ++d)
+        if (first + d < end) get4(first + d, ahead[d]);
+      for (int blk = first; blk < end; ++blk) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[e] = ahead[0][e];
+#pragma unroll
+          for (int d = 0; d + 1 < D; ++d) ahead[d][e] = ahead[d + 1][e];
+        }
+        if (blk + D < end) get4(blk + D, ahead[D - 1]);
+        call(blk, x);
+      }
+    }
+  };
+  auto index_of = [&](int blk, int e) {
+    if (packed >= 0) return base + blk0 * kBlock + (int)short_at[blk * kBlock + 4 * lane + e] - shift;
+    return base + blk * kBlock + 4 * lane + e - shift;
+  };
+  // Building the short list while a pass goes through the part: the elements with in[], in order.
+  int filling = 0;
+  auto pack = [&](int blk, const float (&x)[4], const bool (&in)[4]) {
+    const int mine = in[0] + in[1] + in[2] + in[3], upto = warp_scan(mine, lane);
+    int at = filling + upto - mine;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (in[e]) {
+        if (at < kPack) {
+          short_x[at] = x[e];
+          short_at[at] = (uint16_t)((blk - blk0) * kBlock + 4 * lane + e);
+        }
+        ++at;
+      }
+    filling += __shfl_sync(0xffffffffu, upto, 31);
+  };
+  auto use_pack = [&] {   // (a list that is too short is not used)
+    if (filling <= kPack && per * kBlock <= 65536) {
+      for (int i = filling + lane; i < (filling + kBlock - 1) / kBlock * kBlock; i += 32) short_x[i] = -INFINITY;
+      packed = filling;
+    }
+    __syncwarp();
+  };
+
+  // ---- the largest element (a maximum passes over NaN)
+  const auto larger = [](float x, float y) { return fmaxf(x, y); };
+  float top = -INFINITY, low = INFINITY;   // for top-k also the smallest above -infinity, and how many there are
+  uint32_t finite = 0;
+  each(blk0, blk1, [&](int blk, const float (&x)[4]) {
+    top = fmaxf(top, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+    if (k < V) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool in = x[e] > -INFINITY;
+        finite += in;
+        low = fminf(low, in ? x[e] : INFINITY);
+      }
+    }
+  });
+  top = warp_fold(top, larger);
+  low = warp_min(low);
+  finite = __reduce_add_sync(0xffffffffu, finite);
+  if (lane == 0) {
+    s.red[warp].top = top;
+    s.red[warp].low = low;
+    s.red[warp].finite = finite;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    top = warp_fold(s.red[lane].top, larger);
+    low = warp_min(s.red[lane].low);
+    finite = __reduce_add_sync(0xffffffffu, s.red[lane].finite);
+    if (lane == 0) {
+      s.slot.top = top;
+      s.slot.low = low;
+      s.slot.finite = finite;
+    }
+  }
+  meet();
+  top = peek(&s.slot.top, lane % C);
+  low = peek(&s.slot.low, lane % C);
+  finite = peek(&s.slot.finite, lane % C);
+  top = warp_fold(top, larger);
+  low = warp_min(low);
+  finite = __reduce_add_sync(0xffffffffu, lane < C ? finite : 0u);
+  if (top == -INFINITY || !(temp > 0.0f) || k == 1) {
+    uint32_t first = 0xffffffffu;   // the lowest index that holds it
+    each(blk0, top > -INFINITY ? blk1 : blk0, [&](int blk, const float (&x)[4]) {
+#pragma unroll
+      for (int e = 3; e >= 0; --e)
+        if (x[e] == top) first = min(first, (uint32_t)index_of(blk, e));
+    });
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) s.red[warp].first = first;
+    __syncthreads();
+    if (warp == 0) {
+      first = __reduce_min_sync(0xffffffffu, s.red[lane].first);
+      if (lane == 0) s.slot.first = first;
+    }
+    meet();
+    if (rank == 0 && warp == 0) {
+      first = __reduce_min_sync(0xffffffffu, peek(&s.slot.first, lane % C));
+      if (lane == 0) {
+        a.tokens[b] = top > -INFINITY ? (int)first : 0;
+        if (a.probs) a.probs[b] = top > -INFINITY ? 1.0f : 0.0f;
+      }
+    }
+    meet();   // (rank 0 reads the others' slots)
+    return;
+  }
+  inf = top == INFINITY;
+  if (inf) top = low = 0.0f;
   Weigher W;
-  W.max = (double)top;
-  W.c = 1.4426950408889634074 / (double)temp;
-  W.half_max = 0.5f * top;
-  W.fc2 = (float)fmin(2.0 * W.c, 3.402823466e38);
-  W.frac = a.frac;
+  W.max = wide(top);
+  W.c = 64.0 * 1.4426950408889634074 / (double)temp;
+  const double octave = (double)temp * 0.69314718055994530942;   // a factor of two in the weight
+  W.cut = fmaxf((float)(W.max - 60.0 * octave), -kHuge);
   W.table = s.table;
 
-  // Sum over the cluster of one number per thread (a slot field that the caller chooses).
-  auto cluster_total = [&](u64 x, u64 Slot::* field) -> u64 {
+  // Sum over the cluster of one number per thread.
+  auto cluster_total = [&](double x, double Slot::* field) -> double {
     x = warp_add(x);
+    if (lane == 0) s.scan_d[warp] = x;
     __syncthreads();
-    if (lane == 0) s.scan[warp] = x;
-    __syncthreads();
-    if (tid == 0) {
-      u64 t = 0;
-      for (int w = 0; w < kWarps; ++w) t += s.scan[w];
-      s.slot.*field = t;
+    if (warp == 0) {
+      x = warp_add(s.scan_d[lane]);
+      if (lane == 0) s.slot.*field = x;
     }
-    cluster_sync();
+    meet();
+    return warp_add(lane < C ? peek(&(s.slot.*field), lane) : 0.0);
+  };
+  auto clear_hist = [&](int limbs) {
+    for (int i = tid; i < limbs * kBins; i += kThreads) (&s.hist[0][0])[i] = 0;
+    if (tid == 0) s.list_n = 0;
+    __syncthreads();
+  };
+  // The histograms of the cluster added up, in everyone's `total`: each CTA takes a slice of the bins.
+  auto merge_hist = [&](auto combine) {
+    meet();
+    // (C neighbouring lanes to a bin, each reads its CTA's numbers and writes its CTA's total)
+    for (int j = tid; j < kBins; j += kThreads) {
+      const int i = rank * (kBins / C) + j / C, r = j % C;
+      u64 t = combine(i, r);
+      for (int o = C >> 1; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      poke(&s.total[i], r, t);
+    }
+    if (tid == 0) {
+      s.pick = kBins - 1;
+      s.pick_above = 0;
+      s.pick_front = 0.0;
+    }
+    meet();
+  };
+  auto counts = [&](int i, int r) -> u64 { return peek(&s.hist[0][i], r); };
+  auto limbs = [&](int i, int r) -> u64 {
     u64 t = 0;
-    for (int r = 0; r < C; ++r) t += peek(&(s.slot.*field), r);
+#pragma unroll
+    for (int l = 0; l < kLimbs; ++l) t += (u64)peek(&s.hist[l][i], r) << (l * kLimbBits);
     return t;
   };
-
-  // Narrows down the element (in the vocabulary's order) at which the running count (MASS: weight, of elements above
-  // `floor_key`) first exceeds `target`: `key` is its key, `ties` how many of the elements with that key lie up to and
-  // including it, `equal` how many there are.  The running sum is known to exceed the target somewhere.
-  auto narrow = [&](auto mass, u64 target, u64 all, uint32_t floor_key, uint32_t& key, u64& ties, uint32_t& equal) {
-    constexpr bool MASS = decltype(mass)::value;
-    u64 above = 0;
-    uint32_t klo = MASS ? max(floor_key, 1u) : 1u, khi = key_of(top);
-    float vlo = low;
-    if (MASS) vlo = fmaxf(fmaxf(vlo, top - 124.0f / W.fc2), floor_key ? value_of(floor_key) : -INFINITY);
-    // bins over the values: half the width, so that the difference of two finite numbers stays finite
-    const float width = 0.5f * top - 0.5f * vlo, grain = width > 0.0f ? (float)kBins / width : 0.0f;
-    const bool by_value = grain > 0.0f && grain < INFINITY;
-    // round 0 of MASS adds weights as 32-bit numbers in units of `all` / 2^31 (which finds a few bins that must hold the
-    // place), everything else is exact
-    const float unit = MASS ? 2147483648.0f / (float)((double)all * ldexp(1.0, -a.frac)) : 0.0f;
-    for (int round = 0; round < 8; ++round) {   // (a round over keys cuts their range by 1024: at most five)
-      const bool value_bins = round == 0 && by_value, rough = MASS && round == 0;
-      const uint32_t span = khi - klo;
-      const int shift = max(0, 22 - __clz(span | 1u));   // (span >> shift) < 1024
-      auto bin_of = [&](float x, uint32_t xk) -> int {
-        if (value_bins) return (int)fminf((0.5f * top - 0.5f * x) * grain, (float)(kBins - 1));
-        return (int)((khi - xk) >> shift);
-      };
-      auto candidate = [&](uint32_t xk) { return MASS && round == 0 ? xk > floor_key : (xk >= klo && xk <= khi); };
-      const int limbs = MASS && !rough ? kLimbs : 1;
-      for (int i = tid; i < limbs * kBins; i += kThreads) (&s.hist[0][0])[i] = 0;
-      if (tid == 0) s.list_n = 0;
-      __syncthreads();
-      for (int blk = blk0; blk < blk1; ++blk) {
-        float x[4];
-        get4(blk, x);
+  // A weight of bin i is 2^(-i / 64) (1 + q 2^-36): the bin holds how many there are, and the sums of the lower and upper
+  // halves of q + 2^29.  In units of 2^(-i / 64) 2^-36:
+  auto masses = [&](int i, int r) -> u64 {
+    return (u64)peek(&s.hist[0][i], r) * ((1ull << 36) - (1ull << 29)) + ((u64)peek(&s.hist[2][i], r) << 15) + peek(&s.hist[1][i], r);
+  };
+  // The bin at which the running sum of f(total, bin) first exceeds `want`, and the sum in front of it.
+  auto find_bin = [&](auto zero, auto f, decltype(zero) want, auto* scan, decltype(zero)& in_front) -> int {
+    using N = decltype(zero);
+    constexpr int E = kBins / kThreads;
+    N x[E], sum = zero;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t xk = key_of(x[e]);
-          const bool in = xk != 0u && candidate(xk);
-          if (rough) {
-            const float w = in ? exp2f(W.log2f32(x[e])) * unit : 0.0f;
-            if (w >= 1.0f) atomicAdd(&s.hist[0][bin_of(x[e], xk)], (uint32_t)w);
-          } else if (!MASS) {
-            // (equal logits, as bf16 has many of, meet in one bin: a warp that agrees adds once)
-            const int bin = in ? bin_of(x[e], xk) : -1;
-            const int lead = __shfl_sync(0xffffffffu, bin, 0);
-            const unsigned same = __ballot_sync(0xffffffffu, bin == lead);
-            if (same == 0xffffffffu) {
-              if (lane == 0 && lead >= 0) atomicAdd(&s.hist[0][lead], 32u);
-            } else if (in) {
-              atomicAdd(&s.hist[0][bin], 1u);
-            }
-          } else if (in) {
-            const int bin = bin_of(x[e], xk);
-            u64 w = W(x[e]);
+    for (int e = 0; e < E; ++e) sum += x[e] = f(s.total[tid * E + e], tid * E + e);
+    const N inc = warp_scan(sum, lane);
+    if (lane == 31) scan[warp] = inc;
+    __syncthreads();
+    const N upto = warp_scan(scan[lane], lane), all = __shfl_sync(0xffffffffu, upto, kWarps - 1);
+    N run = __shfl_sync(0xffffffffu, upto, max(warp - 1, 0));
+    run = (warp ? run : zero) + (inc - sum);
+    // (a sum that was formed in another order may end a rounding short of the place)
+    if constexpr (std::is_integral_v<N>) want = all > 0 ? min(want, all - 1) : want;
+    else want = fmin(want, all);
 #pragma unroll
-            for (int l = 0; l < kLimbs; ++l, w >>= kLimbBits)
-              if (w & ((1u << kLimbBits) - 1u)) atomicAdd(&s.hist[l][bin], (uint32_t)w & ((1u << kLimbBits) - 1u));
-          }
-        }
+    for (int e = 0; e < E; ++e) {
+      if (run <= want && run + x[e] > want) {
+        s.pick = tid * E + e;
+        if constexpr (std::is_integral_v<N>) s.pick_above = run;
+        else s.pick_front = run;
       }
-      cluster_sync();
-      // each CTA adds up a slice of the bins over the cluster and hands it to everyone
-      for (int i = rank * (kBins / C) + tid; i < (rank + 1) * (kBins / C); i += kThreads) {
-        u64 t = 0;
-        for (int l = 0; l < limbs; ++l) {
-          u64 x = 0;
-          for (int r = 0; r < C; ++r) x += peek(&s.hist[l][i], r);
-          t += x << (l * kLimbBits);
-        }
-        for (int r = 0; r < C; ++r) poke(&s.total[i], r, t);
-      }
-      if (tid == 0) {
-        s.pick_lo = kBins - 1;
-        s.pick_hi = kBins - 1;
-        s.pick_above = 0;
-      }
-      cluster_sync();
-      {
-        constexpr int E = kBins / kThreads;
-        u64 x[E], sum = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum += x[e] = s.total[tid * E + e];
-        u64 inc = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += y;
-        }
-        if (lane == 31) s.scan[warp] = inc;
-        __syncthreads();
-        u64 run = inc - sum;
-        for (int w = 0; w < warp; ++w) run += s.scan[w];
-        // a rough sum is short by less than one unit an element and off by 2^-16 of itself
-        const u64 want = rough ? (u64)((double)target / (double)all * 2147483648.0) : target - above;
-        const u64 slack_lo = rough ? (u64)V + (1u << 15) : 0, slack_hi = rough ? (1u << 15) + 1 : 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const u64 next = run + x[e];
-          if (run + slack_lo <= want && next + slack_lo > want) {
-            s.pick_lo = tid * E + e;
-            s.pick_above = run;
-          }
-          if (tid * E + e == 0 && slack_lo > want) s.pick_lo = 0;
-          if (run <= want + slack_hi && next > want + slack_hi) s.pick_hi = tid * E + e;
-          run = next;
-        }
-        __syncthreads();
-      }
-      const int lo = s.pick_lo, hi = max(lo, s.pick_hi);
-      if (!rough) above += s.pick_above;
-      // what lies in those bins, and (after a rough round) the exact weight of what lies in front of them
-      u64 front = 0;
-      uint32_t n = 0, kmin = 0xffffffffu, kmax = 0;
-      for (int blk = blk0; blk < blk1; ++blk) {
-        float x[4];
-        get4(blk, x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t xk = key_of(x[e]);
-          if (xk == 0u || !candidate(xk)) continue;
-          const int bin = bin_of(x[e], xk);
-          if (bin < lo) {
-            if (rough) front += W(x[e]);
-          } else if (bin <= hi) {
-            ++n;
-            kmin = min(kmin, xk);
-            kmax = max(kmax, xk);
-            const int at = atomicAdd(&s.list_n, 1);
-            if (at < kList) {
-              s.list_key[at] = xk;
-              s.list_at[at] = base + blk * kBlock + 4 * lane + e;
-            }
-          }
-        }
-      }
-      front = warp_add(front);
-      n = __reduce_add_sync(0xffffffffu, n);
-      kmin = __reduce_min_sync(0xffffffffu, kmin);
-      kmax = __reduce_max_sync(0xffffffffu, kmax);
-      if (lane == 0) {
-        s.red[warp].above = front;
-        s.red[warp].n = n;
-        s.red[warp].kmin = kmin;
-        s.red[warp].kmax = kmax;
-      }
-      __syncthreads();
-      if (tid == 0) {
-        for (int w = 1; w < kWarps; ++w) {
-          front += s.red[w].above;
-          n += s.red[w].n;
-          kmin = min(kmin, s.red[w].kmin);
-          kmax = max(kmax, s.red[w].kmax);
-        }
-        s.slot.above = front;
-        s.slot.n = n;
-        s.slot.kmin = kmin;
-        s.slot.kmax = kmax;
-      }
-      cluster_sync();
-      u64 ahead = 0;
-      n = 0;
-      kmin = 0xffffffffu;
-      kmax = 0;
-      int off = 0;
-      for (int r = 0; r < C; ++r) {
-        ahead += peek(&s.slot.above, r);
-        const uint32_t nr = peek(&s.slot.n, r);
-        if (r < rank) off += (int)nr;
-        n += nr;
-        kmin = min(kmin, peek(&s.slot.kmin, r));
-        kmax = max(kmax, peek(&s.slot.kmax, r));
-      }
-      if (rough) above = ahead;
-      if (n == 0) {   // (not reached while the sums say that the place is there)
-        key = klo;
-        ties = 0;
-        equal = 0;
-        return;
-      }
-      if (kmin == kmax) {
-        key = kmin;
-        equal = n;
-        const u64 w = MASS ? W(value_of(kmin)) : 1;
-        ties = w ? (target - above) / w + 1 : n;
-        if (ties > n) ties = n;
-        return;
-      }
-      if (n <= kList) {   // rank them: every CTA gathers all lists
-        for (int r = 0, o = 0; r < C; ++r) {
-          const int nr = (int)peek(&s.slot.n, r);
-          for (int i = tid; i < nr; i += kThreads) {
-            const uint32_t xk = peek(&s.list_key[i], r);
-            s.all_key[o + i] = xk;
-            s.all_at[o + i] = (int)peek(reinterpret_cast<const uint32_t*>(&s.list_at[i]), r);
-            s.all_w[o + i] = MASS ? W(value_of(xk)) : 1;
-          }
-          o += nr;
-        }
-        __syncthreads();
-        if (tid < (int)n) {
-          const uint32_t xk = s.all_key[tid];
-          const int at = s.all_at[tid];
-          u64 before = above;
-          uint32_t eq = 0, eq_before = 0;
-          for (int i = 0; i < (int)n; ++i) {
-            const uint32_t yk = s.all_key[i];
-            const bool ahead_of = yk > xk || (yk == xk && s.all_at[i] < at);
-            if (ahead_of) before += s.all_w[i];
-            eq += yk == xk;
-            eq_before += yk == xk && ahead_of;
-          }
-          if (before <= target && target < before + s.all_w[tid]) {
-            s.pick_key = xk;
-            s.pick_ties = eq_before + 1;
-            s.slot.eq = eq;
-          }
-        }
-        __syncthreads();
-        key = s.pick_key;
-        ties = s.pick_ties;
-        equal = s.slot.eq;
-        cluster_sync();   // the lists have been read
-        return;
-      }
-      klo = kmin;
-      khi = kmax;
+      run += x[e];
     }
-    key = klo;
-    ties = equal = 0;
+    __syncthreads();
+    if constexpr (std::is_integral_v<N>) in_front = s.pick_above;
+    else in_front = s.pick_front;
+    return s.pick;
   };
 
-  // ---- threshold
-  uint32_t t = 0u, equal = 0;
-  u64 ties = 0;   // t = 0: everything above -infinity is kept
-  if (k < V) {
-    // (fewer than k elements above -infinity: all of them stay)
-    u64 n = 0;
-    for (int blk = blk0; blk < blk1; ++blk) {
-      float x[4];
-      get4(blk, x);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) n += x[e] > -INFINITY;
+  // Candidates of a narrowing step: how many, their keys' range, and (in any order) the first kList of them.
+  struct Found { uint32_t n, kmin, kmax; };
+  auto note = [&](Found& f, uint32_t xk, int at) {
+    ++f.n;
+    f.kmin = min(f.kmin, xk);
+    f.kmax = max(f.kmax, xk);
+    if (*reinterpret_cast<volatile int*>(&s.list_n) > kList) return;
+    const int i = atomicAdd(&s.list_n, 1);
+    if (i < kList) {
+      s.list_key[i] = xk;
+      s.list_at[i] = (uint32_t)at;
     }
-    n = cluster_total(n, &Slot::count);
-    if ((u64)k < n) narrow(std::false_type{}, (u64)k - 1, 0, 0u, t, ties, equal);
+  };
+  // Adds up Found over the cluster.
+  auto gather = [&](Found& f) {
+    f.n = __reduce_add_sync(0xffffffffu, f.n);
+    f.kmin = __reduce_min_sync(0xffffffffu, f.kmin);
+    f.kmax = __reduce_max_sync(0xffffffffu, f.kmax);
+    if (lane == 0) {
+      Slot& r = s.red[warp];
+      r.n = f.n; r.kmin = f.kmin; r.kmax = f.kmax;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      const Slot& r = s.red[lane];
+      const uint32_t n = __reduce_add_sync(0xffffffffu, r.n);
+      const uint32_t lo = __reduce_min_sync(0xffffffffu, r.kmin), hi = __reduce_max_sync(0xffffffffu, r.kmax);
+      if (lane == 0) {
+        s.slot.n = n; s.slot.kmin = lo; s.slot.kmax = hi;
+      }
+    }
+    meet();
+    const int r = lane % C;
+    const uint32_t n = peek(&s.slot.n, r), lo = peek(&s.slot.kmin, r), hi = peek(&s.slot.kmax, r);
+    f.n = __reduce_add_sync(0xffffffffu, lane < C ? n : 0u);
+    f.kmin = __reduce_min_sync(0xffffffffu, lo);
+    f.kmax = __reduce_max_sync(0xffffffffu, hi);
+  };
+  uint32_t t = 0u, equal = 0;   // threshold key (0: everything above -infinity is kept), elements that have it
+  u64 ties = 0;                 // and how many of them are kept, the first ones in index order
+  // Goes on inside the candidates f: the element at which the running count (MASS: weight) exceeds `target`, `above` of
+  // it lies in front of them.  Counts are whole numbers; weights are added as integers here.
+  auto finish = [&](auto mass, Found f, double above, double target) {
+    constexpr bool MASS = decltype(mass)::value;
+    constexpr double one = MASS ? (double)(1ull << kFrac) : 1.0;
+    for (int round = 0; round < 5; ++round) {   // (a round cuts the range of the keys by 1024: at most four)
+      if (f.n == 0) return;   // (not reached: the place is known to be there)
+      const double left = (target - above) * one;
+      const u64 want = left > 0.0 ? (u64)left : 0;
+      if (f.kmin == f.kmax) {
+        const u64 w = MASS ? W.fixed(value_of(f.kmin)) : 1;
+        t = f.kmin;
+        equal = f.n;
+        ties = w ? min(want / w + 1, (u64)f.n) : (u64)f.n;
+        return;
+      }
+      if (f.n <= kRank) {   // every CTA gathers all lists and ranks them
+        const int upto = warp_scan(lane < C ? (int)peek(&s.slot.n, lane % C) : 0, lane);
+        int from = 0, r = 0;   // the list that entry `tid` of all of them is in, and where it begins
+        for (int c = 0; c + 1 < C; ++c) {
+          const int end = __shfl_sync(0xffffffffu, upto, c);
+          if (tid >= end) {
+            from = end;
+            r = c + 1;
+          }
+        }
+        if (tid < (int)f.n) {
+          const uint32_t xk = peek(&s.list_key[tid - from], r);
+          s.all_at[tid] = peek(&s.list_at[tid - from], r);
+          s.all_key[tid] = xk;
+          s.all_w[tid] = MASS ? W.fixed(value_of(xk)) : 1;
+        }
+        __syncthreads();
+        for (int c = warp; c < (int)f.n; c += kWarps) {   // a warp to a candidate, the lanes over all of them
+          const uint32_t xk = s.all_key[c], at = s.all_at[c];
+          u64 before = 0;
+          uint32_t eq = 0, eq_before = 0, place = 0;
+          for (int i = lane; i < (int)f.n; i += 32) {
+            const uint32_t yk = s.all_key[i];
+            const bool first = yk > xk || (yk == xk && s.all_at[i] < at);
+            if (first) before += s.all_w[i];
+            place += first;
+            eq += yk == xk;
+            eq_before += yk == xk && first;
+          }
+          before = warp_fold(before, [](u64 p, u64 q) { return p + q; });
+          place = __reduce_add_sync(0xffffffffu, place);
+          eq = __reduce_add_sync(0xffffffffu, eq);
+          eq_before = __reduce_add_sync(0xffffffffu, eq_before);
+          if (lane == 0 && before <= want && (want < before + s.all_w[c] || place + 1 == f.n)) {
+            s.pick_key = xk;
+            s.pick_ties = eq_before + 1;
+            s.pick_equal = eq;
+          }
+        }
+        __syncthreads();
+        t = s.pick_key;
+        ties = s.pick_ties;
+        equal = s.pick_equal;
+        meet();   // the lists have been read
+        return;
+      }
+      // the list takes the place of the row where it holds all of this CTA's candidates: one to a thread
+      static_assert(kList == kThreads);
+      const bool listed = s.list_n <= kList;
+      const uint32_t my_key = listed && tid < s.list_n ? s.list_key[tid] : 0u, my_at = listed && tid < s.list_n ? s.list_at[tid] : 0u;
+      __syncthreads();
+      const uint32_t klo = f.kmin, khi = f.kmax;
+      const int by = max(0, 22 - __clz((khi - klo) | 1u));   // (khi - klo) >> by < 1024
+      clear_hist(MASS ? kLimbs : 1);
+      auto add = [&](uint32_t xk) {
+        if (xk < klo || xk > khi) return;
+        const int bin = (int)((khi - xk) >> by);
+        if constexpr (MASS) {
+          u64 w = W.fixed(value_of(xk));
+#pragma unroll
+          for (int l = 0; l < kLimbs; ++l, w >>= kLimbBits)
+            if (w & ((1u << kLimbBits) - 1u)) atomicAdd(&s.hist[l][bin], (uint32_t)w & ((1u << kLimbBits) - 1u));
+        } else {
+          atomicAdd(&s.hist[0][bin], 1u);
+        }
+      };
+      if (listed) {
+        add(my_key);
+      } else {
+        each(blk0, blk1, [&](int, const float (&x)[4]) {
+#pragma unroll 1
+          for (int e = 0; e < 4; ++e) add(key_of(e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3]));
+        });
+      }
+      if constexpr (MASS) merge_hist(limbs);
+      else merge_hist(counts);
+      u64 in_front;
+      const int bin = find_bin((u64)0, [](u64 x, int) { return x; }, want, s.scan, in_front);
+      above += (double)in_front / one;
+      f = Found{0u, 0xffffffffu, 0u};
+      auto inside = [&](uint32_t xk) { return xk >= klo && xk <= khi && (int)((khi - xk) >> by) == bin; };
+      if (listed) {
+        if (inside(my_key)) note(f, my_key, (int)my_at);
+      } else {
+        each(blk0, blk1, [&](int blk, const float (&x)[4]) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t xk = key_of(x[e]);
+            if (inside(xk)) note(f, xk, index_of(blk, e));
+          }
+        });
+      }
+      gather(f);
+    }
+  };
+
+  // ---- top-k (fewer than k elements above -infinity: all of them stay; an infinite maximum: so do its equals, unless
+  // there are more than k)
+  if (k < V) {
+    uint32_t n = finite;
+    if (inf) {
+      uint32_t m = 0;
+      each(blk0, blk1, [&](int blk, const float (&x)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m += x[e] == 0.0f;
+      });
+      n = (uint32_t)cluster_total((double)m, &Slot::count);
+    }
+    clear_hist(1);
+    if ((uint32_t)k < n) {
+      // bins over the values (of halves: the difference of two finite numbers stays finite)
+      const float width = 0.5f * top - 0.5f * low, grain = (float)kBins / width;
+      Found f{0u, 0xffffffffu, 0u};
+      double above = 0.0;
+      int bin = -1;
+      auto bin_of = [&](float x) { return (int)fminf((0.5f * top - 0.5f * x) * grain, (float)(kBins - 1)); };
+      const bool by_value = width > 0.0f && grain < INFINITY;
+      if (by_value) {
+        each(blk0, blk1, [&](int blk, const float (&x)[4]) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (x[e] > -INFINITY) atomicAdd(&s.hist[0][bin_of(x[e])], 1u);   // (NaN fails the comparison)
+        });
+        merge_hist(counts);
+        u64 in_front;
+        bin = find_bin((u64)0, [](u64 x, int) { return x; }, (u64)k - 1, s.scan, in_front);
+        above = (double)in_front;
+      }
+      each(blk0, blk1, [&](int blk, const float (&x)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (x[e] > -INFINITY && (!by_value || bin_of(x[e]) == bin)) note(f, key_of(x[e]), index_of(blk, e));
+        bool in[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) in[e] = x[e] > -INFINITY && by_value && bin_of(x[e]) <= bin;
+        if (__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) pack(blk, x, in);
+      });
+      if (by_value) use_pack();
+      gather(f);
+      finish(std::false_type{}, f, above, (double)(k - 1));
+    }
   }
+  // ---- top-p
   if (p < 1.0f) {
-    u64 z = 0;
-    for (int blk = blk0; blk < blk1; ++blk) {
-      float x[4];
-      get4(blk, x);
+    const float tv = t ? value_of(t) : -INFINITY;
+    // the mass above the threshold so far, and its distribution over 64ths of a factor of two (the last bin is everything
+    // below 2^-16: nobody counts it, half a row would add to one number)
+    double z = 0.0;
+    clear_hist(3);
+    each(blk0, blk1, [&](int, const float (&x)[4]) {
+      bool in[4];
+      int bin[4], q[4];
+      double w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        in[e] = x[e] > tv && x[e] >= W.cut;
+        w[e] = W(fmaxf(x[e], W.cut), bin[e], q[e]);
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (key_of(x[e]) > t) z += W(x[e]);
-    }
-    const u64 strictly = cluster_total(z, &Slot::mass);
-    const u64 wt = t ? W(value_of(t)) : 0, all = strictly + ties * wt;
-    const u64 target = p > 0.0f ? __umul64hi((u64)((double)p * 18446744073709551616.0), all) : 0;
+        if (in[e] && bin[e] < kBins - 1) {
+          const uint32_t positive = (uint32_t)(q[e] + (1 << 29));
+          atomicAdd(&s.hist[0][bin[e]], 1u);
+          atomicAdd(&s.hist[1][bin[e]], positive & 0x7fffu);
+          atomicAdd(&s.hist[2][bin[e]], positive >> 15);
+        }
+      z += ((in[0] ? w[0] : 0.0) + (in[1] ? w[1] : 0.0)) + ((in[2] ? w[2] : 0.0) + (in[3] ? w[3] : 0.0));
+    });
+    const double strictly = cluster_total(z, &Slot::mass);
+    const double wt = t ? W(tv) : 0.0;
+    const double target = p > 0.0f ? (double)p * (strictly + (double)ties * wt) : 0.0;
     if (target < strictly) {
-      uint32_t t2;
-      narrow(std::true_type{}, target, strictly, t, t2, ties, equal);
-      t = t2;
-    } else if (wt) {   // the border lies among the ties of top-k
-      ties = min(ties, (target - strictly) / wt + 1);
+      merge_hist(masses);
+      double front;
+      const int bin = find_bin(0.0, [&](u64 x, int i) {
+        const double unit = __hiloint2double(__double2hiint(s.table[-i & 63]) - (((i + 63) >> 6) << 20), __double2loint(s.table[-i & 63]));
+        return i < kBins - 1 ? (double)x * (unit * 0x1p-36) : 1e30;
+      }, target, s.scan_d, front);
+      const float cut = bin == kBins - 1 ? W.cut : fmaxf(W.cut, (float)(W.max - (double)(bin + 1) * (octave / 64.0)));
+      const bool fill = packed < 0;
+      Found f{0u, 0xffffffffu, 0u};
+      filling = 0;
+      if (tid == 0) s.list_n = 0;
+      __syncthreads();
+      each(blk0, blk1, [&](int blk, const float (&x)[4]) {
+        bool in[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) in[e] = x[e] > tv && x[e] >= cut;
+        if (!__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int be = min(W.bin_of(fmaxf(x[e], cut)), kBins - 1);
+          if (in[e] && be == bin) note(f, key_of(x[e]), index_of(blk, e));
+          in[e] = in[e] && be <= bin;
+        }
+        if (fill && filling <= kPack) pack(blk, x, in);
+      });
+      if (fill) use_pack();
+      gather(f);
+      finish(std::true_type{}, f, front, target);
+    } else if (wt > 0.0) {   // the border lies among the ties of top-k
+      ties = min(ties, (u64)((target - strictly) / wt) + 1);
     }
   }
   const bool some = t != 0u && ties < equal;   // only the first of the elements that equal the threshold stay
+  const float tv = t ? value_of(t) : -INFINITY;
   u64 seen0 = 0;                               // ties in front of this warp's part
   if (some) {
     uint32_t eq = 0;
-    for (int blk = blk0; blk < blk1; ++blk) {
-      float x[4];
-      get4(blk, x);
+    each(blk0, blk1, [&](int blk, const float (&x)[4]) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) eq += key_of(x[e]) == t;
-    }
+      for (int e = 0; e < 4; ++e) eq += x[e] == tv;
+    });
     eq = __reduce_add_sync(0xffffffffu, eq);
-    __syncthreads();
     if (lane == 0) s.warp_eq[warp] = eq;
     __syncthreads();
-    if (tid == 0) {
-      uint32_t e = 0;
-      for (int w = 0; w < kWarps; ++w) e += s.warp_eq[w];
-      s.slot.eq = e;
+    if (warp == 0) {
+      eq = __reduce_add_sync(0xffffffffu, s.warp_eq[lane]);
+      if (lane == 0) s.slot.eq = eq;
     }
-    cluster_sync();
-    for (int r = 0; r < rank; ++r) seen0 += peek(&s.slot.eq, r);
-    for (int w = 0; w < warp; ++w) seen0 += s.warp_eq[w];
+    meet();
+    eq = peek(&s.slot.eq, lane % C);
+    seen0 = __reduce_add_sync(0xffffffffu, (lane < rank ? eq : 0u) + (lane < warp ? s.warp_eq[lane] : 0u));
   }
   // ---- kept weights in index order
-  const u64 mfix = mp > 0.0f ? (u64)((double)mp * ldexp(1.0, a.frac)) : 0;
-  auto kept4 = [&](int blk, u64& seen, u64 (&w)[4]) {
-    float x[4];
-    get4(blk, x);
-    u64 rank4 = 0;
-    uint32_t mine = 0;
+  // what cannot be kept is passed over by one comparison: below the threshold, or 1 % below the least weight
+  float cut = fmaxf(W.cut, tv);
+  if (mp > 0.0f) cut = fmaxf(cut, (float)(W.max + ((double)__log2f(mp) - 0.01) * octave));   // (the 32-bit logarithm is good to 2^-20)
+  // a few kept elements of a long part are listed first: a weight costs thirty times the comparison
+  if (packed < 0 && (t || mp > 0.0f)) {
+    filling = 0;
+    each(blk0, blk1, [&](int blk, const float (&x)[4]) {
+      const bool in[4] = {x[0] >= cut, x[1] >= cut, x[2] >= cut, x[3] >= cut};
+      if (filling <= kPack && __any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) pack(blk, x, in);
+    });
+    use_pack();
+  }
+  const double mp_near = mp > 0.0f ? (double)mp * 1.0000001 : 0.0;
+  auto kept4 = [&](const float (&x)[4], u64& seen, double (&w)[4]) -> bool {   // whether any lane has a weight
+    u64 place = 0;
     if (some) {
+      uint32_t mine = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mine += key_of(x[e]) == t;
+      for (int e = 0; e < 4; ++e) mine += x[e] == tv;
       uint32_t inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += y;
       }
-      rank4 = seen + inc - mine;
+      place = seen + inc - mine;
       seen += __shfl_sync(0xffffffffu, inc, 31);
     }
+    bool keep[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t xk = key_of(x[e]);
-      bool keep = xk > t || (t && xk == t);
-      if (some && xk == t) keep = rank4++ < ties;
-      w[e] = 0;
-      if (keep && xk) {
-        w[e] = W(x[e]);
-        if (mp > 0.0f) {
-          const long long d = (long long)(w[e] - mfix);
-          const long long near = (long long)(mfix >> 26) + 2;
-          bool ok = d >= 0;
-          if (d <= near && d >= -near) ok = exp(((double)x[e] - W.max) / (double)temp) >= (double)mp;   // next to the border: in 64 bits
-          if (!ok) w[e] = 0;
-        }
-      }
+      keep[e] = x[e] >= cut;
+      if (some && x[e] == tv) keep[e] = keep[e] && place++ < ties;
+      w[e] = 0.0;
     }
-  };
-  u64 sum = 0, seen = seen0;
-  for (int blk = blk0; blk < blk1; ++blk) {
-    u64 w[4];
-    kept4(blk, seen, w);
-    sum += (w[0] + w[1]) + (w[2] + w[3]);
-  }
-  sum = warp_add(sum);
-  __syncthreads();
-  if (lane == 0) s.warp_sum[warp] = sum;
-  __syncthreads();
-  if (tid == 0) {
-    u64 x = 0;
-    for (int w = 0; w < kWarps; ++w) x += s.warp_sum[w];
-    s.slot.sum = x;
-  }
-  cluster_sync();
-  u64 z = 0, ahead = 0;
-  for (int r = 0; r < C; ++r) {
-    const u64 x = peek(&s.slot.sum, r);
-    if (r < rank) ahead += x;
-    z += x;
-  }
-  for (int w = 0; w < warp; ++w) ahead += s.warp_sum[w];
-  const float u = a.u[b];
-  const double uu = u >= 0.0f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0;
-  const u64 target = __umul64hi((u64)(uu * 18446744073709551616.0), z);
-  if (ahead <= target && target < ahead + sum) {   // the warp that holds the token
-    seen = seen0;
-    for (int blk = blk0; blk < blk1; ++blk) {
-      u64 w[4];
-      kept4(blk, seen, w);
-      const u64 mine = (w[0] + w[1]) + (w[2] + w[3]);
-      u64 inc = mine;
+    if (!__any_sync(0xffffffffu, keep[0] || keep[1] || keep[2] || keep[3])) return false;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 y = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += y;
-      }
-      const unsigned hit = __ballot_sync(0xffffffffu, ahead + inc > target);
-      if (hit) {
-        if (lane == __ffs(hit) - 1) {
-          u64 run = ahead + inc - mine;
-          int e = 0;
-          for (; e < 3 && run + w[e] <= target; ++e) run += w[e];
-          a.tokens[b] = base + blk * kBlock + 4 * lane + e;
-          if (a.probs) a.probs[b] = (float)((double)w[e] / (double)z);
+    for (int e = 0; e < 4; ++e) {
+      int bin;
+      const double x0 = W(fmaxf(x[e], cut), bin);
+      w[e] = keep[e] ? x0 : 0.0;
+    }
+    if (mp > 0.0f) {
+      bool near = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) near = near || (w[e] != 0.0 && w[e] < mp_near);
+      if (near) {   // next to the border of min-p, or below it: with the library's exponential
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) {
+          const double we = e == 0 ? w[0] : e == 1 ? w[1] : e == 2 ? w[2] : w[3];
+          const float xe = e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3];
+          const bool drop = we < mp_near && library_exp(((double)xe - W.max) / (double)temp) < (double)mp;
+          if (drop && e == 0) w[0] = 0.0;
+          if (drop && e == 1) w[1] = 0.0;
+          if (drop && e == 2) w[2] = 0.0;
+          if (drop && e == 3) w[3] = 0.0;
         }
-        break;
       }
-      ahead += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return true;
+  };
+  // Lane i keeps the sum of the i-th group of blocks of its warp, and the ties in front of it: the walk at the end then
+  // goes through one group.
+  const int group = packed >= 0 ? 1 : (per + 7) / 8;
+  double my_group = 0.0;
+  u64 seen = seen0, my_seen = seen0;
+  double in_group = 0.0;
+  bool any = false;
+  int g = 0, to_go = group;
+  each(blk0, blk1, [&](int, const float (&x)[4]) {
+    if (to_go == group && lane == g) my_seen = seen;
+    double w[4];
+    if (kept4(x, seen, w)) {
+      in_group += (w[0] + w[1]) + (w[2] + w[3]);
+      any = true;
+    }
+    if (--to_go == 0) {
+      if (any) {
+        in_group = warp_add(in_group);
+        if (lane == g) my_group = in_group;
+      }
+      in_group = 0.0;
+      any = false;
+      to_go = group;
+      ++g;
+    }
+  });
+  in_group = warp_add(in_group);
+  if (lane == g) my_group = in_group;   // (a last group that is short)
+  const double upto_group = warp_scan(my_group, lane);
+  if (lane == 31) s.warp_sum[warp] = upto_group;
+  __syncthreads();
+  const double upto_warp = warp_scan(s.warp_sum[lane], lane);
+  if (tid == 31) s.slot.sum = upto_warp;
+  meet();
+  // The place u z of the running sum belongs to the last CTA, in it the last warp, in it the last group, and there the last
+  // token with a weight whose front is not past it.  (Roundings between the levels move a border by 2^-52 of the sum.)
+  const double mine = lane < C ? peek(&s.slot.sum, lane % C) : 0.0;
+  if (C > 1) fsvd_tile::cluster_arrive();   // nothing of another CTA is read any more
+  const double upto_cta = warp_scan(mine, lane), z = __shfl_sync(0xffffffffu, upto_cta, 31);
+  const float u = a.u[b];
+  const double target = (u >= 0.0f ? fmin((double)u, 1.0 - 0x1p-24) : 0.0) * z;
+  auto last_not_past = [&](double x, double end, double from) -> int {   // lane of it; x: its part, end: the sum up to it
+    const unsigned ok = __ballot_sync(0xffffffffu, x > 0.0 && from + (end - x) <= target);
+    const unsigned any = __ballot_sync(0xffffffffu, x > 0.0);
+    return ok ? 31 - __clz(ok) : any ? __ffs(any) - 1 : -1;
+  };
+  const int owner = last_not_past(mine, upto_cta, 0.0);
+  if (owner == rank) {
+    double from = __shfl_sync(0xffffffffu, upto_cta - mine, owner);
+    const double wx = s.warp_sum[lane];
+    const int ow = last_not_past(wx, upto_warp, from);
+    if (ow == warp) {
+      from += __shfl_sync(0xffffffffu, upto_warp - wx, ow);
+      const int og = last_not_past(my_group, upto_group, from);
+      from += __shfl_sync(0xffffffffu, upto_group - my_group, og);
+      seen = __shfl_sync(0xffffffffu, my_seen, og);
+      int best = 0;
+      double best_w = 0.0;
+      const int first = blk0 + og * group;
+      each(first, min(blk1, first + group), [&](int blk, const float (&x4)[4]) {
+        if (packed >= 0 && blk != og) return;   // (a short list has a group per block)
+        double w[4];
+        kept4(x4, seen, w);
+        const double x = (w[0] + w[1]) + (w[2] + w[3]), end = warp_scan(x, lane);
+        const int src = last_not_past(x, end, from);
+        const bool here = src >= 0 && (best_w == 0.0 || __shfl_sync(0xffffffffu, from + (end - x), src) <= target);
+        if (here) {
+          double run = from + (end - x), pw = 0.0;
+          int pick = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (w[e] > 0.0 && (pw == 0.0 || run <= target)) {
+              pick = index_of(blk, e);
+              pw = w[e];
+            }
+            run += w[e];
+          }
+          best = __shfl_sync(0xffffffffu, pick, src);
+          best_w = __shfl_sync(0xffffffffu, pw, src);
+        }
+        from += __shfl_sync(0xffffffffu, end, 31);
+      });
+      if (lane == 0) {
+        a.tokens[b] = best;
+        if (a.probs) a.probs[b] = (float)(best_w / z);
+      }
     }
   }
-  cluster_sync();   // (the others may still be reading this CTA's slot)
+  if (C > 1) fsvd_tile::cluster_wait();   // the others have read this CTA's slot
 }
 
 static int fail(int code, const char* msg) {
@@ -657,26 +926,26 @@ extern "C" int fsvd_sample(const void* logits, long long row_stride, int dtype, 
   if (!logits || !uniforms || !tokens) return fail(FSVD_ERR_ARG, "null argument");
   if (dtype != FSVD_DTYPE_F32 && dtype != FSVD_DTYPE_BF16) return fail(FSVD_ERR_ARG, "logits are float32 or bfloat16");
   if (B < 0 || V < 1 || row_stride < 0) return fail(FSVD_ERR_ARG, "bad sizes");
-  if (V > kMaxVocab) return fail(FSVD_ERR_UNSUPPORTED, "a vocabulary beyond 2^22 is unsupported");
+  if (V > kMaxVocab) return fail(FSVD_ERR_UNSUPPORTED, "a vocabulary beyond 2^20 is unsupported");
   if (B > (1 << 24)) return fail(FSVD_ERR_UNSUPPORTED, "more than 2^24 rows are unsupported");
   if (temperature_all != temperature_all || top_p_all != top_p_all || min_p_all != min_p_all)
     return fail(FSVD_ERR_ARG, "NaN setting");
   if (B == 0) return 0;
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  int bits = 0;
-  while ((1 << bits) < V) ++bits;
-  // CTAs of a row: enough that a piece is at most 50 KB (three CTAs per SM), and that few rows use the whole GPU as long
-  // as a CTA has 2048 elements to work on.
+  // CTAs of a row: so many that a piece fits beside the short lists, and as many as give every SM at most one, as long as
+  // each has 4096 elements to work on.
+  const int es = dtype == FSVD_DTYPE_F32 ? 4 : 2;
+  const long long places = V + 16 / es - 1;   // a row may start up to 15 bytes behind a 16-byte boundary
   int C = 1;
-  while (C < kMaxCluster && (V / C > 12800 || (B * C < sms && V / C > 2048))) C *= 2;
+  while (C < kMaxCluster && ((2ll * B * C <= sms && places / C > 4096) || places * es / C > 140 * 1024)) C *= 2;
   Args a;
   a.logits = logits; a.stride = row_stride; a.u = uniforms; a.temperature = temperature; a.top_k = top_k; a.top_p = top_p;
   a.min_p = min_p; a.T_all = temperature_all; a.k_all = top_k_all; a.p_all = top_p_all; a.m_all = min_p_all;
-  a.tokens = tokens; a.probs = probs; a.V = V; a.frac = std::min(46, 62 - bits);
-  a.chunk = ((V + C - 1) / C + kBlock - 1) / kBlock * kBlock;
-  const bool resident = a.chunk <= 48 * 1024;
-  const size_t smem = resident ? (size_t)a.chunk * 4 : 0;
+  a.tokens = tokens; a.probs = probs; a.V = V;
+  a.chunk = (int)(((places + C - 1) / C + kBlock - 1) / kBlock * kBlock);
+  const bool resident = (size_t)a.chunk * es <= 144 * 1024;   // (with the 80 KB that every CTA has)
+  const size_t smem = (size_t)kWarps * (resident ? kPackPiece : kPackAlone) * 6 + (resident ? (size_t)a.chunk * es : 0);
   const void* fn = dtype == FSVD_DTYPE_F32 ? (resident ? (const void*)sample_kernel<float, true> : (const void*)sample_kernel<float, false>)
                                            : (resident ? (const void*)sample_kernel<__nv_bfloat16, true>
                                                        : (const void*)sample_kernel<__nv_bfloat16, false>);
