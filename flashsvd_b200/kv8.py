@@ -75,30 +75,30 @@ class KV8Cache:
     struct: FsvdKv8 = field(init=False, repr=False)
 
     def __post_init__(self):
-        k, ks = self.k, self.k_scale
+        k, v, ks, vs, block = self.k, self.v, self.k_scale, self.v_scale, self.block
         if k.ndim != 4:
             raise ValueError(f"k must be [B, Hk, S_max, Dh], got {tuple(k.shape)}")
-        B, Hk, S, Dh = k.shape
-        if self.block not in BLOCKS:
-            raise ValueError(f"block must be one of {BLOCKS}, got {self.block}")
-        if Dh not in (64, 128):
+        shape = k.shape
+        B, Hk, S, Dh = shape
+        if block not in BLOCKS:
+            raise ValueError(f"block must be one of {BLOCKS}, got {block}")
+        if Dh != 128 and Dh != 64:
             raise ValueError(f"head_dim {Dh} unsupported (64, 128)")
         if B < 1 or Hk < 1 or S < 1:
-            raise ValueError(f"empty cache {tuple(k.shape)}")
-        if self.v.shape != k.shape:
+            raise ValueError(f"empty cache {tuple(shape)}")
+        if v.shape != shape:
             raise ValueError("v shape must match k")
-        if k.dtype != torch.float8_e4m3fn or self.v.dtype != torch.float8_e4m3fn:
+        if k.dtype is not torch.float8_e4m3fn or v.dtype is not torch.float8_e4m3fn:
             raise ValueError("the codes are float8_e4m3fn tensors")
-        want = (B, Hk, -(-S // self.block))
-        for name, t in (("k_scale", ks), ("v_scale", self.v_scale)):
-            if tuple(t.shape) != want or t.dtype != torch.float32:
-                raise ValueError(f"{name} must be float32 {want}, got {t.dtype} {tuple(t.shape)}")
-        for t in (k, self.v, ks, self.v_scale):
-            if not t.is_cuda or t.device != k.device:
-                raise ValueError("the cache is CUDA tensors of one device (there is no CPU path)")
-            if not t.is_contiguous():
-                raise ValueError("the cache needs contiguous tensors")
-        self.struct = FsvdKv8(k.data_ptr(), self.v.data_ptr(), ks.data_ptr(), self.v_scale.data_ptr(), B, Hk, S, Dh, self.block)
+        want = (B, Hk, -(-S // block))
+        if ks.shape != want or vs.shape != want or ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
+            raise ValueError(f"k_scale and v_scale must be float32 {want}, got {ks.dtype} {tuple(ks.shape)} and {vs.dtype} {tuple(vs.shape)}")
+        self.index = index = k.get_device()
+        if index < 0 or not (index == v.get_device() == ks.get_device() == vs.get_device()):
+            raise ValueError("the cache is CUDA tensors of one device (there is no CPU path)")
+        if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+            raise ValueError("the cache needs contiguous tensors")
+        self.struct = FsvdKv8(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), B, Hk, S, Dh, block)
         self.ref = C.byref(self.struct)
 
     @classmethod

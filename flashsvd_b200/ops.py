@@ -294,8 +294,21 @@ def tp_decode_layer(dims: FsvdDims, layer: FsvdLayer, cos, sin, cache_seqlens, x
 
 
 # ---- operators for callers that drive the layers themselves: rotary positions, the 8-bit cache, the next token
-def _raw_stream(device: torch.device):
-    return torch.cuda.current_stream(device).cuda_stream
+# (These are calls of a few microseconds on the device: the checks are written for their cost.)
+_BF16, _F32, _F64, _I32 = torch.bfloat16, torch.float32, torch.float64, torch.int32
+_lib_handle = None
+
+
+def _library():
+    global _lib_handle
+    if _lib_handle is None:
+        _lib_handle = _lib.load()
+    return _lib_handle
+
+
+def _raw_stream(index: int) -> int:
+    """The current stream of a device as an integer."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class _SameDevice:
@@ -303,8 +316,8 @@ class _SameDevice:
 
     __slots__ = ("index", "was")
 
-    def __init__(self, device: torch.device):
-        self.index, self.was = device.index, None
+    def __init__(self, index: int):
+        self.index, self.was = index, None
 
     def __enter__(self):
         now = torch.cuda.current_device()
@@ -317,22 +330,46 @@ class _SameDevice:
             torch.cuda.set_device(self.was)
 
 
-def _want(name: str, t, dtype, device, shape=None, strided: bool = False):
-    """Checks one tensor argument; with `strided` only the last two dimensions have to be contiguous."""
+def _refuse(name: str, t, dtype, index: int, shape, strided: bool):
+    """Says what is wrong with a tensor argument that `_ok` did not take."""
     if not torch.is_tensor(t) or not t.is_cuda:
         raise ValueError(f"{name}: flashsvd_b200 ops need CUDA tensors (there is no CPU path)")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the call's other tensors on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors on cuda:{index}")
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    if strided:
-        if t.numel() and (t.stride(-1) != 1 and t.shape[-1] > 1 or t.stride(-2) != t.shape[-1] and t.shape[-2] > 1):
-            raise ValueError(f"{name}: heads and dimensions must be contiguous")
-    elif not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t
+    raise ValueError(f"{name}: heads and dimensions must be contiguous" if strided else f"{name} must be contiguous")
+
+
+def _ok(name: str, t, dtype, index: int, shape=None):
+    """A contiguous tensor of this type, device and shape; its address."""
+    if not (torch.is_tensor(t) and t.dtype is dtype and t.get_device() == index and (shape is None or t.shape == shape)
+            and t.is_contiguous()):
+        _refuse(name, t, dtype, index, shape, False)
+    return t.data_ptr()
+
+
+def _ok_strided(name: str, t, dtype, index: int, shape):
+    """As `_ok`, with any strides in front of the last two dimensions."""
+    if not (torch.is_tensor(t) and t.dtype is dtype and t.get_device() == index and t.shape == shape):
+        _refuse(name, t, dtype, index, shape, True)
+    if not t.is_contiguous() and t.numel():
+        H, D = shape[-2:]
+        st = t.stride()
+        if (st[-1] != 1 and D > 1) or (st[-2] != D and H > 1):
+            _refuse(name, t, dtype, index, shape, True)
+    return t.data_ptr()
+
+
+def _device_of(name: str, t, ndim: int, what: str) -> int:
+    """Index of the device of the argument that the others go by."""
+    if not torch.is_tensor(t) or not t.is_cuda:
+        raise ValueError(f"{name}: flashsvd_b200 ops need CUDA tensors (there is no CPU path)")
+    if t.ndim != ndim:
+        raise ValueError(f"{name} must be {what}, got {tuple(t.shape)}")
+    return t.get_device()
 
 
 def rope_qk(q, k, positions, inv_freq, *, interleaved=False, scale=1.0, q_out=None, k_out=None):
@@ -342,33 +379,36 @@ def rope_qk(q, k, positions, inv_freq, *, interleaved=False, scale=1.0, q_out=No
     in 64 bits), pairs are (i, i + len(inv_freq)), or (2i, 2i + 1) with ``interleaved``; cos and sin are multiplied by
     ``scale``; the other dimensions are copied.  bfloat16 or float32; tokens may be strided (slices of a packed
     projection).  q_out / k_out may be q / k themselves when those are contiguous."""
-    if q.ndim != 3:
-        raise ValueError(f"q must be [T, H, Dh], got {tuple(q.shape)}")
-    T, H, Dh = q.shape
-    dtype, dev = q.dtype, q.device
+    index = _device_of("q", q, 3, "[T, H, Dh]")
+    shape = q.shape
+    T, H, Dh = shape
+    dtype = q.dtype
     code = _dtype_code(dtype)
-    _want("q", q, dtype, dev, strided=True)
-    _want("positions", positions, torch.int32, dev, (T,))
+    qp = _ok_strided("q", q, dtype, index, shape)
+    pp = _ok("positions", positions, _I32, index, (T,))
+    fp = _ok("inv_freq", inv_freq, _F64, index)
     if inv_freq.ndim != 1:
         raise ValueError("inv_freq must be a vector")
-    _want("inv_freq", inv_freq, torch.float64, dev)
-    Hk = 0
+    Hk, kp, kop, ks = 0, None, None, 0
     if k is not None:
         if k.ndim != 3:
             raise ValueError(f"k must be [T, Hk, Dh], got {tuple(k.shape)}")
         Hk = k.shape[1]
-        _want("k", k, dtype, dev, (T, Hk, Dh), strided=True)
-        k_out = torch.empty((T, Hk, Dh), dtype=dtype, device=dev) if k_out is None else _want("k_out", k_out, dtype, dev, k.shape)
+        kp = _ok_strided("k", k, dtype, index, (T, Hk, Dh))
+        if k_out is None:
+            k_out = k.new_empty((T, Hk, Dh))
+        kop = _ok("k_out", k_out, dtype, index, (T, Hk, Dh))
+        ks = k.stride(0) if T > 1 else 0
     elif k_out is not None:
         raise ValueError("k_out without k")
-    q_out = torch.empty((T, H, Dh), dtype=dtype, device=dev) if q_out is None else _want("q_out", q_out, dtype, dev, q.shape)
+    if q_out is None:
+        q_out = q.new_empty(shape)
+    qop = _ok("q_out", q_out, dtype, index, shape)
     if T == 0:
         return q_out, k_out
-    with _SameDevice(dev):
-        check(_lib.load().fsvd_rope_qk(
-            q.data_ptr(), q.stride(0) if T > 1 else 0, None if k is None else k.data_ptr(), 0 if k is None or T < 2 else k.stride(0),
-            positions.data_ptr(), inv_freq.data_ptr(), 2 * inv_freq.shape[0], int(interleaved), float(scale), q_out.data_ptr(),
-            None if k is None else k_out.data_ptr(), T, H, Hk, Dh, code, _raw_stream(dev)))
+    with _SameDevice(index):
+        check(_library().fsvd_rope_qk(qp, q.stride(0) if T > 1 else 0, kp, ks, pp, fp, 2 * inv_freq.shape[0], 1 if interleaved else 0,
+                                      scale, qop, kop, T, H, Hk, Dh, code, _raw_stream(index)))
     return q_out, k_out
 
 
@@ -381,10 +421,10 @@ def make_kv8_workspace(batch, num_heads, num_kv_heads, head_dim, max_len, device
     return Workspace(torch.zeros(n, dtype=torch.uint8, device=device), n)
 
 
-def _ws_of(ws: Workspace, dev) -> Workspace:
-    if ws.buf.device != dev:
-        raise ValueError(f"the workspace is on {ws.buf.device}, the call's tensors on {dev}")
-    return ws
+def _scratch(ws: Workspace, index: int):
+    if ws.buf.get_device() != index:
+        raise ValueError(f"the workspace is on {ws.buf.device}, the call's tensors on cuda:{index}")
+    return ws.buf.data_ptr()
 
 
 def kv8_append(k, v, cache, cache_seqlens, ws: Workspace, *, new_lens=None, q=None, rotary=None, q_out=None):
@@ -394,84 +434,88 @@ def kv8_append(k, v, cache, cache_seqlens, ws: Workspace, *, new_lens=None, q=No
 
     cache_seqlens (int32 [B]) is not advanced.  A token that does not fit the cache is dropped and sets the workspace
     status, as in ``qkv_rope_append``.  Batch and tokens may be strided."""
-    st, dev = cache.struct, cache.device
+    st, index = cache.struct, cache.index
+    B, Hk, Dh = st.B, st.Hk, st.Dh
     if k.ndim != 4:
-        raise ValueError(f"k must be [B, L, {st.Hk}, {st.Dh}], got {tuple(k.shape)}")
-    B, L = k.shape[0], k.shape[1]
-    _want("k", k, torch.bfloat16, dev, (st.B, L, st.Hk, st.Dh), strided=True)
-    _want("v", v, torch.bfloat16, dev, k.shape, strided=True)
-    if v.stride() != k.stride():
-        v = v.contiguous()
-        k = k.contiguous()
-    _want("cache_seqlens", cache_seqlens, torch.int32, dev, (B,))
-    if new_lens is not None:
-        _want("new_lens", new_lens, torch.int32, dev, (B,))
-    H, qs = 0, (0, 0)
+        raise ValueError(f"k must be [B, L, {Hk}, {Dh}], got {tuple(k.shape)}")
+    L = k.shape[1]
+    shape = (B, L, Hk, Dh)
+    kp = _ok_strided("k", k, _BF16, index, shape)
+    vp = _ok_strided("v", v, _BF16, index, shape)
+    kst = k.stride()
+    if v.stride() != kst:
+        k, v = k.contiguous(), v.contiguous()
+        kp, vp, kst = k.data_ptr(), v.data_ptr(), k.stride()
+    sp = _ok("cache_seqlens", cache_seqlens, _I32, index, (B,))
+    np_ = None if new_lens is None else _ok("new_lens", new_lens, _I32, index, (B,))
+    fp, R, inter, scale = None, 0, 0, 1.0
     if rotary is not None:
-        if rotary.inv_freq.ndim != 1:
+        f = rotary.inv_freq
+        fp = _ok("inv_freq", f, _F64, index)
+        if f.ndim != 1:
             raise ValueError("inv_freq must be a vector")
-        _want("inv_freq", rotary.inv_freq, torch.float64, dev)
+        R, inter, scale = 2 * f.shape[0], 1 if rotary.interleaved else 0, rotary.scale
+    H, qp, qop, qs0, qs1 = 0, None, None, 0, 0
     if q is not None:
         if rotary is None:
             raise ValueError("q is passed to be rotated: rotary is missing")
         if q.ndim != 4:
             raise ValueError(f"q must be [B, L, H, Dh], got {tuple(q.shape)}")
         H = q.shape[2]
-        _want("q", q, torch.bfloat16, dev, (B, L, H, st.Dh), strided=True)
-        qs = (q.stride(0), q.stride(1))
+        qshape = (B, L, H, Dh)
+        qp = _ok_strided("q", q, _BF16, index, qshape)
+        qs0, qs1 = q.stride()[:2]
         if q_out is None:
-            q_out = torch.empty((B, L, H, st.Dh), dtype=torch.bfloat16, device=dev)
-        else:
-            _want("q_out", q_out, torch.bfloat16, dev, q.shape)
+            q_out = q.new_empty(qshape)
+        qop = _ok("q_out", q_out, _BF16, index, qshape)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    _ws_of(ws, dev)
+    wp = _scratch(ws, index)
     if L == 0:
         return q_out
-    with _SameDevice(dev):
-        check(_lib.load().fsvd_kv8_append(
-            cache.ref, k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), cache_seqlens.data_ptr(),
-            None if new_lens is None else new_lens.data_ptr(), None if q is None else q.data_ptr(), *qs,
-            None if q is None else q_out.data_ptr(), None if rotary is None else rotary.inv_freq.data_ptr(),
-            0 if rotary is None else 2 * rotary.inv_freq.shape[0], 0 if rotary is None else int(rotary.interleaved),
-            1.0 if rotary is None else float(rotary.scale), H, L, ws.ptr, ws.nbytes, _raw_stream(dev)))
+    with _SameDevice(index):
+        check(_library().fsvd_kv8_append(cache.ref, kp, vp, kst[0], kst[1], sp, np_, qp, qs0, qs1, qop, fp, R, inter, scale, H, L, wp,
+                                         ws.nbytes, _raw_stream(index)))
     return q_out
 
 
 def kv8_load(cache, start, length, *, cache_seqlens=None, seqlen_add=0, k_out=None, v_out=None):
     """Positions [start, start + length) of the cache as bfloat16 numbers: (k, v), each [B, Hk, length, Dh].  With
     ``cache_seqlens`` rows from cache_seqlens[b] + seqlen_add on are zeros."""
-    st, dev = cache.struct, cache.device
+    st, index = cache.struct, cache.index
     start, length = int(start), int(length)
     if start < 0 or length < 0 or start + length > st.S_max:
         raise ValueError(f"positions {start} + {length} are outside the cache ({st.S_max})")
     shape = (st.B, st.Hk, length, st.Dh)
-    if cache_seqlens is not None:
-        _want("cache_seqlens", cache_seqlens, torch.int32, dev, (st.B,))
-    k_out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if k_out is None else _want("k_out", k_out, torch.bfloat16, dev, shape)
-    v_out = torch.empty(shape, dtype=torch.bfloat16, device=dev) if v_out is None else _want("v_out", v_out, torch.bfloat16, dev, shape)
+    sp = None if cache_seqlens is None else _ok("cache_seqlens", cache_seqlens, _I32, index, (st.B,))
+    if k_out is None:
+        k_out = cache.k.new_empty(shape, dtype=_BF16)
+    if v_out is None:
+        v_out = cache.k.new_empty(shape, dtype=_BF16)
+    kp, vp = _ok("k_out", k_out, _BF16, index, shape), _ok("v_out", v_out, _BF16, index, shape)
     if length == 0:
         return k_out, v_out
-    with _SameDevice(dev):
-        check(_lib.load().fsvd_kv8_load(cache.ref, start, length, None if cache_seqlens is None else cache_seqlens.data_ptr(),
-                                        int(seqlen_add), k_out.data_ptr(), v_out.data_ptr(), _raw_stream(dev)))
+    with _SameDevice(index):
+        check(_library().fsvd_kv8_load(cache.ref, start, length, sp, int(seqlen_add), kp, vp, _raw_stream(index)))
     return k_out, v_out
 
 
 def flash_decode_kv8(q, cache, cache_seqlens, ws: Workspace, *, seqlen_add=0, scale=0.0, out=None):
     """``flash_decode`` over an 8-bit cache: q[B, H, Dh] bfloat16 against positions [0, cache_seqlens[b] + seqlen_add),
     scale <= 0 selects 1/sqrt(Dh); a sequence without positions gives zeros."""
-    st, dev = cache.struct, cache.device
+    st, index = cache.struct, cache.index
     if q.ndim != 3:
         raise ValueError(f"q must be [B, H, Dh], got {tuple(q.shape)}")
     H = q.shape[1]
-    _want("q", q, torch.bfloat16, dev, (st.B, H, st.Dh))
-    _want("cache_seqlens", cache_seqlens, torch.int32, dev, (st.B,))
-    out = torch.empty_like(q) if out is None else _want("out", out, torch.bfloat16, dev, q.shape)
-    _ws_of(ws, dev)
-    with _SameDevice(dev):
-        check(_lib.load().fsvd_flash_decode_kv8(cache.ref, q.data_ptr(), cache_seqlens.data_ptr(), int(seqlen_add), out.data_ptr(),
-                                                H, float(scale), ws.ptr, ws.nbytes, _raw_stream(dev)))
+    shape = (st.B, H, st.Dh)
+    qp = _ok("q", q, _BF16, index, shape)
+    sp = _ok("cache_seqlens", cache_seqlens, _I32, index, (st.B,))
+    if out is None:
+        out = torch.empty_like(q)
+    op = _ok("out", out, _BF16, index, shape)
+    wp = _scratch(ws, index)
+    with _SameDevice(index):
+        check(_library().fsvd_flash_decode_kv8(cache.ref, qp, sp, int(seqlen_add), op, H, scale, wp, ws.nbytes, _raw_stream(index)))
     return out
 
 
@@ -484,33 +528,32 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     those the ones with weight >= ``min_p`` (0: all).  The token is the first one in index order whose running mass
     exceeds uniforms[b] of the kept mass; probs is its share.  temperature <= 0 takes the largest logit.  Each setting
     is a number or a tensor with one value per row (float32; top_k int32)."""
-    if logits.ndim != 2:
-        raise ValueError(f"logits must be [B, V], got {tuple(logits.shape)}")
+    index = _device_of("logits", logits, 2, "[B, V]")
     B, V = logits.shape
-    dev = logits.device
     code = _dtype_code(logits.dtype)
-    if not logits.is_cuda:
-        raise ValueError("logits: flashsvd_b200 ops need CUDA tensors (there is no CPU path)")
     if V < 1:
         raise ValueError("logits of an empty vocabulary")
     if V > 1 and logits.stride(1) != 1:
         raise ValueError("logits: a row must be contiguous")
-    _want("uniforms", uniforms, torch.float32, dev, (B,))
-    ptrs, values = [], []
-    for name, x, dtype in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
-                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)):
-        if torch.is_tensor(x):
-            ptrs.append(_want(name, x, dtype, dev, (B,)).data_ptr())
-            values.append(0)
-        else:
-            ptrs.append(None)
-            values.append(int(x) if dtype == torch.int32 else float(x))
-    out = torch.empty(B, dtype=torch.int32, device=dev) if out is None else _want("out", out, torch.int32, dev, (B,))
-    probs_out = torch.empty(B, dtype=torch.float32, device=dev) if probs_out is None else _want("probs_out", probs_out, torch.float32, dev, (B,))
+    rows = (B,)
+    up = _ok("uniforms", uniforms, _F32, index, rows)
+    tp = kp = pp = mp = None
+    if torch.is_tensor(temperature):
+        tp, temperature = _ok("temperature", temperature, _F32, index, rows), 1.0
+    if torch.is_tensor(top_k):
+        kp, top_k = _ok("top_k", top_k, _I32, index, rows), 0
+    if torch.is_tensor(top_p):
+        pp, top_p = _ok("top_p", top_p, _F32, index, rows), 1.0
+    if torch.is_tensor(min_p):
+        mp, min_p = _ok("min_p", min_p, _F32, index, rows), 0.0
+    if out is None:
+        out = uniforms.new_empty(rows, dtype=_I32)
+    if probs_out is None:
+        probs_out = torch.empty_like(uniforms)
+    op, bp = _ok("out", out, _I32, index, rows), _ok("probs_out", probs_out, _F32, index, rows)
     if B == 0:
         return out, probs_out
-    with _SameDevice(dev):
-        check(_lib.load().fsvd_sample(
-            logits.data_ptr(), logits.stride(0) if B > 1 else V, code, uniforms.data_ptr(), *ptrs, *values, out.data_ptr(),
-            probs_out.data_ptr(), B, V, _raw_stream(dev)))
+    with _SameDevice(index):
+        check(_library().fsvd_sample(logits.data_ptr(), logits.stride(0) if B > 1 else V, code, up, tp, kp, pp, mp, temperature, top_k,
+                                     top_p, min_p, op, bp, B, V, _raw_stream(index)))
     return out, probs_out
