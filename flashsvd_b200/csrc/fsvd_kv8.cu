@@ -434,7 +434,7 @@ static Kv8Ws ws_layout(long long B, long long H, long long Hk, long long Dh) {
   Kv8Ws w;
   w.counters = 256;   // behind the status word (fsvd_workspace_status)
   w.part = w.counters + (size_t)((B * Hk * 4 + 255) / 256 * 256);
-  w.total = w.part + (size_t)kMaxCtas * sm_count() * 2 * (H / Hk) * (Dh + 2) * 4;
+  w.total = w.part + (size_t)kMaxCtas * sm_count() * 2 * (H / Hk) * (Dh + fsvd_kv8_attn::kPad) * 4;
   return w;
 }
 

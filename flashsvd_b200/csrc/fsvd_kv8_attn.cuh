@@ -5,13 +5,15 @@
 // tcgen05.mma kind::f8f6f4 multiplies e4m3 by e4m3 exactly and adds in 32 bits, so the codes go from TMA to the tensor
 // core as they lie in memory.  What is not e4m3 is written as a sum of e4m3 numbers and takes a column of the small
 // operand each: a query row is hi + lo / 16 (a bf16 number has 8 bits, an e4m3 number 4: nothing is lost above 2^-22 of
-// the row's largest), a weight is w0 + w1 / 16 + w2 / 256 + w3 / 4096, which is good to 2^-19 of itself and 2^-26 of the
+// the row's largest), a weight is w0 + w1 / 16 + w2 / 256 + w3 / 4096, which is good to 2^-17 of itself and 2^-24 of the
 // largest.  A tile is 128 tokens: S^T [128 tokens, 2 G] = K8 . q^T, then O^T [Dh, 4 G] = V8^T . w^T, where V8^T is the
 // tile as it lies, read along its other axis.  Scales are applied to the scores in 32 bits: the exponent of a weight is
 // s log2(e) + log2(vs), so that the weight carries its value's scale, and the denominator divides it out.
 //
 // A thread of the four softmax warps owns a token of S^T and a dimension of O^T; one more thread issues the copies, one
-// the products.  O^T is read back after every tile and summed in registers, where a new maximum rescales it.
+// the products.  O^T is read back after every tile and summed in registers, where a new maximum rescales it.  The
+// maximum that weights refer to is one that was, and is renewed when a score passes it by more than 2^4 = the room that the
+// codes are given: nearly every tile then needs one vote of the four warps instead of a maximum per head.
 //
 // The tiles of all (sequence, kv head) pairs form one list that is cut into equal parts, one per CTA, whatever the
 // lengths are; a pair that more than one CTA works on is merged, in the order of its parts, by the CTA that finishes it.
@@ -31,13 +33,15 @@ constexpr int kSoft = 128;      // threads of the softmax warps
 constexpr int kThreads = 192;
 constexpr int kPieces = 4;      // e4m3 numbers of a weight
 constexpr int kMaxGroup = 16;
+constexpr int kPad = 4;         // floats behind a head's partial sums
+constexpr float kRoom = 4.0f;   // log2 of how far a score may pass the maximum that weights refer to
 
 struct Args {
   const float *k_scale, *v_scale;
   const __nv_bfloat16* q;
   __nv_bfloat16* out;
   const int* seqlens;
-  float* part;       // [CTAs][2][G][Dh + 2]: partial sums, maximum, denominator
+  float* part;       // [CTAs][2][G][Dh + kPad]: partial sums, maximum, denominator
   int* counters;     // [B * Hk], zero between launches
   int* status;
   long long wait_limit;
@@ -65,15 +69,22 @@ __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint3
       ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// e4m3 x e4m3 -> fp32, M = 128, N columns; A along its rows (K-major) or along its columns (transposed)
-__device__ __forceinline__ uint32_t idesc_f8(int N, bool a_transposed) {
-  return (1u << 4) | ((a_transposed ? 1u : 0u) << 15) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+// e4m3 x e4m3 -> fp32, M = 128, N columns; both operands along their rows (K-major) or along their columns (transposed)
+__device__ __forceinline__ uint32_t idesc_f8(int N, bool transposed) {
+  return (1u << 4) | ((transposed ? 3u : 0u) << 15) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
 // Operand of rows of ROW bytes (64 or 128) under the swizzle of that span; eight rows are 8 ROW bytes.  The stride
 // between spans is zero: a transposed operand of 64 rows repeats them as rows 64..127 (which nobody reads).
 template <int ROW>
 __device__ __forceinline__ uint64_t desc_f8(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(8 * ROW >> 4) << 32) | (1ull << 46) | ((ROW == 128 ? 2ull : 4ull) << 61);
+}
+// The weights: 128 rows (tokens) of N bytes (columns), read along the columns; rows of 32 and 64 bytes under the swizzle
+// of that span.
+template <int N>
+__device__ __forceinline__ uint64_t desc_weights(uint32_t addr) {
+  const uint64_t at = (uint64_t)((addr >> 4) & 0x3fffu) | (1ull << 46);
+  return N == 16 ? at | (8ull << 16) | (8ull << 32) : at | ((uint64_t)(8 * N >> 4) << 32) | ((N == 32 ? 6ull : 4ull) << 61);
 }
 // byte c of row r of such an operand
 template <int ROW>
@@ -151,6 +162,40 @@ __device__ __forceinline__ void tm_ld<64>(uint32_t taddr, float* v) {
   tm_ld<32>(taddr + 32, v + 32);
 }
 
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Whether any thread of the softmax warps says so.
+__device__ __forceinline__ bool soft_any(bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)x)
+      : "memory");
+  return r != 0;
+}
+// Two fp32 numbers of at most 256, given 16 times, as four e4m3 codes each (x in the low byte of a pair): each code is the
+// nearest to what the ones before leave, times 16.  What the first one leaves is kept as a 16-bit number of 11 bits.
+__device__ __forceinline__ void four_codes(float x16, float y16, uint32_t (&c)[4]) {
+  c[0] = __nv_cvt_float2_to_fp8x2(make_float2(x16 * 0.0625f, y16 * 0.0625f), __NV_SATFINITE, __NV_E4M3);
+  const __half2_raw h0 = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c[0], __NV_E4M3);
+  const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+  __half2 r = __floats2half2_rn(fmaf(f0.x, -16.0f, x16), fmaf(f0.y, -16.0f, y16));
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    c[i] = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&r), __NV_SATFINITE, __NV_E4M3);
+    if (i < 3) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c[i], __NV_E4M3);
+      r = __hmul2(__hsub2(r, *reinterpret_cast<const __half2*>(&h)), __float2half2_rn(16.0f));
+    }
+  }
+}
 // Two fp32 numbers -> their nearest e4m3 codes (x in the low byte), and what the codes stand for.
 __device__ __forceinline__ uint32_t to_codes(float x, float y, float& dx, float& dy) {
   const uint32_t c = __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
@@ -165,7 +210,7 @@ __device__ __forceinline__ uint32_t to_codes(float x, float y, float& dx, float&
 struct Cursor {
   const int* seqlens;
   int add, S_max, Hk, B;
-  int b, hk, tiles, n;       // tiles of the sequence, positions of the sequence
+  int b, hk, tiles, n;       // sequence, kv head, the sequence's tiles and positions
   int tile, left;            // next tile, tiles left for this CTA
   __device__ __forceinline__ int positions(int i) const {
     return (int)min(max((long long)seqlens[i] + add, 0ll), (long long)S_max);
@@ -201,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
   __shared__ __align__(8) unsigned long long kv_full[S::kStages], kv_empty[S::kStages], s_full[2], w_full[2], o_full[2], q_full[2];
   __shared__ uint32_t tmem_slot;
   __shared__ float qfac[2][GP], wmax[2][4][GP], red[4][GP];
-  __shared__ int start_b, start_hk, start_tile, last_sh, giveup_sh;
+  __shared__ int start_b, start_hk, start_tile, start_n, last_sh, giveup_sh;
   __shared__ long long total_sh, base_sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.G;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -259,6 +304,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
         start_b = b0 + lane;
         start_hk = (int)(off / t);
         start_tile = (int)(off % t);
+        start_n = cur.positions(b0 + lane);
         base_sh = before + inc - x;   // list index of the sequence's first tile
       }
       found = __any_sync(0xffffffffu, mine);
@@ -271,8 +317,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
   const long long total = total_sh, per = (total + gridDim.x - 1) / gridDim.x, w0 = per * blockIdx.x;
   cur.left = (int)max(0ll, min(per, total - w0));
   if (cur.left > 0) {
-    cur.b = start_b; cur.hk = start_hk; cur.tile = start_tile;
-    cur.enter();
+    cur.b = start_b; cur.hk = start_hk; cur.tile = start_tile; cur.n = start_n;
+    cur.tiles = (cur.n + kTile - 1) / kTile;
   }
 
   if (warp == 4) {   // ---- copies
@@ -315,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
         const uint32_t v = smem_u32(smem + st * 2 * S::kHalf + S::kHalf), w = smem_u32(ws + buf * S::kW);
 #pragma unroll
         for (int k = 0; k < kTile / 32; ++k)
-          mma_f8(tmem + 2 * S::kNq + buf * S::kNw, desc_f8<DH>(v + 32 * DH * k), desc_f8<128>(w + 32 * k), iw, k > 0);
+          mma_f8(tmem + 2 * S::kNq + buf * S::kNw, desc_f8<DH>(v + 32 * DH * k), desc_weights<S::kNw>(w + 32 * S::kNw * k), iw, k > 0);
         tc_commit(smem_u32(&o_full[buf]));
         tc_commit(smem_u32(&kv_empty[st]));
       };
@@ -340,17 +386,35 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
       if (!*giveup) weigh(n - 1);
     }
   } else {   // ---- softmax
-    // the query rows of (b, hk) as hi + lo / 16, scaled to a largest magnitude in [128, 256)
-    auto build_q = [&](int b, int hk, int which) {
-      constexpr int D = DH / 32;
+    // The query rows of a pair as hi + lo / 16, scaled to a largest magnitude in [128, 256): fetched while the pair before is
+    // begun, written when its first tile is through.
+    constexpr int D = DH / 32, R = (GP + 3) / 4;   // numbers of a lane, rows of a warp
+    uint32_t rows[R][D / 2];
+    auto fetch_q = [&](int b, int hk) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (warp + 4 * r < G) {
+          const __nv_bfloat16* row = a.q + (((size_t)b * a.Hk + hk) * G + warp + 4 * r) * DH + lane * D;
+          if constexpr (D == 4) {
+            const uint2 w = *reinterpret_cast<const uint2*>(row);
+            rows[r][0] = w.x;
+            rows[r][D / 2 - 1] = w.y;
+          } else {
+            rows[r][0] = *reinterpret_cast<const uint32_t*>(row);
+          }
+        }
+    };
+    auto build_q = [&](int which) {
       uint8_t* dst = qs + which * S::kQ;
-      for (int g = warp; g < G; g += 4) {
-        const __nv_bfloat16* row = a.q + (((size_t)b * a.Hk + hk) * G + g) * DH + lane * D;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int g = warp + 4 * r;
+        if (g >= G) break;
         float x[D], top = 0.0f;
         bool fine = true;
 #pragma unroll
         for (int e = 0; e < D; ++e) {
-          x[e] = __bfloat162float(row[e]);
+          x[e] = __uint_as_float((e & 1) ? rows[r][e / 2] & 0xffff0000u : rows[r][e / 2] << 16);
           top = fmaxf(top, fabsf(x[e]));
           fine = fine && isfinite(x[e]);
         }
@@ -388,19 +452,24 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
     long long seq_base = cur.left > 0 ? base_sh : 0;
     int j = 0, seg = 0;
     if (cur.left > 0) {
-      build_q(cur.b, cur.hk, 0);
+      fetch_q(cur.b, cur.hk);
+      build_q(0);
       soft_sync();
     }
     while (cur.left > 0) {
       const int run = cur.run(), first = cur.tile, bh = cur.b * a.Hk + cur.hk, n = cur.n, ntiles = cur.tiles, hk = cur.hk;
+      cur.next(run);
+      const bool more = cur.left > 0;   // (`cur` is the next pair from here on)
+      if (more) fetch_q(cur.b, cur.hk);
       const long long list0 = seq_base + (long long)hk * ntiles;   // list index of the pair's first tile
       const float* ksc = a.k_scale + (size_t)bh * a.nb;
       const float* vsc = a.v_scale + (size_t)bh * a.nb;
-      float m[GP], l[GP], acc[GP], corr[GP];
+      float m[GP], l[GP], acc[GP], corr[GP], qf[GP];   // l and acc: 256 and 16 times the sums
 #pragma unroll
       for (int g = 0; g < GP; ++g) {
         m[g] = -INFINITY;
         l[g] = acc[g] = 0.0f;
+        qf[g] = qfac[seg & 1][g];
       }
       auto collect = [&](int jj, const float (&c)[GP]) {   // acc = acc c + O(jj)
         const int buf = jj & 1;
@@ -424,59 +493,79 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
       for (int i = 0; i < run; ++i, ++j) {
         const int t = first + i, buf = j & 1;
         const bool valid = t * kTile + tid < n;
-        const float kf = ks, lv = log2f(vs), inv = valid ? 1.0f / vs : 0.0f;
+        const float kf = ks, lv = __log2f(vs), inv = valid ? __fdividef(1.0f, vs) : 0.0f;
         if (i + 1 < run) scales(t + 1);
         wait_bar(smem_u32(&s_full[buf]), (j >> 1) & 1, giveup, a.status, a.wait_limit, DS_BARRIER_TIMEOUT);
         tc_fence_after();
         float s[2 * GP], e[GP];
         tm_ld<2 * GP>(tmem + buf * S::kNq + lanes, s);
+        bool higher = false;
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
-          const float x = (s[GP + g] * 0.0625f + s[g]) * (kf * qfac[seg & 1][g]) + lv;
+          const float x = fmaf(fmaf(s[GP + g], 0.0625f, s[g]), kf * qf[g], lv);
           e[g] = valid ? x : -INFINITY;
-          const float top = warp_max(e[g]);
-          if (lane == 0) wmax[buf][warp][g] = top;
+          higher = higher || (g < G && e[g] > m[g] + kRoom);
         }
         if (!valid) {   // the last tile: a row behind the end may hold anything
           uint4* row = reinterpret_cast<uint4*>(smem + (j % S::kStages) * 2 * S::kHalf + S::kHalf + tid * DH);
 #pragma unroll
           for (int x = 0; x < DH / 16; ++x) row[x] = make_uint4(0u, 0u, 0u, 0u);
         }
-        soft_sync();
         float prev[GP];   // rescaling of the tile before, which is collected below
-        uint8_t* dst = ws + buf * S::kW;
 #pragma unroll
         for (int g = 0; g < GP; ++g) {
-          const float top = fmaxf(fmaxf(wmax[buf][0][g], wmax[buf][1][g]), fmaxf(wmax[buf][2][g], wmax[buf][3][g]));
-          const float mn = fmaxf(m[g], top);
           prev[g] = corr[g];
-          corr[g] = m[g] == mn ? 1.0f : exp2f(m[g] - mn);
-          m[g] = mn;
-          e[g] = valid ? exp2f(e[g] - mn) : 0.0f;
-          l[g] = l[g] * corr[g] + e[g] * inv;
-          e[g] *= 256.0f;
+          corr[g] = 1.0f;
+        }
+        if (soft_any(higher)) {
+#pragma unroll
+          for (int g = 0; g < GP; ++g) {
+            const float top = warp_max(e[g]);
+            if (lane == 0) wmax[buf][warp][g] = top;
+          }
+          soft_sync();
+#pragma unroll
+          for (int g = 0; g < GP; ++g) {
+            const float top = fmaxf(fmaxf(wmax[buf][0][g], wmax[buf][1][g]), fmaxf(wmax[buf][2][g], wmax[buf][3][g]));
+            const float mn = fmaxf(m[g], top);
+            corr[g] = m[g] == mn ? 1.0f : ex2(m[g] - mn);
+            m[g] = mn;
+            l[g] *= corr[g];
+          }
         }
 #pragma unroll
-        for (int g = 0; g < GP; g += 2) {
-          float x = e[g], y = GP > 1 ? e[(g + 1) % GP] : 0.0f;
+        for (int g = 0; g < GP; ++g) {
+          e[g] = valid ? ex2(e[g] - m[g] + 8.0f) : 0.0f;   // 256 times the weight, which is at most 2^kRoom
+          l[g] = fmaf(e[g], inv, l[g]);
+        }
+        {
+          uint32_t c[(GP + 1) / 2][4];   // pairs of heads
 #pragma unroll
-          for (int p = 0; p < kPieces; ++p) {
-            float dx, dy;
-            const uint32_t c = to_codes(x, y, dx, dy);
-            dst[swizzled<128>(p * GP + g, tid)] = (uint8_t)(c & 0xffu);
-            if (GP > 1) dst[swizzled<128>(p * GP + g + 1, tid)] = (uint8_t)(c >> 8);
-            x = (x - dx) * 16.0f;
-            y = (y - dy) * 16.0f;
+          for (int g = 0; g < GP; g += 2) four_codes(e[g], GP > 1 ? e[(g + 1) % GP] : 0.0f, c[g / 2]);
+          uint8_t* dst = ws + buf * S::kW + tid * S::kNw;
+          if constexpr (GP == 1) {
+            *reinterpret_cast<uint32_t*>(dst) = __byte_perm(__byte_perm(c[0][0], c[0][1], 0x0040), __byte_perm(c[0][2], c[0][3], 0x0040), 0x5410);
+          } else if constexpr (GP == 2) {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(c[0][0] | (c[0][1] << 16), c[0][2] | (c[0][3] << 16));
+          } else {
+            uint32_t w[GP];   // codes of four heads each, piece by piece
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+#pragma unroll
+              for (int g = 0; g < GP / 4; ++g) w[p * (GP / 4) + g] = c[2 * g][p] | (c[2 * g + 1][p] << 16);
+            const int x = S::kNw == 32 ? (tid >> 2) & 1 : S::kNw == 64 ? (tid >> 1) & 3 : 0;
+#pragma unroll
+            for (int i16 = 0; i16 < GP / 4; ++i16)
+              *reinterpret_cast<uint4*>(dst + ((i16 ^ x) << 4)) = make_uint4(w[4 * i16], w[4 * i16 + 1], w[4 * i16 + 2], w[4 * i16 + 3]);
           }
         }
         tc_fence_before();
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(smem_u32(&w_full[buf]));
+        if (i == 0 && more) build_q((seg + 1) & 1);   // (the products of the pair before the last are done with that buffer)
         if (i > 0) collect(j - 1, prev);
       }
-      cur.next(run);
       if (hk == a.Hk - 1 && first + run == ntiles) seq_base += (long long)a.Hk * ntiles;
-      if (cur.left > 0) build_q(cur.b, cur.hk, (seg + 1) & 1);
       collect(j - 1, corr);
       // denominators
 #pragma unroll
@@ -489,19 +578,19 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
 #pragma unroll
       for (int g = 0; g < GP; ++g) l[g] = (red[0][g] + red[1][g]) + (red[2][g] + red[3][g]);
       __nv_bfloat16* out = a.out + (size_t)bh * G * DH + tid;
-      const int rec = DH + 2;
+      constexpr int rec = DH + kPad;
       if (run == ntiles) {
         if (owns) {
 #pragma unroll
           for (int g = 0; g < GP; ++g)
-            if (g < G) out[g * DH] = __float2bfloat16_rn(acc[g] * (1.0f / 256.0f) / l[g]);
+            if (g < G) out[g * DH] = __float2bfloat16_rn(acc[g] * 16.0f / l[g]);
         }
       } else {
         float* rp = a.part + ((size_t)blockIdx.x * 2 + (seg > 0)) * G * rec;
 #pragma unroll
         for (int g = 0; g < GP; ++g)
           if (g < G) {
-            if (owns) rp[g * rec + tid] = acc[g] * (1.0f / 256.0f);
+            if (owns) rp[g * rec + tid] = acc[g] * 16.0f;   // (256 times the sum, as l)
             if (tid == 0) *reinterpret_cast<float2*>(rp + g * rec + DH) = make_float2(m[g], l[g]);
           }
         __threadfence();
@@ -511,18 +600,63 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
         soft_sync();
         if (last_sh) {
           __threadfence();
-          for (int g = 0; g < G; ++g) {
-            float mm = -INFINITY, ll = 0.0f, o = 0.0f;
-            for (int c = c0; c <= c1; ++c) {
-              const float* r = a.part + (((size_t)c * 2 + (per * c < list0)) * G + g) * rec;
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(r + DH));
-              const float x = owns ? __ldcg(r + tid) : 0.0f;
-              const float mn = fmaxf(mm, ml.x), f0 = mm == mn ? 1.0f : exp2f(mm - mn), f1 = ml.x == mn ? 1.0f : exp2f(ml.x - mn);
+          // maximum and denominator of each head: a warp to a head, its lanes over the parts
+          const float* base = a.part;
+          auto record = [&](int c) { return base + ((size_t)c * 2 + (per * c < list0)) * G * rec; };
+          for (int g = warp; g < G; g += 4) {
+            float mm = -INFINITY, ll = 0.0f;
+            for (int c = c0 + lane; c <= c1; c += 32) {
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(record(c) + g * rec + DH));
+              const float mn = fmaxf(mm, ml.x);
+              ll = ll * (mm == mn ? 1.0f : ex2(mm - mn)) + ml.y * (ml.x == mn ? 1.0f : ex2(ml.x - mn));
               mm = mn;
-              ll = ll * f0 + ml.y * f1;
-              o = o * f0 + x * f1;
             }
-            if (owns) out[g * DH] = __float2bfloat16_rn(o / ll);
+            const float top = warp_max(mm);
+            ll = mm == top ? ll : ll * ex2(mm - top);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+            if (lane == 0) {
+              red[0][g] = top;
+              red[1][g] = ll;
+            }
+          }
+          soft_sync();
+          // four dimensions to a thread; where there are fewer of those than threads, the parts are shared out too and their
+          // sums added in order
+          const int items = G * (DH / 4), shares = max(1, kSoft / items);
+          float4* sums = reinterpret_cast<float4*>(ws);   // (no weights are on their way)
+          for (int x = tid; x < items * shares; x += kSoft) {
+            const int item = x % items, share = x / items, g = item / (DH / 4), d = item % (DH / 4) * 4;
+            const float top = red[0][g];
+            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+            for (int c = c0 + share; c <= c1; c += shares) {
+              const float* r = record(c) + g * rec;
+              const float mc = __ldcg(r + DH);
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(r + d));
+              const float f = mc == top ? 1.0f : ex2(mc - top);
+              o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+            }
+            if (shares > 1) sums[x] = o;
+            else {
+              const float den = red[1][g];
+              *reinterpret_cast<uint2*>(a.out + ((size_t)bh * G + g) * DH + d) =
+                  make_uint2(pack_bf16(o.x / den, o.y / den), pack_bf16(o.z / den, o.w / den));
+            }
+          }
+          if (shares > 1) {
+            soft_sync();
+            if (tid < items) {
+              const int g = tid / (DH / 4), d = tid % (DH / 4) * 4;
+              float4 o = sums[tid];
+              for (int x = 1; x < shares; ++x) {
+                const float4 v = sums[tid + x * items];
+                o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+              }
+              const float den = red[1][g];
+              *reinterpret_cast<uint2*>(a.out + ((size_t)bh * G + g) * DH + d) =
+                  make_uint2(pack_bf16(o.x / den, o.y / den), pack_bf16(o.z / den, o.w / den));
+            }
           }
           if (tid == 0) a.counters[bh] = 0;
         }
