@@ -470,7 +470,7 @@ static int launch_attn(const CUtensorMap& km, const CUtensorMap& vm, const fsvd_
   static_assert(S::kCtas <= kMaxCtas);
   const long long tiles = (long long)a.B * a.Hk * ((a.S_max + fsvd_kv8_attn::kTile - 1) / fsvd_kv8_attn::kTile);
   const unsigned grid = (unsigned)std::min<long long>(tiles, (long long)S::kCtas * sm_count());
-  return launch(fsvd_kv8_attn::attn_kernel<DH, GP>, dim3(grid), fsvd_kv8_attn::kThreads, S::kSmem, stream, km, vm, a);
+  return launch(fsvd_kv8_attn::attn_kernel<DH, GP>, dim3(grid), S::kThreads, S::kSmem, stream, km, vm, a);
 }
 template <int DH>
 static int launch_attn(const CUtensorMap& km, const CUtensorMap& vm, const fsvd_kv8_attn::Args& a, void* stream) {

@@ -29,8 +29,7 @@ using namespace fsvd_tile;
 
 constexpr int kTile = 128;      // tokens
 constexpr int kBox = 32;        // tokens of a TMA box: a short last tile is fetched in as many as it needs
-constexpr int kSoft = 128;      // threads of the softmax warps
-constexpr int kThreads = 192;
+constexpr int kSoft = 128;      // threads of a softmax group
 constexpr int kPieces = 4;      // e4m3 numbers of a weight
 constexpr int kMaxGroup = 16;
 constexpr int kPad = 4;         // floats behind a head's partial sums
@@ -51,8 +50,14 @@ struct Args {
 
 template <int DH, int GP>
 struct Shape {
-  static constexpr int kCtas = GP <= 4 ? 3 : GP <= 8 ? 2 : 1;           // per SM
-  static constexpr int kStages = (GP <= 4 ? 2 : GP <= 8 ? 3 : 5) * (128 / DH);
+  // Heads are shared out to groups of four softmax warps, four heads each: with 8 heads in one group a tile took 1.4 times as
+  // long as its bytes.
+  static constexpr int kGroups = GP > 4 ? GP / 4 : 1, kHeads = GP / kGroups;
+  static constexpr int kThreads = kSoft * kGroups + 64;
+  // CTAs of an SM, and tiles that a CTA has under way.  32 sequences x 32 heads of 128 x 2048 tokens: two CTAs of three tiles
+  // 83 us, three of two 94; heads of 64, 128 ragged sequences: three CTAs of four tiles 41 us, two of six 48.
+  static constexpr int kCtas = GP > 8 ? 1 : DH == 64 && GP <= 4 ? 3 : 2;
+  static constexpr int kStages = GP > 8 ? 5 * (128 / DH) : DH == 128 ? 3 : GP <= 4 ? 4 : 6;
   static constexpr int kNq = 2 * GP < 16 ? 16 : 2 * GP;                 // columns of S
   static constexpr int kNw = kPieces * GP < 16 ? 16 : kPieces * GP;     // columns of O
   static constexpr int kCols = 2 * (kNq + kNw) <= 64 ? 64 : 2 * (kNq + kNw) <= 128 ? 128 : 256;
@@ -101,7 +106,9 @@ __device__ __forceinline__ void tma_box_3d(uint32_t dst, const void* tmap, int x
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// Barriers: of the threads of one softmax group (its number), of all softmax threads.
+__device__ __forceinline__ void group_sync(int group) { asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory"); }
+__device__ __forceinline__ void soft_sync(int threads) { asm volatile("bar.sync 8, %0;" ::"r"(threads) : "memory"); }
 __device__ __forceinline__ float warp_max(float x) {
   float r;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
@@ -167,16 +174,16 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// Whether any thread of the softmax warps says so.
-__device__ __forceinline__ bool soft_any(bool x) {
+// Whether any thread of a softmax group says so.
+__device__ __forceinline__ bool group_any(bool x, int group) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, 1, 128, p;\n\t"
+      "bar.red.or.pred q, %2, 128, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"((uint32_t)x)
+      : "r"((uint32_t)x), "r"(group + 1)
       : "memory");
   return r != 0;
 }
@@ -238,16 +245,19 @@ struct Cursor {
 };
 
 template <int DH, int GP>
-__global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas) attn_kernel(const __grid_constant__ CUtensorMap kmap,
                                                                              const __grid_constant__ CUtensorMap vmap,
                                                                              const Args a) {
   using S = Shape<DH, GP>;
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) unsigned long long kv_full[S::kStages], kv_empty[S::kStages], s_full[2], w_full[2], o_full[2], q_full[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ float qfac[2][GP], wmax[2][4][GP], red[4][GP];
+  __shared__ float qfac[2][GP], wmax[2][4][GP], red2[2][4][GP];
   __shared__ int start_b, start_hk, start_tile, start_n, last_sh, giveup_sh;
-  __shared__ long long total_sh, base_sh;
+  __shared__ int per_sh, total_sh, base_sh;
+  struct Part { int bh, tiles, list; };   // of a pair: which, its tiles, where they begin in the list
+  __shared__ Part part_of[2];
+  constexpr int NG = S::kGroups, GH = S::kHeads, kCopy = 4 * NG, kMma = kCopy + 1;   // (warps)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.G;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* qs = smem + S::kStages * 2 * S::kHalf;
@@ -256,19 +266,22 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
 
   if (tid == 0) {
     giveup_sh = 0;
+    part_of[0].tiles = part_of[1].tiles = 0;
     for (int i = 0; i < S::kStages; ++i) {
       mbar_init(smem_u32(&kv_full[i]), 1);
       mbar_init(smem_u32(&kv_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&s_full[i]), 1);
-      mbar_init(smem_u32(&w_full[i]), kSoft);
+      mbar_init(smem_u32(&w_full[i]), kSoft * NG);
       mbar_init(smem_u32(&o_full[i]), 1);
-      mbar_init(smem_u32(&q_full[i]), kSoft);
+      mbar_init(smem_u32(&q_full[i]), kSoft * NG);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 5) tc_alloc(smem_u32(&tmem_slot), S::kCols);
+  if (warp == kCopy && lane < 2)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(lane ? reinterpret_cast<uint64_t>(&vmap) : reinterpret_cast<uint64_t>(&kmap)) : "memory");
+  if (warp == kMma) tc_alloc(smem_u32(&tmem_slot), S::kCols);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -279,49 +292,59 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
   Cursor cur;
   cur.seqlens = a.seqlens; cur.add = a.seqlen_add; cur.S_max = a.S_max; cur.Hk = a.Hk; cur.B = a.B;
   if (warp == 0) {
-    long long total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-      long long x = b0 + lane < a.B ? (long long)((cur.positions(b0 + lane) + kTile - 1) / kTile) * a.Hk : 0;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-      total += x;
-    }
-    const long long per = (total + gridDim.x - 1) / gridDim.x, w0 = per * blockIdx.x;
-    long long before = 0;
-    int found = 0;
-    for (int b0 = 0; b0 < a.B && !found && w0 < total; b0 += 32) {
-      const int t = b0 + lane < a.B ? (cur.positions(b0 + lane) + kTile - 1) / kTile : 0;
-      const long long x = (long long)t * a.Hk;
-      long long inc = x;
+    auto entries = [&](int i, int& n, int& t) -> int {   // of sequence i
+      n = i < a.B ? cur.positions(i) : 0;
+      t = (n + kTile - 1) / kTile;
+      return t * a.Hk;   // (a list of 2^31 tiles would stand for more memory than there is)
+    };
+    auto prefix = [&](int x) {
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += y;
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
       }
+      return x;
+    };
+    int n, t;
+    const int x0 = entries(lane, n, t), inc0 = prefix(x0);   // the first 32 sequences, often all
+    int total = __shfl_sync(0xffffffffu, inc0, 31);
+    for (int b0 = 32; b0 < a.B; b0 += 32) {
+      int n1, t1;
+      total += __reduce_add_sync(0xffffffffu, entries(b0 + lane, n1, t1));
+    }
+    const int grid = gridDim.x, per = (total + grid - 1) / grid, w0 = per * blockIdx.x;
+    int before = 0, x = x0, inc = inc0;
+    for (int b0 = 0; w0 < total;) {
       const bool mine = w0 >= before + inc - x && w0 < before + inc;
       if (mine) {
-        const long long off = w0 - (before + inc - x);
+        const int off = w0 - (before + inc - x);
         start_b = b0 + lane;
-        start_hk = (int)(off / t);
-        start_tile = (int)(off % t);
-        start_n = cur.positions(b0 + lane);
+        start_hk = off / t;
+        start_tile = off - off / t * t;
+        start_n = n;
         base_sh = before + inc - x;   // list index of the sequence's first tile
       }
-      found = __any_sync(0xffffffffu, mine);
+      b0 += 32;
+      if (__any_sync(0xffffffffu, mine) || b0 >= a.B) break;
       before += __shfl_sync(0xffffffffu, inc, 31);
+      x = entries(b0 + lane, n, t);
+      inc = prefix(x);
     }
-    if (lane == 0) total_sh = total;
+    if (lane == 0) {
+      total_sh = total;
+      per_sh = per;
+    }
   }
   __syncthreads();
   const uint32_t tmem = tmem_slot;
-  const long long total = total_sh, per = (total + gridDim.x - 1) / gridDim.x, w0 = per * blockIdx.x;
-  cur.left = (int)max(0ll, min(per, total - w0));
+  const int per = per_sh;
+  cur.left = max(0, min(per, total_sh - per * (int)blockIdx.x));
   if (cur.left > 0) {
     cur.b = start_b; cur.hk = start_hk; cur.tile = start_tile; cur.n = start_n;
     cur.tiles = (cur.n + kTile - 1) / kTile;
   }
 
-  if (warp == 4) {   // ---- copies
+  if (warp == kCopy) {   // ---- copies
     if (lane == 0 && cur.left > 0) {
       int j = 0;
       while (cur.left > 0) {
@@ -349,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
         wait_bar(smem_u32(&kv_empty[i % S::kStages]), (i / S::kStages) & 1, giveup, a.status, a.wait_limit, DS_COPY_TIMEOUT);
       }
     }
-  } else if (warp == 5) {   // ---- products
+  } else if (warp == kMma) {   // ---- products
     if (lane == 0 && cur.left > 0) {
       const uint32_t iq = idesc_f8(S::kNq, false), iw = idesc_f8(S::kNw, true);
       const int n = cur.left;
@@ -388,33 +411,32 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
   } else {   // ---- softmax
     // The query rows of a pair as hi + lo / 16, scaled to a largest magnitude in [128, 256): fetched while the pair before is
     // begun, written when its first tile is through.
-    constexpr int D = DH / 32, R = (GP + 3) / 4;   // numbers of a lane, rows of a warp
-    uint32_t rows[R][D / 2];
+    const int group = warp >> 2, tl = tid & (kSoft - 1), wl = warp & 3;   // thread and warp within the group
+    const int head0 = group * GH;                                          // its heads
+    constexpr int D = DH / 32;   // numbers of a lane; a warp takes a row
+    static_assert(GP <= 4 * NG);
+    uint32_t rows[D / 2];
     auto fetch_q = [&](int b, int hk) {
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (warp + 4 * r < G) {
-          const __nv_bfloat16* row = a.q + (((size_t)b * a.Hk + hk) * G + warp + 4 * r) * DH + lane * D;
-          if constexpr (D == 4) {
-            const uint2 w = *reinterpret_cast<const uint2*>(row);
-            rows[r][0] = w.x;
-            rows[r][D / 2 - 1] = w.y;
-          } else {
-            rows[r][0] = *reinterpret_cast<const uint32_t*>(row);
-          }
+      if (warp < G) {
+        const __nv_bfloat16* row = a.q + (((size_t)b * a.Hk + hk) * G + warp) * DH + lane * D;
+        if constexpr (D == 4) {
+          const uint2 w = *reinterpret_cast<const uint2*>(row);
+          rows[0] = w.x;
+          rows[D / 2 - 1] = w.y;
+        } else {
+          rows[0] = *reinterpret_cast<const uint32_t*>(row);
         }
+      }
     };
     auto build_q = [&](int which) {
-      uint8_t* dst = qs + which * S::kQ;
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int g = warp + 4 * r;
-        if (g >= G) break;
+      if (warp < G) {
+        const int g = warp;
+        uint8_t* dst = qs + which * S::kQ;
         float x[D], top = 0.0f;
         bool fine = true;
 #pragma unroll
         for (int e = 0; e < D; ++e) {
-          x[e] = __uint_as_float((e & 1) ? rows[r][e / 2] & 0xffff0000u : rows[r][e / 2] << 16);
+          x[e] = __uint_as_float((e & 1) ? rows[e / 2] & 0xffff0000u : rows[e / 2] << 16);
           top = fmaxf(top, fabsf(x[e]));
           fine = fine && isfinite(x[e]);
         }
@@ -433,8 +455,8 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
           lo |= cl << (8 * e);
         }
         if (!fine) hi = lo = 0x7f7f7f7fu;   // a query that is not finite gives no number
-        uint8_t* p0 = dst + swizzled<DH>(g, lane * D);
-        uint8_t* p1 = dst + swizzled<DH>(GP + g, lane * D);
+        uint8_t* p0 = dst + swizzled<DH>(g / GH * 2 * GH + g % GH, lane * D);
+        uint8_t* p1 = dst + swizzled<DH>(g / GH * 2 * GH + GH + g % GH, lane * D);
         if constexpr (D == 4) {
           *reinterpret_cast<uint32_t*>(p0) = hi;
           *reinterpret_cast<uint32_t*>(p1) = lo;
@@ -447,86 +469,126 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(smem_u32(&q_full[which]));
     };
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    const bool owns = tid < DH;   // a dimension of the result
-    long long seq_base = cur.left > 0 ? base_sh : 0;
+    const uint32_t lanes = (uint32_t)(wl * 32) << 16;
+    const bool owns = tl < DH;   // a dimension of the result
+    int seq_base = cur.left > 0 ? base_sh : 0;
     int j = 0, seg = 0;
+    // The pair that is ending: its last product runs while the first tile of the next pair goes through the softmax.
+    float acc[GH], l_end[GH], m_end[GH], c_end[GH];
+    int bh_end = 0, run_end = 0, tiles_end = 0, seg_end = 0, list_end = 0;
+    bool pending = false;
+#pragma unroll
+    for (int g = 0; g < GH; ++g) acc[g] = 0.0f;
+    auto collect = [&](int jj, const float (&c)[GH]) {   // acc = acc c + O(jj)
+      const int buf = jj & 1;
+      wait_bar(smem_u32(&o_full[buf]), (jj >> 1) & 1, giveup, a.status, a.wait_limit, DS_BARRIER_TIMEOUT);
+      tc_fence_after();
+      if (wl * 32 < DH) {
+        float o[kPieces * GH];
+        tm_ld<kPieces * GH>(tmem + 2 * S::kNq + buf * S::kNw + group * kPieces * GH + lanes, o);
+#pragma unroll
+        for (int g = 0; g < GH; ++g)
+          acc[g] = acc[g] * c[g] + (((o[3 * GH + g] * 0.0625f + o[2 * GH + g]) * 0.0625f + o[GH + g]) * 0.0625f + o[g]);
+      }
+    };
+    auto finalise = [&](int last) {
+      float (&red)[4][GP] = red2[seg_end & 1];
+      collect(last, c_end);
+      // denominators
+#pragma unroll
+      for (int g = 0; g < GH; ++g) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l_end[g] += __shfl_xor_sync(0xffffffffu, l_end[g], o);
+        if (lane == 0) red[wl][head0 + g] = l_end[g];
+      }
+      group_sync(group);
+#pragma unroll
+      for (int g = 0; g < GH; ++g) l_end[g] = (red[0][head0 + g] + red[1][head0 + g]) + (red[2][head0 + g] + red[3][head0 + g]);
+      __nv_bfloat16* out = a.out + ((size_t)bh_end * G + head0) * DH + tl;
+      constexpr int rec = DH + kPad;
+      if (run_end == tiles_end) {
+        if (owns) {
+#pragma unroll
+          for (int g = 0; g < GH; ++g)
+            if (head0 + g < G) out[g * DH] = __float2bfloat16_rn(acc[g] * 16.0f / l_end[g]);
+        }
+      } else {
+        float* rp = a.part + ((size_t)blockIdx.x * 2 + (seg_end > 0)) * G * rec + head0 * rec;
+#pragma unroll
+        for (int g = 0; g < GH; ++g)
+          if (head0 + g < G) {
+            if (owns) rp[g * rec + tl] = acc[g] * 16.0f;   // (256 times the sum, as l)
+            if (tl == 0) *reinterpret_cast<float2*>(rp + g * rec + DH) = make_float2(m_end[g], l_end[g]);
+          }
+        if (tid == 0) part_of[seg_end > 0] = Part{bh_end, tiles_end, list_end};
+      }
+#pragma unroll
+      for (int g = 0; g < GH; ++g) acc[g] = 0.0f;
+    };
     if (cur.left > 0) {
       fetch_q(cur.b, cur.hk);
       build_q(0);
-      soft_sync();
+      soft_sync(kSoft * NG);
     }
     while (cur.left > 0) {
       const int run = cur.run(), first = cur.tile, bh = cur.b * a.Hk + cur.hk, n = cur.n, ntiles = cur.tiles, hk = cur.hk;
       cur.next(run);
       const bool more = cur.left > 0;   // (`cur` is the next pair from here on)
       if (more) fetch_q(cur.b, cur.hk);
-      const long long list0 = seq_base + (long long)hk * ntiles;   // list index of the pair's first tile
+      const int list0 = seq_base + hk * ntiles;   // list index of the pair's first tile
       const float* ksc = a.k_scale + (size_t)bh * a.nb;
       const float* vsc = a.v_scale + (size_t)bh * a.nb;
-      float m[GP], l[GP], acc[GP], corr[GP], qf[GP];   // l and acc: 256 and 16 times the sums
+      float m[GH], l[GH], corr[GH], qf[GH];   // l and acc: 256 and 16 times the sums
 #pragma unroll
-      for (int g = 0; g < GP; ++g) {
+      for (int g = 0; g < GH; ++g) {
         m[g] = -INFINITY;
-        l[g] = acc[g] = 0.0f;
-        qf[g] = qfac[seg & 1][g];
+        l[g] = 0.0f;
+        qf[g] = qfac[seg & 1][head0 + g];
       }
-      auto collect = [&](int jj, const float (&c)[GP]) {   // acc = acc c + O(jj)
-        const int buf = jj & 1;
-        wait_bar(smem_u32(&o_full[buf]), (jj >> 1) & 1, giveup, a.status, a.wait_limit, DS_BARRIER_TIMEOUT);
-        tc_fence_after();
-        if (warp * 32 < DH) {
-          float o[kPieces * GP];
-          tm_ld<kPieces * GP>(tmem + 2 * S::kNq + buf * S::kNw + lanes, o);
-#pragma unroll
-          for (int g = 0; g < GP; ++g)
-            acc[g] = acc[g] * c[g] + (((o[3 * GP + g] * 0.0625f + o[2 * GP + g]) * 0.0625f + o[GP + g]) * 0.0625f + o[g]);
-        }
-      };
       float ks = 0.0f, vs = 1.0f;
       auto scales = [&](int t) {
-        const int at = t * kTile + tid;
+        const int at = t * kTile + tl;
         ks = at < n ? ksc[at >> a.block_log2] : 0.0f;
         vs = at < n ? vsc[at >> a.block_log2] : 1.0f;
       };
       scales(first);
       for (int i = 0; i < run; ++i, ++j) {
         const int t = first + i, buf = j & 1;
-        const bool valid = t * kTile + tid < n;
+        const bool valid = t * kTile + tl < n;
         const float kf = ks, lv = __log2f(vs), inv = valid ? __fdividef(1.0f, vs) : 0.0f;
         if (i + 1 < run) scales(t + 1);
         wait_bar(smem_u32(&s_full[buf]), (j >> 1) & 1, giveup, a.status, a.wait_limit, DS_BARRIER_TIMEOUT);
         tc_fence_after();
-        float s[2 * GP], e[GP];
-        tm_ld<2 * GP>(tmem + buf * S::kNq + lanes, s);
+        float s[2 * GH], e[GH];
+        tm_ld<2 * GH>(tmem + buf * S::kNq + group * 2 * GH + lanes, s);
         bool higher = false;
 #pragma unroll
-        for (int g = 0; g < GP; ++g) {
-          const float x = fmaf(fmaf(s[GP + g], 0.0625f, s[g]), kf * qf[g], lv);
+        for (int g = 0; g < GH; ++g) {
+          const float x = fmaf(fmaf(s[GH + g], 0.0625f, s[g]), kf * qf[g], lv);
           e[g] = valid ? x : -INFINITY;
-          higher = higher || (g < G && e[g] > m[g] + kRoom);
+          higher = higher || (head0 + g < G && e[g] > m[g] + kRoom);
         }
-        if (!valid) {   // the last tile: a row behind the end may hold anything
-          uint4* row = reinterpret_cast<uint4*>(smem + (j % S::kStages) * 2 * S::kHalf + S::kHalf + tid * DH);
+        if (!valid && group == 0) {   // the last tile: a row behind the end may hold anything
+          uint4* row = reinterpret_cast<uint4*>(smem + (j % S::kStages) * 2 * S::kHalf + S::kHalf + tl * DH);
 #pragma unroll
-          for (int x = 0; x < DH / 16; ++x) row[x] = make_uint4(0u, 0u, 0u, 0u);
+          for (int x = 0; x < DH / 16; ++x) row[(x + tl) % (DH / 16)] = make_uint4(0u, 0u, 0u, 0u);   // (neighbours in other banks)
         }
-        float prev[GP];   // rescaling of the tile before, which is collected below
+        float prev[GH];   // rescaling of the tile before, which is collected below
 #pragma unroll
-        for (int g = 0; g < GP; ++g) {
+        for (int g = 0; g < GH; ++g) {
           prev[g] = corr[g];
           corr[g] = 1.0f;
         }
-        if (soft_any(higher)) {
+        if (group_any(higher, group)) {
 #pragma unroll
-          for (int g = 0; g < GP; ++g) {
+          for (int g = 0; g < GH; ++g) {
             const float top = warp_max(e[g]);
-            if (lane == 0) wmax[buf][warp][g] = top;
+            if (lane == 0) wmax[buf][wl][head0 + g] = top;
           }
-          soft_sync();
+          group_sync(group);
 #pragma unroll
-          for (int g = 0; g < GP; ++g) {
-            const float top = fmaxf(fmaxf(wmax[buf][0][g], wmax[buf][1][g]), fmaxf(wmax[buf][2][g], wmax[buf][3][g]));
+          for (int g = 0; g < GH; ++g) {
+            const float top = fmaxf(fmaxf(wmax[buf][0][head0 + g], wmax[buf][1][head0 + g]), fmaxf(wmax[buf][2][head0 + g], wmax[buf][3][head0 + g]));
             const float mn = fmaxf(m[g], top);
             corr[g] = m[g] == mn ? 1.0f : ex2(m[g] - mn);
             m[g] = mn;
@@ -534,146 +596,145 @@ __global__ void __launch_bounds__(kThreads, Shape<DH, GP>::kCtas) attn_kernel(co
           }
         }
 #pragma unroll
-        for (int g = 0; g < GP; ++g) {
+        for (int g = 0; g < GH; ++g) {
           e[g] = valid ? ex2(e[g] - m[g] + 8.0f) : 0.0f;   // 256 times the weight, which is at most 2^kRoom
           l[g] = fmaf(e[g], inv, l[g]);
         }
         {
-          uint32_t c[(GP + 1) / 2][4];   // pairs of heads
+          uint32_t c[(GH + 1) / 2][4];   // pairs of heads
 #pragma unroll
-          for (int g = 0; g < GP; g += 2) four_codes(e[g], GP > 1 ? e[(g + 1) % GP] : 0.0f, c[g / 2]);
-          uint8_t* dst = ws + buf * S::kW + tid * S::kNw;
-          if constexpr (GP == 1) {
+          for (int g = 0; g < GH; g += 2) four_codes(e[g], GH > 1 ? e[(g + 1) % GH] : 0.0f, c[g / 2]);
+          uint8_t* dst = ws + buf * S::kW + tl * S::kNw;
+          if constexpr (GH == 1) {
             *reinterpret_cast<uint32_t*>(dst) = __byte_perm(__byte_perm(c[0][0], c[0][1], 0x0040), __byte_perm(c[0][2], c[0][3], 0x0040), 0x5410);
-          } else if constexpr (GP == 2) {
+          } else if constexpr (GH == 2) {
             *reinterpret_cast<uint2*>(dst) = make_uint2(c[0][0] | (c[0][1] << 16), c[0][2] | (c[0][3] << 16));
           } else {
-            uint32_t w[GP];   // codes of four heads each, piece by piece
-#pragma unroll
-            for (int p = 0; p < 4; ++p)
-#pragma unroll
-              for (int g = 0; g < GP / 4; ++g) w[p * (GP / 4) + g] = c[2 * g][p] | (c[2 * g + 1][p] << 16);
-            const int x = S::kNw == 32 ? (tid >> 2) & 1 : S::kNw == 64 ? (tid >> 1) & 3 : 0;
-#pragma unroll
-            for (int i16 = 0; i16 < GP / 4; ++i16)
-              *reinterpret_cast<uint4*>(dst + ((i16 ^ x) << 4)) = make_uint4(w[4 * i16], w[4 * i16 + 1], w[4 * i16 + 2], w[4 * i16 + 3]);
+            const int x = NG == 2 ? (tl >> 2) & 1 : NG == 4 ? (tl >> 1) & 3 : 0;
+            *reinterpret_cast<uint4*>(dst + ((group ^ x) << 4)) =
+                make_uint4(c[0][0] | (c[GH / 2 - 1][0] << 16), c[0][1] | (c[GH / 2 - 1][1] << 16), c[0][2] | (c[GH / 2 - 1][2] << 16),
+                           c[0][3] | (c[GH / 2 - 1][3] << 16));
           }
         }
         tc_fence_before();
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(smem_u32(&w_full[buf]));
         if (i == 0 && more) build_q((seg + 1) & 1);   // (the products of the pair before the last are done with that buffer)
-        if (i > 0) collect(j - 1, prev);
-      }
-      if (hk == a.Hk - 1 && first + run == ntiles) seq_base += (long long)a.Hk * ntiles;
-      collect(j - 1, corr);
-      // denominators
-#pragma unroll
-      for (int g = 0; g < GP; ++g) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l[g] += __shfl_xor_sync(0xffffffffu, l[g], o);
-        if (lane == 0) red[warp][g] = l[g];
-      }
-      soft_sync();
-#pragma unroll
-      for (int g = 0; g < GP; ++g) l[g] = (red[0][g] + red[1][g]) + (red[2][g] + red[3][g]);
-      __nv_bfloat16* out = a.out + (size_t)bh * G * DH + tid;
-      constexpr int rec = DH + kPad;
-      if (run == ntiles) {
-        if (owns) {
-#pragma unroll
-          for (int g = 0; g < GP; ++g)
-            if (g < G) out[g * DH] = __float2bfloat16_rn(acc[g] * 16.0f / l[g]);
+        if (i > 0) {
+          collect(j - 1, prev);
+        } else if (pending) {
+          finalise(j - 1);
+          pending = false;
         }
-      } else {
-        float* rp = a.part + ((size_t)blockIdx.x * 2 + (seg > 0)) * G * rec;
+      }
+      if (hk == a.Hk - 1 && first + run == ntiles) seq_base += a.Hk * ntiles;
 #pragma unroll
-        for (int g = 0; g < GP; ++g)
-          if (g < G) {
-            if (owns) rp[g * rec + tid] = acc[g] * 16.0f;   // (256 times the sum, as l)
-            if (tid == 0) *reinterpret_cast<float2*>(rp + g * rec + DH) = make_float2(m[g], l[g]);
-          }
-        __threadfence();
-        soft_sync();
-        const int c0 = (int)(list0 / per), c1 = (int)((list0 + ntiles - 1) / per);   // the CTAs of this pair
-        if (tid == 0) last_sh = atomicAdd(a.counters + bh, 1) == c1 - c0;
-        soft_sync();
-        if (last_sh) {
-          __threadfence();
-          // maximum and denominator of each head: a warp to a head, its lanes over the parts
-          const float* base = a.part;
-          auto record = [&](int c) { return base + ((size_t)c * 2 + (per * c < list0)) * G * rec; };
-          for (int g = warp; g < G; g += 4) {
-            float mm = -INFINITY, ll = 0.0f;
-            for (int c = c0 + lane; c <= c1; c += 32) {
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(record(c) + g * rec + DH));
-              const float mn = fmaxf(mm, ml.x);
-              ll = ll * (mm == mn ? 1.0f : ex2(mm - mn)) + ml.y * (ml.x == mn ? 1.0f : ex2(ml.x - mn));
-              mm = mn;
-            }
-            const float top = warp_max(mm);
-            ll = mm == top ? ll : ll * ex2(mm - top);
+      for (int g = 0; g < GH; ++g) {
+        l_end[g] = l[g];
+        m_end[g] = m[g];
+        c_end[g] = corr[g];
+      }
+      bh_end = bh; run_end = run; tiles_end = ntiles; seg_end = seg; list_end = list0;
+      if (more) pending = true;
+      else finalise(j - 1);
+      ++seg;
+    }
+    // The pairs that this CTA has worked on a part of (its first and its last one): whoever finishes a pair merges its parts,
+    // in their order.
+    soft_sync(kSoft * NG);   // (the release below covers what the barrier orders in front of it)
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+      const Part pt = part_of[which];
+      if (pt.tiles == 0) continue;
+      constexpr int rec = DH + kPad;
+      const int c0 = pt.list / per, c1 = (pt.list + pt.tiles - 1) / per;   // the CTAs of this pair
+      if (tid == 0) {
+        int arrived;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(arrived) : "l"(a.counters + pt.bh) : "memory");
+        last_sh = arrived == c1 - c0;
+      }
+      soft_sync(kSoft * NG);
+      if (last_sh) {
+        // CTA c's part is its first one if it starts inside the pair's tiles, else its last
+        auto record = [&](int c) { return a.part + ((size_t)c * 2 + (per * c < pt.list)) * G * rec; };
+        __nv_bfloat16* out = a.out + (size_t)pt.bh * G * DH;
+        // Four dimensions to a thread, which goes through the parts eight at a time with a running maximum; where there are many
+        // parts and fewer dimensions than threads, the parts are shared out too.
+        constexpr int kBatch = 8;
+        const int items = G * (DH / 4), shares = c1 - c0 >= kBatch ? max(1, kSoft / items) : 1;
+        float4* sums = reinterpret_cast<float4*>(ws);   // (no weights are on their way any more; at most 128 of each)
+        float2* tops = reinterpret_cast<float2*>(ws + kSoft * sizeof(float4));
+        static_assert(2 * S::kW >= kSoft * (int)(sizeof(float4) + sizeof(float2)));
+        auto store = [&](int item, const float4& o, float den) {
+          *reinterpret_cast<uint2*>(out + item / (DH / 4) * DH + item % (DH / 4) * 4) =
+              make_uint2(pack_bf16(o.x / den, o.y / den), pack_bf16(o.z / den, o.w / den));
+        };
+        for (int x = tid; x < items * shares; x += kSoft * NG) {
+          const int item = x % items, share = x / items, g = item / (DH / 4), d = item % (DH / 4) * 4;
+          float top = -INFINITY, den = 0.0f;
+          float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          for (int cb = c0 + share; cb <= c1; cb += kBatch * shares) {
+            float2 ml[kBatch];
+            float4 v[kBatch];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
-            if (lane == 0) {
-              red[0][g] = top;
-              red[1][g] = ll;
+            for (int c = 0; c < kBatch; ++c) {
+              const float* r = record(min(cb + c * shares, c1)) + g * rec;
+              ml[c] = __ldcg(reinterpret_cast<const float2*>(r + DH));
+              v[c] = __ldcg(reinterpret_cast<const float4*>(r + d));
             }
+            float mn = top;
+#pragma unroll
+            for (int c = 0; c < kBatch; ++c) mn = fmaxf(mn, cb + c * shares <= c1 ? ml[c].x : -INFINITY);
+            const float f0 = top == mn ? 1.0f : ex2(top - mn);
+            top = mn;
+            den *= f0;
+            o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+#pragma unroll
+            for (int c = 0; c < kBatch; ++c)
+              if (cb + c * shares <= c1) {
+                const float f = ml[c].x == mn ? 1.0f : ex2(ml[c].x - mn);
+                den = fmaf(f, ml[c].y, den);
+                o.x = fmaf(f, v[c].x, o.x); o.y = fmaf(f, v[c].y, o.y); o.z = fmaf(f, v[c].z, o.z); o.w = fmaf(f, v[c].w, o.w);
+              }
           }
-          soft_sync();
-          // four dimensions to a thread; where there are fewer of those than threads, the parts are shared out too and their
-          // sums added in order
-          const int items = G * (DH / 4), shares = max(1, kSoft / items);
-          float4* sums = reinterpret_cast<float4*>(ws);   // (no weights are on their way)
-          for (int x = tid; x < items * shares; x += kSoft) {
-            const int item = x % items, share = x / items, g = item / (DH / 4), d = item % (DH / 4) * 4;
-            const float top = red[0][g];
+          if (shares == 1) {
+            store(item, o, den);
+          } else {
+            sums[x] = o;
+            tops[x] = make_float2(top, den);
+          }
+        }
+        if (shares > 1) {
+          soft_sync(kSoft * NG);
+          if (tid < items) {
+            float top = tops[tid].x;
+            for (int x = 1; x < shares; ++x) top = fmaxf(top, tops[tid + x * items].x);
             float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-            for (int c = c0 + share; c <= c1; c += shares) {
-              const float* r = record(c) + g * rec;
-              const float mc = __ldcg(r + DH);
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(r + d));
-              const float f = mc == top ? 1.0f : ex2(mc - top);
+            float den = 0.0f;
+            for (int x = 0; x < shares; ++x) {
+              const float2 ml = tops[tid + x * items];
+              const float4 v = sums[tid + x * items];
+              const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
+              den = fmaf(f, ml.y, den);
               o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
             }
-            if (shares > 1) sums[x] = o;
-            else {
-              const float den = red[1][g];
-              *reinterpret_cast<uint2*>(a.out + ((size_t)bh * G + g) * DH + d) =
-                  make_uint2(pack_bf16(o.x / den, o.y / den), pack_bf16(o.z / den, o.w / den));
-            }
+            store(tid, o, den);
           }
-          if (shares > 1) {
-            soft_sync();
-            if (tid < items) {
-              const int g = tid / (DH / 4), d = tid % (DH / 4) * 4;
-              float4 o = sums[tid];
-              for (int x = 1; x < shares; ++x) {
-                const float4 v = sums[tid + x * items];
-                o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
-              }
-              const float den = red[1][g];
-              *reinterpret_cast<uint2*>(a.out + ((size_t)bh * G + g) * DH + d) =
-                  make_uint2(pack_bf16(o.x / den, o.y / den), pack_bf16(o.z / den, o.w / den));
-            }
-          }
-          if (tid == 0) a.counters[bh] = 0;
         }
+        if (tid == 0) a.counters[pt.bh] = 0;
       }
-      ++seg;
-      soft_sync();   // `red`, `last_sh`
+      soft_sync(kSoft * NG);
     }
     // sequences without positions
     for (int i = blockIdx.x; i < a.B; i += gridDim.x)
       if (cur.positions(i) == 0)
-        for (int x = tid; x < a.Hk * G * DH / 8; x += kSoft)
+        for (int x = tid; x < a.Hk * G * DH / 8; x += kSoft * NG)
           reinterpret_cast<uint4*>(a.out + (size_t)i * a.Hk * G * DH)[x] = make_uint4(0u, 0u, 0u, 0u);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tc_dealloc(tmem, S::kCols);
+  if (warp == kMma) tc_dealloc(tmem, S::kCols);
 }
 
 }  // namespace fsvd_kv8_attn
