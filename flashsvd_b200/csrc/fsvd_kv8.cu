@@ -89,26 +89,13 @@ struct RopeArgs {
   int T, H, Hk, Dh, tokens, heads;   // tokens and heads of a CTA
 };
 
+// A CTA turns `tokens` rows of heads; its threads go through the (token, head, unit) list in steps of kThreads, several units
+// at a time so that their loads are under way together.
 template <typename T, bool WIDE>
-__device__ __forceinline__ void rotate_row(const T* in, T* out, int u, int R, int interleaved, const float (&c)[8],
-                                           const float (&s)[8]) {
-  float a[8], b[8];
-  fsvd_rope::load_unit<WIDE>(in, u, R, interleaved, a, b);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float x = a[i], y = b[i];
-    if (8 * u + i < (R >> 1)) {   // (the others are copied: an infinity times a sine of zero is no number)
-      a[i] = x * c[i] - y * s[i];
-      b[i] = y * c[i] + x * s[i];
-    }
-  }
-  fsvd_rope::store_unit<WIDE>(out, u, R, interleaved, a, b);
-}
-
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const RopeArgs a) {
-  extern __shared__ float2 table[];   // [tokens][R / 2] cosine, sine
-  const int half = a.rot.R >> 1, tid = threadIdx.x;
+__global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
+  constexpr int N = 2;                              // units at a time
+  extern __shared__ __align__(16) float2 table[];   // [tokens][R / 2] cosine, sine
+  const int half = a.rot.R >> 1, tid = threadIdx.x, R = a.rot.R, inter = a.rot.interleaved;
   const int t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.T - t0);
   pdl_begin();
   for (int i = tid; i < nt * half; i += kThreads) {
@@ -118,27 +105,55 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeArgs a) {
     table[i] = make_float2((float)c, (float)s);
   }
   __syncthreads();
-  const int U = a.Dh / 16, u = tid % U, per = kThreads / U;
-  const int h0 = blockIdx.y * a.heads, h1 = min(h0 + a.heads, a.H + a.Hk);
-  if (tid >= per * U) return;
-  for (int t = 0; t < nt; ++t) {
-    float c[8], s[8];
+  const unsigned U = a.Dh / 16;
+  const int h0 = blockIdx.y * a.heads, nh = min(a.heads, a.H + a.Hk - h0);
+  const unsigned items = (unsigned)nt * nh * U;
+  for (unsigned i0 = tid; i0 < items; i0 += N * kThreads) {
+    float x[N][8], y[N][8];
+    T* dst[N];
+    int token[N], unit[N];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int p = 8 * u + i;
-      const float2 cs = p < half ? table[t * half + p] : make_float2(1.0f, 0.0f);
-      c[i] = cs.x;
-      s[i] = cs.y;
+    for (int k = 0; k < N; ++k) {
+      const unsigned i = i0 + k * kThreads;
+      if (i < items) {
+        const unsigned row = i / U, t = row / (unsigned)nh;
+        const int h = h0 + (int)(row - t * nh);
+        const size_t tt = t0 + t;
+        token[k] = (int)t;
+        unit[k] = (int)(i - row * U);
+        const bool q = h < a.H;
+        const T* src = q ? reinterpret_cast<const T*>(a.q) + tt * a.q_stride + (size_t)h * a.Dh
+                         : reinterpret_cast<const T*>(a.k) + tt * a.k_stride + (size_t)(h - a.H) * a.Dh;
+        dst[k] = q ? reinterpret_cast<T*>(a.q_out) + (tt * a.H + h) * a.Dh : reinterpret_cast<T*>(a.k_out) + (tt * a.Hk + h - a.H) * a.Dh;
+        fsvd_rope::load_unit<WIDE>(src, unit[k], R, inter, x[k], y[k]);
+      }
     }
-    const size_t tt = t0 + t;
-    for (int h = h0 + tid / U; h < h1; h += per) {
-      if (h < a.H)
-        rotate_row<T, WIDE>(reinterpret_cast<const T*>(a.q) + tt * a.q_stride + (size_t)h * a.Dh,
-                            reinterpret_cast<T*>(a.q_out) + (tt * a.H + h) * a.Dh, u, a.rot.R, a.rot.interleaved, c, s);
-      else
-        rotate_row<T, WIDE>(reinterpret_cast<const T*>(a.k) + tt * a.k_stride + (size_t)(h - a.H) * a.Dh,
-                            reinterpret_cast<T*>(a.k_out) + (tt * a.Hk + h - a.H) * a.Dh, u, a.rot.R, a.rot.interleaved, c, s);
-    }
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (i0 + k * kThreads < items) {
+        auto turn = [&](int e, float c, float s) {
+          const float xe = x[k][e], ye = y[k][e];
+          x[k][e] = xe * c - ye * s;
+          y[k][e] = ye * c + xe * s;
+        };
+        const float2* cs = table + token[k] * half + 8 * unit[k];
+        // (pairs that are not rotated are copied: an infinity times a sine of zero is no number)
+        if constexpr (WIDE) {
+          if (8 * unit[k] < half) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const float4 two = *reinterpret_cast<const float4*>(cs + e);
+              turn(e, two.x, two.y);
+              turn(e + 1, two.z, two.w);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (8 * unit[k] + e < half) turn(e, cs[e].x, cs[e].y);
+        }
+        fsvd_rope::store_unit<WIDE>(dst[k], unit[k], R, inter, x[k], y[k]);
+      }
   }
 }
 
@@ -217,12 +232,34 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
   const int nq = (int)(min(end_ll, blk0 + BLOCK) - lo), n = max(0, hi - lo);
   const int R = a.rot.R, half = R >> 1, inter = a.rot.interleaved;
   if (R) {
-    for (int i = tid; i < nq * half; i += kThreads) {
-      const int t = i / half;
-      double c, s;
-      fsvd_rope::angle(lo + t, a.rot.inv_freq[i - t * half], a.rot.scale, c, s);
+    // Cosines and sines of the tile's tokens.  More than a few: of every eighth token and of steps 0..7, and the products of
+    // those (64 tokens: 16 evaluations in 64 bits a pair instead of 64).
+    auto put = [&](int i, double c, double s) {
       const float ch = (float)c, sh = (float)s;
       tab[i] = make_float4(ch, (float)(c - (double)ch), sh, (float)(s - (double)sh));
+    };
+    const int coarse = (nq + 7) / 8;
+    if (nq <= 8) {
+      for (int i = tid; i < nq * half; i += kThreads) {
+        const int t = i / half;
+        double c, s;
+        fsvd_rope::angle(lo + t, a.rot.inv_freq[i - t * half], a.rot.scale, c, s);
+        put(i, c, s);
+      }
+    } else {
+      double2* steps = reinterpret_cast<double2*>(tab + min(BLOCK, a.L) * half);   // [8 + coarse][half]
+      for (int i = tid; i < (8 + coarse) * half; i += kThreads) {
+        const int k = i / half;
+        double c, s;
+        fsvd_rope::angle(k < 8 ? k : lo + 8 * (k - 8), a.rot.inv_freq[i - k * half], k < 8 ? 1.0f : a.rot.scale, c, s);
+        steps[i] = make_double2(c, s);
+      }
+      __syncthreads();
+      for (int i = tid; i < nq * half; i += kThreads) {
+        const int t = i / half, p = i - t * half;
+        const double2 x = steps[(8 + (t >> 3)) * half + p], y = steps[(t & 7) * half + p];
+        put(i, x.x * y.x - x.y * y.y, x.y * y.x + x.x * y.y);
+      }
     }
     __syncthreads();
   }
@@ -377,33 +414,47 @@ struct LoadArgs {
   __nv_bfloat16 *k_out, *v_out;
 };
 
+// A CTA reads back kThreads * kLoads sixteen-byte pieces in a row of one plane (a sequence's head, keys or values).
+constexpr int kLoads = 4;
+template <int DH>
 __global__ void __launch_bounds__(kThreads) load_kernel(const LoadArgs a) {
+  constexpr int V = DH / 16;   // pieces of a row
   pdl_begin();
-  const int DH = a.c.Dh, V = DH / 16, nb = (a.c.S_max + a.c.block - 1) / a.c.block;
-  const size_t rows = (size_t)a.c.B * a.c.Hk * a.length, total = rows * V;
-  for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < 2 * total; i += (size_t)gridDim.x * kThreads) {
-    const bool second = i >= total;
-    const size_t at = second ? i - total : i, row = at / V, bh = row / a.length;
-    const int c = (int)(at - row * V), t = a.start + (int)(row - bh * a.length);
-    uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
-    if (!a.seqlens || t < a.seqlens[bh / a.c.Hk] + a.seqlen_add) {
-      const uint4 w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(second ? a.c.v8 : a.c.k8) +
-                                                      (bh * a.c.S_max + t) * DH + 16 * c);
-      const float s = (second ? a.c.v_scale : a.c.k_scale)[bh * nb + t / a.c.block];
-      const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-      uint32_t o[8];
+  const int planes = a.c.B * a.c.Hk, per_plane = (a.length * V + kThreads * kLoads - 1) / (kThreads * kLoads);
+  const int plane2 = blockIdx.x / per_plane, first = (blockIdx.x - plane2 * per_plane) * kThreads * kLoads + threadIdx.x;
+  const bool second = plane2 >= planes;
+  const int bh = second ? plane2 - planes : plane2, nb = (a.c.S_max + a.c.block - 1) / a.c.block;
+  const uint8_t* codes = reinterpret_cast<const uint8_t*>(second ? a.c.v8 : a.c.k8) + ((size_t)bh * a.c.S_max + a.start) * DH;
+  const float* scales = (second ? a.c.v_scale : a.c.k_scale) + (size_t)bh * nb;
+  __nv_bfloat16* out = (second ? a.v_out : a.k_out) + (size_t)bh * a.length * DH;
+  const int end = a.seqlens ? (int)min((long long)a.length, max(0ll, (long long)a.seqlens[bh / a.c.Hk] + a.seqlen_add - a.start)) : a.length;
+  uint4 w[kLoads];
+  float f[kLoads];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 p = decode2(x[e] & 0xffffu), q = decode2(x[e] >> 16);
-        o[2 * e] = fsvd_rope::pack2(p.x * s, p.y * s);
-        o[2 * e + 1] = fsvd_rope::pack2(q.x * s, q.y * s);
-      }
-      lo = make_uint4(o[0], o[1], o[2], o[3]);
-      hi = make_uint4(o[4], o[5], o[6], o[7]);
+  for (int i = 0; i < kLoads; ++i) {
+    const int at = first + i * kThreads, t = at / V;
+    w[i] = make_uint4(0u, 0u, 0u, 0u);
+    f[i] = 0.0f;
+    if (t < end) {
+      w[i] = __ldg(reinterpret_cast<const uint4*>(codes) + at);
+      f[i] = __ldg(scales + (a.start + t) / a.c.block);
     }
-    uint4* out = reinterpret_cast<uint4*>((second ? a.v_out : a.k_out) + row * DH + 16 * c);
-    out[0] = lo;
-    out[1] = hi;
+  }
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int at = first + i * kThreads, t = at / V;
+    if (t >= a.length) break;
+    const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+    uint32_t o[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 p = decode2(x[e] & 0xffffu), q = decode2(x[e] >> 16);
+      o[2 * e] = fsvd_rope::pack2(p.x * f[i], p.y * f[i]);
+      o[2 * e + 1] = fsvd_rope::pack2(q.x * f[i], q.y * f[i]);
+    }
+    uint4* dst = reinterpret_cast<uint4*>(out) + 2 * (size_t)at;
+    dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
@@ -521,8 +572,10 @@ int fsvd_rope_qk(const void* q, long long q_stride, const void* k, long long k_s
   a.q_stride = q_stride; a.k_stride = k_stride; a.positions = positions;
   a.rot = Rotary{inv_freq, rotary_dim, interleaved != 0, rope_scale};
   a.T = T; a.H = H; a.Hk = Hk; a.Dh = Dh;
-  a.tokens = std::min(16, T);
-  a.heads = H + Hk;
+  // One wave of four CTAs per SM, up to 32 tokens each; a few tokens are shared out by heads.
+  a.tokens = std::min(32, (T + 4 * sm_count() - 1) / (4 * sm_count()));
+  const int ctas = (T + a.tokens - 1) / a.tokens, splits = std::max(1, std::min({2 * sm_count() / ctas, (H + Hk) * (Dh / 16) / kThreads, 8}));
+  a.heads = (H + Hk + splits - 1) / splits;
   const dim3 grid((T + a.tokens - 1) / a.tokens, (H + Hk + a.heads - 1) / a.heads);
   const size_t smem = (size_t)a.tokens * (rotary_dim / 2) * sizeof(float2);
   const bool wide = rotary_dim % 16 == 0;
@@ -567,10 +620,14 @@ int fsvd_kv8_append(const fsvd_kv8* cache, const void* k, const void* v, long lo
   a.H = q ? H : 0; a.L = L;
   const int BLOCK = cache->block;
   a.nblk = (int)(((long long)L + BLOCK - 2) / BLOCK + 1);
+  // Heads of a CTA share the table of angles: with rotation as few groups as still give every SM two CTAs.
   a.groups = cache->Hk;
+  if (inv_freq)
+    while (a.groups % 2 == 0 && (long long)cache->B * a.nblk * (a.groups / 2) >= 2ll * sm_count()) a.groups /= 2;
   const long long grid = (long long)cache->B * a.nblk * a.groups;
   if (grid > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many tokens for one call");
-  const size_t smem = (size_t)std::min(BLOCK, L) * (a.rot.R / 2) * sizeof(float4);
+  const int tile = std::min(BLOCK, L);
+  const size_t smem = (size_t)(a.rot.R / 2) * (tile * sizeof(float4) + (tile > 8 ? (8 + (tile + 7) / 8) * sizeof(double2) : 0));
   return cache->Dh == 64 ? launch_append<64>(a, smem, (unsigned)grid, stream) : launch_append<128>(a, smem, (unsigned)grid, stream);
 }
 
@@ -584,9 +641,10 @@ int fsvd_kv8_load(const fsvd_kv8* cache, int start, int length, const int* cache
   if (length == 0) return 0;
   LoadArgs a = {*cache, start, length, seqlen_add, cache_seqlens, reinterpret_cast<__nv_bfloat16*>(k_out),
                 reinterpret_cast<__nv_bfloat16*>(v_out)};
-  const long long items = 2ll * cache->B * cache->Hk * length * (cache->Dh / 16);
-  const long long grid = std::min<long long>((items + kThreads - 1) / kThreads, 16ll * sm_count());
-  return launch(load_kernel, dim3((unsigned)grid), kThreads, 0, stream, a);
+  const long long grid = 2ll * cache->B * cache->Hk * (((long long)length * (cache->Dh / 16) + kThreads * kLoads - 1) / (kThreads * kLoads));
+  if (grid > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many tokens for one call");
+  return cache->Dh == 64 ? launch(load_kernel<64>, dim3((unsigned)grid), kThreads, 0, stream, a)
+                         : launch(load_kernel<128>, dim3((unsigned)grid), kThreads, 0, stream, a);
 }
 
 int fsvd_flash_decode_kv8(const fsvd_kv8* cache, const void* q, const int* cache_seqlens, int seqlen_add, void* out, int H,
