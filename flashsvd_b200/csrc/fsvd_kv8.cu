@@ -88,21 +88,26 @@ struct RopeArgs {
   Rotary rot;
   int T, H, Hk, Dh, tokens, heads;   // tokens and heads of a CTA
 };
+constexpr int kRopeTokens = 32;
 
 // A CTA turns `tokens` rows of heads; its threads go through the (token, head, unit) list in steps of kThreads, several units
 // at a time so that their loads are under way together.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
   constexpr int N = 2;                              // units at a time
-  extern __shared__ __align__(16) float2 table[];   // [tokens][R / 2] cosine, sine
+  extern __shared__ __align__(16) float2 table[];   // per token: cosine and sine of the pairs, in slots (below)
   const int half = a.rot.R >> 1, tid = threadIdx.x, R = a.rot.R, inter = a.rot.interleaved;
   const int t0 = blockIdx.x * a.tokens, nt = min(a.tokens, a.T - t0);
+  // Two neighbouring pairs of a unit share 16 bytes; neighbouring units lie next to each other, so that the lanes of a warp
+  // read from different banks.
+  const int units = (half + 7) / 8, row_slots = 8 * units;
+  auto slot_of = [&](int two, int unit) { return two * units + unit; };
   pdl_begin();
   for (int i = tid; i < nt * half; i += kThreads) {
     double c, s;
-    const int t = i / half;
-    fsvd_rope::angle(a.positions[t0 + t], a.rot.inv_freq[i - t * half], a.rot.scale, c, s);
-    table[i] = make_float2((float)c, (float)s);
+    const int t = i / half, p = i - t * half;
+    fsvd_rope::angle(a.positions[t0 + t], a.rot.inv_freq[p], a.rot.scale, c, s);
+    table[t * row_slots + 2 * slot_of((p & 7) >> 1, p >> 3) + (p & 1)] = make_float2((float)c, (float)s);
   }
   __syncthreads();
   const unsigned U = a.Dh / 16;
@@ -136,21 +141,15 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
           x[k][e] = xe * c - ye * s;
           y[k][e] = ye * c + xe * s;
         };
-        const float2* cs = table + token[k] * half + 8 * unit[k];
+        const float4* cs = reinterpret_cast<const float4*>(table + token[k] * row_slots);
         // (pairs that are not rotated are copied: an infinity times a sine of zero is no number)
-        if constexpr (WIDE) {
-          if (8 * unit[k] < half) {
+        if (8 * unit[k] < half) {
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const float4 two = *reinterpret_cast<const float4*>(cs + e);
-              turn(e, two.x, two.y);
-              turn(e + 1, two.z, two.w);
-            }
+          for (int e = 0; e < 8; e += 2) {
+            const float4 two = cs[slot_of(e >> 1, unit[k])];
+            if (WIDE || 8 * unit[k] + e < half) turn(e, two.x, two.y);
+            if (WIDE || 8 * unit[k] + e + 1 < half) turn(e + 1, two.z, two.w);
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (8 * unit[k] + e < half) turn(e, cs[e].x, cs[e].y);
         }
         fsvd_rope::store_unit<WIDE>(dst[k], unit[k], R, inter, x[k], y[k]);
       }
@@ -190,29 +189,116 @@ __device__ __forceinline__ float2 decode2(uint32_t codes) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// x c - y s for bf16 x, y and (c, s) given as sums of two fp32 numbers each: the error of the result is that of its
-// last rounding, so that a rotated key falls on the same side of a rounding border as in 64 bits.  (Products of a bf16
-// and an fp32 number do not fit 24 bits: their rounding errors are carried along.)
-__device__ __forceinline__ float turn(float x, float y, float ch, float cl, float sh, float sl) {
-  const float p = x * ch, pe = fmaf(x, ch, -p);
-  const float q = y * sh, qe = fmaf(y, sh, -q);
-  const float d = p - q, z = d - p, de = (p - (d - z)) - (q + z);
-  return d + (de + (pe - qe) + (x * cl - y * sl));
+// A bf16 number as fp64 by its bits, finite ones only (the conversion instruction runs at an eighth of the rate; a zero
+// comes out as 2^-127, which no code can tell from it).
+__device__ __forceinline__ double wide(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), 0);
 }
 
-template <int DH, int BLOCK>
-__device__ __forceinline__ int unit_offset(int u, int R, int interleaved, int which) {
-  const bool split = !interleaved && 16 * u < R;
-  return split ? 8 * u + (which ? (R >> 1) : 0) : 16 * u + 8 * which;
+__device__ __forceinline__ uint32_t turn_key(uint32_t w, double2 cs) {
+  const float fx = __uint_as_float(w << 16), fy = __uint_as_float(w & 0xffff0000u);
+  double x = wide(fx), y = wide(fy);
+  if ((w & 0x7f80u) == 0x7f80u) x = (double)fx;
+  if ((w & 0x7f800000u) == 0x7f800000u) y = (double)fy;
+  return fsvd_rope::pack2((float)(x * cs.x - y * cs.y), (float)(y * cs.x + x * cs.y));
+}
+__device__ __forceinline__ uint32_t turn_query(uint32_t w, float c, float s) {
+  const float x = __uint_as_float(w << 16), y = __uint_as_float(w & 0xffff0000u);
+  return fsvd_rope::pack2(x * c - y * s, y * c + x * s);
+}
+
+// Scales and codes of one thread's share of a tile: eight packed pairs of bf16 numbers (a in the low half) per row.
+struct Share {
+  uint32_t top = 0;   // largest magnitude, as the bits of a bf16 number
+  bool odd = false;   // something is not finite
+};
+template <int NIT>
+__device__ __forceinline__ void largest(const uint32_t (&w)[NIT][8], Share& s) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int it = 0; it < NIT; ++it)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[it][i] & 0x7fff7fffu);
+  s.top = max(m & 0xffffu, m >> 16);
+  if (s.top >= 0x7f80u) {   // the finite ones alone
+    s.odd = true;
+    s.top = 0;
+#pragma unroll
+    for (int it = 0; it < NIT; ++it)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t x = w[it][i] & 0x7fffu, y = (w[it][i] >> 16) & 0x7fffu;
+        if (x < 0x7f80u) s.top = max(s.top, x);
+        if (y < 0x7f80u) s.top = max(s.top, y);
+      }
+  }
+}
+__device__ __noinline__ uint32_t careful_codes(uint32_t w, float inv) {
+  float x = __uint_as_float(w << 16) * inv, y = __uint_as_float(w & 0xffff0000u) * inv;
+  if (inv <= 0x1p-120f) {   // 256 * 2^120 is no 32-bit number any more
+    x = fabsf(x) > 240.0f && isfinite(x) ? copysignf(240.0f, x) : x;
+    y = fabsf(y) > 240.0f && isfinite(y) ? copysignf(240.0f, y) : y;
+  }
+  return code2(x, y);
+}
+// Code pairs of one row, times inv (a power of two).
+__device__ __forceinline__ void codes_of(const uint32_t (&w)[8], float inv, bool odd, uint32_t (&cd)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    cd[i] = __nv_cvt_float2_to_fp8x2(make_float2(__uint_as_float(w[i] << 16) * inv, __uint_as_float(w[i] & 0xffff0000u) * inv),
+                                     __NV_SATFINITE, __NV_E4M3);
+  if (odd || inv <= 0x1p-120f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) cd[i] = careful_codes(w[i], inv);
+  }
+}
+template <bool WIDE>
+__device__ __forceinline__ void store_codes(uint8_t* dst, const uint32_t (&cd)[8], int u, int R, int inter) {
+  const int half = R >> 1;
+  if constexpr (WIDE) {
+    const bool split = !inter && 16 * u < R;
+    const uint32_t a03 = __byte_perm(cd[0] | (cd[1] << 16), cd[2] | (cd[3] << 16), 0x6420);
+    const uint32_t a47 = __byte_perm(cd[4] | (cd[5] << 16), cd[6] | (cd[7] << 16), 0x6420);
+    const uint32_t b03 = __byte_perm(cd[0] | (cd[1] << 16), cd[2] | (cd[3] << 16), 0x7531);
+    const uint32_t b47 = __byte_perm(cd[4] | (cd[5] << 16), cd[6] | (cd[7] << 16), 0x7531);
+    const uint2 first = split ? make_uint2(a03, a47) : make_uint2(cd[0] | (cd[1] << 16), cd[2] | (cd[3] << 16));
+    const uint2 second = split ? make_uint2(b03, b47) : make_uint2(cd[4] | (cd[5] << 16), cd[6] | (cd[7] << 16));
+    if (split) {
+      *reinterpret_cast<uint2*>(dst + 8 * u) = first;
+      *reinterpret_cast<uint2*>(dst + 8 * u + half) = second;
+    } else {
+      *reinterpret_cast<uint4*>(dst + 16 * u) = make_uint4(first.x, first.y, second.x, second.y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int2 at = fsvd_rope::pair_at(8 * u + i, R, inter);
+      dst[at.x] = (uint8_t)(cd[i] & 0xffu);
+      dst[at.y] = (uint8_t)(cd[i] >> 8);
+    }
+  }
+}
+
+// Four codes at a larger scale: times f = old scale / new scale.
+__device__ __forceinline__ uint32_t rescaled(uint32_t x, float f) {
+  const float2 p = decode2(x & 0xffffu), q = decode2(x >> 16);
+  return code2(p.x * f, p.y * f) | (code2(q.x * f, q.y * f) << 16);
 }
 
 // One CTA per (sequence, block of the cache, group of kv heads): a tile of at most BLOCK tokens x DH of a head sits in
-// registers (bf16) between the maximum and the rounding, so that each input is read once and each code written once.
+// registers (bf16) between the maximum and the rounding, so that each input is read once and each code written once.  Keys
+// are turned in 64 bits, then rounded to 32 and 16: a rotated key falls on the same side of a rounding border as in
+// exact arithmetic.
+// Threads of a CTA and CTAs of an SM: the table of 128 tokens takes 152 KB, so one larger CTA instead of two.
+// (8192 tokens, 64 and 8 heads: 157 us with 256 threads, 91 with 512.)
+template <int BLOCK> constexpr int kAppendThreads = BLOCK == 128 ? 512 : 256;
+template <int BLOCK> constexpr int kAppendCtas = BLOCK == 128 ? 1 : 2;
 template <int DH, int BLOCK, bool WIDE>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
-  constexpr int U = DH / 16, ROWS = kThreads / U, NIT = (BLOCK + ROWS - 1) / ROWS;
-  extern __shared__ float4 tab[];   // [tokens][R / 2] cosine and sine as (c_hi, c_lo, s_hi, s_lo)
-  __shared__ float red[2][2][kThreads / 32];
+__global__ void __launch_bounds__(kAppendThreads<BLOCK>, kAppendCtas<BLOCK>) append_kernel(const AppendArgs a) {
+  constexpr int kThreads = kAppendThreads<BLOCK>, U = DH / 16, ROWS = kThreads / U, NIT = (BLOCK + ROWS - 1) / ROWS;
+  extern __shared__ double2 tab[];   // per token: cosine and sine of the pairs
+  __shared__ uint32_t red[2][2][kThreads / 32];
   const int tid = threadIdx.x, u = tid % U, r0 = tid / U;
   int idx = blockIdx.x;
   const int grp = idx % a.groups;
@@ -231,178 +317,250 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs a) {
   // (queries of tokens beyond the cache are rotated too: their range is not cut at the capacity)
   const int nq = (int)(min(end_ll, blk0 + BLOCK) - lo), n = max(0, hi - lo);
   const int R = a.rot.R, half = R >> 1, inter = a.rot.interleaved;
-  if (R) {
-    // Cosines and sines of the tile's tokens.  More than a few: of every eighth token and of steps 0..7, and the products of
-    // those (64 tokens: 16 evaluations in 64 bits a pair instead of 64).
-    auto put = [&](int i, double c, double s) {
-      const float ch = (float)c, sh = (float)s;
-      tab[i] = make_float4(ch, (float)(c - (double)ch), sh, (float)(s - (double)sh));
-    };
-    const int coarse = (nq + 7) / 8;
-    if (nq <= 8) {
-      for (int i = tid; i < nq * half; i += kThreads) {
-        const int t = i / half;
-        double c, s;
-        fsvd_rope::angle(lo + t, a.rot.inv_freq[i - t * half], a.rot.scale, c, s);
-        put(i, c, s);
-      }
-    } else {
-      double2* steps = reinterpret_cast<double2*>(tab + min(BLOCK, a.L) * half);   // [8 + coarse][half]
-      for (int i = tid; i < (8 + coarse) * half; i += kThreads) {
-        const int k = i / half;
-        double c, s;
-        fsvd_rope::angle(k < 8 ? k : lo + 8 * (k - 8), a.rot.inv_freq[i - k * half], k < 8 ? 1.0f : a.rot.scale, c, s);
-        steps[i] = make_double2(c, s);
-      }
-      __syncthreads();
-      for (int i = tid; i < nq * half; i += kThreads) {
-        const int t = i / half, p = i - t * half;
-        const double2 x = steps[(8 + (t >> 3)) * half + p], y = steps[(t & 7) * half + p];
-        put(i, x.x * y.x - x.y * y.y, x.y * y.x + x.x * y.y);
-      }
-    }
-    __syncthreads();
-  }
+  // pair p of a token sits in slot (p % 8) * units + p / 8: the lanes of a warp, a unit of eight pairs each, read neighbours
+  const int units = (half + 7) / 8, slots = 8 * units;
   const int Hk = a.c.Hk, nb = (a.c.S_max + BLOCK - 1) / BLOCK;
   const int hk0 = (int)((long long)Hk * grp / a.groups), hk1 = (int)((long long)Hk * (grp + 1) / a.groups);
-  const bool held = start > blk0;   // the block holds tokens already
-  int parity = 0;
-  for (int hk = hk0; hk < hk1 && n > 0; ++hk, parity ^= 1) {
-    uint32_t kreg[NIT][8], vreg[NIT][8];   // packed pairs (a, b)
-    float kmax = 0.0f, vmax = 0.0f;
+  uint32_t kreg[NIT][8], vreg[NIT][8];   // packed pairs (a, b)
+  auto fetch = [&](int hk) {
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
       const int t = r0 + it * ROWS;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) kreg[it][i] = vreg[it][i] = 0u;
       if (t < n) {
         const size_t off = (size_t)b * a.kv_batch + (size_t)(lo - start + t) * a.kv_token + (size_t)hk * DH;
-        float x[8], y[8];
-        fsvd_rope::load_unit<WIDE>(a.v + off, u, R, inter, x, y);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          vreg[it][i] = fsvd_rope::pack2(x[i], y[i]);
-          if (isfinite(x[i])) vmax = fmaxf(vmax, fabsf(x[i]));
-          if (isfinite(y[i])) vmax = fmaxf(vmax, fabsf(y[i]));
+        fsvd_rope::load_pairs<WIDE>(a.k + off, u, R, inter, kreg[it]);
+        fsvd_rope::load_pairs<WIDE>(a.v + off, u, R, inter, vreg[it]);
+      }
+    }
+  };
+  if (n > 0 && hk0 < hk1) fetch(hk0);   // (the first head is under way while the angles are formed)
+  if (R) {
+    // Cosines and sines of the tile's tokens.  More than a few: of every eighth token and of steps 0..7, and the products of
+    // those (64 tokens: 16 evaluations a pair instead of 64).
+    auto pair_of = [&](int slot) { return slot % units * 8 + slot / units; };
+    const int coarse = (nq + 7) / 8;
+    double2* steps = nq <= 8 ? tab : tab + min(BLOCK, a.L) * slots;   // [8 + coarse][slots]
+    for (int i = tid; i < (nq <= 8 ? nq : 8 + coarse) * slots; i += kThreads) {
+      const int k = i / slots, p = pair_of(i - k * slots);
+      if (p >= half) continue;
+      const bool step = nq > 8 && k < 8;
+      double c, s;
+      fsvd_rope::angle(step ? k : nq <= 8 ? lo + k : lo + 8 * (k - 8), a.rot.inv_freq[p], step ? 1.0f : a.rot.scale, c, s);
+      steps[i] = make_double2(c, s);
+    }
+    __syncthreads();
+    if (nq > 8) {
+      for (int s0 = tid % 32; s0 < slots; s0 += 32)
+        for (int t = tid / 32; t < nq; t += kThreads / 32) {
+          const double2 x = steps[(8 + (t >> 3)) * slots + s0], y = steps[(t & 7) * slots + s0];
+          tab[t * slots + s0] = make_double2(x.x * y.x - x.y * y.y, x.y * y.x + x.x * y.y);
         }
-        fsvd_rope::load_unit<WIDE>(a.k + off, u, R, inter, x, y);
+      __syncthreads();
+    }
+  }
+  const bool turns = 8 * u < half;
+  const double2* my_tab = tab + u;   // pair i of this unit: my_tab[token * slots + i * units]
+  const bool held = start > blk0;   // the block holds tokens already
+  int parity = 0;
+  for (int hk = hk0; hk < hk1 && n > 0; ++hk, parity ^= 1) {
+    const size_t si = ((size_t)b * Hk + hk) * nb + blk;
+    const float kold = held ? a.c.k_scale[si] : 0.0f, vold = held ? a.c.v_scale[si] : 0.0f;
+    if (turns) {
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) {
+        const int t = r0 + it * ROWS;
+        if (t >= n) break;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int p = 8 * u + i;
-          if (p < half) {
-            const float4 cs = tab[t * half + p];
-            const float x0 = x[i], y0 = y[i];
-            x[i] = turn(x0, y0, cs.x, cs.y, cs.z, cs.w);
-            y[i] = turn(y0, -x0, cs.x, cs.y, cs.z, cs.w);
-          }
-          kreg[it][i] = fsvd_rope::pack2(x[i], y[i]);
-          x[i] = __uint_as_float(kreg[it][i] << 16);
-          y[i] = __uint_as_float(kreg[it][i] & 0xffff0000u);
-          if (isfinite(x[i])) kmax = fmaxf(kmax, fabsf(x[i]));
-          if (isfinite(y[i])) kmax = fmaxf(kmax, fabsf(y[i]));
+          if (!WIDE && 8 * u + i >= half) break;
+          kreg[it][i] = turn_key(kreg[it][i], my_tab[t * slots + i * units]);
         }
       }
     }
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) {
-      kmax = fmaxf(kmax, __shfl_xor_sync(0xffffffffu, kmax, x));
-      vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, x));
-    }
+    Share ks, vs;
+    largest<NIT>(kreg, ks);
+    largest<NIT>(vreg, vs);
+    const uint32_t kwarp = __reduce_max_sync(0xffffffffu, ks.top), vwarp = __reduce_max_sync(0xffffffffu, vs.top);
     if ((tid & 31) == 0) {
-      red[parity][0][tid >> 5] = kmax;
-      red[parity][1][tid >> 5] = vmax;
+      red[parity][0][tid >> 5] = kwarp;
+      red[parity][1][tid >> 5] = vwarp;
     }
-    const size_t si = ((size_t)b * Hk + hk) * nb + blk;
-    const float kold = held ? a.c.k_scale[si] : 0.0f, vold = held ? a.c.v_scale[si] : 0.0f;
     __syncthreads();   // (two halves of `red` in turn: the next head writes the other one)
+    uint32_t kbits = 0, vbits = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
-      kmax = fmaxf(kmax, red[parity][0][w]);
-      vmax = fmaxf(vmax, red[parity][1][w]);
+      kbits = max(kbits, red[parity][0][w]);
+      vbits = max(vbits, red[parity][1][w]);
     }
-    const int ke = scale_exponent(kmax), ve = scale_exponent(vmax);
-    const float ks = fmaxf(kold, two_to(ke)), vs = fmaxf(vold, two_to(ve));
+    const float kscale = fmaxf(kold, two_to(scale_exponent(__uint_as_float(kbits << 16))));
+    const float vscale = fmaxf(vold, two_to(scale_exponent(__uint_as_float(vbits << 16))));
     const size_t base = (((size_t)b * Hk + hk) * a.c.S_max + (size_t)blk0) * DH;
     uint8_t* kc = reinterpret_cast<uint8_t*>(a.c.k8) + base;
     uint8_t* vc = reinterpret_cast<uint8_t*>(a.c.v8) + base;
     if (held) {   // a larger scale: round what the block holds once more
       const int old_bytes = (int)(start - blk0) * DH;
       for (int which = 0; which < 2; ++which) {
-        const float was = which ? vold : kold, now = which ? vs : ks;
+        const float was = which ? vold : kold, now = which ? vscale : kscale;
         if (!(now > was)) continue;
         uint32_t* w = reinterpret_cast<uint32_t*>(which ? vc : kc);
         const float f = was / now;
         for (int i = tid; i < old_bytes / 4; i += kThreads) {
-          const uint32_t x = w[i];
-          const float2 p = decode2(x & 0xffffu), q = decode2(x >> 16);
-          w[i] = code2(p.x * f, p.y * f) | (code2(q.x * f, q.y * f) << 16);
+          w[i] = rescaled(w[i], f);
         }
       }
     }
-    const float ki = 1.0f / ks, vi = 1.0f / vs;
+    const float ki = 1.0f / kscale, vi = 1.0f / vscale;
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
       const int t = r0 + it * ROWS;
       if (t < n) {
         const size_t row = (size_t)(lo - blk0 + t) * DH;
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-          uint8_t* dst = (which ? vc : kc) + row;
-          const float inv = which ? vi : ki;
-          uint32_t cd[8];   // codes of the pairs: low byte a, high byte b
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t w = which ? vreg[it][i] : kreg[it][i];
-            float x = __uint_as_float(w << 16) * inv, y = __uint_as_float(w & 0xffff0000u) * inv;
-            if (inv <= 0x1p-120f) {   // 256 * 2^120 is no 32-bit number any more
-              x = fabsf(x) > 240.0f && isfinite(x) ? copysignf(240.0f, x) : x;
-              y = fabsf(y) > 240.0f && isfinite(y) ? copysignf(240.0f, y) : y;
-            }
-            cd[i] = code2(x, y);
-          }
-          if constexpr (WIDE) {
-            const bool split = !inter && 16 * u < R;
-            uint2 first, second;
-            const uint32_t a03 = __byte_perm(__byte_perm(cd[0], cd[1], 0x0040), __byte_perm(cd[2], cd[3], 0x0040), 0x5410);
-            const uint32_t a47 = __byte_perm(__byte_perm(cd[4], cd[5], 0x0040), __byte_perm(cd[6], cd[7], 0x0040), 0x5410);
-            const uint32_t b03 = __byte_perm(__byte_perm(cd[0], cd[1], 0x0051), __byte_perm(cd[2], cd[3], 0x0051), 0x5410);
-            const uint32_t b47 = __byte_perm(__byte_perm(cd[4], cd[5], 0x0051), __byte_perm(cd[6], cd[7], 0x0051), 0x5410);
-            first = split ? make_uint2(a03, a47) : make_uint2(cd[0] | (cd[1] << 16), cd[2] | (cd[3] << 16));
-            second = split ? make_uint2(b03, b47) : make_uint2(cd[4] | (cd[5] << 16), cd[6] | (cd[7] << 16));
-            *reinterpret_cast<uint2*>(dst + (split ? 8 * u : 16 * u)) = first;
-            *reinterpret_cast<uint2*>(dst + (split ? 8 * u + half : 16 * u + 8)) = second;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int2 at = fsvd_rope::pair_at(8 * u + i, R, inter);
-              dst[at.x] = (uint8_t)(cd[i] & 0xffu);
-              dst[at.y] = (uint8_t)(cd[i] >> 8);
-            }
-          }
-        }
+        uint32_t cd[8];   // codes of the pairs: low byte a, high byte b
+        codes_of(kreg[it], ki, ks.odd, cd);
+        store_codes<WIDE>(kc + row, cd, u, R, inter);
+        codes_of(vreg[it], vi, vs.odd, cd);
+        store_codes<WIDE>(vc + row, cd, u, R, inter);
       }
     }
     if (tid == 0) {
-      a.c.k_scale[si] = ks;
-      a.c.v_scale[si] = vs;
+      a.c.k_scale[si] = kscale;
+      a.c.v_scale[si] = vscale;
     }
+    if (hk + 1 < hk1) fetch(hk + 1);
   }
   if (!a.q) return;
+  // queries: a thread keeps its token's cosines and sines while it goes through the heads, two at a time
   const int h0 = (int)((long long)a.H * grp / a.groups), h1 = (int)((long long)a.H * (grp + 1) / a.groups);
-  for (int i = r0; i < nq * (h1 - h0); i += ROWS) {
-    const int t = i / (h1 - h0), h = h0 + i - t * (h1 - h0);
-    const size_t tok = (size_t)(lo - start + t);
-    float x[8], y[8];
-    fsvd_rope::load_unit<WIDE>(a.q + (size_t)b * a.q_batch + tok * a.q_token + (size_t)h * DH, u, R, inter, x, y);
+  for (int t = r0; t < nq; t += ROWS) {
+    float c[8], s[8];
+    if (turns) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int p = 8 * u + e;
-      if (p < half) {
-        const float4 cs = tab[t * half + p];
-        const float x0 = x[e], y0 = y[e];
-        x[e] = x0 * cs.x - y0 * cs.z;
-        y[e] = y0 * cs.x + x0 * cs.z;
+      for (int i = 0; i < 8; ++i) {
+        const bool in = WIDE || 8 * u + i < half;
+        const double2 cs = my_tab[t * slots + (in ? i * units : 0)];
+        c[i] = (float)cs.x;
+        s[i] = (float)cs.y;
       }
     }
-    fsvd_rope::store_unit<WIDE>(a.q_out + (((size_t)b * a.L + tok) * a.H + h) * DH, u, R, inter, x, y);
+    const size_t tok = (size_t)(lo - start + t);
+    const __nv_bfloat16* src = a.q + (size_t)b * a.q_batch + tok * a.q_token;
+    __nv_bfloat16* dst = a.q_out + ((size_t)b * a.L + tok) * a.H * DH;
+    constexpr int N = 2;
+    for (int h = h0; h < h1; h += N) {
+      uint32_t w[N][8];
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (h + k < h1) fsvd_rope::load_pairs<WIDE>(src + (size_t)(h + k) * DH, u, R, inter, w[k]);
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (h + k < h1) {
+          if (turns) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if (!WIDE && 8 * u + i >= half) break;
+              w[k][i] = turn_query(w[k][i], c[i], s[i]);
+            }
+          }
+          fsvd_rope::store_pairs<WIDE>(dst + (size_t)(h + k) * DH, u, R, inter, w[k]);
+        }
+    }
+  }
+}
+
+// A single token per sequence: the rows of a CTA are heads, not tokens, so that every thread has a share (the kernel above
+// would leave all rows but one idle: a step of 128 sequences with 32 heads took 32.2 us, here 5.0; of 8 sequences 4.4 and 3.8).
+// Almost all of a small step is latency: one load, one sine in 64 bits (about 1500 clocks), one store.
+template <int DH, bool WIDE>
+__global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs a) {
+  constexpr int U = DH / 16, ROWS = kThreads / U;
+  __shared__ double2 tab[DH / 2];   // pair p in slot (p % 8) * units + p / 8
+  const int tid = threadIdx.x, u = tid % U, lane = tid & 31;
+  const int grp = blockIdx.x % a.groups, b = blockIdx.x / a.groups;
+  const int R = a.rot.R, half = R >> 1, inter = a.rot.interleaved, units = (half + 7) / 8, BLOCK = a.c.block;
+  const int Hk = a.c.Hk, nb = (a.c.S_max + BLOCK - 1) / BLOCK;
+  const int hk = (int)((long long)Hk * grp / a.groups) + tid / U, h = (int)((long long)a.H * grp / a.groups) + tid / U;
+  const bool has_q = h < (int)((long long)a.H * (grp + 1) / a.groups);
+  pdl_begin();
+  if (a.new_lens && a.new_lens[b] <= 0) return;
+  const int start = max(a.seqlens[b], 0);
+  if (start >= a.c.S_max && grp == 0 && tid == 0) atomicCAS(a.status, (int)DS_OK, (int)DS_CACHE_FULL);
+  const bool has_kv = start < a.c.S_max && hk < (int)((long long)Hk * (grp + 1) / a.groups);
+  const int blk = start / BLOCK, old = start - blk * BLOCK;   // tokens that the block holds already
+  const size_t si = ((size_t)b * Hk + hk) * nb + blk;
+  uint32_t kw[1][8], vw[1][8], qw[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) kw[0][i] = vw[0][i] = 0u;
+  float kold = 0.0f, vold = 0.0f;
+  if (has_kv) {
+    const size_t off = (size_t)b * a.kv_batch + (size_t)hk * DH;
+    fsvd_rope::load_pairs<WIDE>(a.k + off, u, R, inter, kw[0]);
+    fsvd_rope::load_pairs<WIDE>(a.v + off, u, R, inter, vw[0]);
+    if (old) {
+      kold = a.c.k_scale[si];
+      vold = a.c.v_scale[si];
+    }
+  }
+  if (has_q) fsvd_rope::load_pairs<WIDE>(a.q + (size_t)b * a.q_batch + (size_t)h * DH, u, R, inter, qw);
+  if (tid < half) {
+    double c, s;
+    fsvd_rope::angle(start, a.rot.inv_freq[tid], a.rot.scale, c, s);
+    tab[(tid & 7) * units + (tid >> 3)] = make_double2(c, s);
+  }
+  __syncthreads();
+  if (8 * u < half) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (!WIDE && 8 * u + i >= half) break;
+      const double2 cs = tab[i * units + u];
+      if (has_kv) kw[0][i] = turn_key(kw[0][i], cs);
+      if (has_q) qw[i] = turn_query(qw[i], (float)cs.x, (float)cs.y);
+    }
+  }
+  if (has_q) fsvd_rope::store_pairs<WIDE>(a.q_out + ((size_t)b * a.H + h) * DH, u, R, inter, qw);
+  Share ks, vs;
+  largest<1>(kw, ks);
+  largest<1>(vw, vs);
+  uint32_t kbits = ks.top, vbits = vs.top;
+#pragma unroll
+  for (int d = 1; d < U; d *= 2) {
+    kbits = max(kbits, __shfl_xor_sync(0xffffffffu, kbits, d));
+    vbits = max(vbits, __shfl_xor_sync(0xffffffffu, vbits, d));
+  }
+  const float kscale = fmaxf(kold, two_to(scale_exponent(__uint_as_float(kbits << 16))));
+  const float vscale = fmaxf(vold, two_to(scale_exponent(__uint_as_float(vbits << 16))));
+  const size_t base = (((size_t)b * Hk + hk) * a.c.S_max + (size_t)blk * BLOCK) * DH;
+  if (has_kv) {
+    uint32_t cd[8];
+    codes_of(kw[0], 1.0f / kscale, ks.odd, cd);
+    store_codes<WIDE>(reinterpret_cast<uint8_t*>(a.c.k8) + base + (size_t)old * DH, cd, u, R, inter);
+    codes_of(vw[0], 1.0f / vscale, vs.odd, cd);
+    store_codes<WIDE>(reinterpret_cast<uint8_t*>(a.c.v8) + base + (size_t)old * DH, cd, u, R, inter);
+    if (u == 0) {
+      a.c.k_scale[si] = kscale;
+      a.c.v_scale[si] = vscale;
+    }
+  }
+  // A larger scale: round what the block holds once more, a warp together for each of its heads.
+  for (int which = 0; which < 2; ++which) {
+    const float was = which ? vold : kold, now = which ? vscale : kscale;
+    for (uint32_t grown = __ballot_sync(0xffffffffu, has_kv && old && u == 0 && now > was); grown; grown &= grown - 1) {
+      const int from = __ffs(grown) - 1;
+      const float f = __shfl_sync(0xffffffffu, was / now, from);
+      uint8_t* codes = reinterpret_cast<uint8_t*>(which ? a.c.v8 : a.c.k8) + __shfl_sync(0xffffffffu, base, from);
+      uint4* p = reinterpret_cast<uint4*>(codes);
+      for (int i = lane; i < old * DH / 16; i += 128) {
+        uint4 x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + 32 * e < old * DH / 16) x[e] = p[i + 32 * e];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + 32 * e < old * DH / 16)
+            p[i + 32 * e] = make_uint4(rescaled(x[e].x, f), rescaled(x[e].y, f), rescaled(x[e].z, f), rescaled(x[e].w, f));
+      }
+    }
   }
 }
 
@@ -532,18 +690,58 @@ static int launch_attn(const CUtensorMap& km, const CUtensorMap& vm, const fsvd_
   return launch_attn<DH, 16>(km, vm, a, stream);
 }
 
+static int launch_rope(RopeArgs& a, int dtype, void* stream) {
+  // One wave of four CTAs per SM, up to 32 tokens each; a few tokens are shared out by heads.
+  const int all = a.H + a.Hk, T = a.T;
+  a.tokens = std::min(kRopeTokens, (T + 4 * sm_count() - 1) / (4 * sm_count()));
+  const int ctas = (T + a.tokens - 1) / a.tokens, splits = std::max(1, std::min({2 * sm_count() / ctas, all * (a.Dh / 16) / kThreads, 8}));
+  a.heads = (all + splits - 1) / splits;
+  const dim3 grid(ctas, (all + a.heads - 1) / a.heads);
+  const size_t smem = (size_t)a.tokens * ((a.rot.R / 2 + 7) / 8 * 8) * sizeof(float2);
+  const bool wide = a.rot.R % 16 == 0;
+  if (dtype == FSVD_DTYPE_F32)
+    return wide ? launch(rope_kernel<float, true>, grid, kThreads, smem, stream, a)
+                : launch(rope_kernel<float, false>, grid, kThreads, smem, stream, a);
+  return wide ? launch(rope_kernel<__nv_bfloat16, true>, grid, kThreads, smem, stream, a)
+              : launch(rope_kernel<__nv_bfloat16, false>, grid, kThreads, smem, stream, a);
+}
+
 template <int DH, int BLOCK>
-static int launch_append(const AppendArgs& a, size_t smem, unsigned grid, void* stream) {
-  if (a.rot.R % 16 == 0) return launch(append_kernel<DH, BLOCK, true>, dim3(grid), kThreads, smem, stream, a);
-  return launch(append_kernel<DH, BLOCK, false>, dim3(grid), kThreads, smem, stream, a);
+static int launch_append(AppendArgs a, void* stream) {
+  // Heads of a CTA share the table of angles.  Of the groupings by halves the one with the least waves x (planes of a CTA +
+  // kTable), the table being worth about as much as four planes (keys, values or queries of a head).  32 heads of 128, us
+  // beside as few groups as give each SM two CTAs: 1024 tokens 15.1 (19.7), 2041 tokens 28.9 (32.3), 2 x 1024 with 16 heads
+  // of 64 9.3 (12.6); 4 x 301 with 64 and 8 heads 15.9 (15.6).
+  constexpr int kTable = 4;
+  const long long tiles = (long long)a.c.B * ((a.L + BLOCK - 1) / BLOCK), fit = (long long)kAppendCtas<BLOCK> * sm_count();
+  auto cost = [&](int g) {
+    return (tiles * g + fit - 1) / fit * (2 * ((a.c.Hk + g - 1) / g) + (a.H + g - 1) / g + (a.rot.R ? kTable : 0));
+  };
+  a.groups = std::max(a.H, a.c.Hk);
+  for (int g = a.groups; g > 1 && g % 2 == 0; g /= 2)
+    if (cost(g / 2) < cost(a.groups)) a.groups = g / 2;
+  const long long grid = (long long)a.c.B * a.nblk * a.groups;
+  if (grid > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many tokens for one call");
+  const int tile = std::min(BLOCK, a.L);
+  const size_t smem = (size_t)((a.rot.R / 2 + 7) / 8 * 8) * (tile + (tile > 8 ? 8 + (tile + 7) / 8 : 0)) * sizeof(double2);
+  return a.rot.R % 16 == 0 ? launch(append_kernel<DH, BLOCK, true>, dim3((unsigned)grid), kAppendThreads<BLOCK>, smem, stream, a)
+                           : launch(append_kernel<DH, BLOCK, false>, dim3((unsigned)grid), kAppendThreads<BLOCK>, smem, stream, a);
 }
 template <int DH>
-static int launch_append(const AppendArgs& a, size_t smem, unsigned grid, void* stream) {
+static int launch_append(AppendArgs a, void* stream) {
+  if (a.L == 1) {
+    constexpr int rows = kThreads / (DH / 16);
+    a.groups = (std::max(a.H, a.c.Hk) + rows - 1) / rows;
+    const long long grid = (long long)a.c.B * a.groups;
+    if (grid > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many heads for one call");
+    return a.rot.R % 16 == 0 ? launch(append_step_kernel<DH, true>, dim3((unsigned)grid), kThreads, 0, stream, a)
+                             : launch(append_step_kernel<DH, false>, dim3((unsigned)grid), kThreads, 0, stream, a);
+  }
   switch (a.c.block) {
-    case 16: return launch_append<DH, 16>(a, smem, grid, stream);
-    case 32: return launch_append<DH, 32>(a, smem, grid, stream);
-    case 64: return launch_append<DH, 64>(a, smem, grid, stream);
-    default: return launch_append<DH, 128>(a, smem, grid, stream);
+    case 16: return launch_append<DH, 16>(a, stream);
+    case 32: return launch_append<DH, 32>(a, stream);
+    case 64: return launch_append<DH, 64>(a, stream);
+    default: return launch_append<DH, 128>(a, stream);
   }
 }
 
@@ -572,18 +770,7 @@ int fsvd_rope_qk(const void* q, long long q_stride, const void* k, long long k_s
   a.q_stride = q_stride; a.k_stride = k_stride; a.positions = positions;
   a.rot = Rotary{inv_freq, rotary_dim, interleaved != 0, rope_scale};
   a.T = T; a.H = H; a.Hk = Hk; a.Dh = Dh;
-  // One wave of four CTAs per SM, up to 32 tokens each; a few tokens are shared out by heads.
-  a.tokens = std::min(32, (T + 4 * sm_count() - 1) / (4 * sm_count()));
-  const int ctas = (T + a.tokens - 1) / a.tokens, splits = std::max(1, std::min({2 * sm_count() / ctas, (H + Hk) * (Dh / 16) / kThreads, 8}));
-  a.heads = (H + Hk + splits - 1) / splits;
-  const dim3 grid((T + a.tokens - 1) / a.tokens, (H + Hk + a.heads - 1) / a.heads);
-  const size_t smem = (size_t)a.tokens * (rotary_dim / 2) * sizeof(float2);
-  const bool wide = rotary_dim % 16 == 0;
-  if (dtype == FSVD_DTYPE_F32)
-    return wide ? launch(rope_kernel<float, true>, grid, kThreads, smem, stream, a)
-                : launch(rope_kernel<float, false>, grid, kThreads, smem, stream, a);
-  return wide ? launch(rope_kernel<__nv_bfloat16, true>, grid, kThreads, smem, stream, a)
-              : launch(rope_kernel<__nv_bfloat16, false>, grid, kThreads, smem, stream, a);
+  return launch_rope(a, dtype, stream);
 }
 
 size_t fsvd_kv8_workspace_bytes(int B, int H, int Hk, int Dh, int S_max) {
@@ -620,15 +807,8 @@ int fsvd_kv8_append(const fsvd_kv8* cache, const void* k, const void* v, long lo
   a.H = q ? H : 0; a.L = L;
   const int BLOCK = cache->block;
   a.nblk = (int)(((long long)L + BLOCK - 2) / BLOCK + 1);
-  // Heads of a CTA share the table of angles: with rotation as few groups as still give every SM two CTAs.
-  a.groups = cache->Hk;
-  if (inv_freq)
-    while (a.groups % 2 == 0 && (long long)cache->B * a.nblk * (a.groups / 2) >= 2ll * sm_count()) a.groups /= 2;
-  const long long grid = (long long)cache->B * a.nblk * a.groups;
-  if (grid > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many tokens for one call");
-  const int tile = std::min(BLOCK, L);
-  const size_t smem = (size_t)(a.rot.R / 2) * (tile * sizeof(float4) + (tile > 8 ? (8 + (tile + 7) / 8) * sizeof(double2) : 0));
-  return cache->Dh == 64 ? launch_append<64>(a, smem, (unsigned)grid, stream) : launch_append<128>(a, smem, (unsigned)grid, stream);
+  if ((long long)cache->B * L > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many tokens for one call");
+  return cache->Dh == 64 ? launch_append<64>(a, stream) : launch_append<128>(a, stream);
 }
 
 int fsvd_kv8_load(const fsvd_kv8* cache, int start, int length, const int* cache_seqlens, int seqlen_add, void* k_out,

@@ -107,4 +107,49 @@ __device__ __forceinline__ void store_unit(T* row, int u, int R, int interleaved
   }
 }
 
+// The same for bf16 rows as packed pairs: a in the low half of a word, b in the high one.
+template <bool WIDE>
+__device__ __forceinline__ void load_pairs(const __nv_bfloat16* row, int u, int R, int interleaved, uint32_t (&w)[8]) {
+  if constexpr (WIDE) {
+    const bool split = !interleaved && 16 * u < R;
+    const uint4 x = *reinterpret_cast<const uint4*>(row + (split ? 8 * u : 16 * u));
+    const uint4 y = *reinterpret_cast<const uint4*>(row + (split ? 8 * u + (R >> 1) : 16 * u + 8));
+    const uint32_t p[4] = {x.x, x.y, x.z, x.w}, q[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[2 * i] = split ? __byte_perm(p[i], q[i], 0x5410) : i < 2 ? p[2 * i] : q[2 * i - 4];
+      w[2 * i + 1] = split ? __byte_perm(p[i], q[i], 0x7632) : i < 2 ? p[2 * i + 1] : q[2 * i - 3];
+    }
+  } else {
+    const uint16_t* r = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int2 at = pair_at(8 * u + i, R, interleaved);
+      w[i] = (uint32_t)r[at.x] | ((uint32_t)r[at.y] << 16);
+    }
+  }
+}
+template <bool WIDE>
+__device__ __forceinline__ void store_pairs(__nv_bfloat16* row, int u, int R, int interleaved, const uint32_t (&w)[8]) {
+  if constexpr (WIDE) {
+    const bool split = !interleaved && 16 * u < R;
+    uint32_t p[4], q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      p[i] = split ? __byte_perm(w[2 * i], w[2 * i + 1], 0x5410) : w[i];
+      q[i] = split ? __byte_perm(w[2 * i], w[2 * i + 1], 0x7632) : w[4 + i];
+    }
+    *reinterpret_cast<uint4*>(row + (split ? 8 * u : 16 * u)) = make_uint4(p[0], p[1], p[2], p[3]);
+    *reinterpret_cast<uint4*>(row + (split ? 8 * u + (R >> 1) : 16 * u + 8)) = make_uint4(q[0], q[1], q[2], q[3]);
+  } else {
+    uint16_t* r = reinterpret_cast<uint16_t*>(row);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int2 at = pair_at(8 * u + i, R, interleaved);
+      r[at.x] = (uint16_t)(w[i] & 0xffffu);
+      r[at.y] = (uint16_t)(w[i] >> 16);
+    }
+  }
+}
+
 }  // namespace fsvd_rope
