@@ -160,6 +160,14 @@ class DecodeEngine:
         self._reserve_positions(int(n_steps))
         check(self.lib.fsvd_model_step(self.handle, int(n_steps), torch.cuda.current_stream().cuda_stream))
 
+    def sample(self, uniforms: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
+        """Draws the next token of every sequence from the logits of the last step or prompt (``ops.sample``: uniforms
+        float32 [B] in [0, 1), settings as numbers or tensors with one value per sequence) and makes it the input of the
+        next step, in place of the largest logit that the step chose.  Returns the tokens (int32 [B], the engine's own
+        buffer: the next step overwrites it); no synchronisation.  ``token_log`` keeps the step's own choice."""
+        return ops.sample(self.logits, uniforms, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
+                          out=self.tokens)[0]
+
     def reset(self) -> None:
         self._fill_positions(0)
         self.step_counter.zero_()
@@ -423,6 +431,20 @@ class EngineGroup:
         for e in self.engines:
             e.prefill(prompt[o:o + e.B])
             o += e.B
+
+    def sample(self, uniforms: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> torch.Tensor:
+        """``DecodeEngine.sample`` for all sequences; a copy of their tokens."""
+        if tuple(uniforms.shape) != (self.B,):
+            raise ValueError(f"uniforms must be [{self.B}], got {list(uniforms.shape)}")
+        settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        for name, x in settings.items():
+            if torch.is_tensor(x) and tuple(x.shape) != (self.B,):
+                raise ValueError(f"{name} must be [{self.B}], got {list(x.shape)}")
+        o = 0
+        for e in self.engines:
+            e.sample(uniforms[o:o + e.B], **{n: x[o:o + e.B] if torch.is_tensor(x) else x for n, x in settings.items()})
+            o += e.B
+        return self.tokens
 
     def last_tokens(self, n: int) -> torch.Tensor:
         return torch.cat([e.last_tokens(n) for e in self.engines], dim=1)

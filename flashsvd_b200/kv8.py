@@ -2,7 +2,8 @@
 
 ``KV8Cache`` holds e4m3 codes with one power-of-two scale per block of tokens and kv head; ``ops.kv8_append`` writes
 it, ``ops.kv8_load`` reads it back as bfloat16, ``ops.flash_decode_kv8`` attends over it.  Half the bytes of the bf16
-cache of ``runtime.FlashSVDV15DenseKVCache``, for the same number of tokens.
+cache of ``runtime.FlashSVDV15DenseKVCache``, for the same number of tokens; ``runtime.FlashSVDV15KV8Cache`` holds one per
+layer of a model.
 """
 from __future__ import annotations
 
@@ -62,7 +63,7 @@ def rotary(rotary_dim: int, *, theta: float = 10000.0, scaling: str = "none", fa
     return Rotary(f.to(device), interleaved, scale)
 
 
-@dataclass
+@dataclass(frozen=True)
 class KV8Cache:
     """``k`` / ``v`` [B, Hk, S_max, Dh] float8_e4m3fn codes (a head's tokens lie together: a tile of them is one piece
     of memory), ``k_scale`` / ``v_scale`` [B, Hk, ceil(S_max / block)] float32.  A code stands for code * scale."""
@@ -72,7 +73,7 @@ class KV8Cache:
     k_scale: torch.Tensor
     v_scale: torch.Tensor
     block: int = 64
-    struct: FsvdKv8 = field(init=False, repr=False)
+    struct: FsvdKv8 = field(init=False, repr=False, compare=False)
 
     def __post_init__(self):
         k, v, ks, vs, block = self.k, self.v, self.k_scale, self.v_scale, self.block
@@ -92,14 +93,17 @@ class KV8Cache:
             raise ValueError("the codes are float8_e4m3fn tensors")
         want = (B, Hk, -(-S // block))
         if ks.shape != want or vs.shape != want or ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
-            raise ValueError(f"k_scale and v_scale must be float32 {want}, got {ks.dtype} {tuple(ks.shape)} and {vs.dtype} {tuple(vs.shape)}")
-        self.index = index = k.get_device()
+            raise ValueError(f"k_scale and v_scale must be float32 {want}, got {ks.dtype} {tuple(ks.shape)} and {vs.dtype} "
+                             f"{tuple(vs.shape)}")
+        index = k.get_device()
         if index < 0 or not (index == v.get_device() == ks.get_device() == vs.get_device()):
             raise ValueError("the cache is CUDA tensors of one device (there is no CPU path)")
         if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
             raise ValueError("the cache needs contiguous tensors")
-        self.struct = FsvdKv8(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), B, Hk, S, Dh, block)
-        self.ref = C.byref(self.struct)
+        put = object.__setattr__   # (frozen: the addresses below are those of the tensors above)
+        put(self, "index", index)
+        put(self, "struct", FsvdKv8(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), B, Hk, S, Dh, block))
+        put(self, "ref", C.byref(self.struct))
 
     @classmethod
     def empty(cls, batch: int, max_len: int, num_kv_heads: int, head_dim: int, *, block: int = 64, device="cuda") -> "KV8Cache":

@@ -107,6 +107,7 @@ class LlamaRotaryEmbedding(nn.Module):
         self.dim, self.max_position_embeddings, self.base = int(dim), int(max_position_embeddings), float(base)
         inv = 1.0 / (self.base ** (torch.arange(0, self.dim, 2, dtype=torch.float32, device=device) / self.dim))
         self.register_buffer("inv_freq", inv, persistent=False)
+        self._inv_freq64: dict = {}
 
     @torch.no_grad()
     def forward(self, x: torch.Tensor, position_ids: Optional[torch.Tensor] = None, seq_len: Optional[int] = None):
@@ -117,6 +118,14 @@ class LlamaRotaryEmbedding(nn.Module):
         freqs = pos[..., None] * self.inv_freq.to(x.device)
         emb = torch.cat([freqs, freqs], dim=-1)
         return emb.cos().to(x.dtype), emb.sin().to(x.dtype)
+
+    @torch.no_grad()
+    def rotate(self, q: torch.Tensor, k: Optional[torch.Tensor], position_ids: torch.Tensor):
+        """q [T, H, dim] and k [T, Hk, dim] (or None) at positions [T], by ``ops.rope_qk``: angles in 64 bits, no tables."""
+        key = str(q.device)
+        if key not in self._inv_freq64:
+            self._inv_freq64[key] = self.base ** (-torch.arange(0, self.dim, 2, dtype=torch.float64, device=q.device) / self.dim)
+        return ops.rope_qk(q, k, position_ids.to(device=q.device, dtype=torch.int32), self._inv_freq64[key])
 
 
 def enable_flashsvd_llama_layer_tail_cuda_graph() -> bool:
@@ -220,6 +229,10 @@ class SVD_LlamaAttention(_WithWorkspace):
         del cache_bindings
         x, cache = hidden_states, past_key_value
         B, L, d = x.shape
+        if getattr(cache, "holds_codes", False):
+            if L != 1:
+                raise ValueError("decode path: CUDA hidden state [B, 1, d]")
+            return self._kv8_forward(x, cache, cache_position, advance=advance_cache)
         if L != 1 or not _decode_ok(x):
             raise ValueError("decode path: CUDA hidden state [B, 1, d] with B <= 8 (bf16) or 4 (fp32)")
         H, Hk, Dh, li = self.num_heads, self.num_key_value_heads, self.head_dim, self.layer_idx
@@ -252,14 +265,55 @@ class SVD_LlamaAttention(_WithWorkspace):
             cache.advance_after_fa2(li, q_len=1, cache_position=cache_position)
         return y.reshape(B, 1, d)
 
+    def _kv8_forward(self, x, cache, cache_position=None, *, advance: bool = True):
+        """Attention output [B, L, d] over an 8-bit cache: keys and queries are rotated, keys and values rounded to codes
+        as they are appended; a single token attends over the codes, a prompt over what is read back of them."""
+        if not x.is_cuda:
+            raise RuntimeError("flashsvd_b200 modules run on CUDA tensors only (there is no CPU path)")
+        if x.dtype != torch.bfloat16:
+            raise ValueError(f"the 8-bit cache serves bfloat16 models, got {x.dtype}")
+        B, L, d = x.shape
+        H, Hk, Dh, li = self.num_heads, self.num_key_value_heads, self.head_dim, self.layer_idx
+        own = _decode_ok(x)   # the sizes that the projection kernels take
+        ws = None
+        if own:
+            key = (str(x.device), x.dtype, B, "kv8")
+            if key not in self._ws:
+                self._ws[key] = ops.make_workspace(
+                    ops.make_dims(dtype=x.dtype, B=B, d=d, H=H, Hk=Hk, Dh=Dh, Rq=self.q_u_proj.in_features,
+                                  Rk=self.k_u_proj.in_features, Rv=self.v_u_proj.in_features,
+                                  Ro=self.o_v_proj.out_features), x.device)
+            ws = self._ws[key]
+
+        def project(y, v, u):
+            return ops.lowrank_proj(y.reshape(B, -1).contiguous(), v.weight, u.weight, ws).view(B, 1, -1) if own else u(v(y))
+
+        q = project(x, self.q_v_proj, self.q_u_proj).view(B, L, H, Dh)
+        k = project(x, self.k_v_proj, self.k_u_proj).view(B, L, Hk, Dh)
+        v = project(x, self.v_v_proj, self.v_u_proj).view(B, L, Hk, Dh)
+        if L == 1:
+            a = cache.decode_step(q, k, v, li, cache_position=cache_position, advance=advance)
+        else:
+            _, start, q = cache.append(k, v, li, query_states=q, cache_position=cache_position, advance=advance)
+            kk, vv = ops.kv8_load(cache.layer(li, B), 0, start + L)
+            if Hk != H:
+                kk, vv = kk.repeat_interleave(H // Hk, 1), vv.repeat_interleave(H // Hk, 1)
+            pos = torch.arange(start, start + L, device=x.device)
+            mask = torch.arange(start + L, device=x.device)[None, :] <= pos[:, None]
+            a = F.scaled_dot_product_attention(q.transpose(1, 2), kk, vv, attn_mask=mask[None, None], scale=1.0 / math.sqrt(Dh))
+            a = a.transpose(1, 2)
+        return project(a.reshape(B, L, H * Dh), self.o_v_proj, self.o_u_proj)
+
     def forward(self, hidden_states: torch.Tensor, attention_mask=None, position_ids=None, past_key_values=None,
                 cache_position: Optional[torch.Tensor] = None, position_embeddings=None, **kwargs):
         """Returns (attn_output[B, L, d], None) like the transformers attention protocol.
-        ``past_key_values`` is a ``runtime.FlashSVDV15DenseKVCache``."""
+        ``past_key_values`` is a ``runtime.FlashSVDV15DenseKVCache``, or a ``runtime.FlashSVDV15KV8Cache``."""
         x, cache = hidden_states, past_key_values
         if cache is None:
             raise ValueError("SVD_LlamaAttention needs past_key_values (a FlashSVDV15DenseKVCache)")
         B, L, d = x.shape
+        if getattr(cache, "holds_codes", False):
+            return self._kv8_forward(x, cache, cache_position), None
         H, Hk, Dh, li = self.num_heads, self.num_key_value_heads, self.head_dim, self.layer_idx
         cache._ensure_layer_spec(li, h=Hk, dh=Dh)
         cos, sin = cache.get_rope_tables(cache.max_cache_len, Dh, device=x.device, dtype=x.dtype)

@@ -293,6 +293,198 @@ class FlashSVDV15DenseKVCache(_CacheBase):
         return out
 
 
+class FlashSVDV15KV8Cache(_CacheBase):
+    """``FlashSVDV15DenseKVCache`` in 8 bits, for bfloat16 models on CUDA: ``layers8[l]`` is a ``kv8.KV8Cache`` (e4m3 codes,
+    a power-of-two scale per ``block`` tokens and kv head), shaped on first use.  Keys are stored after the rotation
+    ``rotary`` (a ``kv8.Rotary``; default: all dimensions, ``config.rope_theta``), whose angles are formed in 64 bits.
+    Tokens are appended at the end: writing in front of it cuts the sequence there."""
+
+    is_compileable = False
+    holds_codes = True
+
+    def __init__(self, config, *, max_batch_size: int, max_cache_len: int, device=None, block: int = 64, rotary=None,
+                 layer_device_map: Optional[dict] = None) -> None:
+        try:
+            super().__init__(layers=[])
+        except TypeError:
+            super().__init__()
+        self._max_batch_size, self._max_cache_len, self._block = int(max_batch_size), int(max_cache_len), int(block)
+        self._rope_theta = float(getattr(config, "rope_theta", 10000.0))
+        self._rotary = rotary
+        self._rotaries: dict = {}
+        self._spaces: dict = {}
+        self._views: dict = {}
+        self._seqlens: dict = {}
+        n = int(getattr(config, "num_hidden_layers", 0))
+        self._seen = [0] * n
+        self.layers8: list = [None] * n
+        self._layer_device = []
+        for idx in range(n):
+            d = device if layer_device_map is None else layer_device_map[idx]
+            d = torch.device("cuda", d) if isinstance(d, int) else torch.device(d if d is not None else "cuda")
+            if d.type != "cuda":
+                raise ValueError("the 8-bit cache lives on CUDA devices (there is no CPU path)")
+            self._layer_device.append(d)
+
+    @property
+    def max_batch_size(self) -> int:
+        return self._max_batch_size
+
+    @property
+    def max_cache_len(self) -> int:
+        return self._max_cache_len
+
+    def __len__(self) -> int:
+        return len(self.layers8)
+
+    def nbytes(self) -> int:
+        return sum(c.nbytes() for c in self.layers8 if c is not None)
+
+    def _ensure_layer_spec(self, layer_idx: int, *, h: int, dh: int) -> None:
+        from . import kv8
+
+        c = self.layers8[layer_idx]
+        if c is None:
+            self.layers8[layer_idx] = kv8.KV8Cache.empty(self._max_batch_size, self._max_cache_len, int(h), int(dh),
+                                                         block=self._block, device=self._layer_device[layer_idx])
+        elif (c.k.shape[1], c.k.shape[3]) != (int(h), int(dh)):
+            raise RuntimeError(f"FlashSVDV15KV8Cache shape changed after init for layer {layer_idx}: "
+                               f"old={(c.k.shape[1], c.k.shape[3])}, new={(int(h), int(dh))}")
+
+    def layer(self, layer_idx: int, batch_size: int):
+        """The first ``batch_size`` sequences of a layer, as the operators take them."""
+        from . import kv8
+
+        c, B = self.layers8[layer_idx], int(batch_size)
+        if B == c.batch:
+            return c
+        if B > c.batch:
+            raise RuntimeError(f"batch {B} exceeds max_batch_size {c.batch}")
+        key = (int(layer_idx), B)
+        if key not in self._views:
+            self._views[key] = kv8.KV8Cache(c.k[:B], c.v[:B], c.k_scale[:B], c.v_scale[:B], c.block)
+        return self._views[key]
+
+    def rotary(self, head_dim: int, device):
+        """The rotation of the keys on a device."""
+        from . import kv8
+
+        key = (int(head_dim), str(device))
+        if key not in self._rotaries:
+            r = self._rotary
+            self._rotaries[key] = kv8.rotary(int(head_dim), theta=self._rope_theta, device=device) if r is None else \
+                kv8.Rotary(r.inv_freq.to(device), r.interleaved, r.scale)
+        return self._rotaries[key]
+
+    def workspace(self, layer_idx: int, batch_size: int, num_heads: int):
+        from . import ops
+
+        c = self.layer(layer_idx, batch_size)
+        Hk, Dh = c.k.shape[1], c.k.shape[3]
+        key = (str(c.device), int(batch_size), int(num_heads), Hk, Dh)
+        if key not in self._spaces:
+            self._spaces[key] = ops.make_kv8_workspace(batch_size, num_heads, Hk, Dh, self._max_cache_len, c.device)
+        return self._spaces[key]
+
+    def _place(self, layer_idx: int, B: int, L: int, cache_position):
+        """(int32 [B] of the positions in front of the new tokens, the largest of them or None where only the device
+        knows it).  Several tokens take consecutive positions, the same in every sequence; a single one may have one
+        position per sequence."""
+        dev = self._layer_device[layer_idx]
+        key = (int(layer_idx), int(B))
+        if key not in self._seqlens:
+            self._seqlens[key] = torch.empty(B, dtype=torch.int32, device=dev)
+        sl = self._seqlens[key]
+        start = cache_position
+        if cache_position is None:
+            start = self._seen[layer_idx]
+        elif torch.is_tensor(cache_position):
+            pos = cache_position.reshape(-1)
+            if int(pos.numel()) != (L if L > 1 or int(pos.numel()) != B else B):
+                raise ValueError(f"cache_position has {int(pos.numel())} entries for {L} new token(s) of {B} sequence(s)")
+            if L > 1 or not pos.is_cuda:
+                at = pos.tolist()
+                if L > 1 and at != list(range(at[0], at[0] + L)):
+                    raise ValueError("the 8-bit cache appends consecutive positions")
+                if min(at) < 0:
+                    raise IndexError(f"FlashSVDV15KV8Cache write position out of range: {min(at)}")
+                start = at[0] if L > 1 else max(at)
+            else:
+                start = None   # (a token that does not fit is dropped by the kernel and flags the workspace)
+            if start is None or (start + L <= self._max_cache_len and L == 1):
+                sl.copy_(pos.expand(B) if int(pos.numel()) == 1 else pos)
+                return sl, start
+        start = int(start)
+        if start < 0 or start + L > self._max_cache_len:
+            raise IndexError(f"FlashSVDV15KV8Cache write position out of range: start={start} q_len={L} max={self._max_cache_len}")
+        sl.fill_(start)
+        return sl, start
+
+    def _advance(self, layer_idx: int, start: Optional[int], L: int) -> None:
+        self._seen[layer_idx] = (self._seen[layer_idx] if start is None else start) + L
+
+    def append(self, key_states, value_states, layer_idx: int, *, query_states=None, rotate: bool = True, cache_position=None,
+               advance: bool = True):
+        """Appends [B, L, Hk, Dh] keys and values; with ``rotate`` the keys are rotated first, and so are the queries
+        [B, L, H, Dh].  Returns (positions in front of the new tokens int32 [B], their largest or None, rotated queries
+        or None)."""
+        from . import ops
+
+        layer_idx = int(layer_idx)
+        B, L, Hk, Dh = (int(n) for n in key_states.shape)
+        if L < 1:
+            raise ValueError("no tokens to append")
+        if key_states.dtype != torch.bfloat16:
+            raise ValueError(f"the 8-bit cache takes bfloat16 keys and values, got {key_states.dtype}")
+        self._ensure_layer_spec(layer_idx, h=Hk, dh=Dh)
+        c = self.layer(layer_idx, B)
+        H = Hk if query_states is None else int(query_states.shape[2])
+        ws = self.workspace(layer_idx, B, H)
+        sl, start = self._place(layer_idx, B, L, cache_position)
+        q = ops.kv8_append(key_states, value_states, c, sl, ws, q=query_states if rotate else None,
+                           rotary=self.rotary(Dh, c.device) if rotate else None)
+        if advance:
+            self._advance(layer_idx, start, L)
+        return sl, start, q if rotate else query_states
+
+    def decode_step(self, query_states, key_states, value_states, layer_idx: int, *, cache_position=None, advance: bool = True):
+        """One new token per sequence: rotation, append and attention over the sequence with it.  query_states
+        [B, 1, H, Dh], key_states / value_states [B, 1, Hk, Dh]; returns [B, H, Dh]."""
+        from . import ops
+
+        sl, _, q = self.append(key_states, value_states, layer_idx, query_states=query_states, cache_position=cache_position,
+                               advance=advance)
+        B, _, H, _ = q.shape
+        return ops.flash_decode_kv8(q[:, 0], self.layer(layer_idx, B), sl, self.workspace(layer_idx, B, H), seqlen_add=1)
+
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int, cache_kwargs: Optional[dict] = None):
+        """The transformers protocol: key_states (after their rotation), value_states [B, Hk, L, Dh] are appended; returns
+        the sequence so far as bfloat16 [B, Hk, S, Dh], read back from the codes."""
+        from . import ops
+
+        pos = None if cache_kwargs is None else cache_kwargs.get("cache_position")
+        if torch.is_tensor(pos):
+            pos = pos.cpu()
+        _, start, _ = self.append(key_states.transpose(1, 2).contiguous(), value_states.transpose(1, 2).contiguous(), layer_idx,
+                                  rotate=False, cache_position=pos)
+        B, _, L, _ = key_states.shape
+        return ops.kv8_load(self.layer(int(layer_idx), B), 0, start + L)
+
+    def get_seq_length(self, layer_idx: Optional[int] = 0) -> int:
+        return self._seen[int(layer_idx or 0)] if self._seen else 0
+
+    def get_max_cache_shape(self) -> Optional[int]:
+        return self._max_cache_len
+
+    def get_mask_sizes(self, cache_position, layer_idx: int = 0):
+        q_len = int(cache_position.shape[0]) if torch.is_tensor(cache_position) else int(cache_position)
+        return q_len + self.get_seq_length(), 0
+
+    def reset(self) -> None:
+        """Forgets the tokens (the next append starts its block's scale anew, so the codes need no clearing)."""
+        self._seen = [0] * len(self._seen)
+
+
 class FlashSVDLegacySparseKVCache:
     """Name of the reference's rank-space cache (runtime/cache/attn_legacy_sparse_kv.py:23-257: it
     keeps x . k_v^T and x . v_v^T per position and rebuilds keys and values inside its own decode
@@ -644,16 +836,22 @@ def _sample_next_token(logits: torch.Tensor, *, do_sample: bool, temperature: fl
 
 @torch.inference_mode()
 def generate_text(model: Any, tokenizer: Any, *, prompt: str, max_new_tokens: int = 64, device=None,
-                  do_sample: bool = False, temperature: float = 0.8, top_p: float = 0.95) -> dict:
+                  do_sample: bool = False, temperature: float = 0.8, top_p: float = 0.95, top_k: int = 0, min_p: float = 0.0,
+                  uniforms: Optional[torch.Tensor] = None) -> dict:
     """Single-prompt generation (greedy, or sampled with temperature / top_p) on a ``DecodeEngine``; returns the reference's result dict
     (prompt_token_count, generated_token_count, output_ids, completion_ids, text, completion_text).
-    Generation stops after an end-of-sequence token, like the reference loop."""
+    Generation stops after an end-of-sequence token, like the reference loop.
+
+    With ``uniforms`` (float32 [max_new_tokens] in [0, 1)), ``top_k`` or ``min_p`` the tokens are drawn by ``ops.sample``
+    on the device (from ``uniforms``, else from torch's CUDA generator) and the host reads none of them before the end."""
     from .engine import DecodeEngine, engine_for_model, has_lowrank_modules
 
     if not isinstance(model, DecodeEngine):
         if not has_lowrank_modules(model):
             if not callable(model) or not hasattr(model, "parameters"):
                 raise TypeError("generate_text takes a DecodeEngine, a model with low-rank modules or a transformers model")
+            if uniforms is not None or top_k or min_p:
+                raise ValueError("uniforms, top_k and min_p need a DecodeEngine or a model with low-rank modules")
             return _generate_text_generic(model, tokenizer, prompt=prompt, max_new_tokens=max_new_tokens, device=device,
                                           do_sample=do_sample, temperature=temperature, top_p=top_p)
         enc0 = tokenizer(prompt, return_tensors="pt", add_special_tokens=False)
@@ -667,10 +865,24 @@ def generate_text(model: Any, tokenizer: Any, *, prompt: str, max_new_tokens: in
     max_new_tokens = int(max_new_tokens)
     if prompt_len + max_new_tokens > model.S_max:
         raise IndexError(f"prompt of {prompt_len} tokens + {max_new_tokens} new tokens exceeds the cache length {model.S_max}")
+    on_device = do_sample and float(temperature) > 0.0 and max_new_tokens and (uniforms is not None or top_k or min_p)
+    if on_device:
+        if uniforms is None:
+            uniforms = torch.rand(max_new_tokens, dtype=torch.float32, device=model.device)
+        if tuple(uniforms.shape) != (max_new_tokens,):
+            raise ValueError(f"uniforms must be [{max_new_tokens}], got {list(uniforms.shape)}")
+        uniforms = uniforms.to(device=model.device, dtype=torch.float32)
     model.reset()
     model.prefill(input_ids)
     eos = getattr(tokenizer, "eos_token_id", None)
-    if do_sample and float(temperature) > 0.0 and max_new_tokens:
+    if on_device:
+        drawn = torch.empty(max_new_tokens, dtype=torch.int32, device=model.device)
+        for i in range(max_new_tokens):
+            drawn[i:i + 1] = model.sample(uniforms[i:i + 1], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            if i + 1 < max_new_tokens:
+                model.step(1)
+        new = drawn.tolist()
+    elif do_sample and float(temperature) > 0.0 and max_new_tokens:
         # sampled: the kernel leaves the logits of every step on the device; the token drawn from them
         # on the host side of the API is written back as the next step's input (the kernel's own greedy
         # choice is overwritten), one launch per token
