@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 
 import torch
 
@@ -63,20 +63,13 @@ def rotary(rotary_dim: int, *, theta: float = 10000.0, scaling: str = "none", fa
     return Rotary(f.to(device), interleaved, scale)
 
 
-@dataclass(frozen=True)
 class KV8Cache:
     """``k`` / ``v`` [B, Hk, S_max, Dh] float8_e4m3fn codes (a head's tokens lie together: a tile of them is one piece
     of memory), ``k_scale`` / ``v_scale`` [B, Hk, ceil(S_max / block)] float32.  A code stands for code * scale."""
 
-    k: torch.Tensor
-    v: torch.Tensor
-    k_scale: torch.Tensor
-    v_scale: torch.Tensor
-    block: int = 64
-    struct: FsvdKv8 = field(init=False, repr=False, compare=False)
+    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "_block", "index", "struct", "ref")
 
-    def __post_init__(self):
-        k, v, ks, vs, block = self.k, self.v, self.k_scale, self.v_scale, self.block
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, block: int = 64):
         if k.ndim != 4:
             raise ValueError(f"k must be [B, Hk, S_max, Dh], got {tuple(k.shape)}")
         shape = k.shape
@@ -92,18 +85,24 @@ class KV8Cache:
         if k.dtype is not torch.float8_e4m3fn or v.dtype is not torch.float8_e4m3fn:
             raise ValueError("the codes are float8_e4m3fn tensors")
         want = (B, Hk, -(-S // block))
-        if ks.shape != want or vs.shape != want or ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
-            raise ValueError(f"k_scale and v_scale must be float32 {want}, got {ks.dtype} {tuple(ks.shape)} and {vs.dtype} "
-                             f"{tuple(vs.shape)}")
+        if k_scale.shape != want or v_scale.shape != want or k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32:
+            raise ValueError(f"k_scale and v_scale must be float32 {want}, got {k_scale.dtype} {tuple(k_scale.shape)} and "
+                             f"{v_scale.dtype} {tuple(v_scale.shape)}")
         index = k.get_device()
-        if index < 0 or not (index == v.get_device() == ks.get_device() == vs.get_device()):
+        if index < 0 or not (index == v.get_device() == k_scale.get_device() == v_scale.get_device()):
             raise ValueError("the cache is CUDA tensors of one device (there is no CPU path)")
-        if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        if not (k.is_contiguous() and v.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
             raise ValueError("the cache needs contiguous tensors")
-        put = object.__setattr__   # (frozen: the addresses below are those of the tensors above)
-        put(self, "index", index)
-        put(self, "struct", FsvdKv8(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), B, Hk, S, Dh, block))
-        put(self, "ref", C.byref(self.struct))
+        self._k, self._v, self._k_scale, self._v_scale, self._block, self.index = k, v, k_scale, v_scale, block, index
+        self.struct = FsvdKv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, Hk, S, Dh, block)
+        self.ref = C.byref(self.struct)
+
+    # (the tensors cannot be exchanged: `struct` holds their addresses)
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    k_scale = property(lambda self: self._k_scale)
+    v_scale = property(lambda self: self._v_scale)
+    block = property(lambda self: self._block)
 
     @classmethod
     def empty(cls, batch: int, max_len: int, num_kv_heads: int, head_dim: int, *, block: int = 64, device="cuda") -> "KV8Cache":

@@ -320,7 +320,7 @@ class _SameDevice:
         self.index, self.was = index, None
 
     def __enter__(self):
-        now = torch.cuda.current_device()
+        now = torch._C._cuda_getDevice()
         if now != self.index:
             self.was = now
             torch.cuda.set_device(self.index)
@@ -372,6 +372,11 @@ def _device_of(name: str, t, ndim: int, what: str) -> int:
     return t.get_device()
 
 
+def _room_like(t):
+    """A contiguous tensor of the same size (`empty_like` costs half of `new_empty`, and keeps other strides)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def rope_qk(q, k, positions, inv_freq, *, interleaved=False, scale=1.0, q_out=None, k_out=None):
     """Rotates q[T, H, Dh] and k[T, Hk, Dh] (or None) at positions[T] (int32); returns (q_out, k_out).
 
@@ -396,13 +401,13 @@ def rope_qk(q, k, positions, inv_freq, *, interleaved=False, scale=1.0, q_out=No
         Hk = k.shape[1]
         kp = _ok_strided("k", k, dtype, index, (T, Hk, Dh))
         if k_out is None:
-            k_out = k.new_empty((T, Hk, Dh))
+            k_out = _room_like(k)
         kop = _ok("k_out", k_out, dtype, index, (T, Hk, Dh))
         ks = k.stride(0) if T > 1 else 0
     elif k_out is not None:
         raise ValueError("k_out without k")
     if q_out is None:
-        q_out = q.new_empty(shape)
+        q_out = _room_like(q)
     qop = _ok("q_out", q_out, dtype, index, shape)
     if T == 0:
         return q_out, k_out
@@ -466,7 +471,7 @@ def kv8_append(k, v, cache, cache_seqlens, ws: Workspace, *, new_lens=None, q=No
         qp = _ok_strided("q", q, _BF16, index, qshape)
         qs0, qs1 = q.stride()[:2]
         if q_out is None:
-            q_out = q.new_empty(qshape)
+            q_out = _room_like(q)
         qop = _ok("q_out", q_out, _BF16, index, qshape)
     elif q_out is not None:
         raise ValueError("q_out without q")
