@@ -35,7 +35,7 @@ constexpr int kLimbs = 4, kLimbBits = 12;   // such an integer as four numbers o
 constexpr int kList = 1024;                 // candidates of a CTA that are listed
 constexpr int kRank = 192;                  // candidates of a row that are ranked directly
 constexpr int kBlock = 128;                 // elements of a warp's step: four neighbours per lane
-constexpr int kPackPiece = 256, kPackAlone = 1024;   // elements that a warp's short list holds, beside the piece and without
+constexpr int kPackPiece = 256, kPackAlone = 896;   // elements that a warp's short list holds, beside the piece and without
 constexpr int kMaxCluster = 8;
 constexpr int kMaxVocab = 1 << 20;          // (2^17 elements of a CTA fit a bin's 32-bit sums of 15-bit numbers)
 constexpr float kHuge = 3.402823466e38f;
@@ -933,18 +933,22 @@ extern "C" int fsvd_sample(const void* logits, long long row_stride, int dtype, 
   if (B == 0) return 0;
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  // CTAs of a row: so many that a piece fits beside the short lists, and as many as give every SM at most one, as long as
-  // each has 4096 elements to work on.
+  // CTAs of a row, by waves x time of a CTA: 20 us for its steps one after the other, and 0.28 us per 1000 elements where they
+  // fit its shared memory, 0.36 where every pass reads them again from L2.
   const int es = dtype == FSVD_DTYPE_F32 ? 4 : 2;
   const long long places = V + 16 / es - 1;   // a row may start up to 15 bytes behind a 16-byte boundary
+  const auto chunk_of = [&](int c) { return ((places + c - 1) / c + kBlock - 1) / kBlock * kBlock; };
+  const auto fits = [&](int c) { return chunk_of(c) * es <= 144 * 1024; };   // (with the 80 KB that every CTA has)
+  const auto cost = [&](int c) { return (double)(((long long)B * c + sms - 1) / sms) * (20.0 + chunk_of(c) * (fits(c) ? 0.28e-3 : 0.36e-3)); };
   int C = 1;
-  while (C < kMaxCluster && ((2ll * B * C <= sms && places / C > 4096) || places * es / C > 140 * 1024)) C *= 2;
+  for (int c = 2; c <= kMaxCluster; c *= 2)
+    if (places / c > 2048 && cost(c) < cost(C)) C = c;
   Args a;
   a.logits = logits; a.stride = row_stride; a.u = uniforms; a.temperature = temperature; a.top_k = top_k; a.top_p = top_p;
   a.min_p = min_p; a.T_all = temperature_all; a.k_all = top_k_all; a.p_all = top_p_all; a.m_all = min_p_all;
   a.tokens = tokens; a.probs = probs; a.V = V;
-  a.chunk = (int)(((places + C - 1) / C + kBlock - 1) / kBlock * kBlock);
-  const bool resident = (size_t)a.chunk * es <= 144 * 1024;   // (with the 80 KB that every CTA has)
+  a.chunk = (int)chunk_of(C);
+  const bool resident = fits(C);
   const size_t smem = (size_t)kWarps * (resident ? kPackPiece : kPackAlone) * 6 + (resident ? (size_t)a.chunk * es : 0);
   const void* fn = dtype == FSVD_DTYPE_F32 ? (resident ? (const void*)sample_kernel<float, true> : (const void*)sample_kernel<float, false>)
                                            : (resident ? (const void*)sample_kernel<__nv_bfloat16, true>

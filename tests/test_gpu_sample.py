@@ -124,3 +124,18 @@ def test_sample_in_a_graph():
         u.copy_(torch.rand(3, device=DEV))
         graph.replay()
         assert torch.equal(out, ops.sample(x, u, top_p=0.9, top_k=100)[0])
+
+
+@pytest.mark.parametrize("dtype,B,V", [(torch.float32, 1, 300001), (torch.float32, 2, 1 << 20), (torch.bfloat16, 1, 1 << 20),
+                                       (torch.float32, 140, 50001), (torch.bfloat16, 149, 80003), (torch.float32, 75, 61007)])
+def test_rows_longer_than_shared_memory_and_many_rows(dtype, B, V):
+    from flashsvd_b200 import ops
+
+    gen = torch.Generator().manual_seed(B + V)
+    x = (4 * torch.randn(B, V, generator=gen)).to(dtype)
+    u = torch.rand(B, generator=gen)
+    rows = [0] if B == 1 else [0, 1] if B == 2 else [0, B // 2, B - 1]
+    for T, k, p, m in ((1.0, 0, 1.0, 0.0), (0.8, 0, 0.9, 0.0), (1.2, 50, 0.9, 0.02), (2.5, V // 3, 0.99, 0.0), (0.0, 0, 1.0, 0.0),
+                       (1.0, 0, 1.0, 0.1)):
+        tokens, probs = ops.sample(x.to(DEV), u.to(DEV), temperature=T, top_k=k, top_p=p, min_p=m)
+        _check(x[rows], u[rows], T, k, p, m, tokens[rows], probs[rows])
