@@ -306,20 +306,26 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   // Building the short list while a pass goes through the part: the elements with in[], in order.
   int filling = 0;
   auto pack = [&](int blk, const float (&x)[4], const bool (&in)[4]) {
-    const int mine = in[0] + in[1] + in[2] + in[3], upto = warp_scan(mine, lane);
-    int at = filling + upto - mine;
+    const uint32_t in_front = (1u << lane) - 1u;
+    uint32_t who[4];
+    int at = filling;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      who[e] = __ballot_sync(0xffffffffu, in[e]);
+      at += __popc(who[e] & in_front);
+      filling += __popc(who[e]);
+    }
+    if (filling > kPack) return;   // (a list that is too short is not used)
+    const int place = (blk - blk0) * kBlock + 4 * lane;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (in[e]) {
-        if (at < kPack) {
-          short_x[at] = x[e];
-          short_at[at] = (uint16_t)((blk - blk0) * kBlock + 4 * lane + e);
-        }
+        short_x[at] = x[e];
+        short_at[at] = (uint16_t)(place + e);
         ++at;
       }
-    filling += __shfl_sync(0xffffffffu, upto, 31);
   };
-  auto use_pack = [&] {   // (a list that is too short is not used)
+  auto use_pack = [&] {
     if (filling <= kPack && per * kBlock <= 65536) {
       for (int i = filling + lane; i < (filling + kBlock - 1) / kBlock * kBlock; i += 32) short_x[i] = -INFINITY;
       packed = filling;
@@ -402,6 +408,24 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   W.cut = fmaxf((float)(W.max - 60.0 * octave), -kHuge);
   W.table = s.table;
 
+  // The least number from W.cut on whose bin is at most `bin`.  Bins fall with the number, so 32 lanes narrow the range of
+  // keys 33 times a step; first the 32 keys around the place by the formula.
+  auto least_of = [&](int bin) -> float {
+    uint32_t lo = key_of(W.cut), hi = key_of((float)W.max);   // lo: not yet, unless W.cut itself is; hi: is
+    if (W.bin_of(W.cut) <= bin) return W.cut;
+    const uint32_t guess = key_of(fmaxf(W.cut, fminf((float)W.max, (float)(W.max - ((double)bin + 0.5) * (octave / 64.0)))));
+    uint32_t from = max(lo, guess > 16 ? guess - 16 : 0u), step = 1;
+    while (hi - lo > 1) {
+      const uint32_t mine = from + step * (uint32_t)lane;
+      const unsigned is = __ballot_sync(0xffffffffu, mine < hi && mine > lo && W.bin_of(value_of(mine)) <= bin);
+      const unsigned in = __ballot_sync(0xffffffffu, mine < hi && mine > lo);
+      if (is) hi = from + step * (uint32_t)(__ffs(is) - 1);
+      if (in & ~is) lo = from + step * (uint32_t)(31 - __clz(in & ~is));
+      step = (hi - lo + 32) / 33;
+      from = lo + step;
+    }
+    return value_of(hi);
+  };
   // Sum over the cluster of one number per thread.
   auto cluster_total = [&](double x, double Slot::* field) -> double {
     x = warp_add(x);
@@ -713,7 +737,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         const double unit = __hiloint2double(__double2hiint(s.table[-i & 63]) - (((i + 63) >> 6) << 20), __double2loint(s.table[-i & 63]));
         return i < kBins - 1 ? (double)x * (unit * 0x1p-36) : 1e30;
       }, target, s.scan_d, front);
-      const float cut = bin == kBins - 1 ? W.cut : fmaxf(W.cut, (float)(W.max - (double)(bin + 1) * (octave / 64.0)));
+      // the least numbers of this bin and of the one above it: the pass below only compares
+      const float cut = bin == kBins - 1 ? W.cut : least_of(bin), end = bin ? least_of(bin - 1) : INFINITY;
       const bool fill = packed < 0;
       Found f{0u, 0xffffffffu, 0u};
       filling = 0;
@@ -725,11 +750,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         for (int e = 0; e < 4; ++e) in[e] = x[e] > tv && x[e] >= cut;
         if (!__any_sync(0xffffffffu, in[0] || in[1] || in[2] || in[3])) return;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int be = min(W.bin_of(fmaxf(x[e], cut)), kBins - 1);
-          if (in[e] && be == bin) note(f, key_of(x[e]), index_of(blk, e));
-          in[e] = in[e] && be <= bin;
-        }
+        for (int e = 0; e < 4; ++e)
+          if (in[e] && x[e] < end) note(f, key_of(x[e]), index_of(blk, e));
         if (fill && filling <= kPack) pack(blk, x, in);
       });
       if (fill) use_pack();
