@@ -5,7 +5,7 @@
 // sort: a histogram of 1024 bins over the values narrows the threshold to a few of them, and a hundred candidates are
 // then ranked directly; where there are more, bins over the integer keys inside narrow it on.
 //
-// Weights exp((l - max) / T) are 64-bit numbers good to 2^-34, and every sum has a fixed order, or is one of integers where
+// Weights exp((l - max) / T) are 64-bit numbers good to 2^-39, and every sum has a fixed order, or is one of integers where
 // its terms come in any order.  32-bit weights would put a draw from a flat row of 10^5 tokens on another token than exact
 // arithmetic once in 10^4 rows.
 //
@@ -30,6 +30,7 @@ typedef unsigned long long u64;
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
 static_assert(kWarps == 32, "a warp folds one number of every warp");
 constexpr int kBins = 1024;
+constexpr int kPer = 32, kPerLog = 5;       // bins of a factor of two in the weight
 constexpr int kFrac = 40;                   // bits behind the point of a weight as an integer (at most one; 2^20 of them fit)
 constexpr int kLimbs = 4, kLimbBits = 12;   // such an integer as four numbers of 12 bits: 2^20 of them fit 32-bit sums
 constexpr int kList = 1024;                 // candidates of a CTA that are listed
@@ -62,18 +63,17 @@ struct Slot {
 struct Shared {
   uint32_t hist[kLimbs][kBins];
   u64 total[kBins];
-  double table[64];
+  double table[kPer];
   double warp_sum[kWarps], scan_d[kWarps];
   u64 scan[kWarps];
   uint32_t warp_eq[kWarps];
   uint32_t list_key[kList], list_at[kList];
-  uint32_t all_key[kRank], all_at[kRank];
-  u64 all_w[kRank];
+  u64 all_key[kRank], all_w[kRank];
   Slot slot, red[kWarps];
   int pick, list_n;
   u64 pick_above;
   double pick_front;
-  uint32_t pick_key, pick_ties, pick_equal;
+  u64 pick_key;
 };
 
 // Ascending keys for ascending numbers above -infinity (the zeros share theirs); 0 for -infinity and NaN.
@@ -147,23 +147,23 @@ __device__ __forceinline__ double wide(float x) {
   return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + 0x38000000u)), (int)(b << 29));
 }
 
-// exp((x - max) / T) = 2^(k / 64) 2^(r / 64) with k whole and |r| <= 1/2: a table of 64, a polynomial of degree three
-// (Taylor; the next term is below 2^-34), and k / 64 into the exponent.  For x >= cut; callers raise what is below to it and
+// exp((x - max) / T) = 2^(k / 32) 2^(r / 32) with k whole and |r| <= 1/2: a table of 32, a polynomial of degree four
+// (Taylor; the next term is below 2^-39), and k / 32 into the exponent.  For x >= cut; callers raise what is below to it and
 // drop the result, so that four weights are formed side by side without a branch (each is a chain of a dozen steps).
 struct Weigher {
-  double max, c;           // c = 64 log2(e) / T
+  double max, c;           // c = 32 log2(e) / T
   float cut;               // below it a weight is under 2^-60 and counts as zero; finite
-  const double* table;     // 2^(j / 64)
-  __device__ __forceinline__ double operator()(float x, int& bin, int& q) const {   // q: w = 2^(-bin / 64) (1 + q 2^-36)
-    constexpr double magic = 6755399441055744.0, a = 0.010830424696249145459;   // 1.5 * 2^52; ln(2) / 64
+  const double* table;     // 2^(j / 32)
+  __device__ __forceinline__ double operator()(float x, int& bin, int& q) const {   // q: w = 2^(-bin / 32) (1 + q 2^-35)
+    constexpr double magic = 6755399441055744.0, a = 0.69314718055994530942 / kPer;   // 1.5 * 2^52; ln(2) / 32
     const double d = wide(x) - max, k = fma(d, c, magic);
     const int lo = __double2loint(k);
     const double r = fma(d, c, -(k - magic));
-    const double e = fma(r, fma(r, fma(r, a * a * a / 6.0, a * a / 2.0), a), 1.0);
-    const double w = table[lo & 63] * e;
-    bin = -lo;             // 64ths of a factor of two below the maximum
-    q = __double2loint(e + 98304.0);   // (1.5 * 2^16: the low word counts 2^-36)
-    return __hiloint2double(__double2hiint(w) + ((lo >> 6) << 20), __double2loint(w));
+    const double e = fma(r, fma(r, fma(r, fma(r, a * a * a * a / 24.0, a * a * a / 6.0), a * a / 2.0), a), 1.0);
+    const double w = table[lo & (kPer - 1)] * e;
+    bin = -lo;             // 32nds of a factor of two below the maximum
+    q = __double2loint(e + 196608.0);   // (1.5 * 2^17: the low word counts 2^-35; below 2^29 as |e - 1| < 2^-6.5)
+    return __hiloint2double(__double2hiint(w) + ((lo >> kPerLog) << 20), __double2loint(w));
   }
   __device__ __forceinline__ double operator()(float x, int& bin) const {
     int q;
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   const int base = rank * a.chunk, i_end = min(base + a.chunk, V + shift), i_begin = max(base, shift);
   const int len = max(0, i_end - base);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (tid < 64) s.table[tid] = exp2((double)tid / 64.0);
+  if (tid < kPer) s.table[tid] = exp2((double)tid / kPer);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float temp = fminf(a.temperature ? a.temperature[b] : a.T_all, kHuge);
   int k = a.top_k ? a.top_k[b] : a.k_all;
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   if (inf) top = low = 0.0f;
   Weigher W;
   W.max = wide(top);
-  W.c = 64.0 * 1.4426950408889634074 / (double)temp;
+  W.c = kPer * 1.4426950408889634074 / (double)temp;
   const double octave = (double)temp * 0.69314718055994530942;   // a factor of two in the weight
   W.cut = fmaxf((float)(W.max - 60.0 * octave), -kHuge);
   W.table = s.table;
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   auto least_of = [&](int bin) -> float {
     uint32_t lo = key_of(W.cut), hi = key_of((float)W.max);   // lo: not yet, unless W.cut itself is; hi: is
     if (W.bin_of(W.cut) <= bin) return W.cut;
-    const uint32_t guess = key_of(fmaxf(W.cut, fminf((float)W.max, (float)(W.max - ((double)bin + 0.5) * (octave / 64.0)))));
+    const uint32_t guess = key_of(fmaxf(W.cut, fminf((float)W.max, (float)(W.max - ((double)bin + 0.5) * (octave / kPer)))));
     uint32_t from = max(lo, guess > 16 ? guess - 16 : 0u), step = 1;
     while (hi - lo > 1) {
       const uint32_t mine = from + step * (uint32_t)lane;
@@ -467,10 +467,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     for (int l = 0; l < kLimbs; ++l) t += (u64)peek(&s.hist[l][i], r) << (l * kLimbBits);
     return t;
   };
-  // A weight of bin i is 2^(-i / 64) (1 + q 2^-36): the bin holds how many there are, and the sums of the lower and upper
-  // halves of q + 2^29.  In units of 2^(-i / 64) 2^-36:
+  // A weight of bin i is 2^(-i / 32) (1 + q 2^-35): the bin holds how many there are, and the sums of the lower and upper
+  // halves of q + 2^29.  In units of 2^(-i / 32) 2^-35:
   auto masses = [&](int i, int r) -> u64 {
-    return (u64)peek(&s.hist[0][i], r) * ((1ull << 36) - (1ull << 29)) + ((u64)peek(&s.hist[2][i], r) << 15) + peek(&s.hist[1][i], r);
+    return (u64)peek(&s.hist[0][i], r) * ((1ull << 35) - (1ull << 29)) + ((u64)peek(&s.hist[2][i], r) << 15) + peek(&s.hist[1][i], r);
   };
   // The bin at which the running sum of f(total, bin) first exceeds `want`, and the sum in front of it.
   auto find_bin = [&](auto zero, auto f, decltype(zero) want, auto* scan, decltype(zero)& in_front) -> int {
@@ -571,37 +571,39 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         }
         if (tid < (int)f.n) {
           const uint32_t xk = peek(&s.list_key[tid - from], r);
-          s.all_at[tid] = peek(&s.list_at[tid - from], r);
-          s.all_key[tid] = xk;
+          s.all_key[tid] = ((u64)xk << 32) | ~peek(&s.list_at[tid - from], r);   // larger: in front
           s.all_w[tid] = MASS ? W.fixed(value_of(xk)) : 1;
         }
         __syncthreads();
-        for (int c = warp; c < (int)f.n; c += kWarps) {   // a warp to a candidate, the lanes over all of them
-          const uint32_t xk = s.all_key[c], at = s.all_at[c];
+        for (int c0 = 4 * warp; c0 < (int)f.n; c0 += 4 * kWarps) {   // eight lanes to a candidate, over all of them
+          const int c = min(c0 + lane / 8, (int)f.n - 1);
+          const u64 key = s.all_key[c];
           u64 before = 0;
-          uint32_t eq = 0, eq_before = 0, place = 0;
-          for (int i = lane; i < (int)f.n; i += 32) {
-            const uint32_t yk = s.all_key[i];
-            const bool first = yk > xk || (yk == xk && s.all_at[i] < at);
-            if (first) before += s.all_w[i];
-            place += first;
-            eq += yk == xk;
-            eq_before += yk == xk && first;
+          uint32_t place = 0;
+#pragma unroll 4
+          for (int i = lane & 7; i < (int)f.n; i += 8)
+            if (s.all_key[i] > key) {
+              before += s.all_w[i];
+              ++place;
+            }
+#pragma unroll
+          for (int o = 1; o < 8; o *= 2) {
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+            place += __shfl_xor_sync(0xffffffffu, place, o);
           }
-          before = warp_fold(before, [](u64 p, u64 q) { return p + q; });
-          place = __reduce_add_sync(0xffffffffu, place);
-          eq = __reduce_add_sync(0xffffffffu, eq);
-          eq_before = __reduce_add_sync(0xffffffffu, eq_before);
-          if (lane == 0 && before <= want && (want < before + s.all_w[c] || place + 1 == f.n)) {
-            s.pick_key = xk;
-            s.pick_ties = eq_before + 1;
-            s.pick_equal = eq;
-          }
+          if (before <= want && (want < before + s.all_w[c] || place + 1 == f.n)) s.pick_key = key;
         }
         __syncthreads();
-        t = s.pick_key;
-        ties = s.pick_ties;
-        equal = s.pick_equal;
+        const u64 key = s.pick_key;
+        uint32_t eq = 0, eq_upto = 0;
+        for (int i = lane; i < (int)f.n; i += 32) {
+          const bool same = (uint32_t)(s.all_key[i] >> 32) == (uint32_t)(key >> 32);
+          eq += same;
+          eq_upto += same && s.all_key[i] >= key;
+        }
+        t = (uint32_t)(key >> 32);
+        ties = __reduce_add_sync(0xffffffffu, eq_upto);
+        equal = __reduce_add_sync(0xffffffffu, eq);
         meet();   // the lists have been read
         return;
       }
@@ -704,8 +706,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   // ---- top-p
   if (p < 1.0f) {
     const float tv = t ? value_of(t) : -INFINITY;
-    // the mass above the threshold so far, and its distribution over 64ths of a factor of two (the last bin is everything
-    // below 2^-16: nobody counts it, half a row would add to one number)
+    // the mass above the threshold so far, and its distribution over 32nds of a factor of two (the last bin is everything
+    // below 2^-32, which is hardly ever where the border lies: nobody counts it, half a row may add to one number)
     double z = 0.0;
     clear_hist(3);
     each(blk0, blk1, [&](int, const float (&x)[4]) {
@@ -734,8 +736,9 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
       merge_hist(masses);
       double front;
       const int bin = find_bin(0.0, [&](u64 x, int i) {
-        const double unit = __hiloint2double(__double2hiint(s.table[-i & 63]) - (((i + 63) >> 6) << 20), __double2loint(s.table[-i & 63]));
-        return i < kBins - 1 ? (double)x * (unit * 0x1p-36) : 1e30;
+        const double of = s.table[-i & (kPer - 1)];
+        const double unit = __hiloint2double(__double2hiint(of) - (((i + kPer - 1) >> kPerLog) << 20), __double2loint(of));
+        return i < kBins - 1 ? (double)x * (unit * 0x1p-35) : 1e30;
       }, target, s.scan_d, front);
       // the least numbers of this bin and of the one above it: the pass below only compares
       const float cut = bin == kBins - 1 ? W.cut : least_of(bin), end = bin ? least_of(bin - 1) : INFINITY;
