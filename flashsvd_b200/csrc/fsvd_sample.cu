@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     f.kmax = __reduce_max_sync(0xffffffffu, hi);
   };
   uint32_t t = 0u, equal = 0;   // threshold key (0: everything above -infinity is kept), elements that have it
-  u64 ties = 0;                 // and how many of them are kept, the first ones in index order
+  uint32_t ties = 0;            // and how many of them are kept, the first ones in index order
   // Goes on inside the candidates f: the element at which the running count (MASS: weight) exceeds `target`, `above` of
   // it lies in front of them.  Counts are whole numbers; weights are added as integers here.
   auto finish = [&](auto mass, Found f, double above, double target) {
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         const u64 w = MASS ? W.fixed(value_of(f.kmin)) : 1;
         t = f.kmin;
         equal = f.n;
-        ties = w ? min(want / w + 1, (u64)f.n) : (u64)f.n;
+        ties = w ? (uint32_t)min(want / w + 1, (u64)f.n) : f.n;
         return;
       }
       if (f.n <= kRank) {   // every CTA gathers all lists and ranks them
@@ -704,6 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     }
   }
   // ---- top-p
+  bool tried = false;   // to list what top-p keeps
   if (p < 1.0f) {
     const float tv = t ? value_of(t) : -INFINITY;
     // the mass above the threshold so far, and its distribution over 32nds of a factor of two (the last bin is everything
@@ -743,6 +744,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
       // the least numbers of this bin and of the one above it: the pass below only compares
       const float cut = bin == kBins - 1 ? W.cut : least_of(bin), end = bin ? least_of(bin - 1) : INFINITY;
       const bool fill = packed < 0;
+      tried = true;
       Found f{0u, 0xffffffffu, 0u};
       filling = 0;
       if (tid == 0) s.list_n = 0;
@@ -761,12 +763,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
       gather(f);
       finish(std::true_type{}, f, front, target);
     } else if (wt > 0.0) {   // the border lies among the ties of top-k
-      ties = min(ties, (u64)((target - strictly) / wt) + 1);
+      ties = (uint32_t)min((u64)ties, (u64)((target - strictly) / wt) + 1);
     }
   }
   const bool some = t != 0u && ties < equal;   // only the first of the elements that equal the threshold stay
   const float tv = t ? value_of(t) : -INFINITY;
-  u64 seen0 = 0;                               // ties in front of this warp's part
+  uint32_t seen0 = 0;                          // ties in front of this warp's part
   if (some) {
     uint32_t eq = 0;
     each(blk0, blk1, [&](int blk, const float (&x)[4]) {
@@ -789,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   float cut = fmaxf(W.cut, tv);
   if (mp > 0.0f) cut = fmaxf(cut, (float)(W.max + ((double)__log2f(mp) - 0.01) * octave));   // (the 32-bit logarithm is good to 2^-20)
   // a few kept elements of a long part are listed first: a weight costs thirty times the comparison
-  if (packed < 0 && (t || mp > 0.0f)) {
+  if (packed < 0 && ((t && !tried) || mp > 0.0f)) {
     filling = 0;
     each(blk0, blk1, [&](int blk, const float (&x)[4]) {
       const bool in[4] = {x[0] >= cut, x[1] >= cut, x[2] >= cut, x[3] >= cut};
@@ -798,8 +800,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     use_pack();
   }
   const double mp_near = mp > 0.0f ? (double)mp * 1.0000001 : 0.0;
-  auto kept4 = [&](const float (&x)[4], u64& seen, double (&w)[4]) -> bool {   // whether any lane has a weight
-    u64 place = 0;
+  auto kept4 = [&](const float (&x)[4], uint32_t& seen, double (&w)[4]) -> bool {   // whether any lane has a weight
+    uint32_t place = 0;
     if (some) {
       uint32_t mine = 0;
 #pragma unroll
@@ -850,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   // goes through one group.
   const int group = packed >= 0 ? 1 : (per + 7) / 8;
   double my_group = 0.0;
-  u64 seen = seen0, my_seen = seen0;
+  uint32_t seen = seen0, my_seen = seen0;
   double in_group = 0.0;
   bool any = false;
   int g = 0, to_go = group;
