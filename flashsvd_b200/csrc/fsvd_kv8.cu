@@ -290,13 +290,13 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t x, float f) {
 // registers (bf16) between the maximum and the rounding, so that each input is read once and each code written once.  Keys
 // are turned in 64 bits, then rounded to 32 and 16: a rotated key falls on the same side of a rounding border as in
 // exact arithmetic.
-// Threads of a CTA and CTAs of an SM: the table of 128 tokens takes 152 KB, so one larger CTA instead of two.
-// (8192 tokens, 64 and 8 heads: 157 us with 256 threads, 91 with 512.)
-template <int BLOCK> constexpr int kAppendThreads = BLOCK == 128 ? 512 : 256;
-template <int BLOCK> constexpr int kAppendCtas = BLOCK == 128 ? 1 : 2;
-template <int DH, int BLOCK, bool WIDE>
-__global__ void __launch_bounds__(kAppendThreads<BLOCK>, kAppendCtas<BLOCK>) append_kernel(const AppendArgs a) {
-  constexpr int kThreads = kAppendThreads<BLOCK>, U = DH / 16, ROWS = kThreads / U, NIT = (BLOCK + ROWS - 1) / ROWS;
+// A thread to a unit of the tile.  CTAS of them to an SM: 512 threads of 128 registers, where a thread has its reads of the
+// table under way together, or 1024 of 64 (MANY), which overlap better once there is much to do.
+template <int DH, int BLOCK> constexpr int kAppendThreads = BLOCK * DH / 16;
+template <int DH, int BLOCK, bool MANY> constexpr int kAppendCtas = std::max(1, (MANY ? 1024 : 512) / kAppendThreads<DH, BLOCK>);
+template <int DH, int BLOCK, bool WIDE, bool MANY>
+__global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLOCK, MANY>) append_kernel(const AppendArgs a) {
+  constexpr int kThreads = kAppendThreads<DH, BLOCK>, U = DH / 16, ROWS = kThreads / U, NIT = (BLOCK + ROWS - 1) / ROWS;
   extern __shared__ double2 tab[];   // per token: cosine and sine of the pairs
   __shared__ uint32_t red[2][2][kThreads / 32];
   const int tid = threadIdx.x, u = tid % U, r0 = tid / U;
@@ -698,14 +698,13 @@ static int launch_rope(RopeArgs& a, int dtype, void* stream) {
               : launch(rope_kernel<__nv_bfloat16, false>, grid, kThreads, smem, stream, a);
 }
 
-template <int DH, int BLOCK>
+template <int DH, int BLOCK, bool MANY>
 static int launch_append(AppendArgs a, void* stream) {
   // Heads of a CTA share the table of angles.  Of the groupings by halves the one with the least waves x (planes of a CTA +
-  // kTable), the table being worth about as much as four planes (keys, values or queries of a head).  32 heads of 128, us
-  // beside as few groups as give each SM two CTAs: 1024 tokens 15.1 (19.7), 2041 tokens 28.9 (32.3), 2 x 1024 with 16 heads
-  // of 64 9.3 (12.6); 4 x 301 with 64 and 8 heads 15.9 (15.6).
+  // kTable), the table being worth about as much as four planes (keys, values or queries of a head).  Beside as few groups
+  // as give each SM two CTAs: 1024 tokens with 32 heads of 128 15.1 us (19.7), 2 x 1024 with 16 heads of 64 9.3 (12.6).
   constexpr int kTable = 4;
-  const long long tiles = (long long)a.c.B * ((a.L + BLOCK - 1) / BLOCK), fit = (long long)kAppendCtas<BLOCK> * sm_count();
+  const long long tiles = (long long)a.c.B * ((a.L + BLOCK - 1) / BLOCK), fit = (long long)kAppendCtas<DH, BLOCK, MANY> * sm_count();
   auto cost = [&](int g) {
     return (tiles * g + fit - 1) / fit * (2 * ((a.c.Hk + g - 1) / g) + (a.H + g - 1) / g + (a.rot.R ? kTable : 0));
   };
@@ -716,11 +715,21 @@ static int launch_append(AppendArgs a, void* stream) {
   if (grid > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many tokens for one call");
   const int tile = std::min(BLOCK, a.L);
   const size_t smem = (size_t)((a.rot.R / 2 + 7) / 8 * 8) * (tile + (tile > 8 ? 8 + (tile + 7) / 8 : 0)) * sizeof(double2);
-  return a.rot.R % 16 == 0 ? launch(append_kernel<DH, BLOCK, true>, dim3((unsigned)grid), kAppendThreads<BLOCK>, smem, stream, a)
-                           : launch(append_kernel<DH, BLOCK, false>, dim3((unsigned)grid), kAppendThreads<BLOCK>, smem, stream, a);
+  return a.rot.R % 16 == 0 ? launch(append_kernel<DH, BLOCK, true, MANY>, dim3((unsigned)grid), kAppendThreads<DH, BLOCK>, smem, stream, a)
+                           : launch(append_kernel<DH, BLOCK, false, MANY>, dim3((unsigned)grid), kAppendThreads<DH, BLOCK>, smem, stream, a);
+}
+template <int DH, int BLOCK>
+static int launch_append(const AppendArgs& a, void* stream) {
+  // Rows (a head's token of keys, values or queries) of an SM from which the 1024 threads are ahead; us at 512 and 1024
+  // threads, heads of 128: 512 tokens with 32 heads (331 rows) 9.7 and 11.1, 1024 (662) 14.8 and 15.8, 2041 (1320) 30.5 and
+  // 28.0, 4096 with 32 and 8 (1328) 28.6 and 25.1, 4 x 1024 with 64 and 8 in blocks of 32 (2213) 46.3 and 38.6.  Without
+  // rotation there is no table to wait for: 2041 tokens 18.4 and 13.3.
+  const bool many = !a.rot.R || (long long)a.c.B * a.L * (2 * a.c.Hk + a.H) >= 1024ll * sm_count();
+  return many ? launch_append<DH, BLOCK, true>(a, stream) : launch_append<DH, BLOCK, false>(a, stream);
 }
 template <int DH>
-static int launch_append(AppendArgs a, void* stream) {
+static int launch_append(const AppendArgs& given, void* stream) {
+  AppendArgs a = given;
   if (a.L == 1) {
     constexpr int rows = kThreads / (DH / 16);
     a.groups = (std::max(a.H, a.c.Hk) + rows - 1) / rows;
