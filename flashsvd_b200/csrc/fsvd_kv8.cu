@@ -208,30 +208,25 @@ __device__ __forceinline__ uint32_t turn_query(uint32_t w, float c, float s) {
   return fsvd_rope::pack2(x * c - y * s, y * c + x * s);
 }
 
-// Scales and codes of one thread's share of a tile: eight packed pairs of bf16 numbers (a in the low half) per row.
+// Scales and codes of one thread's share of a tile: eight packed pairs of bf16 numbers (a in the low half).
 struct Share {
   uint32_t top = 0;   // largest magnitude, as the bits of a bf16 number
   bool odd = false;   // something is not finite
 };
-template <int NIT>
-__device__ __forceinline__ void largest(const uint32_t (&w)[NIT][8], Share& s) {
+__device__ __forceinline__ void largest(const uint32_t (&w)[8], Share& s) {
   uint32_t m = 0;
 #pragma unroll
-  for (int it = 0; it < NIT; ++it)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[it][i] & 0x7fff7fffu);
+  for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
   s.top = max(m & 0xffffu, m >> 16);
   if (s.top >= 0x7f80u) {   // the finite ones alone
     s.odd = true;
     s.top = 0;
 #pragma unroll
-    for (int it = 0; it < NIT; ++it)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t x = w[it][i] & 0x7fffu, y = (w[it][i] >> 16) & 0x7fffu;
-        if (x < 0x7f80u) s.top = max(s.top, x);
-        if (y < 0x7f80u) s.top = max(s.top, y);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t x = w[i] & 0x7fffu, y = (w[i] >> 16) & 0x7fffu;
+      if (x < 0x7f80u) s.top = max(s.top, x);
+      if (y < 0x7f80u) s.top = max(s.top, y);
+    }
   }
 }
 __device__ __noinline__ uint32_t careful_codes(uint32_t w, float inv) {
@@ -296,10 +291,10 @@ template <int DH, int BLOCK> constexpr int kAppendThreads = BLOCK * DH / 16;
 template <int DH, int BLOCK, bool MANY> constexpr int kAppendCtas = std::max(1, (MANY ? 1024 : 512) / kAppendThreads<DH, BLOCK>);
 template <int DH, int BLOCK, bool WIDE, bool MANY>
 __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLOCK, MANY>) append_kernel(const AppendArgs a) {
-  constexpr int kThreads = kAppendThreads<DH, BLOCK>, U = DH / 16, ROWS = kThreads / U, NIT = (BLOCK + ROWS - 1) / ROWS;
+  constexpr int kThreads = kAppendThreads<DH, BLOCK>, U = DH / 16;
   extern __shared__ double2 tab[];   // per token: cosine and sine of the pairs
   __shared__ uint32_t red[2][2][kThreads / 32];
-  const int tid = threadIdx.x, u = tid % U, r0 = tid / U;
+  const int tid = threadIdx.x, u = tid % U, t = tid / U;   // this thread's unit and token of the tile
   int idx = blockIdx.x;
   const int grp = idx % a.groups;
   idx /= a.groups;
@@ -321,18 +316,14 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
   const int units = (half + 7) / 8, slots = 8 * units;
   const int Hk = a.c.Hk, nb = (a.c.S_max + BLOCK - 1) / BLOCK;
   const int hk0 = (int)((long long)Hk * grp / a.groups), hk1 = (int)((long long)Hk * (grp + 1) / a.groups);
-  uint32_t kreg[NIT][8], vreg[NIT][8];   // packed pairs (a, b)
+  uint32_t kreg[8], vreg[8];   // packed pairs (a, b)
   auto fetch = [&](int hk) {
 #pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-      const int t = r0 + it * ROWS;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) kreg[it][i] = vreg[it][i] = 0u;
-      if (t < n) {
-        const size_t off = (size_t)b * a.kv_batch + (size_t)(lo - start + t) * a.kv_token + (size_t)hk * DH;
-        fsvd_rope::load_pairs<WIDE>(a.k + off, u, R, inter, kreg[it]);
-        fsvd_rope::load_pairs<WIDE>(a.v + off, u, R, inter, vreg[it]);
-      }
+    for (int i = 0; i < 8; ++i) kreg[i] = vreg[i] = 0u;
+    if (t < n) {
+      const size_t off = (size_t)b * a.kv_batch + (size_t)(lo - start + t) * a.kv_token + (size_t)hk * DH;
+      fsvd_rope::load_pairs<WIDE>(a.k + off, u, R, inter, kreg);
+      fsvd_rope::load_pairs<WIDE>(a.v + off, u, R, inter, vreg);
     }
   };
   if (n > 0 && hk0 < hk1) fetch(hk0);   // (the first head is under way while the angles are formed)
@@ -353,9 +344,9 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
     __syncthreads();
     if (nq > 8) {
       for (int s0 = tid % 32; s0 < slots; s0 += 32)
-        for (int t = tid / 32; t < nq; t += kThreads / 32) {
-          const double2 x = steps[(8 + (t >> 3)) * slots + s0], y = steps[(t & 7) * slots + s0];
-          tab[t * slots + s0] = make_double2(x.x * y.x - x.y * y.y, x.y * y.x + x.x * y.y);
+        for (int k = tid / 32; k < nq; k += kThreads / 32) {
+          const double2 x = steps[(8 + (k >> 3)) * slots + s0], y = steps[(k & 7) * slots + s0];
+          tab[k * slots + s0] = make_double2(x.x * y.x - x.y * y.y, x.y * y.x + x.x * y.y);
         }
       __syncthreads();
     }
@@ -367,21 +358,16 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
   for (int hk = hk0; hk < hk1 && n > 0; ++hk, parity ^= 1) {
     const size_t si = ((size_t)b * Hk + hk) * nb + blk;
     const float kold = held ? a.c.k_scale[si] : 0.0f, vold = held ? a.c.v_scale[si] : 0.0f;
-    if (turns) {
+    if (turns && t < n) {
 #pragma unroll
-      for (int it = 0; it < NIT; ++it) {
-        const int t = r0 + it * ROWS;
-        if (t >= n) break;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (!WIDE && 8 * u + i >= half) break;
-          kreg[it][i] = turn_key(kreg[it][i], my_tab[t * slots + i * units]);
-        }
+      for (int i = 0; i < 8; ++i) {
+        if (!WIDE && 8 * u + i >= half) break;
+        kreg[i] = turn_key(kreg[i], my_tab[t * slots + i * units]);
       }
     }
     Share ks, vs;
-    largest<NIT>(kreg, ks);
-    largest<NIT>(vreg, vs);
+    largest(kreg, ks);
+    largest(vreg, vs);
     const uint32_t kwarp = __reduce_max_sync(0xffffffffu, ks.top), vwarp = __reduce_max_sync(0xffffffffu, vs.top);
     if ((tid & 31) == 0) {
       red[parity][0][tid >> 5] = kwarp;
@@ -406,23 +392,17 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
         if (!(now > was)) continue;
         uint32_t* w = reinterpret_cast<uint32_t*>(which ? vc : kc);
         const float f = was / now;
-        for (int i = tid; i < old_bytes / 4; i += kThreads) {
-          w[i] = rescaled(w[i], f);
-        }
+        for (int i = tid; i < old_bytes / 4; i += kThreads) w[i] = rescaled(w[i], f);
       }
     }
     const float ki = 1.0f / kscale, vi = 1.0f / vscale;
-#pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-      const int t = r0 + it * ROWS;
-      if (t < n) {
-        const size_t row = (size_t)(lo - blk0 + t) * DH;
-        uint32_t cd[8];   // codes of the pairs: low byte a, high byte b
-        codes_of(kreg[it], ki, ks.odd, cd);
-        store_codes<WIDE>(kc + row, cd, u, R, inter);
-        codes_of(vreg[it], vi, vs.odd, cd);
-        store_codes<WIDE>(vc + row, cd, u, R, inter);
-      }
+    if (t < n) {
+      const size_t row = (size_t)(lo - blk0 + t) * DH;
+      uint32_t cd[8];   // codes of the pairs: low byte a, high byte b
+      codes_of(kreg, ki, ks.odd, cd);
+      store_codes<WIDE>(kc + row, cd, u, R, inter);
+      codes_of(vreg, vi, vs.odd, cd);
+      store_codes<WIDE>(vc + row, cd, u, R, inter);
     }
     if (tid == 0) {
       a.c.k_scale[si] = kscale;
@@ -430,42 +410,40 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
     }
     if (hk + 1 < hk1) fetch(hk + 1);
   }
-  if (!a.q) return;
+  if (!a.q || t >= nq) return;
   // queries: a thread keeps its token's cosines and sines while it goes through the heads, two at a time
   const int h0 = (int)((long long)a.H * grp / a.groups), h1 = (int)((long long)a.H * (grp + 1) / a.groups);
-  for (int t = r0; t < nq; t += ROWS) {
-    float c[8], s[8];
-    if (turns) {
+  float c[8], s[8];
+  if (turns) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool in = WIDE || 8 * u + i < half;
-        const double2 cs = my_tab[t * slots + (in ? i * units : 0)];
-        c[i] = (float)cs.x;
-        s[i] = (float)cs.y;
-      }
+    for (int i = 0; i < 8; ++i) {
+      const bool in = WIDE || 8 * u + i < half;
+      const double2 cs = my_tab[t * slots + (in ? i * units : 0)];
+      c[i] = (float)cs.x;
+      s[i] = (float)cs.y;
     }
-    const size_t tok = (size_t)(lo - start + t);
-    const __nv_bfloat16* src = a.q + (size_t)b * a.q_batch + tok * a.q_token;
-    __nv_bfloat16* dst = a.q_out + ((size_t)b * a.L + tok) * a.H * DH;
-    constexpr int N = 2;
-    for (int h = h0; h < h1; h += N) {
-      uint32_t w[N][8];
+  }
+  const size_t tok = (size_t)(lo - start + t);
+  const __nv_bfloat16* src = a.q + (size_t)b * a.q_batch + tok * a.q_token;
+  __nv_bfloat16* dst = a.q_out + ((size_t)b * a.L + tok) * a.H * DH;
+  constexpr int N = 2;
+  for (int h = h0; h < h1; h += N) {
+    uint32_t w[N][8];
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (h + k < h1) fsvd_rope::load_pairs<WIDE>(src + (size_t)(h + k) * DH, u, R, inter, w[k]);
+    for (int k = 0; k < N; ++k)
+      if (h + k < h1) fsvd_rope::load_pairs<WIDE>(src + (size_t)(h + k) * DH, u, R, inter, w[k]);
 #pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (h + k < h1) {
-          if (turns) {
+    for (int k = 0; k < N; ++k)
+      if (h + k < h1) {
+        if (turns) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if (!WIDE && 8 * u + i >= half) break;
-              w[k][i] = turn_query(w[k][i], c[i], s[i]);
-            }
+          for (int i = 0; i < 8; ++i) {
+            if (!WIDE && 8 * u + i >= half) break;
+            w[k][i] = turn_query(w[k][i], c[i], s[i]);
           }
-          fsvd_rope::store_pairs<WIDE>(dst + (size_t)(h + k) * DH, u, R, inter, w[k]);
         }
-    }
+        fsvd_rope::store_pairs<WIDE>(dst + (size_t)(h + k) * DH, u, R, inter, w[k]);
+      }
   }
 }
 
@@ -489,14 +467,14 @@ __global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs 
   const bool has_kv = start < a.c.S_max && hk < (int)((long long)Hk * (grp + 1) / a.groups);
   const int blk = start / BLOCK, old = start - blk * BLOCK;   // tokens that the block holds already
   const size_t si = ((size_t)b * Hk + hk) * nb + blk;
-  uint32_t kw[1][8], vw[1][8], qw[8];
+  uint32_t kw[8], vw[8], qw[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) kw[0][i] = vw[0][i] = 0u;
+  for (int i = 0; i < 8; ++i) kw[i] = vw[i] = 0u;
   float kold = 0.0f, vold = 0.0f;
   if (has_kv) {
     const size_t off = (size_t)b * a.kv_batch + (size_t)hk * DH;
-    fsvd_rope::load_pairs<WIDE>(a.k + off, u, R, inter, kw[0]);
-    fsvd_rope::load_pairs<WIDE>(a.v + off, u, R, inter, vw[0]);
+    fsvd_rope::load_pairs<WIDE>(a.k + off, u, R, inter, kw);
+    fsvd_rope::load_pairs<WIDE>(a.v + off, u, R, inter, vw);
     if (old) {
       kold = a.c.k_scale[si];
       vold = a.c.v_scale[si];
@@ -514,14 +492,14 @@ __global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs 
     for (int i = 0; i < 8; ++i) {
       if (!WIDE && 8 * u + i >= half) break;
       const double2 cs = tab[i * units + u];
-      if (has_kv) kw[0][i] = turn_key(kw[0][i], cs);
+      if (has_kv) kw[i] = turn_key(kw[i], cs);
       if (has_q) qw[i] = turn_query(qw[i], (float)cs.x, (float)cs.y);
     }
   }
   if (has_q) fsvd_rope::store_pairs<WIDE>(a.q_out + ((size_t)b * a.H + h) * DH, u, R, inter, qw);
   Share ks, vs;
-  largest<1>(kw, ks);
-  largest<1>(vw, vs);
+  largest(kw, ks);
+  largest(vw, vs);
   uint32_t kbits = ks.top, vbits = vs.top;
 #pragma unroll
   for (int d = 1; d < U; d *= 2) {
@@ -531,11 +509,12 @@ __global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs 
   const float kscale = fmaxf(kold, two_to(scale_exponent(__uint_as_float(kbits << 16))));
   const float vscale = fmaxf(vold, two_to(scale_exponent(__uint_as_float(vbits << 16))));
   const size_t base = (((size_t)b * Hk + hk) * a.c.S_max + (size_t)blk * BLOCK) * DH;
+  __syncwarp();   // (a row's lanes have read its scales)
   if (has_kv) {
     uint32_t cd[8];
-    codes_of(kw[0], 1.0f / kscale, ks.odd, cd);
+    codes_of(kw, 1.0f / kscale, ks.odd, cd);
     store_codes<WIDE>(reinterpret_cast<uint8_t*>(a.c.k8) + base + (size_t)old * DH, cd, u, R, inter);
-    codes_of(vw[0], 1.0f / vscale, vs.odd, cd);
+    codes_of(vw, 1.0f / vscale, vs.odd, cd);
     store_codes<WIDE>(reinterpret_cast<uint8_t*>(a.c.v8) + base + (size_t)old * DH, cd, u, R, inter);
     if (u == 0) {
       a.c.k_scale[si] = kscale;
@@ -722,10 +701,11 @@ template <int DH, int BLOCK>
 static int launch_append(const AppendArgs& a, void* stream) {
   // Rows (a head's token of keys, values or queries) of an SM from which the 1024 threads are ahead; us at 512 and 1024
   // threads, heads of 128: 512 tokens with 32 heads (331 rows) 9.7 and 11.1, 1024 (662) 14.8 and 15.8, 2041 (1320) 30.5 and
-  // 28.0, 4096 with 32 and 8 (1328) 28.6 and 25.1, 4 x 1024 with 64 and 8 in blocks of 32 (2213) 46.3 and 38.6.  Without
+  // 27.3, 4096 with 32 and 8 (1328) 28.6 and 23.8, 4 x 1024 with 64 and 8 in blocks of 32 (2213) 46.3 and 36.9.  Without
   // rotation there is no table to wait for: 2041 tokens 18.4 and 13.3.
-  const bool many = !a.rot.R || (long long)a.c.B * a.L * (2 * a.c.Hk + a.H) >= 1024ll * sm_count();
-  return many ? launch_append<DH, BLOCK, true>(a, stream) : launch_append<DH, BLOCK, false>(a, stream);
+  if constexpr (kAppendThreads<DH, BLOCK> < 1024)
+    if (a.rot.R && (long long)a.c.B * a.L * (2 * a.c.Hk + a.H) < 1024ll * sm_count()) return launch_append<DH, BLOCK, false>(a, stream);
+  return launch_append<DH, BLOCK, true>(a, stream);
 }
 template <int DH>
 static int launch_append(const AppendArgs& given, void* stream) {

@@ -352,7 +352,7 @@ int fsvd_tp_decode_layer(const fsvd_dims* dims, const fsvd_layer* layer, const v
  * 64 bits, so that far positions keep their phase.  rotary_dim is even, 2..Dh.
  *
  * q_out / k_out [T, H|Hk, Dh] (contiguous) may be the inputs when those are contiguous.  k and k_out
- * may both be NULL.  dtype bf16 or f32, Dh a multiple of 8 up to 256. */
+ * may both be NULL.  dtype bf16 or f32, Dh a multiple of 16 up to 256. */
 int fsvd_rope_qk(const void* q, long long q_stride, const void* k, long long k_stride, const int* positions,
                  const double* inv_freq, int rotary_dim, int interleaved, float rope_scale, void* q_out, void* k_out,
                  int T, int H, int Hk, int Dh, int dtype, void* stream);
@@ -375,10 +375,13 @@ size_t fsvd_kv8_workspace_bytes(int B, int H, int Hk, int Dh, int S_max);
  * + new_lens[b] - 1 (new_lens NULL: L each).  With inv_freq the keys, and q [B, L, H, Dh] -> q_out when
  * q is given, are rotated at their positions first (a key is rounded to bf16 before it is quantised).
  * A block's scale is the smallest power of two >= 2^-60 for which its largest finite magnitude fits
- * 448 * scale; codes are rounded to nearest even (down where a code times 2^120 would pass the 32-bit range).  When a later token needs a larger scale, the codes
- * that the block already holds are rounded again to the new one.  Values that are not finite are stored as
- * NaN and take no part in the scale.  Scales of blocks that hold tokens must be positive and finite.
- * cache_seqlens is not advanced.  A token at a position >= S_max is dropped and sets status 4. */
+ * 448 * scale; codes are rounded to nearest even (down where a code times 2^120 would pass the 32-bit
+ * range).  When a later token needs a larger scale, the codes that the block already holds are rounded
+ * again to the new one.  Values that are not finite are stored as NaN and take no part in the scale.
+ * Scales of blocks that hold tokens must be positive and finite.  Tokens are appended behind
+ * cache_seqlens[b] (a negative one counts as 0): what the block of the last one held there is not kept.
+ * cache_seqlens is not advanced.  A token at a position >= S_max is dropped and sets status 4; its query
+ * is rotated all the same. */
 int fsvd_kv8_append(const fsvd_kv8* cache, const void* k, const void* v, long long kv_batch_stride, long long kv_token_stride,
                     const int* cache_seqlens, const int* new_lens, const void* q, long long q_batch_stride,
                     long long q_token_stride, void* q_out, const double* inv_freq, int rotary_dim, int interleaved,
@@ -398,10 +401,11 @@ int fsvd_flash_decode_kv8(const fsvd_kv8* cache, const void* q, const int* cache
  * mass is at most top_p times the mass of all of them (>= 1: all), of those the ones with weight >=
  * min_p (<= 0: all); at least one.  The token is the first kept one in index order whose running mass
  * exceeds uniforms[b] times the kept mass; probs (may be NULL) gets its share of that mass.  A
- * temperature <= 0 (or NaN) takes the largest logit, an infinite one counts as the largest finite number.  NaN counts as -infinity; a row without anything above
- * -infinity gives token 0 with share 0.  temperature, top_k, top_p, min_p: one value per row in
- * device memory, or NULL and the value for all rows.  Masses are integer sums of weights in fixed point:
- * the result does not depend on the order of additions. */
+ * temperature <= 0 (or NaN) takes the largest logit, an infinite one counts as the largest finite number.
+ * NaN counts as -infinity; a row without anything above -infinity gives token 0 with share 0; where +infinity
+ * is the largest, the elements that are infinite share everything.  temperature, top_k, top_p, min_p: one
+ * value per row in device memory, or NULL and the value for all rows.  Weights are 64-bit numbers, their
+ * sums have a fixed order or are sums of integers: the same call gives the same token.  V up to 2^20. */
 int fsvd_sample(const void* logits, long long row_stride, int dtype, const float* uniforms, const float* temperature,
                 const int* top_k, const float* top_p, const float* min_p, float temperature_all, int top_k_all,
                 float top_p_all, float min_p_all, int* tokens, float* probs, int B, int V, void* stream);
