@@ -89,6 +89,7 @@ struct RopeArgs {
   int T, H, Hk, Dh, tokens, heads;   // tokens and heads of a CTA
 };
 constexpr int kRopeTokens = 32;
+constexpr int kMaxHeads = 1 << 16;
 
 // A CTA turns `tokens` rows of heads; its threads go through the (token, head, unit) list in steps of kThreads, several units
 // at a time so that their loads are under way together.
@@ -663,9 +664,10 @@ static int launch_attn(const CUtensorMap& km, const CUtensorMap& vm, const fsvd_
 
 static int launch_rope(RopeArgs& a, int dtype, void* stream) {
   // One wave of four CTAs per SM, up to 32 tokens each; a few tokens are shared out by heads.
-  const int all = a.H + a.Hk, T = a.T;
-  a.tokens = std::min(kRopeTokens, (T + 4 * sm_count() - 1) / (4 * sm_count()));
-  const int ctas = (T + a.tokens - 1) / a.tokens, splits = std::max(1, std::min({2 * sm_count() / ctas, all * (a.Dh / 16) / kThreads, 8}));
+  const int all = a.H + a.Hk;
+  const long long T = a.T;
+  a.tokens = (int)std::min<long long>(kRopeTokens, (T + 4 * sm_count() - 1) / (4 * sm_count()));
+  const int ctas = (int)((T + a.tokens - 1) / a.tokens), splits = std::max(1, std::min({2 * sm_count() / ctas, all * (a.Dh / 16) / kThreads, 8}));
   a.heads = (all + splits - 1) / splits;
   const dim3 grid(ctas, (all + a.heads - 1) / a.heads);
   const size_t smem = (size_t)a.tokens * ((a.rot.R / 2 + 7) / 8 * 8) * sizeof(float2);
@@ -738,6 +740,7 @@ int fsvd_rope_qk(const void* q, long long q_stride, const void* k, long long k_s
   if (!q || !positions || !inv_freq || !q_out || (k != nullptr) != (k_out != nullptr)) return fail(FSVD_ERR_ARG, "null argument");
   if (dtype != FSVD_DTYPE_BF16 && dtype != FSVD_DTYPE_F32) return fail(FSVD_ERR_ARG, "bad dtype %d", dtype);
   if (T < 0 || H < 1 || (k && Hk < 1)) return fail(FSVD_ERR_ARG, "bad sizes T=%d H=%d Hk=%d", T, H, Hk);
+  if (H > kMaxHeads || Hk > kMaxHeads) return fail(FSVD_ERR_UNSUPPORTED, "more than %d heads", kMaxHeads);
   if (Dh < 16 || Dh > 256 || Dh % 16) return fail(FSVD_ERR_UNSUPPORTED, "head_dim %d unsupported (multiples of 16 up to 256)", Dh);
   if (int e = check_rotary(inv_freq, rotary_dim, Dh)) return e;
   const int es = dtype == FSVD_DTYPE_F32 ? 4 : 2;
@@ -768,6 +771,7 @@ int fsvd_kv8_append(const fsvd_kv8* cache, const void* k, const void* v, long lo
   if (q && !inv_freq) return fail(FSVD_ERR_ARG, "queries are passed to be rotated: inv_freq is missing");
   if (int e = check_rotary(inv_freq, rotary_dim, cache->Dh)) return e;
   if (L < 0 || (q && H < 1)) return fail(FSVD_ERR_ARG, "bad sizes L=%d H=%d", L, H);
+  if (q && H > kMaxHeads) return fail(FSVD_ERR_UNSUPPORTED, "more than %d heads", kMaxHeads);
   if (kv_batch_stride < 0 || kv_token_stride < 0 || q_batch_stride < 0 || q_token_stride < 0) return fail(FSVD_ERR_ARG, "negative stride");
   if (!aligned16(k) || !aligned16(v) || !aligned16(q) || !aligned16(q_out) || kv_batch_stride % 8 || kv_token_stride % 8 ||
       (q && (q_batch_stride % 8 || q_token_stride % 8)))

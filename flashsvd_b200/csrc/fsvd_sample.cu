@@ -38,7 +38,8 @@ constexpr int kRank = 192;                  // candidates of a row that are rank
 constexpr int kBlock = 128;                 // elements of a warp's step: four neighbours per lane
 constexpr int kPackPiece = 256, kPackAlone = 896;   // elements that a warp's short list holds, beside the piece and without
 constexpr int kMaxCluster = 8;
-constexpr int kMaxVocab = 1 << 20;          // (2^17 elements of a CTA fit a bin's 32-bit sums of 15-bit numbers)
+constexpr int kMaxVocab = 1 << 20;
+constexpr int kMaxPiece = (1 << 17) + kBlock;        // elements of a CTA: so many of 27800 (see `masses`) fit a bin's 32-bit sum
 constexpr float kHuge = 3.402823466e38f;
 
 struct Args {
@@ -154,7 +155,7 @@ struct Weigher {
   double max, c;           // c = 32 log2(e) / T
   float cut;               // below it a weight is under 2^-60 and counts as zero; finite
   const double* table;     // 2^(j / 32)
-  __device__ __forceinline__ double operator()(float x, int& bin, int& q) const {   // q: w = 2^(-bin / 32) (1 + q 2^-35)
+  __device__ __forceinline__ double operator()(float x, int& bin, int& q) const {   // q: w = 2^(-bin / 32) (1 + q 2^-34)
     constexpr double magic = 6755399441055744.0, a = 0.69314718055994530942 / kPer;   // 1.5 * 2^52; ln(2) / 32
     const double d = wide(x) - max, k = fma(d, c, magic);
     const int lo = __double2loint(k);
@@ -162,7 +163,7 @@ struct Weigher {
     const double e = fma(r, fma(r, fma(r, fma(r, a * a * a * a / 24.0, a * a * a / 6.0), a * a / 2.0), a), 1.0);
     const double w = table[lo & (kPer - 1)] * e;
     bin = -lo;             // 32nds of a factor of two below the maximum
-    q = __double2loint(e + 196608.0);   // (1.5 * 2^17: the low word counts 2^-35; below 2^29 as |e - 1| < 2^-6.5)
+    q = __double2loint(e + 393216.0);   // (1.5 * 2^18: the low word counts 2^-34; |q| < 1.9e8 as |e - 1| < 0.011)
     return __hiloint2double(__double2hiint(w) + ((lo >> kPerLog) << 20), __double2loint(w));
   }
   __device__ __forceinline__ double operator()(float x, int& bin) const {
@@ -467,10 +468,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     for (int l = 0; l < kLimbs; ++l) t += (u64)peek(&s.hist[l][i], r) << (l * kLimbBits);
     return t;
   };
-  // A weight of bin i is 2^(-i / 32) (1 + q 2^-35): the bin holds how many there are, and the sums of the lower and upper
-  // halves of q + 2^29.  In units of 2^(-i / 32) 2^-35:
+  // A weight of bin i is 2^(-i / 32) (1 + q 2^-34): the bin holds how many there are, and the sums of the 14 lower bits and
+  // the upper ones (below 27800) of q + 2^28.  In units of 2^(-i / 32) 2^-34:
   auto masses = [&](int i, int r) -> u64 {
-    return (u64)peek(&s.hist[0][i], r) * ((1ull << 35) - (1ull << 29)) + ((u64)peek(&s.hist[2][i], r) << 15) + peek(&s.hist[1][i], r);
+    return (u64)peek(&s.hist[0][i], r) * ((1ull << 34) - (1ull << 28)) + ((u64)peek(&s.hist[2][i], r) << 14) + peek(&s.hist[1][i], r);
   };
   // The bin at which the running sum of f(total, bin) first exceeds `want`, and the sum in front of it.
   auto find_bin = [&](auto zero, auto f, decltype(zero) want, auto* scan, decltype(zero)& in_front) -> int {
@@ -723,10 +724,10 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (in[e] && bin[e] < kBins - 1) {
-          const uint32_t positive = (uint32_t)(q[e] + (1 << 29));
+          const uint32_t positive = (uint32_t)(q[e] + (1 << 28));
           atomicAdd(&s.hist[0][bin[e]], 1u);
-          atomicAdd(&s.hist[1][bin[e]], positive & 0x7fffu);
-          atomicAdd(&s.hist[2][bin[e]], positive >> 15);
+          atomicAdd(&s.hist[1][bin[e]], positive & 0x3fffu);
+          atomicAdd(&s.hist[2][bin[e]], positive >> 14);
         }
       z += ((in[0] ? w[0] : 0.0) + (in[1] ? w[1] : 0.0)) + ((in[2] ? w[2] : 0.0) + (in[3] ? w[3] : 0.0));
     });
@@ -739,7 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
       const int bin = find_bin(0.0, [&](u64 x, int i) {
         const double of = s.table[-i & (kPer - 1)];
         const double unit = __hiloint2double(__double2hiint(of) - (((i + kPer - 1) >> kPerLog) << 20), __double2loint(of));
-        return i < kBins - 1 ? (double)x * (unit * 0x1p-35) : 1e30;
+        return i < kBins - 1 ? (double)x * (unit * 0x1p-34) : 1e30;
       }, target, s.scan_d, front);
       // the least numbers of this bin and of the one above it: the pass below only compares
       const float cut = bin == kBins - 1 ? W.cut : least_of(bin), end = bin ? least_of(bin - 1) : INFINITY;
@@ -961,14 +962,16 @@ extern "C" int fsvd_sample(const void* logits, long long row_stride, int dtype, 
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   // CTAs of a row, by waves x time of a CTA: 20 us for its steps one after the other, and 0.28 us per 1000 elements where they
-  // fit its shared memory, 0.36 where every pass reads them again from L2.
+  // fit its shared memory, 0.36 where every pass reads them again from L2.  (128 rows of 100003: one CTA each 52 us with top-k,
+  // top-p and min-p and 77 with top-p alone; four each, which hold them, 116 and 186.)
   const int es = dtype == FSVD_DTYPE_F32 ? 4 : 2;
   const long long places = V + 16 / es - 1;   // a row may start up to 15 bytes behind a 16-byte boundary
   const auto chunk_of = [&](int c) { return ((places + c - 1) / c + kBlock - 1) / kBlock * kBlock; };
   const auto fits = [&](int c) { return chunk_of(c) * es <= 144 * 1024; };   // (with the 80 KB that every CTA has)
   const auto cost = [&](int c) { return (double)(((long long)B * c + sms - 1) / sms) * (20.0 + chunk_of(c) * (fits(c) ? 0.28e-3 : 0.36e-3)); };
   int C = 1;
-  for (int c = 2; c <= kMaxCluster; c *= 2)
+  while (chunk_of(C) > kMaxPiece) C *= 2;   // (at most kMaxCluster)
+  for (int c = 2 * C; c <= kMaxCluster; c *= 2)
     if (places / c > 2048 && cost(c) < cost(C)) C = c;
   Args a;
   a.logits = logits; a.stride = row_stride; a.u = uniforms; a.temperature = temperature; a.top_k = top_k; a.top_p = top_p;

@@ -426,6 +426,13 @@ def make_kv8_workspace(batch, num_heads, num_kv_heads, head_dim, max_len, device
     return Workspace(torch.zeros(n, dtype=torch.uint8, device=device), n)
 
 
+def _add(n) -> int:
+    n = int(n)
+    if not -(1 << 31) <= n < 1 << 31:
+        raise ValueError(f"seqlen_add {n} is no 32-bit number")
+    return n
+
+
 def _scratch(ws: Workspace, index: int):
     if ws.buf.get_device() != index:
         raise ValueError(f"the workspace is on {ws.buf.device}, the call's tensors on cuda:{index}")
@@ -501,7 +508,7 @@ def kv8_load(cache, start, length, *, cache_seqlens=None, seqlen_add=0, k_out=No
     if length == 0:
         return k_out, v_out
     with _SameDevice(index):
-        check(_library().fsvd_kv8_load(cache.ref, start, length, sp, int(seqlen_add), kp, vp, _raw_stream(index)))
+        check(_library().fsvd_kv8_load(cache.ref, start, length, sp, _add(seqlen_add), kp, vp, _raw_stream(index)))
     return k_out, v_out
 
 
@@ -520,7 +527,7 @@ def flash_decode_kv8(q, cache, cache_seqlens, ws: Workspace, *, seqlen_add=0, sc
     op = _ok("out", out, _BF16, index, shape)
     wp = _scratch(ws, index)
     with _SameDevice(index):
-        check(_library().fsvd_flash_decode_kv8(cache.ref, qp, sp, int(seqlen_add), op, H, scale, wp, ws.nbytes, _raw_stream(index)))
+        check(_library().fsvd_flash_decode_kv8(cache.ref, qp, sp, _add(seqlen_add), op, H, scale, wp, ws.nbytes, _raw_stream(index)))
     return out
 
 
@@ -547,6 +554,8 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
         tp, temperature = _ok("temperature", temperature, _F32, index, rows), 1.0
     if torch.is_tensor(top_k):
         kp, top_k = _ok("top_k", top_k, _I32, index, rows), 0
+    elif top_k > V:
+        top_k = 0
     if torch.is_tensor(top_p):
         pp, top_p = _ok("top_p", top_p, _F32, index, rows), 1.0
     if torch.is_tensor(min_p):

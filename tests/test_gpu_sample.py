@@ -139,3 +139,32 @@ def test_rows_longer_than_shared_memory_and_many_rows(dtype, B, V):
                        (1.0, 0, 1.0, 0.1)):
         tokens, probs = ops.sample(x.to(DEV), u.to(DEV), temperature=T, top_k=k, top_p=p, min_p=m)
         _check(x[rows], u[rows], T, k, p, m, tokens[rows], probs[rows])
+
+
+@pytest.mark.parametrize("B,V", [(140, 262144), (1, (1 << 20) - 1), (148, 160001)])
+def test_masses_of_many_equal_logits(B, V):
+    """More than half the row in one bin of the histogram and the rest in the next ones: its sums hold them all."""
+    from flashsvd_b200 import ops
+
+    # (32 log2(e) x = -64.49 and -64.51 sit at the two ends of the bins -64 and -65: residuals of either sign, all bits set)
+    step = math.log(2.0) / 32
+    for off in (64.49, 64.499, 64.02, 64.51):
+        x = torch.full((V,), -off * step)
+        x[V * 3 // 5:] = -(off + 2.0) * step
+        x[7] = 0.0
+        rows = x[None].expand(B, V).contiguous()
+        u = torch.linspace(0.01, 0.99, B)
+        tokens, probs = ops.sample(rows.to(DEV), u.to(DEV), top_p=0.75)
+        e = torch.exp(x.double())
+        order = torch.argsort(e, descending=True, stable=True)
+        mass = torch.cumsum(e[order], 0)
+        n = int((mass - e[order] <= 0.75 * mass[-1]).sum())   # kept: those whose preceding mass is at most the share
+        kept = torch.zeros(V, dtype=torch.bool)
+        kept[order[:n]] = True
+        run = torch.cumsum(torch.where(kept, e, 0.0), 0)
+        for b in {0, B // 2, B - 1}:
+            # (equal weights by the thousand: sums of 10^5 rounded terms are good to 2^-36 of themselves, which is less than
+            # half a weight, so the place is off by one at most on either side)
+            want = int(torch.searchsorted(run, float(u[b]) * run[-1], right=True))
+            assert abs(int(tokens[b]) - want) <= 1
+            assert abs(float(probs[b]) - float(e[want] / run[-1])) <= float(e[want] / run[-1]) * 2.0 ** -16
