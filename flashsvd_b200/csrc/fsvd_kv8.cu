@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
   const int count = a.new_lens ? min(max(a.new_lens[b], 0), a.L) : a.L;
   const long long end_ll = (long long)start + count;
   const int end = (int)min(end_ll, (long long)a.c.S_max);
-  if (end_ll > a.c.S_max && j == 0 && grp == 0 && tid == 0) atomicCAS(a.status, (int)DS_OK, (int)DS_CACHE_FULL);
+  if (count > 0 && end_ll > a.c.S_max && j == 0 && grp == 0 && tid == 0) atomicCAS(a.status, (int)DS_OK, (int)DS_CACHE_FULL);
   const int blk = start / BLOCK + j;
   const long long blk0 = (long long)blk * BLOCK;
   if (blk0 >= end_ll) return;

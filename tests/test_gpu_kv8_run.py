@@ -405,3 +405,113 @@ def test_rotary_module_rotates_without_tables():
     for y, x in zip(got, (q, k)):
         want = ref.rotate(x, pos, f)
         assert bool(((y.double().cpu() - want).abs() <= want.abs() * 2.0 ** -8 + 2.0 ** -20 * float(x.abs().max())).all())
+
+
+def test_model_step_over_the_8bit_cache_eager_and_captured():
+    """A transformers Llama of these modules: prompt at once or token by token fill the caches alike up to the projections'
+    own roundings; a step with its position on the device, captured and replayed, equals the eager one bit for bit."""
+    from flashsvd_b200 import runtime as R
+    from tests.test_gpu_boundary import _hf_model
+
+    shape, dev = O.TINY_GQA, torch.device(DEV)
+    w = O.make_model_weights(shape, seed=4, dtype=torch.bfloat16)
+    model = _hf_model(shape, w, torch.bfloat16, dev)
+    with torch.inference_mode():
+        layers = len(model.model.layers)
+        ids = torch.randint(0, shape.vocab, (2, 12), generator=torch.Generator().manual_seed(8)).to(dev)
+        runs = []
+        for captured in (False, True):
+            cache = R.FlashSVDV15KV8Cache(model.config, max_batch_size=2, max_cache_len=32, device=dev, block=16)
+            logits = [R.manual_llama_decode_step(model, ids[:, :6], past_key_values=cache, cache_position=torch.arange(6)).logits.clone()]
+            assert [cache.get_seq_length(i) for i in range(layers)] == [6] * layers
+            if captured:
+                tok, pos = ids[:, :1].clone(), torch.tensor([31], device=dev)
+                R.manual_llama_decode_step(model, tok, past_key_values=cache, cache_position=pos)   # (workspaces, at a place not used)
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    out = R.manual_llama_decode_step(model, tok, past_key_values=cache, cache_position=pos).logits
+            for t in range(6, 12):
+                if captured:
+                    tok.copy_(ids[:, t:t + 1])
+                    pos.fill_(t)
+                    graph.replay()
+                    logits.append(out.clone())
+                else:
+                    logits.append(R.manual_llama_decode_step(model, ids[:, t:t + 1], past_key_values=cache,
+                                                             cache_position=torch.tensor([t])).logits.clone())
+            runs.append((logits, [(c.k.view(torch.uint8)[:, :, :12].clone(), c.v.view(torch.uint8)[:, :, :12].clone()) for c in cache.layers8]))
+        for x, y in zip(*(r[0] for r in runs)):
+            assert bool(torch.isfinite(x).all()) and torch.equal(x, y)
+        for x, y in zip(*(r[1] for r in runs)):
+            assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+        with pytest.raises(IndexError):
+            R.manual_llama_decode_step(model, ids[:, :1], past_key_values=cache, cache_position=torch.tensor([32]))
+
+
+def test_calls_beside_each_other_with_workspaces_of_their_own():
+    """Append, read-back, attention and sampling of two models on two streams at once, many times over."""
+    models = [_Loop(4, 8, 2, 128, 400, 5003, 64, bool(i)) for i in range(2)]
+    ids = torch.arange(400).view(4, 100)
+    us = torch.rand(20, 4, generator=torch.Generator().manual_seed(1)).to(DEV)
+    want = []
+    for m in models:
+        m.prompt(ids, [100, 64, 3, 0])
+        trace = []
+        for u in us:
+            m.u.copy_(u)
+            q, a, logits, share = m.step()
+            trace += [a, m.tokens.clone(), share]
+        want.append(trace)
+    torch.cuda.synchronize()
+    again = [_Loop(4, 8, 2, 128, 400, 5003, 64, bool(i)) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in again]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for m, s in zip(again, streams):
+        with torch.cuda.stream(s):
+            m.prompt(ids, [100, 64, 3, 0])
+    for u in us:
+        for i, (m, s) in enumerate(zip(again, streams)):
+            with torch.cuda.stream(s):
+                m.u.copy_(u)
+                q, a, logits, share = m.step()
+                got[i] += [a, m.tokens.clone(), share]
+    torch.cuda.synchronize()
+    for x, y in zip(want, got):
+        assert all(torch.equal(p, q) for p, q in zip(x, y))
+
+
+def test_lengths_at_and_past_their_ends():
+    """Negative and huge lengths: nothing is read or written outside, the flag is set where a token was dropped."""
+    from flashsvd_b200 import kv8, ops
+
+    B, H, Hk, Dh, S, block = 5, 4, 2, 64, 40, 16
+    gen = torch.Generator().manual_seed(17)
+    for L in (1, 3):
+        cache = kv8.KV8Cache.empty(B, S, Hk, Dh, block=block, device=DEV)
+        ws = ops.make_kv8_workspace(B, H, Hk, Dh, S, DEV)
+        x = torch.randn(B, S, Hk, Dh, generator=gen).to(torch.bfloat16).to(DEV)
+        ops.kv8_append(x, x, cache, torch.zeros(B, dtype=torch.int32, device=DEV), ws)
+        before = [t.clone() for t in (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)]
+        lens = torch.tensor([S, 2 ** 31 - 1, 7, 39, -5], dtype=torch.int32, device=DEV)
+        new = torch.tensor([L, L, -3, 0, 0], dtype=torch.int32, device=DEV)
+        y = torch.randn(B, L, Hk, Dh, generator=gen).to(torch.bfloat16).to(DEV)
+        ops.kv8_append(y, y, cache, lens, ws, new_lens=new)
+        after = (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)
+        assert all(torch.equal(a, b) for a, b in zip(before, after))
+        assert ws.raw_status() != 0
+        ws.clear_status()
+        ops.kv8_append(y, y, cache, lens, ws, new_lens=torch.tensor([0, 0, L + 5, 1, 0], dtype=torch.int32, device=DEV))
+        assert ws.status() == 0
+        k = ops.kv8_load(cache, 0, S)[0]
+        old = (before[0].view(torch.float8_e4m3fn).float() * before[2].repeat_interleave(block, 2)[:, :, :S, None]).to(torch.bfloat16)
+        assert torch.equal(k[0], old[0]) and torch.equal(k[1], old[1]) and torch.equal(k[4], old[4])
+        q = torch.randn(B, H, Dh, generator=gen).to(torch.bfloat16).to(DEV)
+        full = ops.flash_decode_kv8(q, cache, torch.tensor([S, S, 10, S, 0], dtype=torch.int32, device=DEV), ws)
+        assert torch.equal(full, ops.flash_decode_kv8(q, cache, torch.tensor([2 ** 31 - 1, S, 10, S + 1, -9], dtype=torch.int32, device=DEV), ws))
+        assert torch.equal(full, ops.flash_decode_kv8(q, cache, torch.tensor([2 ** 31 - 1, S - 3, 7, S, -2 ** 31], dtype=torch.int32,
+                                                                             device=DEV), ws, seqlen_add=3))
+        k2 = ops.kv8_load(cache, 2, 9, cache_seqlens=torch.tensor([2 ** 31 - 1, -1, 3, -2 ** 31, 11], dtype=torch.int32, device=DEV))[0]
+        for b, n in enumerate((9, 0, 1, 0, 9)):
+            assert torch.equal(k2[b, :, :n], k[b, :, 2:2 + n]) and not bool(k2[b, :, n:].any())

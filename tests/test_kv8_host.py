@@ -146,3 +146,13 @@ def test_the_reference_forms():
     x = x.clamp(-448, 448)
     assert torch.equal(ref.e4m3(x.double()).float(), x.to(torch.float8_e4m3fn).float())
     assert ref.exponent(448.0) == 0 and ref.exponent(448.1) == 1 and ref.exponent(3.5) == -7 and ref.exponent(0.0) == -60
+
+
+def test_sizes_that_would_not_fit_their_types(lib):
+    from flashsvd_b200 import ops
+
+    _refused(lib, -2, lib.fsvd_rope_qk(P, 1 << 24, P, 64, P, P, 64, 0, 1.0, P, P, 3, 1 << 17, 1, 64, 0, None), "heads")
+    _refused(lib, -2, lib.fsvd_kv8_append(_cache(), P, P, 256, 256, P, None, P, 256, 256, P, P, 64, 0, 1.0, 1 << 17, 1, P, 1 << 20, None), "heads")
+    for n in (1 << 31, -(1 << 31) - 1):
+        with pytest.raises(ValueError):
+            ops._add(n)
