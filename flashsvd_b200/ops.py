@@ -311,23 +311,15 @@ def _raw_stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-class _SameDevice:
-    """Makes the device of the tensors current for the launch (nothing to do when it is)."""
-
-    __slots__ = ("index", "was")
-
-    def __init__(self, index: int):
-        self.index, self.was = index, None
-
-    def __enter__(self):
-        now = torch._C._cuda_getDevice()
-        if now != self.index:
-            self.was = now
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.was is not None:
-            torch.cuda.set_device(self.was)
+def _launch(index: int, entry, *args) -> None:
+    """A call into the library with the tensors' device current; its status."""
+    if torch._C._cuda_getDevice() == index:
+        status = entry(*args)
+    else:
+        with torch.cuda.device(index):
+            status = entry(*args)
+    if status:
+        check(status)
 
 
 def _refuse(name: str, t, dtype, index: int, shape, strided: bool):
@@ -345,15 +337,21 @@ def _refuse(name: str, t, dtype, index: int, shape, strided: bool):
 
 def _ok(name: str, t, dtype, index: int, shape=None):
     """A contiguous tensor of this type, device and shape; its address."""
-    if not (torch.is_tensor(t) and t.dtype is dtype and t.get_device() == index and (shape is None or t.shape == shape)
-            and t.is_contiguous()):
-        _refuse(name, t, dtype, index, shape, False)
-    return t.data_ptr()
+    try:
+        if t.dtype is dtype and t.get_device() == index and (shape is None or t.shape == shape) and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:   # (no tensor)
+        pass
+    _refuse(name, t, dtype, index, shape, False)
 
 
 def _ok_strided(name: str, t, dtype, index: int, shape):
     """As `_ok`, with any strides in front of the last two dimensions."""
-    if not (torch.is_tensor(t) and t.dtype is dtype and t.get_device() == index and t.shape == shape):
+    try:
+        fits = t.dtype is dtype and t.get_device() == index and t.shape == shape
+    except AttributeError:
+        fits = False
+    if not fits:
         _refuse(name, t, dtype, index, shape, True)
     if not t.is_contiguous() and t.numel():
         H, D = shape[-2:]
@@ -402,18 +400,21 @@ def rope_qk(q, k, positions, inv_freq, *, interleaved=False, scale=1.0, q_out=No
         kp = _ok_strided("k", k, dtype, index, (T, Hk, Dh))
         if k_out is None:
             k_out = _room_like(k)
-        kop = _ok("k_out", k_out, dtype, index, (T, Hk, Dh))
+            kop = k_out.data_ptr()
+        else:
+            kop = _ok("k_out", k_out, dtype, index, (T, Hk, Dh))
         ks = k.stride(0) if T > 1 else 0
     elif k_out is not None:
         raise ValueError("k_out without k")
     if q_out is None:
         q_out = _room_like(q)
-    qop = _ok("q_out", q_out, dtype, index, shape)
+        qop = q_out.data_ptr()
+    else:
+        qop = _ok("q_out", q_out, dtype, index, shape)
     if T == 0:
         return q_out, k_out
-    with _SameDevice(index):
-        check(_library().fsvd_rope_qk(qp, q.stride(0) if T > 1 else 0, kp, ks, pp, fp, 2 * inv_freq.shape[0], 1 if interleaved else 0,
-                                      scale, qop, kop, T, H, Hk, Dh, code, _raw_stream(index)))
+    _launch(index, _library().fsvd_rope_qk, qp, q.stride(0) if T > 1 else 0, kp, ks, pp, fp, 2 * inv_freq.shape[0],
+            1 if interleaved else 0, scale, qop, kop, T, H, Hk, Dh, code, _raw_stream(index))
     return q_out, k_out
 
 
@@ -479,15 +480,16 @@ def kv8_append(k, v, cache, cache_seqlens, ws: Workspace, *, new_lens=None, q=No
         qs0, qs1 = q.stride()[:2]
         if q_out is None:
             q_out = _room_like(q)
-        qop = _ok("q_out", q_out, _BF16, index, qshape)
+            qop = q_out.data_ptr()
+        else:
+            qop = _ok("q_out", q_out, _BF16, index, qshape)
     elif q_out is not None:
         raise ValueError("q_out without q")
     wp = _scratch(ws, index)
     if L == 0:
         return q_out
-    with _SameDevice(index):
-        check(_library().fsvd_kv8_append(cache.ref, kp, vp, kst[0], kst[1], sp, np_, qp, qs0, qs1, qop, fp, R, inter, scale, H, L, wp,
-                                         ws.nbytes, _raw_stream(index)))
+    _launch(index, _library().fsvd_kv8_append, cache.ref, kp, vp, kst[0], kst[1], sp, np_, qp, qs0, qs1, qop, fp, R, inter, scale,
+            H, L, wp, ws.nbytes, _raw_stream(index))
     return q_out
 
 
@@ -502,13 +504,17 @@ def kv8_load(cache, start, length, *, cache_seqlens=None, seqlen_add=0, k_out=No
     sp = None if cache_seqlens is None else _ok("cache_seqlens", cache_seqlens, _I32, index, (st.B,))
     if k_out is None:
         k_out = cache.k.new_empty(shape, dtype=_BF16)
+        kp = k_out.data_ptr()
+    else:
+        kp = _ok("k_out", k_out, _BF16, index, shape)
     if v_out is None:
-        v_out = cache.k.new_empty(shape, dtype=_BF16)
-    kp, vp = _ok("k_out", k_out, _BF16, index, shape), _ok("v_out", v_out, _BF16, index, shape)
+        v_out = torch.empty_like(k_out)
+        vp = v_out.data_ptr()
+    else:
+        vp = _ok("v_out", v_out, _BF16, index, shape)
     if length == 0:
         return k_out, v_out
-    with _SameDevice(index):
-        check(_library().fsvd_kv8_load(cache.ref, start, length, sp, _add(seqlen_add), kp, vp, _raw_stream(index)))
+    _launch(index, _library().fsvd_kv8_load, cache.ref, start, length, sp, _add(seqlen_add), kp, vp, _raw_stream(index))
     return k_out, v_out
 
 
@@ -524,10 +530,11 @@ def flash_decode_kv8(q, cache, cache_seqlens, ws: Workspace, *, seqlen_add=0, sc
     sp = _ok("cache_seqlens", cache_seqlens, _I32, index, (st.B,))
     if out is None:
         out = torch.empty_like(q)
-    op = _ok("out", out, _BF16, index, shape)
+        op = out.data_ptr()
+    else:
+        op = _ok("out", out, _BF16, index, shape)
     wp = _scratch(ws, index)
-    with _SameDevice(index):
-        check(_library().fsvd_flash_decode_kv8(cache.ref, qp, sp, _add(seqlen_add), op, H, scale, wp, ws.nbytes, _raw_stream(index)))
+    _launch(index, _library().fsvd_flash_decode_kv8, cache.ref, qp, sp, _add(seqlen_add), op, H, scale, wp, ws.nbytes, _raw_stream(index))
     return out
 
 
@@ -561,13 +568,17 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     if torch.is_tensor(min_p):
         mp, min_p = _ok("min_p", min_p, _F32, index, rows), 0.0
     if out is None:
-        out = uniforms.new_empty(rows, dtype=_I32)
+        out = torch.empty_like(uniforms, dtype=_I32)
+        op = out.data_ptr()
+    else:
+        op = _ok("out", out, _I32, index, rows)
     if probs_out is None:
         probs_out = torch.empty_like(uniforms)
-    op, bp = _ok("out", out, _I32, index, rows), _ok("probs_out", probs_out, _F32, index, rows)
+        bp = probs_out.data_ptr()
+    else:
+        bp = _ok("probs_out", probs_out, _F32, index, rows)
     if B == 0:
         return out, probs_out
-    with _SameDevice(index):
-        check(_library().fsvd_sample(logits.data_ptr(), logits.stride(0) if B > 1 else V, code, up, tp, kp, pp, mp, temperature, top_k,
-                                     top_p, min_p, op, bp, B, V, _raw_stream(index)))
+    _launch(index, _library().fsvd_sample, logits.data_ptr(), logits.stride(0) if B > 1 else V, code, up, tp, kp, pp, mp, temperature,
+            top_k, top_p, min_p, op, bp, B, V, _raw_stream(index))
     return out, probs_out
