@@ -10,6 +10,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <atomic>
 
 #include "../../include/flashsvd_b200.h"
@@ -412,7 +413,8 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
     if (hk + 1 < hk1) fetch(hk + 1);
   }
   if (!a.q || t >= nq) return;
-  // queries: a thread keeps its token's cosines and sines while it goes through the heads, two at a time
+  // queries: a thread keeps its token's cosines and sines while it goes through the heads, several at a time
+  constexpr int kHeads = MANY ? 2 : 4;
   const int h0 = (int)((long long)a.H * grp / a.groups), h1 = (int)((long long)a.H * (grp + 1) / a.groups);
   float c[8], s[8];
   if (turns) {
@@ -427,25 +429,26 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
   const size_t tok = (size_t)(lo - start + t);
   const __nv_bfloat16* src = a.q + (size_t)b * a.q_batch + tok * a.q_token;
   __nv_bfloat16* dst = a.q_out + ((size_t)b * a.L + tok) * a.H * DH;
-  constexpr int N = 2;
-  for (int h = h0; h < h1; h += N) {
+  auto turn_heads = [&](auto many, int h) {
+    constexpr int N = decltype(many)::value;
     uint32_t w[N][8];
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (h + k < h1) fsvd_rope::load_pairs<WIDE>(src + (size_t)(h + k) * DH, u, R, inter, w[k]);
+    for (int k = 0; k < N; ++k) fsvd_rope::load_pairs<WIDE>(src + (size_t)(h + k) * DH, u, R, inter, w[k]);
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (h + k < h1) {
-        if (turns) {
+    for (int k = 0; k < N; ++k) {
+      if (turns) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (!WIDE && 8 * u + i >= half) break;
-            w[k][i] = turn_query(w[k][i], c[i], s[i]);
-          }
+        for (int i = 0; i < 8; ++i) {
+          if (!WIDE && 8 * u + i >= half) break;
+          w[k][i] = turn_query(w[k][i], c[i], s[i]);
         }
-        fsvd_rope::store_pairs<WIDE>(dst + (size_t)(h + k) * DH, u, R, inter, w[k]);
       }
-  }
+      fsvd_rope::store_pairs<WIDE>(dst + (size_t)(h + k) * DH, u, R, inter, w[k]);
+    }
+  };
+  int h = h0;
+  for (; h + kHeads <= h1; h += kHeads) turn_heads(std::integral_constant<int, kHeads>{}, h);
+  for (; h < h1; ++h) turn_heads(std::integral_constant<int, 1>{}, h);
 }
 
 // A single token per sequence: the rows of a CTA are heads, not tokens, so that every thread has a share (the kernel above
