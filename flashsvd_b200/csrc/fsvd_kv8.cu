@@ -24,6 +24,10 @@ namespace fsvd_kv8_impl {
 using fsvd::DS_CACHE_FULL;
 using fsvd::DS_OK;
 using fsvd::SyncState;
+using fsvd_rope::Form;
+using fsvd_rope::kSingle;
+using fsvd_rope::kTogether;
+using fsvd_rope::kVectors;
 using fsvd_rope::Rotary;
 
 static int fail(int code, const char* fmt, ...) {
@@ -36,6 +40,7 @@ static int fail(int code, const char* fmt, ...) {
   return code;
 }
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
 
 static int sm_count() {
   static std::atomic<int> cache[16];
@@ -88,13 +93,14 @@ struct RopeArgs {
   const int* positions;
   Rotary rot;
   int T, H, Hk, Dh, tokens, heads;   // tokens and heads of a CTA
+  bool on32;                         // all rows begin on boundaries of 32 bytes
 };
 constexpr int kRopeTokens = 32;
 constexpr int kMaxHeads = 1 << 16;
 
 // A CTA turns `tokens` rows of heads; its threads go through the (token, head, unit) list in steps of kThreads, several units
 // at a time so that their loads are under way together.
-template <typename T, bool WIDE>
+template <typename T, Form FORM>
 __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
   constexpr int N = 2;                              // units at a time
   extern __shared__ __align__(16) float2 table[];   // per token: cosine and sine of the pairs, in slots (below)
@@ -132,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
         const T* src = q ? reinterpret_cast<const T*>(a.q) + tt * a.q_stride + (size_t)h * a.Dh
                          : reinterpret_cast<const T*>(a.k) + tt * a.k_stride + (size_t)(h - a.H) * a.Dh;
         dst[k] = q ? reinterpret_cast<T*>(a.q_out) + (tt * a.H + h) * a.Dh : reinterpret_cast<T*>(a.k_out) + (tt * a.Hk + h - a.H) * a.Dh;
-        fsvd_rope::load_unit<WIDE>(src, unit[k], R, inter, x[k], y[k]);
+        fsvd_rope::load_unit<FORM>(src, unit[k], R, inter, x[k], y[k]);
       }
     }
 #pragma unroll
@@ -149,11 +155,11 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
             const float4 two = cs[slot_of(e >> 1, unit[k])];
-            if (WIDE || 8 * unit[k] + e < half) turn(e, two.x, two.y);
-            if (WIDE || 8 * unit[k] + e + 1 < half) turn(e + 1, two.z, two.w);
+            if (FORM != kSingle || 8 * unit[k] + e < half) turn(e, two.x, two.y);
+            if (FORM != kSingle || 8 * unit[k] + e + 1 < half) turn(e + 1, two.z, two.w);
           }
         }
-        fsvd_rope::store_unit<WIDE>(dst[k], unit[k], R, inter, x[k], y[k]);
+        fsvd_rope::store_unit<FORM>(dst[k], unit[k], R, inter, x[k], y[k]);
       }
   }
 }
@@ -169,6 +175,7 @@ struct AppendArgs {
   Rotary rot;       // R = 0: no rotation
   int H, L, groups; // groups: head groups of a (sequence, block)
   int nblk;         // blocks that L tokens can touch
+  bool on32;   // all rows of k, v and q begin on boundaries of 32 bytes
 };
 
 // Exponent of the scale for a largest magnitude: the smallest e >= -60 with amax <= 448 2^e (448 = 1.75 * 2^8).
@@ -250,10 +257,10 @@ __device__ __forceinline__ void codes_of(const uint32_t (&w)[8], float inv, bool
     for (int i = 0; i < 8; ++i) cd[i] = careful_codes(w[i], inv);
   }
 }
-template <bool WIDE>
+template <Form FORM>
 __device__ __forceinline__ void store_codes(uint8_t* dst, const uint32_t (&cd)[8], int u, int R, int inter) {
   const int half = R >> 1;
-  if constexpr (WIDE) {
+  if constexpr (FORM != kSingle) {
     const bool split = !inter && 16 * u < R;
     const uint32_t a03 = __byte_perm(cd[0] | (cd[1] << 16), cd[2] | (cd[3] << 16), 0x6420);
     const uint32_t a47 = __byte_perm(cd[4] | (cd[5] << 16), cd[6] | (cd[7] << 16), 0x6420);
@@ -291,7 +298,7 @@ __device__ __forceinline__ uint32_t rescaled(uint32_t x, float f) {
 // table under way together, or 1024 of 64 (MANY), which overlap better once there is much to do.
 template <int DH, int BLOCK> constexpr int kAppendThreads = BLOCK * DH / 16;
 template <int DH, int BLOCK, bool MANY> constexpr int kAppendCtas = std::max(1, (MANY ? 1024 : 512) / kAppendThreads<DH, BLOCK>);
-template <int DH, int BLOCK, bool WIDE, bool MANY>
+template <int DH, int BLOCK, Form FORM, bool MANY>
 __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLOCK, MANY>) append_kernel(const AppendArgs a) {
   constexpr int kThreads = kAppendThreads<DH, BLOCK>, U = DH / 16;
   extern __shared__ double2 tab[];   // per token: cosine and sine of the pairs
@@ -324,8 +331,8 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
     for (int i = 0; i < 8; ++i) kreg[i] = vreg[i] = 0u;
     if (t < n) {
       const size_t off = (size_t)b * a.kv_batch + (size_t)(lo - start + t) * a.kv_token + (size_t)hk * DH;
-      fsvd_rope::load_pairs<WIDE>(a.k + off, u, R, inter, kreg);
-      fsvd_rope::load_pairs<WIDE>(a.v + off, u, R, inter, vreg);
+      fsvd_rope::load_pairs<FORM>(a.k + off, u, R, inter, kreg);
+      fsvd_rope::load_pairs<FORM>(a.v + off, u, R, inter, vreg);
     }
   };
   if (n > 0 && hk0 < hk1) fetch(hk0);   // (the first head is under way while the angles are formed)
@@ -363,7 +370,7 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
     if (turns && t < n) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (!WIDE && 8 * u + i >= half) break;
+        if (FORM == kSingle && 8 * u + i >= half) break;
         kreg[i] = turn_key(kreg[i], my_tab[t * slots + i * units]);
       }
     }
@@ -402,9 +409,9 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
       const size_t row = (size_t)(lo - blk0 + t) * DH;
       uint32_t cd[8];   // codes of the pairs: low byte a, high byte b
       codes_of(kreg, ki, ks.odd, cd);
-      store_codes<WIDE>(kc + row, cd, u, R, inter);
+      store_codes<FORM>(kc + row, cd, u, R, inter);
       codes_of(vreg, vi, vs.odd, cd);
-      store_codes<WIDE>(vc + row, cd, u, R, inter);
+      store_codes<FORM>(vc + row, cd, u, R, inter);
     }
     if (tid == 0) {
       a.c.k_scale[si] = kscale;
@@ -420,7 +427,7 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
   if (turns) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const bool in = WIDE || 8 * u + i < half;
+      const bool in = FORM != kSingle || 8 * u + i < half;
       const double2 cs = my_tab[t * slots + (in ? i * units : 0)];
       c[i] = (float)cs.x;
       s[i] = (float)cs.y;
@@ -433,17 +440,17 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
     constexpr int N = decltype(many)::value;
     uint32_t w[N][8];
 #pragma unroll
-    for (int k = 0; k < N; ++k) fsvd_rope::load_pairs<WIDE>(src + (size_t)(h + k) * DH, u, R, inter, w[k]);
+    for (int k = 0; k < N; ++k) fsvd_rope::load_pairs<FORM>(src + (size_t)(h + k) * DH, u, R, inter, w[k]);
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       if (turns) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if (!WIDE && 8 * u + i >= half) break;
+          if (FORM == kSingle && 8 * u + i >= half) break;
           w[k][i] = turn_query(w[k][i], c[i], s[i]);
         }
       }
-      fsvd_rope::store_pairs<WIDE>(dst + (size_t)(h + k) * DH, u, R, inter, w[k]);
+      fsvd_rope::store_pairs<FORM>(dst + (size_t)(h + k) * DH, u, R, inter, w[k]);
     }
   };
   int h = h0;
@@ -454,7 +461,7 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
 // A single token per sequence: the rows of a CTA are heads, not tokens, so that every thread has a share (the kernel above
 // would leave all rows but one idle: a step of 128 sequences with 32 heads took 32.2 us, here 5.0; of 8 sequences 4.4 and 3.8).
 // Almost all of a small step is latency: one load, one sine in 64 bits (about 1500 clocks), one store.
-template <int DH, bool WIDE>
+template <int DH, Form FORM>
 __global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs a) {
   constexpr int U = DH / 16;
   __shared__ double2 tab[DH / 2];   // pair p in slot (p % 8) * units + p / 8
@@ -477,14 +484,14 @@ __global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs 
   float kold = 0.0f, vold = 0.0f;
   if (has_kv) {
     const size_t off = (size_t)b * a.kv_batch + (size_t)hk * DH;
-    fsvd_rope::load_pairs<WIDE>(a.k + off, u, R, inter, kw);
-    fsvd_rope::load_pairs<WIDE>(a.v + off, u, R, inter, vw);
+    fsvd_rope::load_pairs<FORM>(a.k + off, u, R, inter, kw);
+    fsvd_rope::load_pairs<FORM>(a.v + off, u, R, inter, vw);
     if (old) {
       kold = a.c.k_scale[si];
       vold = a.c.v_scale[si];
     }
   }
-  if (has_q) fsvd_rope::load_pairs<WIDE>(a.q + (size_t)b * a.q_batch + (size_t)h * DH, u, R, inter, qw);
+  if (has_q) fsvd_rope::load_pairs<FORM>(a.q + (size_t)b * a.q_batch + (size_t)h * DH, u, R, inter, qw);
   if (tid < half) {
     double c, s;
     fsvd_rope::angle(start, a.rot.inv_freq[tid], a.rot.scale, c, s);
@@ -494,13 +501,13 @@ __global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs 
   if (8 * u < half) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (!WIDE && 8 * u + i >= half) break;
+      if (FORM == kSingle && 8 * u + i >= half) break;
       const double2 cs = tab[i * units + u];
       if (has_kv) kw[i] = turn_key(kw[i], cs);
       if (has_q) qw[i] = turn_query(qw[i], (float)cs.x, (float)cs.y);
     }
   }
-  if (has_q) fsvd_rope::store_pairs<WIDE>(a.q_out + ((size_t)b * a.H + h) * DH, u, R, inter, qw);
+  if (has_q) fsvd_rope::store_pairs<FORM>(a.q_out + ((size_t)b * a.H + h) * DH, u, R, inter, qw);
   Share ks, vs;
   largest(kw, ks);
   largest(vw, vs);
@@ -517,9 +524,9 @@ __global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs 
   if (has_kv) {
     uint32_t cd[8];
     codes_of(kw, 1.0f / kscale, ks.odd, cd);
-    store_codes<WIDE>(reinterpret_cast<uint8_t*>(a.c.k8) + base + (size_t)old * DH, cd, u, R, inter);
+    store_codes<FORM>(reinterpret_cast<uint8_t*>(a.c.k8) + base + (size_t)old * DH, cd, u, R, inter);
     codes_of(vw, 1.0f / vscale, vs.odd, cd);
-    store_codes<WIDE>(reinterpret_cast<uint8_t*>(a.c.v8) + base + (size_t)old * DH, cd, u, R, inter);
+    store_codes<FORM>(reinterpret_cast<uint8_t*>(a.c.v8) + base + (size_t)old * DH, cd, u, R, inter);
     if (u == 0) {
       a.c.k_scale[si] = kscale;
       a.c.v_scale[si] = vscale;
@@ -553,6 +560,7 @@ struct LoadArgs {
   int start, length, seqlen_add;
   const int* seqlens;
   __nv_bfloat16 *k_out, *v_out;
+  bool on32;   // which begin on boundaries of 32 bytes
 };
 
 // A thread reads back one sixteen-byte piece, counted through all planes (a sequence's head, keys or values): a short plane
@@ -587,8 +595,12 @@ __global__ void __launch_bounds__(kThreads) load_kernel(const LoadArgs a) {
     o[2 * e + 1] = fsvd_rope::pack2(q.x * f, q.y * f);
   }
   uint4* dst = reinterpret_cast<uint4*>(second ? a.v_out : a.k_out) + 2 * ((size_t)bh * pieces + at);
-  dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  if (a.on32) {
+    fsvd_rope::store32(dst, o);
+  } else {
+    dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  }
 }
 
 // ------------------------------------------------------------------------------------------ host
@@ -674,15 +686,19 @@ static int launch_rope(RopeArgs& a, int dtype, void* stream) {
   a.heads = (all + splits - 1) / splits;
   const dim3 grid(ctas, (all + a.heads - 1) / a.heads);
   const size_t smem = (size_t)a.tokens * ((a.rot.R / 2 + 7) / 8 * 8) * sizeof(float2);
-  const bool wide = a.rot.R % 16 == 0;
+  const Form form = a.rot.R % 16 ? kSingle : dtype == FSVD_DTYPE_BF16 && a.rot.interleaved && a.on32 ? kTogether : kVectors;
   if (dtype == FSVD_DTYPE_F32)
-    return wide ? launch(rope_kernel<float, true>, grid, kThreads, smem, stream, a)
-                : launch(rope_kernel<float, false>, grid, kThreads, smem, stream, a);
-  return wide ? launch(rope_kernel<__nv_bfloat16, true>, grid, kThreads, smem, stream, a)
-              : launch(rope_kernel<__nv_bfloat16, false>, grid, kThreads, smem, stream, a);
+    return form == kSingle ? launch(rope_kernel<float, kSingle>, grid, kThreads, smem, stream, a)
+                           : launch(rope_kernel<float, kVectors>, grid, kThreads, smem, stream, a);
+  return form == kSingle    ? launch(rope_kernel<__nv_bfloat16, kSingle>, grid, kThreads, smem, stream, a)
+         : form == kVectors ? launch(rope_kernel<__nv_bfloat16, kVectors>, grid, kThreads, smem, stream, a)
+                            : launch(rope_kernel<__nv_bfloat16, kTogether>, grid, kThreads, smem, stream, a);
 }
 
-template <int DH, int BLOCK, bool MANY>
+static Form form_of(const AppendArgs& a) {
+  return a.rot.R % 16 ? kSingle : a.on32 && (a.rot.interleaved || !a.rot.R) ? kTogether : kVectors;
+}
+template <int DH, int BLOCK, Form FORM, bool MANY>
 static int launch_append(AppendArgs a, void* stream) {
   // Heads of a CTA share the table of angles.  Of the groupings by halves the one with the least waves x (planes of a CTA +
   // kTable), the table being worth about as much as four planes (keys, values or queries of a head).  Beside as few groups
@@ -699,18 +715,26 @@ static int launch_append(AppendArgs a, void* stream) {
   if (grid > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many tokens for one call");
   const int tile = std::min(BLOCK, a.L);
   const size_t smem = (size_t)((a.rot.R / 2 + 7) / 8 * 8) * (tile + (tile > 8 ? 8 + (tile + 7) / 8 : 0)) * sizeof(double2);
-  return a.rot.R % 16 == 0 ? launch(append_kernel<DH, BLOCK, true, MANY>, dim3((unsigned)grid), kAppendThreads<DH, BLOCK>, smem, stream, a)
-                           : launch(append_kernel<DH, BLOCK, false, MANY>, dim3((unsigned)grid), kAppendThreads<DH, BLOCK>, smem, stream, a);
+  return launch(append_kernel<DH, BLOCK, FORM, MANY>, dim3((unsigned)grid), kAppendThreads<DH, BLOCK>, smem, stream, a);
 }
-template <int DH, int BLOCK>
+template <int DH, int BLOCK, Form FORM>
 static int launch_append(const AppendArgs& a, void* stream) {
   // Rows (a head's token of keys, values or queries) of an SM from which the 1024 threads are ahead; us at 512 and 1024
   // threads, heads of 128: 512 tokens with 32 heads (331 rows) 9.7 and 11.1, 1024 (662) 14.8 and 15.8, 2041 (1320) 30.5 and
   // 27.3, 4096 with 32 and 8 (1328) 28.6 and 23.8, 4 x 1024 with 64 and 8 in blocks of 32 (2213) 46.3 and 36.9.  Without
   // rotation there is no table to wait for: 2041 tokens 18.4 and 13.3.
   if constexpr (kAppendThreads<DH, BLOCK> < 1024)
-    if (a.rot.R && (long long)a.c.B * a.L * (2 * a.c.Hk + a.H) < 1024ll * sm_count()) return launch_append<DH, BLOCK, false>(a, stream);
-  return launch_append<DH, BLOCK, true>(a, stream);
+    if (FORM == kSingle || (a.rot.R && (long long)a.c.B * a.L * (2 * a.c.Hk + a.H) < 1024ll * sm_count()))
+      return launch_append<DH, BLOCK, FORM, false>(a, stream);
+  if constexpr (kAppendThreads<DH, BLOCK> >= 1024 || FORM != kSingle) return launch_append<DH, BLOCK, FORM, true>(a, stream);
+  return 0;   // (not reached)
+}
+template <int DH, int BLOCK>
+static int launch_append(const AppendArgs& a, void* stream) {
+  const Form form = form_of(a);
+  return form == kSingle    ? launch_append<DH, BLOCK, kSingle>(a, stream)
+         : form == kVectors ? launch_append<DH, BLOCK, kVectors>(a, stream)
+                            : launch_append<DH, BLOCK, kTogether>(a, stream);
 }
 template <int DH>
 static int launch_append(const AppendArgs& given, void* stream) {
@@ -720,8 +744,10 @@ static int launch_append(const AppendArgs& given, void* stream) {
     a.groups = (std::max(a.H, a.c.Hk) + rows - 1) / rows;
     const long long grid = (long long)a.c.B * a.groups;
     if (grid > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many heads for one call");
-    return a.rot.R % 16 == 0 ? launch(append_step_kernel<DH, true>, dim3((unsigned)grid), kThreads, 0, stream, a)
-                             : launch(append_step_kernel<DH, false>, dim3((unsigned)grid), kThreads, 0, stream, a);
+    const Form form = form_of(a);
+    return form == kSingle    ? launch(append_step_kernel<DH, kSingle>, dim3((unsigned)grid), kThreads, 0, stream, a)
+           : form == kVectors ? launch(append_step_kernel<DH, kVectors>, dim3((unsigned)grid), kThreads, 0, stream, a)
+                              : launch(append_step_kernel<DH, kTogether>, dim3((unsigned)grid), kThreads, 0, stream, a);
   }
   switch (a.c.block) {
     case 16: return launch_append<DH, 16>(a, stream);
@@ -757,6 +783,7 @@ int fsvd_rope_qk(const void* q, long long q_stride, const void* k, long long k_s
   a.q_stride = q_stride; a.k_stride = k_stride; a.positions = positions;
   a.rot = Rotary{inv_freq, rotary_dim, interleaved != 0, rope_scale};
   a.T = T; a.H = H; a.Hk = Hk; a.Dh = Dh;
+  a.on32 = aligned32(q) && aligned32(k) && aligned32(q_out) && aligned32(k_out) && q_stride * es % 32 == 0 && k_stride * es % 32 == 0;
   return launch_rope(a, dtype, stream);
 }
 
@@ -793,6 +820,8 @@ int fsvd_kv8_append(const fsvd_kv8* cache, const void* k, const void* v, long lo
   a.status = &reinterpret_cast<SyncState*>(ws)->status;
   a.rot = Rotary{inv_freq, inv_freq ? rotary_dim : 0, interleaved != 0, rope_scale};
   a.H = q ? H : 0; a.L = L;
+  a.on32 = aligned32(k) && aligned32(v) && aligned32(q) && aligned32(q_out) && kv_batch_stride % 16 == 0 && kv_token_stride % 16 == 0 &&
+           q_batch_stride % 16 == 0 && q_token_stride % 16 == 0;
   const int BLOCK = cache->block;
   a.nblk = (int)(((long long)L + BLOCK - 2) / BLOCK + 1);
   if ((long long)cache->B * L > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many tokens for one call");
@@ -808,7 +837,7 @@ int fsvd_kv8_load(const fsvd_kv8* cache, int start, int length, const int* cache
   if (!aligned16(k_out) || !aligned16(v_out)) return fail(FSVD_ERR_ALIGN, "outputs must be 16-byte aligned");
   if (length == 0) return 0;
   LoadArgs a = {*cache, start, length, seqlen_add, cache_seqlens, reinterpret_cast<__nv_bfloat16*>(k_out),
-                reinterpret_cast<__nv_bfloat16*>(v_out)};
+                reinterpret_cast<__nv_bfloat16*>(v_out), aligned32(k_out) && aligned32(v_out)};
   const long long pieces = (long long)length * (cache->Dh / 16);
   const long long grid = (2ll * cache->B * cache->Hk * pieces + kThreads - 1) / kThreads;
   if (grid > 0x7fffffffll || pieces > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many tokens for one call");

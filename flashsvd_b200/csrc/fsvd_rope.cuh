@@ -3,12 +3,16 @@
 // A head of Dh dimensions is Dh / 2 pairs: pair p < R / 2 turns by position * inv_freq[p] and is made of dimensions
 // (p, p + R / 2), or (2 p, 2 p + 1) when interleaved; the pairs behind them, (R + 2 j, R + 2 j + 1), stay.  A thread
 // owns a unit of eight consecutive pairs of a row: it reads all 16 numbers before it writes any, so that a row can be
-// rotated in place.  When R is a multiple of 16 a unit is two 16-byte vectors (WIDE); else 16 single numbers.
+// rotated in place.
 #pragma once
 #include <cuda_bf16.h>
 #include <stdint.h>
 
 namespace fsvd_rope {
+
+// How a thread reads its unit: sixteen numbers one by one (R no multiple of 16), two vectors of eight, or one of sixteen
+// (bf16; interleaved, or no rotation; rows on boundaries of 32 bytes).
+enum Form { kSingle, kVectors, kTogether };
 
 struct Rotary {
   const double* inv_freq;   // [R / 2], radians per position
@@ -61,11 +65,34 @@ __device__ __forceinline__ float num(float x) { return x; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 __device__ __forceinline__ void put(float* p, float x) { *p = x; }
 
+// 32 bytes on a boundary of 32.  Where a thread's share of a row lies together, two accesses of 16 bytes would each touch every
+// other half of the warp's sectors.
+__device__ __forceinline__ void load32(const void* p, uint32_t (&w)[8]) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 // The eight pairs of unit u as (a[i], b[i]).
-template <bool WIDE, typename T>
+template <Form FORM, typename T>
 __device__ __forceinline__ void load_unit(const T* row, int u, int R, int interleaved, float (&a)[8], float (&b)[8]) {
-  if constexpr (WIDE) {
+  if constexpr (FORM != kSingle) {
     const bool split = !interleaved && 16 * u < R;   // (16 u = twice the first pair)
+    if constexpr (FORM == kTogether) {
+      uint32_t w[8];
+      load32(row + 16 * u, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a[i] = __uint_as_float(w[i] << 16);
+        b[i] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+      return;
+    }
     float x[8], y[8];
     load8(row + (split ? 8 * u : 16 * u), x);
     load8(row + (split ? 8 * u + (R >> 1) : 16 * u + 8), y);
@@ -84,10 +111,17 @@ __device__ __forceinline__ void load_unit(const T* row, int u, int R, int interl
     }
   }
 }
-template <bool WIDE, typename T>
+template <Form FORM, typename T>
 __device__ __forceinline__ void store_unit(T* row, int u, int R, int interleaved, const float (&a)[8], const float (&b)[8]) {
-  if constexpr (WIDE) {
+  if constexpr (FORM != kSingle) {
     const bool split = !interleaved && 16 * u < R;
+    if constexpr (FORM == kTogether) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = pack2(a[i], b[i]);
+      store32(row + 16 * u, w);
+      return;
+    }
     float x[8], y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -108,10 +142,14 @@ __device__ __forceinline__ void store_unit(T* row, int u, int R, int interleaved
 }
 
 // The same for bf16 rows as packed pairs: a in the low half of a word, b in the high one.
-template <bool WIDE>
+template <Form FORM>
 __device__ __forceinline__ void load_pairs(const __nv_bfloat16* row, int u, int R, int interleaved, uint32_t (&w)[8]) {
-  if constexpr (WIDE) {
+  if constexpr (FORM != kSingle) {
     const bool split = !interleaved && 16 * u < R;
+    if constexpr (FORM == kTogether) {
+      load32(row + 16 * u, w);
+      return;
+    }
     const uint4 x = *reinterpret_cast<const uint4*>(row + (split ? 8 * u : 16 * u));
     const uint4 y = *reinterpret_cast<const uint4*>(row + (split ? 8 * u + (R >> 1) : 16 * u + 8));
     const uint32_t p[4] = {x.x, x.y, x.z, x.w}, q[4] = {y.x, y.y, y.z, y.w};
@@ -129,10 +167,14 @@ __device__ __forceinline__ void load_pairs(const __nv_bfloat16* row, int u, int 
     }
   }
 }
-template <bool WIDE>
+template <Form FORM>
 __device__ __forceinline__ void store_pairs(__nv_bfloat16* row, int u, int R, int interleaved, const uint32_t (&w)[8]) {
-  if constexpr (WIDE) {
+  if constexpr (FORM != kSingle) {
     const bool split = !interleaved && 16 * u < R;
+    if constexpr (FORM == kTogether) {
+      store32(row + 16 * u, w);
+      return;
+    }
     uint32_t p[4], q[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -515,3 +515,37 @@ def test_lengths_at_and_past_their_ends():
         k2 = ops.kv8_load(cache, 2, 9, cache_seqlens=torch.tensor([2 ** 31 - 1, -1, 3, -2 ** 31, 11], dtype=torch.int32, device=DEV))[0]
         for b, n in enumerate((9, 0, 1, 0, 9)):
             assert torch.equal(k2[b, :, :n], k[b, :, 2:2 + n]) and not bool(k2[b, :, n:].any())
+
+
+@pytest.mark.parametrize("inter,R", [(True, 64), (True, 128), (False, 128), (False, 64), (True, 36), (False, 0)])
+def test_rows_on_boundaries_of_16_bytes_only(inter, R):
+    """The same call with every tensor 16 bytes behind a boundary of 32."""
+    from flashsvd_b200 import kv8, ops
+
+    B, H, Hk, Dh, S = 2, 6, 2, 128, 90
+    gen = torch.Generator().manual_seed(R)
+
+    def off(t):
+        return torch.empty(t.numel() + 8, dtype=t.dtype, device=DEV)[8:].view(t.shape).copy_(t)
+
+    rot = kv8.rotary(R, interleaved=inter, device=DEV) if R else None
+    ws = ops.make_kv8_workspace(B, H, Hk, Dh, S, DEV)
+    caches = [kv8.KV8Cache.empty(B, S, Hk, Dh, block=32, device=DEV) for _ in range(2)]
+    lens = torch.tensor([0, 5], dtype=torch.int32, device=DEV)
+    for L in (70, 1):
+        q, k, v = (torch.randn(B, L, n, Dh, generator=gen).to(torch.bfloat16).to(DEV) for n in (H, Hk, Hk))
+        a = ops.kv8_append(k, v, caches[0], lens, ws, q=q if R else None, rotary=rot)
+        b = ops.kv8_append(off(k), off(v), caches[1], lens, ws, q=off(q) if R else None, rotary=rot,
+                           q_out=off(torch.zeros_like(q)) if R else None)
+        assert (a is None and b is None) or torch.equal(a, b)
+        lens = lens + L
+        assert torch.equal(caches[0].k.view(torch.uint8), caches[1].k.view(torch.uint8))
+        assert torch.equal(caches[0].v.view(torch.uint8), caches[1].v.view(torch.uint8))
+        if R:
+            pos = torch.arange(L, dtype=torch.int32, device=DEV)
+            a = ops.rope_qk(q[0], k[0], pos, rot.inv_freq, interleaved=inter)
+            b = ops.rope_qk(off(q[0]), off(k[0]), pos, rot.inv_freq, interleaved=inter, q_out=off(q[0]), k_out=off(k[0]))
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    a = ops.kv8_load(caches[0], 3, 60)
+    b = ops.kv8_load(caches[0], 3, 60, k_out=off(torch.zeros_like(a[0])), v_out=off(torch.zeros_like(a[1])))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
