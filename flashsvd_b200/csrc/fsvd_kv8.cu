@@ -565,7 +565,7 @@ struct LoadArgs {
 
 // A thread reads back one sixteen-byte piece, counted through all planes (a sequence's head, keys or values): a short plane
 // leaves no thread idle, and many small CTAs hide the way from memory better than several pieces of a thread do (8 x 191
-// tokens with 32 heads of 128: 7.2 us, with two pieces 8.3, with four 10.4).
+// tokens with 32 heads of 128: 7.2 us, with two pieces 8.3, with four 10.4; 6.7 with stores of 32 bytes).
 template <int DH>
 __global__ void __launch_bounds__(kThreads) load_kernel(const LoadArgs a) {
   constexpr int V = DH / 16;   // pieces of a row
@@ -702,7 +702,7 @@ template <int DH, int BLOCK, Form FORM, bool MANY>
 static int launch_append(AppendArgs a, void* stream) {
   // Heads of a CTA share the table of angles.  Of the groupings by halves the one with the least waves x (planes of a CTA +
   // kTable), the table being worth about as much as four planes (keys, values or queries of a head).  Beside as few groups
-  // as give each SM two CTAs: 1024 tokens with 32 heads of 128 15.1 us (19.7), 2 x 1024 with 16 heads of 64 9.3 (12.6).
+  // as give each SM two CTAs, then: 1024 tokens with 32 heads of 128 15.1 us (19.7), 2 x 1024 with 16 heads of 64 9.3 (12.6).
   constexpr int kTable = 4;
   const long long tiles = (long long)a.c.B * ((a.L + BLOCK - 1) / BLOCK), fit = (long long)kAppendCtas<DH, BLOCK, MANY> * sm_count();
   auto cost = [&](int g) {
@@ -719,15 +719,18 @@ static int launch_append(AppendArgs a, void* stream) {
 }
 template <int DH, int BLOCK, Form FORM>
 static int launch_append(const AppendArgs& a, void* stream) {
-  // Rows (a head's token of keys, values or queries) of an SM from which the 1024 threads are ahead; us at 512 and 1024
-  // threads, heads of 128: 512 tokens with 32 heads (331 rows) 9.7 and 11.1, 1024 (662) 14.8 and 15.8, 2041 (1320) 30.5 and
-  // 27.3, 4096 with 32 and 8 (1328) 28.6 and 23.8, 4 x 1024 with 64 and 8 in blocks of 32 (2213) 46.3 and 36.9.  Without
-  // rotation there is no table to wait for: 2041 tokens 18.4 and 13.3.
-  if constexpr (kAppendThreads<DH, BLOCK> < 1024)
-    if (FORM == kSingle || (a.rot.R && (long long)a.c.B * a.L * (2 * a.c.Hk + a.H) < 1024ll * sm_count()))
-      return launch_append<DH, BLOCK, FORM, false>(a, stream);
-  if constexpr (kAppendThreads<DH, BLOCK> >= 1024 || FORM != kSingle) return launch_append<DH, BLOCK, FORM, true>(a, stream);
-  return 0;   // (not reached)
+  // Rows (a head's token of keys, values or queries) of an SM from which 1024 threads are ahead; us at 512 and 1024 threads,
+  // heads of 128: 512 tokens with 32 heads (331 rows) 9.8 and 10.7, 1024 (662) 14.6 and 15.2, 2041 (1320) 27.7 and 25.7, 4096
+  // with 32 and 8 (1328) 22.5 and 21.3, 4 x 1024 with 64 and 8 in blocks of 32 (2213) 32.1 and 30.8.  Without rotation there
+  // is no table to wait for: 2041 tokens 18.4 and 13.4.  Heads of 64: 2 x 2000 with 32 heads (2595) 25.9 and 27.0.
+  if constexpr (kAppendThreads<DH, BLOCK> >= 1024) {
+    return launch_append<DH, BLOCK, FORM, true>(a, stream);
+  } else if constexpr (DH == 64 || FORM == kSingle) {
+    return launch_append<DH, BLOCK, FORM, false>(a, stream);
+  } else {
+    const bool many = !a.rot.R || (long long)a.c.B * a.L * (2 * a.c.Hk + a.H) >= 1024ll * sm_count();
+    return many ? launch_append<DH, BLOCK, FORM, true>(a, stream) : launch_append<DH, BLOCK, FORM, false>(a, stream);
+  }
 }
 template <int DH, int BLOCK>
 static int launch_append(const AppendArgs& a, void* stream) {
