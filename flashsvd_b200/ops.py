@@ -371,8 +371,8 @@ def _device_of(name: str, t, ndim: int, what: str) -> int:
 
 
 def _room_like(t):
-    """A contiguous tensor of the same size (`empty_like` costs half of `new_empty`, and keeps other strides)."""
-    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+    """A contiguous tensor of the same size."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def rope_qk(q, k, positions, inv_freq, *, interleaved=False, scale=1.0, q_out=None, k_out=None):
