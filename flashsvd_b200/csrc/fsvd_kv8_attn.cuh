@@ -542,8 +542,7 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
 #pragma unroll
       for (int g = 0; g < GH; ++g) {
         m[g] = -INFINITY;
-        l[g] = 0.0f;
-        qf[g] = qfac[seg & 1][head0 + g];
+        l[g] = qf[g] = 0.0f;
       }
       float ks = 0.0f, vs = 1.0f;
       auto scales = [&](int t) {
@@ -559,6 +558,10 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
         if (i + 1 < run) scales(t + 1);
         wait_bar(smem_u32(&s_full[buf]), (j >> 1) & 1, giveup, a.status, a.wait_limit, DS_BARRIER_TIMEOUT);
         tc_fence_after();
+        if (i == 0) {   // (this product was issued when every warp had written its factors: before it nothing orders them)
+#pragma unroll
+          for (int g = 0; g < GH; ++g) qf[g] = qfac[seg & 1][head0 + g];
+        }
         float s[2 * GH], e[GH];
         tm_ld<2 * GH>(tmem + buf * S::kNq + group * 2 * GH + lanes, s);
         bool higher = false;
