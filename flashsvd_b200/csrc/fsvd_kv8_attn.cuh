@@ -5,15 +5,16 @@
 // tcgen05.mma kind::f8f6f4 multiplies e4m3 by e4m3 exactly and adds in 32 bits, so the codes go from TMA to the tensor
 // core as they lie in memory.  What is not e4m3 is written as a sum of e4m3 numbers and takes a column of the small
 // operand each: a query row is hi + lo / 16 (a bf16 number has 8 bits, an e4m3 number 4: nothing is lost above 2^-22 of
-// the row's largest), a weight is w0 + w1 / 16 + w2 / 256 + w3 / 4096, which is good to 2^-17 of itself and 2^-24 of the
-// largest.  A tile is 128 tokens: S^T [128 tokens, 2 G] = K8 . q^T, then O^T [Dh, 4 G] = V8^T . w^T, where V8^T is the
-// tile as it lies, read along its other axis.  Scales are applied to the scores in 32 bits: the exponent of a weight is
-// s log2(e) + log2(vs), so that the weight carries its value's scale, and the denominator divides it out.
+// the row's largest), a weight is eight digits of base 16, which keep all 24 bits of an fp32 number down to 2^-16 and reach
+// to 2^-39 of the largest (`digits_of`).  A tile is 128 tokens: S^T [128 tokens, 2 G] = K8 . q^T, then
+// O^T [Dh, 8 G] = V8^T . w^T, where V8^T is the tile as it lies, read along its other axis.  Scales are applied to the
+// scores in 32 bits: the exponent of a weight is s log2(e) + log2(vs), so that the weight carries its value's scale, and the
+// denominator divides it out.
 //
 // A thread of the four softmax warps owns a token of S^T and a dimension of O^T; one more thread issues the copies, one
 // the products.  O^T is read back after every tile and summed in registers, where a new maximum rescales it.  The
-// maximum that weights refer to is one that was, and is renewed when a score passes it by more than 2^4 = the room that the
-// codes are given: nearly every tile then needs one vote of the four warps instead of a maximum per head.
+// maximum that weights refer to is one that was, and is renewed when a score passes it by more than the room that the
+// digits are given (2^2): nearly every tile then needs one vote of the four warps instead of a maximum per head.
 //
 // The tiles of all (sequence, kv head) pairs form one list that is cut into equal parts, one per CTA, whatever the
 // lengths are; a pair that more than one CTA works on is merged, in the order of its parts, by the CTA that finishes it.
@@ -30,10 +31,11 @@ using namespace fsvd_tile;
 constexpr int kTile = 128;      // tokens
 constexpr int kBox = 32;        // tokens of a TMA box: a short last tile is fetched in as many as it needs
 constexpr int kSoft = 128;      // threads of a softmax group
-constexpr int kPieces = 4;      // e4m3 numbers of a weight
+constexpr int kDigits = 8;      // e4m3 numbers of a weight
 constexpr int kMaxGroup = 16;
 constexpr int kPad = 4;         // floats behind a head's partial sums
-constexpr float kRoom = 4.0f;   // log2 of how far a score may pass the maximum that weights refer to
+constexpr int kRoom = 2;        // log2 of how far a weight may pass the largest one when the maximum was renewed
+constexpr float kUnit = 1.0f / (1 << (7 - kRoom));   // of the sums that the digits give (`digits_of`)
 
 struct Args {
   const float *k_scale, *v_scale;
@@ -59,11 +61,14 @@ struct Shape {
   static constexpr int kCtas = GP > 8 ? 1 : DH == 64 && GP <= 4 ? 3 : 2;
   static constexpr int kStages = GP > 8 ? 5 * (128 / DH) : DH == 128 ? 3 : GP <= 4 ? 4 : 6;
   static constexpr int kNq = 2 * GP < 16 ? 16 : 2 * GP;                 // columns of S
-  static constexpr int kNw = kPieces * GP < 16 ? 16 : kPieces * GP;     // columns of O
-  static constexpr int kCols = 2 * (kNq + kNw) <= 64 ? 64 : 2 * (kNq + kNw) <= 128 ? 128 : 256;
+  static constexpr int kNw = kDigits * GP < 16 ? 16 : kDigits * GP;     // columns of O
+  static constexpr int kUsed = 2 * (kNq + kNw), kCols = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
+  static_assert(kCols * kCtas <= 512, "tensor memory of an SM");
   static constexpr int kHalf = kTile * DH;                              // bytes of a K or V tile
   static constexpr int kQ = kNq * DH < 1024 ? 1024 : kNq * DH, kW = kNw * kTile;
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * 2 * kHalf + 2 * kQ + 2 * kW;
+  // The weights take the place of the tile's keys, which nobody reads once there are scores.
+  static constexpr bool kOver = kW <= kHalf;
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * 2 * kHalf + 2 * kQ + (kOver ? 0 : 2 * kW);
 };
 
 __device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -84,12 +89,19 @@ template <int ROW>
 __device__ __forceinline__ uint64_t desc_f8(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(8 * ROW >> 4) << 32) | (1ull << 46) | ((ROW == 128 ? 2ull : 4ull) << 61);
 }
-// The weights: 128 rows (tokens) of N bytes (columns), read along the columns; rows of 32 and 64 bytes under the swizzle
-// of that span.
+// The weights: 128 rows (tokens) of N bytes (columns), read along the columns; rows of 32, 64 and 128 bytes under the
+// swizzle of that span.
 template <int N>
 __device__ __forceinline__ uint64_t desc_weights(uint32_t addr) {
   const uint64_t at = (uint64_t)((addr >> 4) & 0x3fffu) | (1ull << 46);
-  return N == 16 ? at | (8ull << 16) | (8ull << 32) : at | ((uint64_t)(8 * N >> 4) << 32) | ((N == 32 ? 6ull : 4ull) << 61);
+  return N == 16 ? at | (8ull << 16) | (8ull << 32)
+                 : at | ((uint64_t)(8 * N >> 4) << 32) | ((N == 32 ? 6ull : N == 64 ? 4ull : 2ull) << 61);
+}
+// Where 16-byte piece c of row r of them lies.
+template <int N>
+__device__ __forceinline__ uint32_t weights_at(int r, int c) {
+  const int x = N == 32 ? (r >> 2) & 1 : N == 64 ? (r >> 1) & 3 : N == 128 ? r & 7 : 0;
+  return (uint32_t)(r * N + ((c ^ x) << 4));
 }
 // byte c of row r of such an operand
 template <int ROW>
@@ -187,21 +199,26 @@ __device__ __forceinline__ bool group_any(bool x, int group) {
       : "memory");
   return r != 0;
 }
-// Two fp32 numbers of at most 256, given 16 times, as four e4m3 codes each (x in the low byte of a pair): each code is the
-// nearest to what the ones before leave, times 16.  What the first one leaves is kept as a 16-bit number of 11 bits.
-__device__ __forceinline__ void four_codes(float x16, float y16, uint32_t (&c)[4]) {
-  c[0] = __nv_cvt_float2_to_fp8x2(make_float2(x16 * 0.0625f, y16 * 0.0625f), __NV_SATFINITE, __NV_E4M3);
-  const __half2_raw h0 = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c[0], __NV_E4M3);
-  const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-  __half2 r = __floats2half2_rn(fmaf(f0.x, -16.0f, x16), fmaf(f0.y, -16.0f, y16));
-#pragma unroll
-  for (int i = 1; i < 4; ++i) {
-    c[i] = __nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&r), __NV_SATFINITE, __NV_E4M3);
-    if (i < 3) {
-      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)c[i], __NV_E4M3);
-      r = __hmul2(__hsub2(r, *reinterpret_cast<const __half2*>(&h)), __float2half2_rn(16.0f));
-    }
-  }
+__device__ __forceinline__ uint32_t prmt(uint32_t x, uint32_t y, uint32_t selector) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(y), "r"(selector));
+  return r;
+}
+// A weight 0 <= u < 2^(kRoom + 1) as eight e4m3 numbers d_i 2^s, d_i the digits 0..15 of a 32-bit whole number W with
+// W 2^s = u 2^(35 - kRoom): sum over i of 16^(i - 7) d_i 2^s = u / kUnit.  All of d 2^s with s = -6..4 are e4m3 numbers, so s
+// follows the weight for ten binades, in which W is the significand with eight zeros behind it; below them s stays and W
+// loses a bit per binade: nothing of the 24 down to 2^(kRoom - 18), less than 2^(kRoom - 41) in all.  A CTA goes through
+// about 2^23 tokens at most (the card's memory in equal parts): what is cut off stays below 2^-15 of the largest value.
+// Digits become codes by a table in registers: a selector of 0..7 takes a byte, one with the upper bit set takes the
+// byte's sign, which is zero; the upper half of the table is asked for the digits with that bit turned.
+__device__ __forceinline__ void digits_of(float u, uint32_t& low, uint32_t& high) {
+  const uint32_t bits = __float_as_uint(u);
+  const int up = (int)(bits >> 23) - (127 + kRoom - 10);
+  const uint32_t w = __funnelshift_rc((bits << 8) | 0x80000000u, 0u, (uint32_t)max(-up, 0)), v = w ^ 0x88888888u;
+  const uint32_t more = (uint32_t)max(up, 0) * 0x08080808u;   // 2^s = 2^-6 2^up; a zero stays one
+  const uint32_t t0 = 0x14100800u + (more & 0xffffff00u), t1 = 0x1e1c1a18u + more, t2 = 0x23222120u + more, t3 = 0x27262524u + more;
+  low = prmt(t0, t1, w) | prmt(t2, t3, v);
+  high = prmt(t0, t1, w >> 16) | prmt(t2, t3, v >> 16);
 }
 // Two fp32 numbers -> their nearest e4m3 codes (x in the low byte), and what the codes stand for.
 __device__ __forceinline__ uint32_t to_codes(float x, float y, float& dx, float& dy) {
@@ -261,7 +278,9 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = a.G;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* qs = smem + S::kStages * 2 * S::kHalf;
-  uint8_t* ws = qs + 2 * S::kQ;
+  auto weights = [&](int j) {   // of tile j
+    return S::kOver ? smem + (j % S::kStages) * 2 * S::kHalf : qs + 2 * S::kQ + (j & 1) * S::kW;
+  };
   volatile int* giveup = &giveup_sh;
 
   if (tid == 0) {
@@ -381,7 +400,7 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
         const int st = j % S::kStages, buf = j & 1;
         wait_bar(smem_u32(&w_full[buf]), (j >> 1) & 1, giveup, a.status, a.wait_limit, DS_BARRIER_TIMEOUT);
         tc_fence_after();
-        const uint32_t v = smem_u32(smem + st * 2 * S::kHalf + S::kHalf), w = smem_u32(ws + buf * S::kW);
+        const uint32_t v = smem_u32(smem + st * 2 * S::kHalf + S::kHalf), w = smem_u32(weights(j));
 #pragma unroll
         for (int k = 0; k < kTile / 32; ++k)
           mma_f8(tmem + 2 * S::kNq + buf * S::kNw, desc_f8<DH>(v + 32 * DH * k), desc_weights<S::kNw>(w + 32 * S::kNw * k), iw, k > 0);
@@ -484,11 +503,19 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
       wait_bar(smem_u32(&o_full[buf]), (jj >> 1) & 1, giveup, a.status, a.wait_limit, DS_BARRIER_TIMEOUT);
       tc_fence_after();
       if (wl * 32 < DH) {
-        float o[kPieces * GH];
-        tm_ld<kPieces * GH>(tmem + 2 * S::kNq + buf * S::kNw + group * kPieces * GH + lanes, o);
+        constexpr int N = GH < 2 ? GH : 2;   // heads at a time
 #pragma unroll
-        for (int g = 0; g < GH; ++g)
-          acc[g] = acc[g] * c[g] + (((o[3 * GH + g] * 0.0625f + o[2 * GH + g]) * 0.0625f + o[GH + g]) * 0.0625f + o[g]);
+        for (int g0 = 0; g0 < GH; g0 += N) {
+          float o[kDigits * N];
+          tm_ld<kDigits * N>(tmem + 2 * S::kNq + buf * S::kNw + (head0 + g0) * kDigits + lanes, o);
+#pragma unroll
+          for (int g = 0; g < N; ++g) {
+            float sum = o[g * kDigits];
+#pragma unroll
+            for (int d = 1; d < kDigits; ++d) sum = fmaf(sum, 0.0625f, o[g * kDigits + d]);
+            acc[g0 + g] = fmaf(acc[g0 + g], c[g0 + g], sum);
+          }
+        }
       }
     };
     auto finalise = [&](int last) {
@@ -510,14 +537,14 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
         if (owns) {
 #pragma unroll
           for (int g = 0; g < GH; ++g)
-            if (head0 + g < G) out[g * DH] = __float2bfloat16_rn(acc[g] * 16.0f / l_end[g]);
+            if (head0 + g < G) out[g * DH] = __float2bfloat16_rn(acc[g] * kUnit / l_end[g]);
         }
       } else {
         float* rp = a.part + ((size_t)blockIdx.x * 2 + (seg_end > 0)) * G * rec + head0 * rec;
 #pragma unroll
         for (int g = 0; g < GH; ++g)
           if (head0 + g < G) {
-            if (owns) rp[g * rec + tl] = acc[g] * 16.0f;   // (256 times the sum, as l)
+            if (owns) rp[g * rec + tl] = acc[g] * kUnit;
             if (tl == 0) *reinterpret_cast<float2*>(rp + g * rec + DH) = make_float2(m_end[g], l_end[g]);
           }
         if (tid == 0) part_of[seg_end > 0] = Part{bh_end, tiles_end, list_end};
@@ -538,7 +565,7 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
       const int list0 = seq_base + hk * ntiles;   // list index of the pair's first tile
       const float* ksc = a.k_scale + (size_t)bh * a.nb;
       const float* vsc = a.v_scale + (size_t)bh * a.nb;
-      float m[GH], l[GH], corr[GH], qf[GH];   // l and acc: 256 and 16 times the sums
+      float m[GH], l[GH], corr[GH], qf[GH];   // (acc: the sums divided by kUnit)
 #pragma unroll
       for (int g = 0; g < GH; ++g) {
         m[g] = -INFINITY;
@@ -569,7 +596,7 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
         for (int g = 0; g < GH; ++g) {
           const float x = fmaf(fmaf(s[GH + g], 0.0625f, s[g]), kf * qf[g], lv);
           e[g] = valid ? x : -INFINITY;
-          higher = higher || (head0 + g < G && e[g] > m[g] + kRoom);
+          higher = higher || (head0 + g < G && e[g] > m[g] + (float)kRoom);
         }
         if (!valid && group == 0) {   // the last tile: a row behind the end may hold anything
           uint4* row = reinterpret_cast<uint4*>(smem + (j % S::kStages) * 2 * S::kHalf + S::kHalf + tl * DH);
@@ -600,23 +627,23 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
         }
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
-          e[g] = valid ? ex2(e[g] - m[g] + 8.0f) : 0.0f;   // 256 times the weight, which is at most 2^kRoom
+          e[g] = valid ? ex2(e[g] - m[g]) : 0.0f;   // at most 2^kRoom
           l[g] = fmaf(e[g], inv, l[g]);
         }
         {
-          uint32_t c[(GH + 1) / 2][4];   // pairs of heads
-#pragma unroll
-          for (int g = 0; g < GH; g += 2) four_codes(e[g], GH > 1 ? e[(g + 1) % GH] : 0.0f, c[g / 2]);
-          uint8_t* dst = ws + buf * S::kW + tl * S::kNw;
+          uint8_t* dst = weights(j);
           if constexpr (GH == 1) {
-            *reinterpret_cast<uint32_t*>(dst) = __byte_perm(__byte_perm(c[0][0], c[0][1], 0x0040), __byte_perm(c[0][2], c[0][3], 0x0040), 0x5410);
-          } else if constexpr (GH == 2) {
-            *reinterpret_cast<uint2*>(dst) = make_uint2(c[0][0] | (c[0][1] << 16), c[0][2] | (c[0][3] << 16));
+            uint2 c;
+            digits_of(e[0], c.x, c.y);
+            *reinterpret_cast<uint2*>(dst + tl * S::kNw) = c;
           } else {
-            const int x = NG == 2 ? (tl >> 2) & 1 : NG == 4 ? (tl >> 1) & 3 : 0;
-            *reinterpret_cast<uint4*>(dst + ((group ^ x) << 4)) =
-                make_uint4(c[0][0] | (c[GH / 2 - 1][0] << 16), c[0][1] | (c[GH / 2 - 1][1] << 16), c[0][2] | (c[GH / 2 - 1][2] << 16),
-                           c[0][3] | (c[GH / 2 - 1][3] << 16));
+#pragma unroll
+            for (int g = 0; g < GH; g += 2) {   // two heads to a piece
+              uint4 c;
+              digits_of(e[g], c.x, c.y);
+              digits_of(e[g + 1], c.z, c.w);
+              *reinterpret_cast<uint4*>(dst + weights_at<S::kNw>(tl, (head0 + g) / 2)) = c;
+            }
           }
         }
         tc_fence_before();
@@ -665,9 +692,9 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
         // parts and fewer dimensions than threads, the parts are shared out too.
         constexpr int kBatch = 8;
         const int items = G * (DH / 4), shares = c1 - c0 >= kBatch ? max(1, kSoft / items) : 1;
-        float4* sums = reinterpret_cast<float4*>(ws);   // (no weights are on their way any more; at most 128 of each)
-        float2* tops = reinterpret_cast<float2*>(ws + kSoft * sizeof(float4));
-        static_assert(2 * S::kW >= kSoft * (int)(sizeof(float4) + sizeof(float2)));
+        float4* sums = reinterpret_cast<float4*>(smem);   // (no tile is on its way any more; at most 128 of each)
+        float2* tops = reinterpret_cast<float2*>(smem + kSoft * sizeof(float4));
+        static_assert(S::kHalf >= kSoft * (int)(sizeof(float4) + sizeof(float2)));
         auto store = [&](int item, const float4& o, float den) {
           *reinterpret_cast<uint2*>(out + item / (DH / 4) * DH + item % (DH / 4) * 4) =
               make_uint2(pack_bf16(o.x / den, o.y / den), pack_bf16(o.z / den, o.w / den));

@@ -1,0 +1,109 @@
+"""Softmax weights and queries of the attention over the 8-bit cache where few of their bits carry the result.
+
+The weights of a tile are fp32 numbers; nothing of a weight may leave the numerator that the denominator counts."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _codes(x):
+    return x.to(torch.float8_e4m3fn)
+
+
+def _cache(B, Hk, S, Dh, block=128):
+    from flashsvd_b200 import kv8
+
+    return kv8.KV8Cache.empty(B, S, Hk, Dh, block=block, device=DEV)
+
+
+@pytest.mark.parametrize("Dh,G,pairs,n,steps", [(64, 1, 640, 2000, (20, 22.9, 24.4, 25.9, 26.1, 28, 30)),
+                                                (128, 2, 320, 2000, (20, 24.4, 26.1)), (64, 4, 320, 2000, (20, 24.4, 26.1)),
+                                                (128, 8, 320, 2000, (20, 24.4, 26.1)), (128, 16, 160, 2000, (20, 24.4, 26.1)),
+                                                (64, 16, 160, 2000, (24.4,)), (64, 8, 320, 2000, (24.4,)),
+                                                (64, 1, 300, 131071, (20, 22.9, 25.9, 26.1, 28, 30)), (128, 8, 80, 131071, (26.1,)),
+                                                (64, 1, 64, 1 << 20, (22.9, 26.1, 28, 30))])
+def test_a_dominant_token_in_front_of_a_long_flat_context(Dh, G, pairs, n, steps):
+    """One token whose value is zero, and n - 1 equal ones at 2^-step of its weight: they alone are the result.
+
+    Tolerance: half a bf16 step and 2^-14 of the largest value, as for attention at large.  Enough pairs that a CTA goes
+    through a whole context, or most of it, with one running maximum."""
+    from flashsvd_b200 import ops
+
+    cache = _cache(pairs, 1, n, Dh)
+    gen = torch.Generator(device=DEV).manual_seed(n + Dh + G)
+    values = _codes(torch.rand(pairs, 1, 1, Dh, device=DEV, generator=gen) + 0.5)
+    cache.v.view(torch.uint8).copy_(values.view(torch.uint8).expand(pairs, 1, n, Dh))
+    at = torch.randint(0, n, (pairs,), generator=torch.Generator().manual_seed(n))
+    at[0], at[1], at[2] = 0, n - 1, n // 2
+    rows = torch.arange(pairs, device=DEV)
+    cache.v.view(torch.uint8)[rows, 0, at.to(DEV)] = 0
+    cache.k.view(torch.uint8)[rows, 0, at.to(DEV), 3] = int(_codes(torch.ones(1)).view(torch.uint8))
+    q = torch.zeros(pairs, G, Dh, device=DEV, dtype=torch.bfloat16)
+    q[:, :, 3] = 1.0
+    lens = torch.full((pairs,), n, dtype=torch.int32, device=DEV)
+    ws = ops.make_kv8_workspace(pairs, G, 1, Dh, n, DEV)
+    v = values.double()[:, 0]
+    for step in steps:
+        scale = torch.tensor(step * math.log(2.0), dtype=torch.float32).item()
+        tail = (n - 1) * math.exp(-scale)
+        want = (v * tail / (1.0 + tail)).expand(pairs, G, Dh)
+        got = ops.flash_decode_kv8(q, cache, lens, ws, scale=scale).double()
+        assert bool(((got - want).abs() <= want * 2.0 ** -8 + 2.0 ** -14 * 1.5).all()), step
+    assert ws.status() == 0
+
+
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("G", [1, 2, 4, 8, 16])
+def test_weights_have_their_bits(Dh, G):
+    """Two tokens of values +448 and -448 and almost equal weights 1 and w: the result is 448 (1 - w) / (1 + w).
+
+    Scores are exact (one product each; the smaller is at most 2^-6) but for a few roundings of 2^-24 of it, the
+    exponential is good to 2^-22 and the sums of two terms to 2^-23: w within 2^-21, the result within 448 * 2^-22, and half
+    a bf16 step.  448 * 2^-20 leaves room for what the exponential's argument adds."""
+    from flashsvd_b200 import ops
+
+    pairs = 512
+    cache = _cache(pairs, 1, 2, Dh, block=16)
+    one, big = (int(_codes(torch.tensor([x])).view(torch.uint8)) for x in (1.0, 448.0))
+    cache.v.view(torch.uint8)[:, 0, 0], cache.v.view(torch.uint8)[:, 0, 1] = big, big | 0x80
+    cache.k.view(torch.uint8)[:, 0, 1, 7] = one
+    gen = torch.Generator().manual_seed(G + Dh)
+    q = torch.zeros(pairs, G, Dh)
+    q[:, :, 7] = -(2.0 ** (-14 + 8 * torch.rand(pairs, G, generator=gen)))
+    q = q.to(torch.bfloat16)
+    ws = ops.make_kv8_workspace(pairs, G, 1, Dh, 2, DEV)
+    got = ops.flash_decode_kv8(q.to(DEV), cache, torch.full((pairs,), 2, dtype=torch.int32, device=DEV), ws, scale=1.0).double().cpu()
+    w = torch.exp(q[:, :, 7].double())
+    want = (448 * (1 - w) / (1 + w))[..., None].expand(pairs, G, Dh)
+    assert bool(((got - want).abs() <= want.abs() * 2.0 ** -8 + 448 * 2.0 ** -20).all())
+
+
+@pytest.mark.parametrize("Dh", [64, 128])
+def test_weights_over_thirty_binades_beside_a_dominant_one(Dh):
+    """Random scores over 26 units below one token of value zero, values of one sign: a mean, so errors are relative to it.
+
+    Half a bf16 step; weights to 2^-20 of themselves (scores of up to 40 to 2^-24 each, four roundings); the weights below
+    2^-33 of the largest are 2^-16 of the others together at most."""
+    from flashsvd_b200 import ops
+
+    B, Hk, G, S = 16, 40, 2, 3000
+    gen = torch.Generator(device=DEV).manual_seed(Dh)
+    cache = _cache(B, Hk, S, Dh, block=64)
+    v = _codes(torch.rand(B, Hk, S, Dh, device=DEV, generator=gen) + 0.5)
+    v[:, :, 1234].view(torch.uint8).zero_()
+    cache.v.view(torch.uint8).copy_(v.view(torch.uint8))
+    k = _codes(torch.randint(-15, 16, (B, Hk, S, Dh), device=DEV, generator=gen).float())
+    k[..., 1:] = 0 * k[..., 1:].float().to(torch.float8_e4m3fn).float()
+    k[:, :, 1234, 0] = _codes(torch.tensor([28.0], device=DEV))[0]
+    cache.k.view(torch.uint8).copy_(k.view(torch.uint8))
+    q = torch.zeros(B, Hk * G, Dh, device=DEV, dtype=torch.bfloat16)
+    q[:, 0::2, 0], q[:, 1::2, 0] = 0.5, 0.6015625
+    ws = ops.make_kv8_workspace(B, Hk * G, Hk, Dh, S, DEV)
+    got = ops.flash_decode_kv8(q, cache, torch.full((B,), S, dtype=torch.int32, device=DEV), ws, scale=1.0).double()
+    s = torch.einsum("bhgd,bhnd->bhgn", q.double().view(B, Hk, G, Dh), k.double())
+    want = (torch.softmax(s, -1) @ v.double()).view(B, Hk * G, Dh)
+    assert bool(((got - want).abs() <= want * (2.0 ** -8 + 2.0 ** -14)).all())
