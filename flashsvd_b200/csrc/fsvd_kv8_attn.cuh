@@ -4,9 +4,9 @@
 //
 // tcgen05.mma kind::f8f6f4 multiplies e4m3 by e4m3 exactly and adds in 32 bits, so the codes go from TMA to the tensor
 // core as they lie in memory.  What is not e4m3 is written as a sum of e4m3 numbers and takes a column of the small
-// operand each: a query row is hi + lo / 16 (a bf16 number has 8 bits, an e4m3 number 4: nothing is lost above 2^-22 of
-// the row's largest), a weight is eight digits of base 16, which keep all 24 bits of an fp32 number down to 2^-16 and reach
-// to 2^-39 of the largest (`digits_of`).  A tile is 128 tokens: S^T [128 tokens, 2 G] = K8 . q^T, then
+// operand each: a query row is q0 + q1 / 16 + q2 / 256 (a bf16 number has 8 bits, an e4m3 number 4: nothing is lost of the
+// numbers above 2^-17 of the row's largest, less than 2^-25 of it below), a weight is eight digits of base 16, which keep all 24 bits of an fp32 number down to 2^-16 and reach
+// to 2^-39 of the largest (`digits_of`).  A tile is 128 tokens: S^T [128 tokens, 4 G] = K8 . q^T, then
 // O^T [Dh, 8 G] = V8^T . w^T, where V8^T is the tile as it lies, read along its other axis.  Scales are applied to the
 // scores in 32 bits: the exponent of a weight is s log2(e) + log2(vs), so that the weight carries its value's scale, and the
 // denominator divides it out.
@@ -32,6 +32,7 @@ constexpr int kTile = 128;      // tokens
 constexpr int kBox = 32;        // tokens of a TMA box: a short last tile is fetched in as many as it needs
 constexpr int kSoft = 128;      // threads of a softmax group
 constexpr int kDigits = 8;      // e4m3 numbers of a weight
+constexpr int kParts = 4;       // columns of a query: three e4m3 numbers, and one that nobody reads
 constexpr int kMaxGroup = 16;
 constexpr int kPad = 4;         // floats behind a head's partial sums
 constexpr int kRoom = 2;        // log2 of how far a weight may pass the largest one when the maximum was renewed
@@ -60,7 +61,7 @@ struct Shape {
   // 83 us, three of two 94; heads of 64, 128 ragged sequences: three CTAs of four tiles 41 us, two of six 48.
   static constexpr int kCtas = GP > 8 ? 1 : DH == 64 && GP <= 4 ? 3 : 2;
   static constexpr int kStages = GP > 8 ? 5 * (128 / DH) : DH == 128 ? 3 : GP <= 4 ? 4 : 6;
-  static constexpr int kNq = 2 * GP < 16 ? 16 : 2 * GP;                 // columns of S
+  static constexpr int kNq = kParts * GP < 16 ? 16 : kParts * GP;       // columns of S
   static constexpr int kNw = kDigits * GP < 16 ? 16 : kDigits * GP;     // columns of O
   static constexpr int kUsed = 2 * (kNq + kNw), kCols = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
   static_assert(kCols * kCtas <= 512, "tensor memory of an SM");
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
       if (!*giveup) weigh(n - 1);
     }
   } else {   // ---- softmax
-    // The query rows of a pair as hi + lo / 16, scaled to a largest magnitude in [128, 256): fetched while the pair before is
+    // The query rows of a pair as q0 + q1 / 16 + q2 / 256, scaled to a largest magnitude in [128, 256): fetched while the pair before is
     // begun, written when its first tile is through.
     const int group = warp >> 2, tl = tid & (kSoft - 1), wl = warp & 3;   // thread and warp within the group
     const int head0 = group * GH;                                          // its heads
@@ -464,24 +465,24 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
         const int e2 = (int)(__float_as_uint(top) >> 23) - 127;          // top in [2^e2, 2^(e2 + 1))
         const int up = fine ? min(max(7 - e2, -120), 120) : 0;
         const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-        uint32_t hi = 0, lo = 0;
+        uint32_t c[3] = {0, 0, 0};
 #pragma unroll
         for (int e = 0; e < D; e += 2) {
-          float h0, h1, l0, l1;
-          const float x0 = x[e] * f, x1 = x[e + 1] * f;
-          const uint32_t ch = to_codes(x0, x1, h0, h1), cl = to_codes((x0 - h0) * 16.0f, (x1 - h1) * 16.0f, l0, l1);
-          hi |= ch << (8 * e);
-          lo |= cl << (8 * e);
+          float x0 = x[e] * f, x1 = x[e + 1] * f;
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            float d0, d1;
+            c[i] |= to_codes(x0, x1, d0, d1) << (8 * e);
+            x0 = (x0 - d0) * 16.0f;
+            x1 = (x1 - d1) * 16.0f;
+          }
         }
-        if (!fine) hi = lo = 0x7f7f7f7fu;   // a query that is not finite gives no number
-        uint8_t* p0 = dst + swizzled<DH>(g / GH * 2 * GH + g % GH, lane * D);
-        uint8_t* p1 = dst + swizzled<DH>(g / GH * 2 * GH + GH + g % GH, lane * D);
-        if constexpr (D == 4) {
-          *reinterpret_cast<uint32_t*>(p0) = hi;
-          *reinterpret_cast<uint32_t*>(p1) = lo;
-        } else {
-          *reinterpret_cast<uint16_t*>(p0) = (uint16_t)hi;
-          *reinterpret_cast<uint16_t*>(p1) = (uint16_t)lo;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          if (!fine) c[i] = 0x7f7f7f7fu;   // a query that is not finite gives no number
+          uint8_t* p = dst + swizzled<DH>(g / GH * kParts * GH + i * GH + g % GH, lane * D);
+          if constexpr (D == 4) *reinterpret_cast<uint32_t*>(p) = c[i];
+          else *reinterpret_cast<uint16_t*>(p) = (uint16_t)c[i];
         }
         if (lane == 0) qfac[which][g] = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)(127 - up) << 23);
       }
@@ -589,12 +590,12 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
 #pragma unroll
           for (int g = 0; g < GH; ++g) qf[g] = qfac[seg & 1][head0 + g];
         }
-        float s[2 * GH], e[GH];
-        tm_ld<2 * GH>(tmem + buf * S::kNq + group * 2 * GH + lanes, s);
+        float s[kParts * GH], e[GH];
+        tm_ld<kParts * GH>(tmem + buf * S::kNq + group * kParts * GH + lanes, s);
         bool higher = false;
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
-          const float x = fmaf(fmaf(s[GH + g], 0.0625f, s[g]), kf * qf[g], lv);
+          const float x = fmaf(fmaf(fmaf(s[2 * GH + g], 0.0625f, s[GH + g]), 0.0625f, s[g]), kf * qf[g], lv);
           e[g] = valid ? x : -INFINITY;
           higher = higher || (head0 + g < G && e[g] > m[g] + (float)kRoom);
         }

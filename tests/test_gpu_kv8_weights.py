@@ -107,3 +107,61 @@ def test_weights_over_thirty_binades_beside_a_dominant_one(Dh):
     s = torch.einsum("bhgd,bhnd->bhgn", q.double().view(B, Hk, G, Dh), k.double())
     want = (torch.softmax(s, -1) @ v.double()).view(B, Hk * G, Dh)
     assert bool(((got - want).abs() <= want * (2.0 ** -8 + 2.0 ** -14)).all())
+
+
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("G", [1, 2, 4, 8, 16])
+def test_small_query_numbers_beside_a_dominant_token(Dh, G):
+    """The two opposite values again, beside a token that outweighs them 2^j times and whose value is zero: their weights
+    differ by a query number far below the row's largest.
+
+    Each number of the row has its 8 bits down to 2^-17 of the largest, below that it is off by 2^-26 of it."""
+    from flashsvd_b200 import ops
+
+    pairs = 512
+    one, big = (int(_codes(torch.tensor([x])).view(torch.uint8)) for x in (1.0, 448.0))
+    gen = torch.Generator().manual_seed(G + Dh)
+    q = torch.zeros(pairs, G, Dh)
+    q[:, :, 7] = -(2.0 ** (-14 + 8 * torch.rand(pairs, G, generator=gen)))
+    q = q.to(torch.bfloat16)
+    ws = ops.make_kv8_workspace(pairs, G, 1, Dh, 3, DEV)
+    w = torch.exp(q[:, :, 7].double())
+    cache = _cache(pairs, 1, 3, Dh, block=16)
+    cache.v.view(torch.uint8)[:, 0, 0], cache.v.view(torch.uint8)[:, 0, 1] = big, big | 0x80
+    cache.k.view(torch.uint8)[:, 0, 1, 7] = one
+    cache.k.view(torch.uint8)[:, 0, 2, 9] = one
+    three = torch.full((pairs,), 3, dtype=torch.int32, device=DEV)
+    for j in (1, 5, 9, 12):
+        top = torch.tensor(j * math.log(2.0)).to(torch.bfloat16)
+        q[:, :, 9] = top
+        got = ops.flash_decode_kv8(q.to(DEV), cache, three, ws, scale=1.0).double().cpu()
+        want = (448 * (1 - w) / (1 + w + math.exp(float(top))))[..., None].expand(pairs, G, Dh)
+        # (the scores below the largest one carry its roundings: 9 * 2^-23, relative to the two weights)
+        assert bool(((got - want).abs() <= want.abs() * 2.0 ** -8 + 448 * math.exp(-float(top)) * 2.0 ** -19).all()), j
+
+
+@pytest.mark.parametrize("Dh,G", [(64, 1), (128, 2), (64, 4), (128, 8), (64, 16), (128, 16)])
+@pytest.mark.parametrize("up", [0, 8, 14, 15, 60])
+def test_query_rows_with_one_large_number(Dh, G, up):
+    """The row's largest number meets keys of zero: the scores come from numbers 2^up below it.
+
+    Up to 2^15 they have all their bits, and the bound is attention's own.  At 2^60 they vanish (2^-25 of the largest is
+    what a row keeps): every score is zero and the result the mean."""
+    from flashsvd_b200 import kv8, ops
+    from tests import kv8_reference as ref
+
+    B, Hk, S = 3, 2, 200
+    gen = torch.Generator().manual_seed(up + Dh + G)
+    k, v = (torch.randn(B, S, Hk, Dh, generator=gen).to(torch.bfloat16) for _ in range(2))
+    k[..., 5] = 0.0
+    q = torch.randn(B, Hk * G, Dh, generator=gen)
+    q = q.sign() * q.abs().clamp(0.5, 1.99)
+    q[:, :, 5] = -1.5 * 2.0 ** up
+    q = q.to(torch.bfloat16)
+    cache = kv8.KV8Cache.empty(B, S, Hk, Dh, block=32, device=DEV)
+    ws = ops.make_kv8_workspace(B, Hk * G, Hk, Dh, S, DEV)
+    ops.kv8_append(k.to(DEV), v.to(DEV), cache, torch.zeros(B, dtype=torch.int32, device=DEV), ws)
+    kk, vv = (x.double().cpu() for x in ops.kv8_load(cache, 0, S))
+    got = ops.flash_decode_kv8(q.to(DEV), cache, torch.full((B,), S, dtype=torch.int32, device=DEV), ws).double().cpu()
+    want = ref.attend(q if up < 60 else torch.zeros_like(q), kk, vv, [S] * B, Dh ** -0.5)
+    assert bool(((got - want).abs() <= want.abs() * 2.0 ** -8 + 2.0 ** -14 * float(vv.abs().max())).all())
