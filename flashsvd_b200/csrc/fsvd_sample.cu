@@ -959,15 +959,21 @@ extern "C" int fsvd_sample(const void* logits, long long row_stride, int dtype, 
   if (temperature_all != temperature_all || top_p_all != top_p_all || min_p_all != min_p_all)
     return fail(FSVD_ERR_ARG, "NaN setting");
   if (B == 0) return 0;
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  int dev = 0, sms = 148, optin = 227 * 1024;
+  if (cudaGetDevice(&dev) == cudaSuccess) {
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+  }
   // CTAs of a row, by waves x time of a CTA: 20 us for its steps one after the other, and 0.28 us per 1000 elements where they
   // fit its shared memory, 0.36 where every pass reads them again from L2.  (128 rows of 100003: one CTA each 52 us with top-k,
   // top-p and min-p and 77 with top-p alone; four each, which hold them, 116 and 186.)
   const int es = dtype == FSVD_DTYPE_F32 ? 4 : 2;
   const long long places = V + 16 / es - 1;   // a row may start up to 15 bytes behind a 16-byte boundary
   const auto chunk_of = [&](int c) { return ((places + c - 1) / c + kBlock - 1) / kBlock * kBlock; };
-  const auto fits = [&](int c) { return chunk_of(c) * es <= 144 * 1024; };   // (with the 80 KB that every CTA has)
+  const auto lists = [](bool resident) { return kWarps * (resident ? kPackPiece : kPackAlone) * 6; };
+  const long long room = optin - (long long)sizeof(Shared) - lists(true);   // 141 KB
+  static_assert(sizeof(Shared) + kWarps * kPackAlone * 6 <= 227 * 1024);
+  const auto fits = [&](int c) { return chunk_of(c) * es <= room; };
   const auto cost = [&](int c) { return (double)(((long long)B * c + sms - 1) / sms) * (20.0 + chunk_of(c) * (fits(c) ? 0.28e-3 : 0.36e-3)); };
   int C = 1;
   while (chunk_of(C) > kMaxPiece) C *= 2;   // (at most kMaxCluster)
@@ -979,7 +985,7 @@ extern "C" int fsvd_sample(const void* logits, long long row_stride, int dtype, 
   a.tokens = tokens; a.probs = probs; a.V = V;
   a.chunk = (int)chunk_of(C);
   const bool resident = fits(C);
-  const size_t smem = (size_t)kWarps * (resident ? kPackPiece : kPackAlone) * 6 + (resident ? (size_t)a.chunk * es : 0);
+  const size_t smem = (size_t)lists(resident) + (resident ? (size_t)a.chunk * es : 0);
   const void* fn = dtype == FSVD_DTYPE_F32 ? (resident ? (const void*)sample_kernel<float, true> : (const void*)sample_kernel<float, false>)
                                            : (resident ? (const void*)sample_kernel<__nv_bfloat16, true>
                                                        : (const void*)sample_kernel<__nv_bfloat16, false>);

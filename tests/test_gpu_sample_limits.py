@@ -1,0 +1,50 @@
+"""`sample` at the limits of its variants: rows that just fit a CTA's shared memory and rows that just do not, the largest
+vocabulary, the calls it refuses.
+
+Shares: weights are rounded to 2^-38 or finer and the share once to fp32: 2^-24 of the value and 2^-30."""
+import pytest
+import torch
+
+from tests import kv8_reference as ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _check(x, u, T, k, p, m, tokens, probs, rows):
+    for b in rows:
+        want, share = ref.sample_row(x[b].double(), float(u[b]), float(torch.tensor(T)), k, float(torch.tensor(p)), float(torch.tensor(m)))
+        assert int(tokens[b]) == want, (b, int(tokens[b]), want)
+        assert abs(float(probs[b]) - share) <= share * 2.0 ** -24 + 2.0 ** -30
+
+
+@pytest.mark.parametrize("dtype,B,V", [(torch.float32, 128, V) for V in (36092, 36093, 36094, 36500, 36861, 36862)]
+                         + [(torch.bfloat16, 128, V) for V in (72183, 72190, 72500, 73000, 73721)]
+                         + [(torch.float32, 37, V) for V in (144381, 144382, 145900, 147453, 147454)]
+                         + [(torch.float32, 1, V) for V in (288765, 288766, 290000, 294909, 294910)]
+                         + [(torch.float32, 8, 291003), (torch.bfloat16, 37, 288800), (torch.bfloat16, 1, 577600), (torch.bfloat16, 8, 585003)])
+def test_rows_at_the_limit_of_shared_memory(dtype, B, V):
+    from flashsvd_b200 import ops
+
+    gen = torch.Generator().manual_seed(B + V)
+    x = (4 * torch.randn(B, V, generator=gen)).to(dtype)
+    u = torch.rand(B, generator=gen)
+    for T, k, p, m in ((0.8, 0, 0.9, 0.0), (1.2, 50, 0.9, 0.02)):
+        tokens, probs = ops.sample(x.to(DEV), u.to(DEV), temperature=T, top_k=k, top_p=p, min_p=m)
+        _check(x, u, T, k, p, m, tokens, probs, {0, B - 1})
+    # a row that begins off a 16-byte boundary has up to 15 bytes more
+    wide = torch.zeros(B, V + 5, dtype=dtype, device=DEV)
+    wide[:, 3:V + 3] = x.to(DEV)
+    again, _ = ops.sample(wide[:, 3:V + 3], u.to(DEV), temperature=1.2, top_k=50, top_p=0.9, min_p=0.02)
+    assert torch.equal(again, tokens)
+
+
+def test_vocabularies_beyond_the_limit_are_refused():
+    from flashsvd_b200 import _lib, ops
+
+    u = torch.zeros(1, device=DEV)
+    for V in ((1 << 20) + 1, 1 << 22):
+        with pytest.raises((_lib.FsvdError, ValueError)):
+            ops.sample(torch.zeros(1, V, device=DEV), u)
+    tokens, _ = ops.sample(torch.zeros(1, 1 << 20, device=DEV), u)
+    assert int(tokens) == 0
