@@ -16,6 +16,7 @@
 #include "../../include/flashsvd_b200.h"
 #include "fsvd_kv8_attn.cuh"
 #include "fsvd_rope.cuh"
+#include "fsvd_smem.h"
 #include "fsvd_stage.h"
 #include "fsvd_tile.h"
 
@@ -59,13 +60,14 @@ __device__ __forceinline__ void pdl_begin() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
-template <typename... Params, typename... Args>
-static int launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, void* stream, const Args&... args) {
-  // Above the 48 KB that a kernel has by itself the limit is raised at every such launch: a setting of the current
-  // device, so nothing is remembered.
+template <auto KERNEL, typename... Args>
+static int launch(dim3 grid, int threads, size_t smem, void* stream, const Args&... args) {
+  // Above the 48 KB that a kernel has by itself its limit is raised, to all that there is: another thread's launch of another
+  // size finds it as it needs it.
+  cudaError_t e = cudaSuccess;
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return fail(FSVD_ERR_CUDA, "shared memory of %zu bytes: %s", smem, cudaGetErrorString(e));
+    static fsvd_tile::SmemLimit limit;
+    e = limit.raise(KERNEL);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
@@ -77,7 +79,7 @@ static int launch(void (*kernel)(Params...), dim3 grid, int threads, size_t smem
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, KERNEL, args...);
   if (e != cudaSuccess) return fail(FSVD_ERR_CUDA, "kernel launch failed: %s", cudaGetErrorString(e));
   fsvd_tile_count_launch();
   return 0;
@@ -666,7 +668,7 @@ static int launch_attn(const CUtensorMap& km, const CUtensorMap& vm, const fsvd_
   static_assert(S::kCtas <= kMaxCtas);
   const long long tiles = (long long)a.B * a.Hk * ((a.S_max + fsvd_kv8_attn::kTile - 1) / fsvd_kv8_attn::kTile);
   const unsigned grid = (unsigned)std::min<long long>(tiles, (long long)S::kCtas * sm_count());
-  return launch(fsvd_kv8_attn::attn_kernel<DH, GP>, dim3(grid), S::kThreads, S::kSmem, stream, km, vm, a);
+  return launch<fsvd_kv8_attn::attn_kernel<DH, GP>>(dim3(grid), S::kThreads, S::kSmem, stream, km, vm, a);
 }
 template <int DH>
 static int launch_attn(const CUtensorMap& km, const CUtensorMap& vm, const fsvd_kv8_attn::Args& a, void* stream) {
@@ -688,11 +690,11 @@ static int launch_rope(RopeArgs& a, int dtype, void* stream) {
   const size_t smem = (size_t)a.tokens * ((a.rot.R / 2 + 7) / 8 * 8) * sizeof(float2);
   const Form form = a.rot.R % 16 ? kSingle : dtype == FSVD_DTYPE_BF16 && a.rot.interleaved && a.on32 ? kTogether : kVectors;
   if (dtype == FSVD_DTYPE_F32)
-    return form == kSingle ? launch(rope_kernel<float, kSingle>, grid, kThreads, smem, stream, a)
-                           : launch(rope_kernel<float, kVectors>, grid, kThreads, smem, stream, a);
-  return form == kSingle    ? launch(rope_kernel<__nv_bfloat16, kSingle>, grid, kThreads, smem, stream, a)
-         : form == kVectors ? launch(rope_kernel<__nv_bfloat16, kVectors>, grid, kThreads, smem, stream, a)
-                            : launch(rope_kernel<__nv_bfloat16, kTogether>, grid, kThreads, smem, stream, a);
+    return form == kSingle ? launch<rope_kernel<float, kSingle>>(grid, kThreads, smem, stream, a)
+                           : launch<rope_kernel<float, kVectors>>(grid, kThreads, smem, stream, a);
+  return form == kSingle    ? launch<rope_kernel<__nv_bfloat16, kSingle>>(grid, kThreads, smem, stream, a)
+         : form == kVectors ? launch<rope_kernel<__nv_bfloat16, kVectors>>(grid, kThreads, smem, stream, a)
+                            : launch<rope_kernel<__nv_bfloat16, kTogether>>(grid, kThreads, smem, stream, a);
 }
 
 static Form form_of(const AppendArgs& a) {
@@ -715,7 +717,7 @@ static int launch_append(AppendArgs a, void* stream) {
   if (grid > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many tokens for one call");
   const int tile = std::min(BLOCK, a.L);
   const size_t smem = (size_t)((a.rot.R / 2 + 7) / 8 * 8) * (tile + (tile > 8 ? 8 + (tile + 7) / 8 : 0)) * sizeof(double2);
-  return launch(append_kernel<DH, BLOCK, FORM, MANY>, dim3((unsigned)grid), kAppendThreads<DH, BLOCK>, smem, stream, a);
+  return launch<append_kernel<DH, BLOCK, FORM, MANY>>(dim3((unsigned)grid), kAppendThreads<DH, BLOCK>, smem, stream, a);
 }
 template <int DH, int BLOCK, Form FORM>
 static int launch_append(const AppendArgs& a, void* stream) {
@@ -748,9 +750,9 @@ static int launch_append(const AppendArgs& given, void* stream) {
     const long long grid = (long long)a.c.B * a.groups;
     if (grid > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many heads for one call");
     const Form form = form_of(a);
-    return form == kSingle    ? launch(append_step_kernel<DH, kSingle>, dim3((unsigned)grid), kThreads, 0, stream, a)
-           : form == kVectors ? launch(append_step_kernel<DH, kVectors>, dim3((unsigned)grid), kThreads, 0, stream, a)
-                              : launch(append_step_kernel<DH, kTogether>, dim3((unsigned)grid), kThreads, 0, stream, a);
+    return form == kSingle    ? launch<append_step_kernel<DH, kSingle>>(dim3((unsigned)grid), kThreads, 0, stream, a)
+           : form == kVectors ? launch<append_step_kernel<DH, kVectors>>(dim3((unsigned)grid), kThreads, 0, stream, a)
+                              : launch<append_step_kernel<DH, kTogether>>(dim3((unsigned)grid), kThreads, 0, stream, a);
   }
   switch (a.c.block) {
     case 16: return launch_append<DH, 16>(a, stream);
@@ -844,8 +846,8 @@ int fsvd_kv8_load(const fsvd_kv8* cache, int start, int length, const int* cache
   const long long pieces = (long long)length * (cache->Dh / 16);
   const long long grid = (2ll * cache->B * cache->Hk * pieces + kThreads - 1) / kThreads;
   if (grid > 0x7fffffffll || pieces > 0x7fffffffll) return fail(FSVD_ERR_UNSUPPORTED, "too many tokens for one call");
-  return cache->Dh == 64 ? launch(load_kernel<64>, dim3((unsigned)grid), kThreads, 0, stream, a)
-                         : launch(load_kernel<128>, dim3((unsigned)grid), kThreads, 0, stream, a);
+  return cache->Dh == 64 ? launch<load_kernel<64>>(dim3((unsigned)grid), kThreads, 0, stream, a)
+                         : launch<load_kernel<128>>(dim3((unsigned)grid), kThreads, 0, stream, a);
 }
 
 int fsvd_flash_decode_kv8(const fsvd_kv8* cache, const void* q, const int* cache_seqlens, int seqlen_add, void* out, int H,

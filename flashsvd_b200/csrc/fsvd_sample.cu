@@ -21,6 +21,7 @@
 #include <type_traits>
 
 #include "../../include/flashsvd_b200.h"
+#include "fsvd_smem.h"
 #include "fsvd_tc.cuh"
 #include "fsvd_tile.h"
 
@@ -986,11 +987,12 @@ extern "C" int fsvd_sample(const void* logits, long long row_stride, int dtype, 
   a.chunk = (int)chunk_of(C);
   const bool resident = fits(C);
   const size_t smem = (size_t)lists(resident) + (resident ? (size_t)a.chunk * es : 0);
-  const void* fn = dtype == FSVD_DTYPE_F32 ? (resident ? (const void*)sample_kernel<float, true> : (const void*)sample_kernel<float, false>)
-                                           : (resident ? (const void*)sample_kernel<__nv_bfloat16, true>
-                                                       : (const void*)sample_kernel<__nv_bfloat16, false>);
-  cudaError_t e = cudaSuccess;
-  if (smem > 16 * 1024) e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  typedef void (*Kernel)(Args);
+  static const Kernel kernels[4] = {sample_kernel<float, false>, sample_kernel<float, true>, sample_kernel<__nv_bfloat16, false>,
+                                    sample_kernel<__nv_bfloat16, true>};
+  static fsvd_tile::SmemLimit limits[4];
+  const int which = (dtype == FSVD_DTYPE_F32 ? 0 : 2) + resident;
+  cudaError_t e = limits[which].raise(kernels[which]);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(B * C));
@@ -1006,7 +1008,7 @@ extern "C" int fsvd_sample(const void* logits, long long row_stride, int dtype, 
     cfg.attrs = at;
     cfg.numAttrs = 2;
     void* params[] = {&a};
-    e = cudaLaunchKernelExC(&cfg, fn, params);
+    e = cudaLaunchKernelExC(&cfg, (const void*)kernels[which], params);
   }
   if (e != cudaSuccess) {
     char msg[160];

@@ -53,6 +53,7 @@
 
 #include "../../include/flashsvd_b200.h"
 #include "fsvd_exchange.h"
+#include "fsvd_smem.h"
 #include "fsvd_stage.h"
 #include "fsvd_tc.cuh"
 #include "fsvd_tile.h"
@@ -1461,21 +1462,6 @@ template <typename... KArgs, typename... Args>
 static cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args&&... args) {
   return launch_pdl_cluster(kern, grid, block, smem, 0u, st, std::forward<Args>(args)...);
 }
-
-// A kernel's dynamic shared-memory limit belongs to a device: raised on the current one, once.
-class SmemLimit {
-  std::atomic<unsigned long long> raised{0};   // a bit per device
- public:
-  template <typename K>
-  cudaError_t raise(K* kern, int bytes) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess || (dev < 64 && (raised.load(std::memory_order_relaxed) >> dev & 1))) return e;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && dev < 64) raised.fetch_or(1ull << dev);
-    return e;
-  }
-};
 
 // (takes the error off the thread, so that no later check of the caller's reports it again)
 static int launch_failed(const char* what) {
