@@ -37,6 +37,7 @@ static int fail(int code, const char* fmt, ...) {
   va_start(ap, fmt);
   vsnprintf(msg, sizeof(msg), fmt, ap);
   va_end(ap);
+  if (code == FSVD_ERR_CUDA) cudaGetLastError();   // (off the thread: no later check of the caller's reports it again)
   fsvd_tile_set_error(code, msg);
   return code;
 }

@@ -942,6 +942,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
 }
 
 static int fail(int code, const char* msg) {
+  if (code == FSVD_ERR_CUDA) cudaGetLastError();   // (off the thread: no later check of the caller's reports it again)
   fsvd_tile_set_error(code, msg);
   return code;
 }
