@@ -629,11 +629,14 @@ constexpr int kMaxCtas = 3;   // attention CTAs of an SM, at most
 struct Kv8Ws {
   size_t counters, part, total;
 };
-static Kv8Ws ws_layout(long long B, long long H, long long Hk, long long Dh) {
+// The counters' place and number depend on the device alone: what a call of other sizes leaves in its partial sums is never
+// read as a counter.
+static Kv8Ws ws_layout(long long H, long long Hk, long long Dh) {
   Kv8Ws w;
+  const size_t ctas = (size_t)kMaxCtas * sm_count();
   w.counters = 256;   // behind the status word (fsvd_workspace_status)
-  w.part = w.counters + (size_t)((B * Hk * 4 + 255) / 256 * 256);
-  w.total = w.part + (size_t)kMaxCtas * sm_count() * 2 * (H / Hk) * (Dh + fsvd_kv8_attn::kPad) * 4;
+  w.part = w.counters + (ctas * 4 + 255) / 256 * 256;
+  w.total = w.part + ctas * 2 * (H / Hk) * (Dh + fsvd_kv8_attn::kPad) * 4;
   return w;
 }
 
@@ -795,7 +798,7 @@ int fsvd_rope_qk(const void* q, long long q_stride, const void* k, long long k_s
 
 size_t fsvd_kv8_workspace_bytes(int B, int H, int Hk, int Dh, int S_max) {
   if (B < 1 || H < 1 || Hk < 1 || (Dh != 64 && Dh != 128) || S_max < 1) return 0;
-  return ws_layout(B, H, Hk, Dh).total;
+  return ws_layout(H, Hk, Dh).total;
 }
 
 int fsvd_kv8_append(const fsvd_kv8* cache, const void* k, const void* v, long long kv_batch_stride, long long kv_token_stride,
@@ -860,7 +863,7 @@ int fsvd_flash_decode_kv8(const fsvd_kv8* cache, const void* q, const int* cache
   if (G > fsvd_kv8_attn::kMaxGroup)
     return fail(FSVD_ERR_UNSUPPORTED, "H/Hk=%d unsupported (1..%d)", G, fsvd_kv8_attn::kMaxGroup);
   if (!aligned16(q) || !aligned16(out)) return fail(FSVD_ERR_ALIGN, "q and out must be 16-byte aligned");
-  const Kv8Ws L = ws_layout(cache->B, H, cache->Hk, cache->Dh);
+  const Kv8Ws L = ws_layout(H, cache->Hk, cache->Dh);
   if (!ws) return fail(FSVD_ERR_WORKSPACE, "null workspace");
   if (!aligned16(ws)) return fail(FSVD_ERR_ALIGN, "workspace is not 16-byte aligned");
   if (ws_bytes < L.total) return fail(FSVD_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", ws_bytes, L.total);

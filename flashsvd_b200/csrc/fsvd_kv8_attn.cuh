@@ -44,7 +44,7 @@ struct Args {
   __nv_bfloat16* out;
   const int* seqlens;
   float* part;       // [CTAs][2][G][Dh + kPad]: partial sums, maximum, denominator
-  int* counters;     // [B * Hk], zero between launches
+  int* counters;     // [CTAs], zero between launches: of the pair that begins in a CTA and goes on in the next one
   int* status;
   long long wait_limit;
   int B, Hk, S_max, block_log2, nb, G, seqlen_add;
@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
       const int c0 = pt.list / per, c1 = (pt.list + pt.tiles - 1) / per;   // the CTAs of this pair
       if (tid == 0) {
         int arrived;
-        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(arrived) : "l"(a.counters + pt.bh) : "memory");
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(arrived) : "l"(a.counters + c0) : "memory");
         last_sh = arrived == c1 - c0;
       }
       soft_sync(kSoft * NG);
@@ -752,7 +752,7 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
             store(tid, o, den);
           }
         }
-        if (tid == 0) a.counters[pt.bh] = 0;
+        if (tid == 0) a.counters[c0] = 0;
       }
       soft_sync(kSoft * NG);
     }

@@ -419,7 +419,8 @@ def rope_qk(q, k, positions, inv_freq, *, interleaved=False, scale=1.0, q_out=No
 
 
 def make_kv8_workspace(batch, num_heads, num_kv_heads, head_dim, max_len, device) -> Workspace:
-    """Scratch of ``kv8_append`` and ``flash_decode_kv8`` for these sizes; launches that share one must be ordered."""
+    """Scratch of ``kv8_append`` and ``flash_decode_kv8`` for these sizes, and for all that need no more (as many heads per kv
+    head, or fewer); launches that share one must be ordered."""
     n = int(_lib.load().fsvd_kv8_workspace_bytes(int(batch), int(num_heads), int(num_kv_heads), int(head_dim), int(max_len)))
     if n == 0:
         raise ValueError(f"no 8-bit cache of these sizes: batch {batch}, heads {num_heads}/{num_kv_heads}, head_dim {head_dim}, "

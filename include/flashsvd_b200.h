@@ -369,7 +369,8 @@ typedef struct fsvd_kv8 {
 } fsvd_kv8;
 /* Scratch of fsvd_kv8_append and fsvd_flash_decode_kv8 for H query heads: status word (read with
  * fsvd_workspace_status), arrival counters, partial results of the key splits.  Zero it once
- * (fsvd_workspace_init).  Launches that share one must be ordered on the device. */
+ * (fsvd_workspace_init).  Launches that share one must be ordered on the device; it serves calls of all
+ * sizes whose own scratch is no larger. */
 size_t fsvd_kv8_workspace_bytes(int B, int H, int Hk, int Dh, int S_max);
 /* New tokens k / v [B, L, Hk, Dh] (batch and token strides given) go to positions cache_seqlens[b] ..
  * + new_lens[b] - 1 (new_lens NULL: L each).  With inv_freq the keys, and q [B, L, H, Dh] -> q_out when
