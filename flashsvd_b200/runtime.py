@@ -316,7 +316,8 @@ class FlashSVDV15KV8Cache(_CacheBase):
         self._views: dict = {}
         self._seqlens: dict = {}
         n = int(getattr(config, "num_hidden_layers", 0))
-        self._seen = [0] * n
+        self._seen: list = [0] * n   # None: only the device knows (`_last`)
+        self._last: list = [None] * n
         self.layers8: list = [None] * n
         self._layer_device = []
         for idx in range(n):
@@ -386,18 +387,18 @@ class FlashSVDV15KV8Cache(_CacheBase):
             self._spaces[key] = ops.make_kv8_workspace(batch_size, num_heads, Hk, Dh, self._max_cache_len, c.device)
         return self._spaces[key]
 
-    def _place(self, layer_idx: int, B: int, L: int, cache_position):
+    def _place(self, layer_idx: int, B: int, L: int, cache_position, advance: bool):
         """(int32 [B] of the positions in front of the new tokens, the largest of them or None where only the device
         knows it).  Several tokens take consecutive positions, the same in every sequence; a single one may have one
         position per sequence."""
         dev = self._layer_device[layer_idx]
-        key = (int(layer_idx), int(B))
+        key = (int(layer_idx), int(B), bool(advance))   # (a call that does not advance leaves the positions of those that do)
         if key not in self._seqlens:
             self._seqlens[key] = torch.empty(B, dtype=torch.int32, device=dev)
         sl = self._seqlens[key]
         start = cache_position
         if cache_position is None:
-            start = self._seen[layer_idx]
+            start = self.get_seq_length(layer_idx)
         elif torch.is_tensor(cache_position):
             pos = cache_position.reshape(-1)
             if int(pos.numel()) != (L if L > 1 or int(pos.numel()) != B else B):
@@ -420,8 +421,9 @@ class FlashSVDV15KV8Cache(_CacheBase):
         sl.fill_(start)
         return sl, start
 
-    def _advance(self, layer_idx: int, start: Optional[int], L: int) -> None:
-        self._seen[layer_idx] = (self._seen[layer_idx] if start is None else start) + L
+    def _advance(self, layer_idx: int, start: Optional[int], L: int, seqlens: torch.Tensor) -> None:
+        self._seen[layer_idx] = None if start is None else start + L
+        self._last[layer_idx] = seqlens if start is None else None
 
     def append(self, key_states, value_states, layer_idx: int, *, query_states=None, rotate: bool = True, cache_position=None,
                advance: bool = True):
@@ -440,11 +442,11 @@ class FlashSVDV15KV8Cache(_CacheBase):
         c = self.layer(layer_idx, B)
         H = Hk if query_states is None else int(query_states.shape[2])
         ws = self.workspace(layer_idx, B, H)
-        sl, start = self._place(layer_idx, B, L, cache_position)
+        sl, start = self._place(layer_idx, B, L, cache_position, advance)
         q = ops.kv8_append(key_states, value_states, c, sl, ws, q=query_states if rotate else None,
                            rotary=self.rotary(Dh, c.device) if rotate else None)
         if advance:
-            self._advance(layer_idx, start, L)
+            self._advance(layer_idx, start, L, sl)
         return sl, start, q if rotate else query_states
 
     def decode_step(self, query_states, key_states, value_states, layer_idx: int, *, cache_position=None, advance: bool = True):
@@ -471,7 +473,17 @@ class FlashSVDV15KV8Cache(_CacheBase):
         return ops.kv8_load(self.layer(int(layer_idx), B), 0, start + L)
 
     def get_seq_length(self, layer_idx: Optional[int] = 0) -> int:
-        return self._seen[int(layer_idx or 0)] if self._seen else 0
+        """Tokens of the longest sequence.  After a step whose position was given as a CUDA tensor this waits for the step and
+        reads the position back (of the last replay, where a graph made the step)."""
+        layer_idx = int(layer_idx or 0)
+        if not self._seen:
+            return 0
+        if self._seen[layer_idx] is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the cache's length is on the device: pass cache_position to a step that is captured")
+            # (a position in front of the cache counts as 0, a token behind its end was dropped)
+            return min(max(int(self._last[layer_idx].max().item()), 0) + 1, self._max_cache_len)
+        return self._seen[layer_idx]
 
     def get_max_cache_shape(self) -> Optional[int]:
         return self._max_cache_len
@@ -483,6 +495,7 @@ class FlashSVDV15KV8Cache(_CacheBase):
     def reset(self) -> None:
         """Forgets the tokens (the next append starts its block's scale anew, so the codes need no clearing)."""
         self._seen = [0] * len(self._seen)
+        self._last = [None] * len(self._last)
 
 
 class FlashSVDLegacySparseKVCache:

@@ -1,0 +1,67 @@
+"""The cache class of the 8-bit cache: where it takes the length from, what it keeps for later calls, what it refuses."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+H, Hk, Dh = 4, 2, 64
+
+
+def _cache(layers=1, S=24, batch=3, block=16):
+    from flashsvd_b200 import runtime as R
+
+    return R.FlashSVDV15KV8Cache(SimpleNamespace(num_hidden_layers=layers, rope_theta=10000.0), max_batch_size=batch, max_cache_len=S,
+                                 device=DEV, block=block)
+
+
+def _qkv(B, L, seed):
+    x = torch.randn(B, L, H + 2 * Hk, Dh, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16).to(DEV)
+    return x[:, :, :H].contiguous(), x[:, :, H:H + Hk].contiguous(), x[:, :, H + Hk:].contiguous()
+
+
+@pytest.mark.parametrize("device", ["cpu", DEV])
+def test_writing_in_front_of_the_end_cuts_the_sequence(device):
+    """The same steps with positions that the host knows and positions that only the device knows."""
+    cache = _cache()
+    q, k, v = _qkv(2, 10, 1)
+    cache.append(k, v, 0, query_states=q)
+    assert cache.get_seq_length() == 10
+    q, k, v = _qkv(2, 1, 2)
+    cache.decode_step(q, k, v, 0, cache_position=torch.tensor([5], device=device))
+    assert cache.get_seq_length() == 6
+    # a step that does not advance is no part of the sequence
+    cache.decode_step(q, k, v, 0, cache_position=torch.tensor([20], device=device), advance=False)
+    assert cache.get_seq_length() == 6 and cache.get_mask_sizes(1) == (7, 0)
+    # the next one without a position goes behind the cut
+    sl, start, _ = cache.append(k, v, 0, query_states=q)
+    assert sl.tolist() == [6, 6] and start == 6 and cache.get_seq_length() == 7
+    cache.decode_step(q, k, v, 0, cache_position=torch.tensor([7, 3], device=device))
+    assert cache.get_seq_length() == 8
+    cache.reset()
+    assert cache.get_seq_length() == 0
+
+
+def test_the_length_follows_a_replayed_step():
+    cache = _cache()
+    q, k, v = _qkv(2, 4, 3)
+    cache.append(k, v, 0, query_states=q)
+    q, k, v = _qkv(2, 1, 4)
+    pos = torch.tensor([4], device=DEV)
+    cache.decode_step(q, k, v, 0, cache_position=pos)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.decode_step(q, k, v, 0, cache_position=pos)
+        with pytest.raises(RuntimeError, match="cache_position"):
+            cache.get_seq_length()
+    for t in (5, 6, 9):
+        pos.fill_(t)
+        graph.replay()
+        assert cache.get_seq_length() == t + 1
+    pos.fill_(1000)   # dropped
+    graph.replay()
+    assert cache.get_seq_length() == 24
+    cache.append(k, v, 0, query_states=q, cache_position=10)
+    assert cache.get_seq_length() == 11
