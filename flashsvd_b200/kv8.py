@@ -18,6 +18,17 @@ from ._lib import FsvdKv8
 BLOCKS = (16, 32, 64, 128)
 
 
+def made_once(what: str, device, make):
+    """What ``make`` puts on a device for later calls to keep.  They may come from any stream, so it is complete when this
+    returns; a graph capture would only record how to make it, so there it is refused."""
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what} made at the first use, which cannot be captured: make such a call before the capture")
+        made = make()
+        torch.cuda.current_stream().synchronize()
+    return made
+
+
 @dataclass
 class Rotary:
     """``inv_freq``: float64 CUDA tensor [rotary_dim / 2], radians per position; ``interleaved``: pairs (2i, 2i + 1)

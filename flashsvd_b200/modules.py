@@ -17,7 +17,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import ops
+from . import kv8, ops
 
 
 def svd_rank(out_features: int, in_features: int, ratio: float) -> int:
@@ -124,7 +124,8 @@ class LlamaRotaryEmbedding(nn.Module):
         """q [T, H, dim] and k [T, Hk, dim] (or None) at positions [T], by ``ops.rope_qk``: angles in 64 bits, no tables."""
         key = str(q.device)
         if key not in self._inv_freq64:
-            self._inv_freq64[key] = self.base ** (-torch.arange(0, self.dim, 2, dtype=torch.float64, device=q.device) / self.dim)
+            self._inv_freq64[key] = kv8.made_once("rotary frequencies are", q.device, lambda: self.base ** (
+                -torch.arange(0, self.dim, 2, dtype=torch.float64, device=q.device) / self.dim))
         return ops.rope_qk(q, k, position_ids.to(device=q.device, dtype=torch.int32), self._inv_freq64[key])
 
 
@@ -279,10 +280,10 @@ class SVD_LlamaAttention(_WithWorkspace):
         if own:
             key = (str(x.device), x.dtype, B, "kv8")
             if key not in self._ws:
-                self._ws[key] = ops.make_workspace(
+                self._ws[key] = kv8.made_once("a workspace is", x.device, lambda: ops.make_workspace(
                     ops.make_dims(dtype=x.dtype, B=B, d=d, H=H, Hk=Hk, Dh=Dh, Rq=self.q_u_proj.in_features,
                                   Rk=self.k_u_proj.in_features, Rv=self.v_u_proj.in_features,
-                                  Ro=self.o_v_proj.out_features), x.device)
+                                  Ro=self.o_v_proj.out_features), x.device))
             ws = self._ws[key]
 
         def project(y, v, u):

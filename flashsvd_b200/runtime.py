@@ -346,8 +346,9 @@ class FlashSVDV15KV8Cache(_CacheBase):
 
         c = self.layers8[layer_idx]
         if c is None:
-            self.layers8[layer_idx] = kv8.KV8Cache.empty(self._max_batch_size, self._max_cache_len, int(h), int(dh),
-                                                         block=self._block, device=self._layer_device[layer_idx])
+            dev = self._layer_device[layer_idx]
+            self.layers8[layer_idx] = kv8.made_once("a layer's cache is", dev, lambda: kv8.KV8Cache.empty(
+                self._max_batch_size, self._max_cache_len, int(h), int(dh), block=self._block, device=dev))
         elif (c.k.shape[1], c.k.shape[3]) != (int(h), int(dh)):
             raise RuntimeError(f"FlashSVDV15KV8Cache shape changed after init for layer {layer_idx}: "
                                f"old={(c.k.shape[1], c.k.shape[3])}, new={(int(h), int(dh))}")
@@ -373,18 +374,20 @@ class FlashSVDV15KV8Cache(_CacheBase):
         key = (int(head_dim), str(device))
         if key not in self._rotaries:
             r = self._rotary
-            self._rotaries[key] = kv8.rotary(int(head_dim), theta=self._rope_theta, device=device) if r is None else \
-                kv8.Rotary(r.inv_freq.to(device), r.interleaved, r.scale)
+            self._rotaries[key] = kv8.made_once("rotary frequencies are", device, lambda: kv8.rotary(
+                int(head_dim), theta=self._rope_theta, device=device) if r is None else
+                kv8.Rotary(r.inv_freq.to(device), r.interleaved, r.scale))
         return self._rotaries[key]
 
     def workspace(self, layer_idx: int, batch_size: int, num_heads: int):
-        from . import ops
+        from . import kv8, ops
 
         c = self.layer(layer_idx, batch_size)
         Hk, Dh = c.k.shape[1], c.k.shape[3]
         key = (str(c.device), int(batch_size), int(num_heads), Hk, Dh)
         if key not in self._spaces:
-            self._spaces[key] = ops.make_kv8_workspace(batch_size, num_heads, Hk, Dh, self._max_cache_len, c.device)
+            self._spaces[key] = kv8.made_once("a workspace is", c.device, lambda: ops.make_kv8_workspace(
+                batch_size, num_heads, Hk, Dh, self._max_cache_len, c.device))
         return self._spaces[key]
 
     def _place(self, layer_idx: int, B: int, L: int, cache_position, advance: bool):

@@ -65,3 +65,54 @@ def test_the_length_follows_a_replayed_step():
     assert cache.get_seq_length() == 24
     cache.append(k, v, 0, query_states=q, cache_position=10)
     assert cache.get_seq_length() == 11
+
+
+def _rotary_module():
+    from flashsvd_b200 import modules as M
+
+    return M.LlamaRotaryEmbedding(Dh, base=777.0)
+
+
+def test_first_uses_cannot_be_captured():
+    """A capture computes nothing, and what a replay makes it makes again every time: the call says so and keeps nothing."""
+    rope, cache = _rotary_module(), _cache()
+    q, k, v = _qkv(2, 1, 5)
+    pos = torch.zeros(2, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for call in (lambda: rope.rotate(q[:, 0], k[:, 0], pos), lambda: cache.rotary(Dh, torch.device(DEV)),
+                     lambda: cache.append(k, v, 0, query_states=q, cache_position=pos)):
+            with pytest.raises(RuntimeError, match="before the capture"):
+                call()
+        pos.add_(1)
+    graph.replay()
+    cache.append(k, v, 0, query_states=q, cache_position=pos)
+    want = rope.rotate(q[:, 0], k[:, 0], pos)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        rope.rotate(q[:, 0], k[:, 0], pos)
+        cache.append(k, v, 0, query_states=q, cache_position=pos)
+    assert torch.equal(rope.rotate(q[:, 0], k[:, 0], pos)[0], want[0])
+
+
+def test_first_uses_on_a_busy_stream_serve_other_streams():
+    """What the first call makes is there when a second call on another stream asks for it."""
+    q, k, v = _qkv(3, 4, 6)
+    pos = torch.arange(12, device=DEV).view(3, 4)[:, 0].contiguous()
+    good_rope, good = _rotary_module(), _cache()
+    want = good_rope.rotate(q[:, 0], k[:, 0], pos)
+    _, _, wq = good.append(k, v, 0, query_states=q)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    # (memory that the allocator hands out again on that stream holds other numbers)
+    with torch.cuda.stream(side):
+        torch.full((1 << 20,), 3.0, dtype=torch.float64, device=DEV)
+        torch.cuda.synchronize()
+        rope, cache = _rotary_module(), _cache()
+        torch.cuda._sleep(400_000_000)
+        rope.rotate(q[:, 0], k[:, 0], pos)
+        cache.append(k, v, 0, query_states=q)
+    got = rope.rotate(q[:, 0], k[:, 0], pos)
+    _, _, gq = cache.append(k, v, 0, query_states=q, cache_position=0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(gq, wq)
