@@ -464,16 +464,16 @@ class FlashSVDV15KV8Cache(_CacheBase):
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int, cache_kwargs: Optional[dict] = None):
         """The transformers protocol: key_states (after their rotation), value_states [B, Hk, L, Dh] are appended; returns
-        the sequence so far as bfloat16 [B, Hk, S, Dh], read back from the codes."""
+        the sequence so far as bfloat16 [B, Hk, S, Dh], read back from the codes (zeros behind the end of a shorter one)."""
         from . import ops
 
         pos = None if cache_kwargs is None else cache_kwargs.get("cache_position")
         if torch.is_tensor(pos):
             pos = pos.cpu()
-        _, start, _ = self.append(key_states.transpose(1, 2).contiguous(), value_states.transpose(1, 2).contiguous(), layer_idx,
-                                  rotate=False, cache_position=pos)
+        sl, start, _ = self.append(key_states.transpose(1, 2).contiguous(), value_states.transpose(1, 2).contiguous(), layer_idx,
+                                   rotate=False, cache_position=pos)
         B, _, L, _ = key_states.shape
-        return ops.kv8_load(self.layer(int(layer_idx), B), 0, start + L)
+        return ops.kv8_load(self.layer(int(layer_idx), B), 0, start + L, cache_seqlens=sl, seqlen_add=L)
 
     def get_seq_length(self, layer_idx: Optional[int] = 0) -> int:
         """Tokens of the longest sequence.  After a step whose position was given as a CUDA tensor this waits for the step and

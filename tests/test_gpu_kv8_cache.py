@@ -116,3 +116,17 @@ def test_first_uses_on_a_busy_stream_serve_other_streams():
     _, _, gq = cache.append(k, v, 0, query_states=q, cache_position=0)
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in zip(got, want)) and torch.equal(gq, wq)
+
+
+def test_update_gives_zeros_behind_a_shorter_sequence():
+    """What a cut or forgotten sequence left there, NaN among it, is not handed out."""
+    cache = _cache()
+    _, k, v = _qkv(3, 12, 7)
+    k[2, 9, 0, 3] = float("nan")
+    cache.append(k, v, 0, rotate=False)
+    cache.reset()
+    _, k, v = _qkv(3, 1, 8)
+    kk, vv = cache.update(k.transpose(1, 2), v.transpose(1, 2), 0, {"cache_position": torch.tensor([10, 0, 4])})
+    assert kk.shape == vv.shape == (3, Hk, 11, Dh)
+    for b, n in enumerate((11, 1, 5)):
+        assert bool(kk[b, :, n - 1].any()) and not bool(kk[b, :, n:].any()) and not bool(vv[b, :, n:].any())
