@@ -457,6 +457,8 @@ class FlashSVDV15KV8Cache(_CacheBase):
         [B, 1, H, Dh], key_states / value_states [B, 1, Hk, Dh]; returns [B, H, Dh]."""
         from . import ops
 
+        if query_states.ndim != 4 or query_states.shape[1] != 1:
+            raise ValueError(f"decode_step takes one token per sequence: query_states [B, 1, H, Dh], got {tuple(query_states.shape)}")
         sl, _, q = self.append(key_states, value_states, layer_idx, query_states=query_states, cache_position=cache_position,
                                advance=advance)
         B, _, H, _ = q.shape

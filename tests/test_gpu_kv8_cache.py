@@ -130,3 +130,17 @@ def test_update_gives_zeros_behind_a_shorter_sequence():
     assert kk.shape == vv.shape == (3, Hk, 11, Dh)
     for b, n in enumerate((11, 1, 5)):
         assert bool(kk[b, :, n - 1].any()) and not bool(kk[b, :, n:].any()) and not bool(vv[b, :, n:].any())
+
+
+def test_decode_step_refuses_several_tokens():
+    """It attends with the first query alone: the others would be lost.  Nothing is appended."""
+    cache = _cache()
+    q, k, v = _qkv(2, 3, 9)
+    cache.append(k, v, 0, query_states=q)
+    before = cache.layers8[0].k.view(torch.uint8).clone()
+    for bad in (q, q[:, 0], q[:, :0]):
+        with pytest.raises(ValueError, match="one token"):
+            cache.decode_step(bad, k, v, 0)
+    with pytest.raises(ValueError):
+        cache.decode_step(q[:, :1], k, v, 0)   # (a query for some of the tokens)
+    assert cache.get_seq_length() == 3 and torch.equal(cache.layers8[0].k.view(torch.uint8), before)
