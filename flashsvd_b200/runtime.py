@@ -390,6 +390,18 @@ class FlashSVDV15KV8Cache(_CacheBase):
                 batch_size, num_heads, Hk, Dh, self._max_cache_len, c.device))
         return self._spaces[key]
 
+    def status(self) -> int:
+        """Blocking: 0, or IndexError where a step whose position only the device knew (a CUDA ``cache_position``) had a token
+        that did not fit: the kernel drops it and says so in the workspace."""
+        for ws in self._spaces.values():
+            ws.status()
+        return 0
+
+    def clear_status(self) -> None:
+        for ws in self._spaces.values():
+            with torch.cuda.device(ws.buf.device):
+                ws.clear_status()
+
     def _place(self, layer_idx: int, B: int, L: int, cache_position, advance: bool):
         """(int32 [B] of the positions in front of the new tokens, the largest of them or None where only the device
         knows it).  Several tokens take consecutive positions, the same in every sequence; a single one may have one

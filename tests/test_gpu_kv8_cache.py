@@ -144,3 +144,18 @@ def test_decode_step_refuses_several_tokens():
     with pytest.raises(ValueError):
         cache.decode_step(q[:, :1], k, v, 0)   # (a query for some of the tokens)
     assert cache.get_seq_length() == 3 and torch.equal(cache.layers8[0].k.view(torch.uint8), before)
+
+
+def test_a_dropped_token_is_reported():
+    cache = _cache(layers=2)
+    q, k, v = _qkv(2, 1, 10)
+    for layer in (0, 1):
+        cache.decode_step(q, k, v, layer, cache_position=torch.tensor([23], device=DEV))
+    assert cache.status() == 0
+    before = [c.k.view(torch.uint8).clone() for c in cache.layers8]
+    cache.decode_step(q, k, v, 1, cache_position=torch.tensor([24, 3], device=DEV))
+    with pytest.raises(IndexError):
+        cache.status()
+    assert torch.equal(cache.layers8[1].k.view(torch.uint8)[0], before[1][0])
+    cache.clear_status()
+    assert cache.status() == 0
