@@ -32,7 +32,7 @@ constexpr int kThreads = 1024, kWarps = kThreads / 32;
 static_assert(kWarps == 32, "a warp folds one number of every warp");
 constexpr int kBins = 1024;
 constexpr int kPer = 32, kPerLog = 5;       // bins of a factor of two in the weight
-constexpr int kFrac = 40;                   // bits behind the point of a weight as an integer (at most one; 2^20 of them fit)
+constexpr int kFrac = 40;                   // bits of a weight as an integer, beside the largest candidate's (2^20 of them fit)
 constexpr int kLimbs = 4, kLimbBits = 12;   // such an integer as four numbers of 12 bits: 2^20 of them fit 32-bit sums
 constexpr int kList = 1024;                 // candidates of a CTA that are listed
 constexpr int kRank = 192;                  // candidates of a row that are ranked directly
@@ -40,7 +40,9 @@ constexpr int kBlock = 128;                 // elements of a warp's step: four n
 constexpr int kPackPiece = 256, kPackAlone = 896;   // elements that a warp's short list holds, beside the piece and without
 constexpr int kMaxCluster = 8;
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kMaxPiece = (1 << 17) + kBlock;        // elements of a CTA: so many of 27800 (see `masses`) fit a bin's 32-bit sum
+constexpr int kMaxPiece = (1 << 17) + kBlock;        // elements of a CTA
+constexpr u64 kMostUpper = 27802;                    // of what `masses` adds in 32 bits
+static_assert(kMaxPiece * kMostUpper < (1ull << 32) && kMaxPiece * 16383ull < (1ull << 32));
 constexpr float kHuge = 3.402823466e38f;
 
 struct Args {
@@ -176,7 +178,7 @@ struct Weigher {
     int bin;
     return x >= cut ? (*this)(x, bin) : 0.0;
   }
-  __device__ __forceinline__ u64 fixed(float x) const { return (u64)__double2ll_rn((*this)(x) * (double)(1ull << kFrac)); }
+  __device__ __forceinline__ u64 fixed(float x, double one) const { return (u64)__double2ll_rn((*this)(x) * one); }
 };
 
 // (out of line: it is hardly ever called)
@@ -470,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     return t;
   };
   // A weight of bin i is 2^(-i / 32) (1 + q 2^-34): the bin holds how many there are, and the sums of the 14 lower bits and
-  // the upper ones (below 27800) of q + 2^28.  In units of 2^(-i / 32) 2^-34:
+  // the upper ones (at most (2^34 (2^(1/64) - 1) + 2^28) / 2^14 = kMostUpper) of q + 2^28.  In units of 2^(-i / 32) 2^-34:
   auto masses = [&](int i, int r) -> u64 {
     return (u64)peek(&s.hist[0][i], r) * ((1ull << 34) - (1ull << 28)) + ((u64)peek(&s.hist[2][i], r) << 14) + peek(&s.hist[1][i], r);
   };
@@ -546,16 +548,19 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   uint32_t t = 0u, equal = 0;   // threshold key (0: everything above -infinity is kept), elements that have it
   uint32_t ties = 0;            // and how many of them are kept, the first ones in index order
   // Goes on inside the candidates f: the element at which the running count (MASS: weight) exceeds `target`, `above` of
-  // it lies in front of them.  Counts are whole numbers; weights are added as integers here.
+  // it lies in front of them.  Counts are whole numbers; weights are added as integers here, in units that give the largest
+  // candidate kFrac bits: a border far down in the tail is as sharp as one among the likely tokens.
   auto finish = [&](auto mass, Found f, double above, double target) {
     constexpr bool MASS = decltype(mass)::value;
-    constexpr double one = MASS ? (double)(1ull << kFrac) : 1.0;
     for (int round = 0; round < 5; ++round) {   // (a round cuts the range of the keys by 1024: at most four)
       if (f.n == 0) return;   // (not reached: the place is known to be there)
+      double one = 1.0;
+      if constexpr (MASS)   // 2^kFrac over the largest weight's power of two
+        one = __hiloint2double((1023 + 1022 + kFrac - (__double2hiint(W(value_of(f.kmax))) >> 20)) << 20, 0);
       const double left = (target - above) * one;
       const u64 want = left > 0.0 ? (u64)left : 0;
       if (f.kmin == f.kmax) {
-        const u64 w = MASS ? W.fixed(value_of(f.kmin)) : 1;
+        const u64 w = MASS ? W.fixed(value_of(f.kmin), one) : 1;
         t = f.kmin;
         equal = f.n;
         ties = w ? (uint32_t)min(want / w + 1, (u64)f.n) : f.n;
@@ -574,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         if (tid < (int)f.n) {
           const uint32_t xk = peek(&s.list_key[tid - from], r);
           s.all_key[tid] = ((u64)xk << 32) | ~peek(&s.list_at[tid - from], r);   // larger: in front
-          s.all_w[tid] = MASS ? W.fixed(value_of(xk)) : 1;
+          s.all_w[tid] = MASS ? W.fixed(value_of(xk), one) : 1;
         }
         __syncthreads();
         for (int c0 = 4 * warp; c0 < (int)f.n; c0 += 4 * kWarps) {   // eight lanes to a candidate, over all of them
@@ -621,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
         if (xk < klo || xk > khi) return;
         const int bin = (int)((khi - xk) >> by);
         if constexpr (MASS) {
-          u64 w = W.fixed(value_of(xk));
+          u64 w = W.fixed(value_of(xk), one);
 #pragma unroll
           for (int l = 0; l < kLimbs; ++l, w >>= kLimbBits)
             if (w & ((1u << kLimbBits) - 1u)) atomicAdd(&s.hist[l][bin], (uint32_t)w & ((1u << kLimbBits) - 1u));

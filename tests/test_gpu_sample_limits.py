@@ -48,3 +48,34 @@ def test_vocabularies_beyond_the_limit_are_refused():
             ops.sample(torch.zeros(1, V, device=DEV), u)
     tokens, _ = ops.sample(torch.zeros(1, 1 << 20, device=DEV), u)
     assert int(tokens) == 0
+
+
+@pytest.mark.parametrize("B,V", [(1, 1 << 20), (130, 600001), (2, 90001)])
+@pytest.mark.parametrize("octaves", [33.5, 36.3, 30.7])
+def test_a_border_far_down_in_the_tail(B, V, octaves):
+    """One likely token in front of V - 1 equal ones at 2^-octaves of its weight, and a top-p that ends among them.
+
+    The likely token's weight is one exactly; the tail's weights, all alike, are good to 2^-39, which over V of them is far
+    less than one; the sums' roundings (2^-50 of the mass) are 2^-12 of a tail weight: the number kept, and with it the place
+    of a draw in the tail, is off by one at most."""
+    import math
+
+    from flashsvd_b200 import ops
+
+    x = torch.full((V,), -octaves * math.log(2.0))
+    x[5] = 0.0
+    w = math.exp(float(x[0].double()))
+    tail = (V - 1) * w
+    p = float(torch.tensor(1.0 - 0.6 * tail / (1.0 + tail), dtype=torch.float32))
+    if p * (1.0 + tail) - 1.0 < 10 * w:   # (a 32-bit p has no value between the token's share and one)
+        pytest.skip("no 32-bit top-p ends in this tail")
+    kept = math.floor((p * (1.0 + tail) - 1.0) / w) + 1   # of the tail: those whose preceding mass is at most p of all
+    z = 1.0 + kept * w
+    u = torch.tensor([1.0 - 2.0 ** -24 * (1 + b % 3) for b in range(B)])
+    tokens, probs = ops.sample(x[None].expand(B, V).contiguous().to(DEV), u.to(DEV), top_p=p)
+    for b in range(B):
+        # (five tail tokens lie in front of the likely one)
+        place = float(u[b].double()) * z
+        want = 5 if place < 1.0 + 5 * w else 6 + math.floor((place - 1.0) / w) - 5
+        assert abs(int(tokens[b]) - want) <= 1, (int(tokens[b]), want)
+        assert abs(float(probs[b]) - (w if want != 5 else 1.0) / z) <= 2.0 ** -24 * (w if want != 5 else 1.0)
