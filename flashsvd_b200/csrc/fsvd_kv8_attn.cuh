@@ -9,7 +9,9 @@
 // to 2^-39 of the largest (`digits_of`).  A tile is 128 tokens: S^T [128 tokens, 4 G] = K8 . q^T, then
 // O^T [Dh, 8 G] = V8^T . w^T, where V8^T is the tile as it lies, read along its other axis.  Scales are applied to the
 // scores in 32 bits: the exponent of a weight is s log2(e) + log2(vs), so that the weight carries its value's scale, and the
-// denominator divides it out.
+// denominator divides it out.  (A token whose scale is 2^kSpan below the largest has its weight formed with a larger one, so
+// that it does not leave the 32-bit range, and multiplied down for the product.)  Maxima are whole numbers: a change of them
+// rounds nothing.
 //
 // A thread of the four softmax warps owns a token of S^T and a dimension of O^T; one more thread issues the copies, one
 // the products.  O^T is read back after every tile and summed in registers, where a new maximum rescales it.  The
@@ -36,6 +38,7 @@ constexpr int kParts = 4;       // columns of a query: three e4m3 numbers, and o
 constexpr int kMaxGroup = 16;
 constexpr int kPad = 4;         // floats behind a head's partial sums
 constexpr int kRoom = 2;        // log2 of how far a weight may pass the largest one when the maximum was renewed
+constexpr float kSpan = 60.0f, kSlack = 30.0f;   // binades below the largest value's scale when it was renewed, and above it
 constexpr float kUnit = 1.0f / (1 << (7 - kRoom));   // of the sums that the digits give (`digits_of`)
 
 struct Args {
@@ -187,6 +190,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// x 2^-up, for an `up` whose power alone may leave the 32-bit range
+__device__ __forceinline__ float lowered(float x, float up) {
+  const float f = ex2(-0.5f * up);
+  return x * f * f;
+}
 // Whether any thread of a softmax group says so.
 __device__ __forceinline__ bool group_any(bool x, int group) {
   uint32_t r;
@@ -270,7 +278,8 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
   extern __shared__ uint8_t raw[];
   __shared__ __align__(8) unsigned long long kv_full[S::kStages], kv_empty[S::kStages], s_full[2], w_full[2], o_full[2], q_full[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ float qfac[2][GP], wmax[2][4][GP], red2[2][4][GP];
+  __shared__ float qfac[2][GP], red2[2][4][GP], wtop[2][S::kGroups][4];
+  __shared__ float2 wmax[2][4][GP];
   __shared__ int start_b, start_hk, start_tile, start_n, last_sh, giveup_sh;
   __shared__ int per_sh, total_sh, base_sh;
   struct Part { int bh, tiles, list; };   // of a pair: which, its tiles, where they begin in the list
@@ -567,11 +576,9 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
       const float* ksc = a.k_scale + (size_t)bh * a.nb;
       const float* vsc = a.v_scale + (size_t)bh * a.nb;
       float m[GH], l[GH], corr[GH], qf[GH];   // (acc: the sums divided by kUnit)
+      float vmax = 0.0f, floor = -INFINITY;           // largest log2(vs), and the least that weights are formed with
 #pragma unroll
-      for (int g = 0; g < GH; ++g) {
-        m[g] = -INFINITY;
-        l[g] = qf[g] = 0.0f;
-      }
+      for (int g = 0; g < GH; ++g) m[g] = l[g] = qf[g] = 0.0f;
       float ks = 0.0f, vs = 1.0f;
       auto scales = [&](int t) {
         const int at = t * kTile + tl;
@@ -582,7 +589,7 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
       for (int i = 0; i < run; ++i, ++j) {
         const int t = first + i, buf = j & 1;
         const bool valid = t * kTile + tl < n;
-        const float kf = ks, lv = __log2f(vs), inv = valid ? __fdividef(1.0f, vs) : 0.0f;
+        const float kf = ks, lv = __log2f(vs);
         if (i + 1 < run) scales(t + 1);
         wait_bar(smem_u32(&s_full[buf]), (j >> 1) & 1, giveup, a.status, a.wait_limit, DS_BARRIER_TIMEOUT);
         tc_fence_after();
@@ -592,12 +599,13 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
         }
         float s[kParts * GH], e[GH];
         tm_ld<kParts * GH>(tmem + buf * S::kNq + group * kParts * GH + lanes, s);
-        bool higher = false;
+        float used = fmaxf(lv, floor);
+        bool higher = i == 0 || (valid && lv > vmax + kSlack);
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
-          const float x = fmaf(fmaf(fmaf(s[2 * GH + g], 0.0625f, s[GH + g]), 0.0625f, s[g]), kf * qf[g], lv);
-          e[g] = valid ? x : -INFINITY;
-          higher = higher || (head0 + g < G && e[g] > m[g] + (float)kRoom);
+          s[g] = fmaf(fmaf(s[2 * GH + g], 0.0625f, s[GH + g]), 0.0625f, s[g]);
+          e[g] = fmaf(s[g], kf * qf[g], used - m[g]);
+          higher = higher || (valid && head0 + g < G && e[g] > (float)kRoom);
         }
         if (!valid && group == 0) {   // the last tile: a row behind the end may hold anything
           uint4* row = reinterpret_cast<uint4*>(smem + (j % S::kStages) * 2 * S::kHalf + S::kHalf + tl * DH);
@@ -613,23 +621,41 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
         if (group_any(higher, group)) {
 #pragma unroll
           for (int g = 0; g < GH; ++g) {
-            const float top = warp_max(e[g]);
-            if (lane == 0) wmax[buf][wl][head0 + g] = top;
+            const float top = warp_max(valid ? e[g] : -INFINITY), score = warp_max(valid ? e[g] - used : -INFINITY);
+            if (lane == 0) wmax[buf][wl][head0 + g] = make_float2(top, score);
           }
+          const float vtop = warp_max(valid ? lv : -INFINITY);
+          if (lane == 0) wtop[buf][group][wl] = vtop;
           group_sync(group);
+          const float v4 = fmaxf(fmaxf(wtop[buf][group][0], wtop[buf][group][1]), fmaxf(wtop[buf][group][2], wtop[buf][group][3]));
+          vmax = i == 0 ? v4 : fmaxf(vmax, v4);
+          floor = vmax - kSpan;
+          used = fmaxf(lv, floor);
 #pragma unroll
           for (int g = 0; g < GH; ++g) {
-            const float top = fmaxf(fmaxf(wmax[buf][0][head0 + g], wmax[buf][1][head0 + g]), fmaxf(wmax[buf][2][head0 + g], wmax[buf][3][head0 + g]));
-            const float mn = fmaxf(m[g], top);
-            corr[g] = m[g] == mn ? 1.0f : ex2(m[g] - mn);
-            m[g] = mn;
-            l[g] *= corr[g];
+            float2 top = wmax[buf][0][head0 + g];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) {
+              const float2 y = wmax[buf][w][head0 + g];
+              top.x = fmaxf(top.x, y.x);
+              top.y = fmaxf(top.y, y.y);
+            }
+            // (the first tile's maximum may be below zero; where nothing is above -infinity there is nothing to refer to)
+            const float most = ceilf(fmaxf(top.x, top.y + floor)), up = most > -INFINITY ? (i == 0 ? most : fmaxf(most, 0.0f)) : 0.0f;
+            if (i > 0) {   // (before it there are no sums)
+              corr[g] = ex2(-up);
+              l[g] = lowered(l[g], up);
+            }
+            m[g] += up;
+            e[g] = fmaf(s[g], kf * qf[g], used - m[g]);
           }
         }
+        const float inv = valid ? ex2(-used) : 0.0f, down = ex2(lv - used);
 #pragma unroll
         for (int g = 0; g < GH; ++g) {
-          e[g] = valid ? ex2(e[g] - m[g]) : 0.0f;   // at most 2^kRoom
+          e[g] = valid ? ex2(e[g]) : 0.0f;   // at most 2^kRoom
           l[g] = fmaf(e[g], inv, l[g]);
+          e[g] *= down;
         }
         {
           uint8_t* dst = weights(j);
@@ -716,15 +742,15 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
             float mn = top;
 #pragma unroll
             for (int c = 0; c < kBatch; ++c) mn = fmaxf(mn, cb + c * shares <= c1 ? ml[c].x : -INFINITY);
-            const float f0 = top == mn ? 1.0f : ex2(top - mn);
+            const float gone = top > -INFINITY ? mn - top : 0.0f, f0 = ex2(-gone);
             top = mn;
-            den *= f0;
+            den = lowered(den, gone);
             o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
 #pragma unroll
             for (int c = 0; c < kBatch; ++c)
               if (cb + c * shares <= c1) {
-                const float f = ml[c].x == mn ? 1.0f : ex2(ml[c].x - mn);
-                den = fmaf(f, ml[c].y, den);
+                const float f = ex2(ml[c].x - mn);
+                den += lowered(ml[c].y, mn - ml[c].x);
                 o.x = fmaf(f, v[c].x, o.x); o.y = fmaf(f, v[c].y, o.y); o.z = fmaf(f, v[c].z, o.z); o.w = fmaf(f, v[c].w, o.w);
               }
           }
@@ -745,8 +771,8 @@ __global__ void __launch_bounds__(Shape<DH, GP>::kThreads, Shape<DH, GP>::kCtas)
             for (int x = 0; x < shares; ++x) {
               const float2 ml = tops[tid + x * items];
               const float4 v = sums[tid + x * items];
-              const float f = ml.x == top ? 1.0f : ex2(ml.x - top);
-              den = fmaf(f, ml.y, den);
+              const float f = ex2(ml.x - top);
+              den += ml.x > -INFINITY ? lowered(ml.y, top - ml.x) : ml.y;
               o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
             }
             store(tid, o, den);

@@ -165,3 +165,64 @@ def test_query_rows_with_one_large_number(Dh, G, up):
     got = ops.flash_decode_kv8(q.to(DEV), cache, torch.full((B,), S, dtype=torch.int32, device=DEV), ws).double().cpu()
     want = ref.attend(q if up < 60 else torch.zeros_like(q), kk, vv, [S] * B, Dh ** -0.5)
     assert bool(((got - want).abs() <= want.abs() * 2.0 ** -8 + 2.0 ** -14 * float(vv.abs().max())).all())
+
+
+@pytest.mark.parametrize("Dh,G", [(64, 1), (128, 2), (64, 4), (128, 8), (64, 16)])
+def test_scales_of_the_whole_range_in_one_sequence(Dh, G):
+    """Blocks of tiny values, of values near bf16's largest and of zeros, wherever the likely tokens are.
+
+    Every weight counts in the denominator, whatever its value's scale.  The results are means of numbers of one sign, so that
+    errors are relative to them: half a bf16 step, and the weights' own."""
+    from flashsvd_b200 import kv8, ops
+
+    block, S = 16, 16 * 40
+    gen = torch.Generator().manual_seed(Dh + G)
+    size = torch.zeros(S)
+    for b, x in {0: 1e-25, 3: 1e30, 7: 0.0, 8: 1.0, 9: 3e37, 17: 1e-18, 20: 1e24, 33: 0.0, 39: 1e10}.items():
+        size[b * block:(b + 1) * block] = x
+    v = ((torch.rand(1, S, 1, Dh, generator=gen) + 0.5) * size[None, :, None, None]).to(torch.bfloat16)
+    for likely in range(0, 40, 1):
+        k = torch.zeros(1, S, 1, Dh, dtype=torch.bfloat16)
+        k[:, likely * block:(likely + 1) * block, :, 3] = 1.0
+        cache = kv8.KV8Cache.empty(1, S, 1, Dh, block=block, device=DEV)
+        ws = ops.make_kv8_workspace(1, G, 1, Dh, S, DEV)
+        ops.kv8_append(k.to(DEV), v.to(DEV), cache, torch.zeros(1, dtype=torch.int32, device=DEV), ws)
+        kk, vv = (x.double().cpu()[0, 0] for x in ops.kv8_load(cache, 0, S))
+        q = torch.zeros(1, G, Dh)
+        q[0, :, 3] = torch.linspace(2.0, 60.0, G) if G > 1 else 20.0
+        q = q.to(torch.bfloat16)
+        for n in (S, S - 5, 16 * 10):
+            got = ops.flash_decode_kv8(q.to(DEV), cache, torch.tensor([n], dtype=torch.int32, device=DEV), ws, scale=1.0).double().cpu()[0]
+            p = torch.softmax(q[0].double() @ kk[:n].T, -1)
+            want = p @ vv[:n]
+            # (scores of at most 60 log2(e) to 2^-22 of themselves: weights to 2^-15)
+            assert bool(((got - want).abs() <= want.abs() * (2.0 ** -8 + 2.0 ** -14)).all()), (likely, n)
+
+
+@pytest.mark.parametrize("Dh,G", [(64, 1), (128, 2), (128, 8), (64, 16)])
+@pytest.mark.parametrize("base", [-400.0, -90.0, 300.0])
+def test_scores_far_from_zero(Dh, G, base):
+    """All scores lie around `base`; they rise from tile to tile, or fall."""
+    from flashsvd_b200 import kv8, ops
+    from tests import kv8_reference as ref
+
+    B, S = 2, 700
+    gen = torch.Generator().manual_seed(Dh + G)
+    for slope in (0.0, 1.0, -1.0):
+        k = torch.zeros(B, S, 1, Dh)
+        k[..., 0] = 1.0
+        k[..., 1] = slope * (torch.arange(S) // 128 * 8)[None, :, None]   # (steps of 8: exact codes)
+        k[..., 2] = torch.randint(-15, 16, (B, S, 1), generator=gen).float()
+        v = torch.randn(B, S, 1, Dh, generator=gen)
+        q = torch.zeros(B, G, Dh)
+        q[:, :, 0], q[:, :, 1], q[:, :, 2] = base, 1.0, 0.125
+        q = q.to(torch.bfloat16)
+        cache = kv8.KV8Cache.empty(B, S, 1, Dh, block=32, device=DEV)
+        ws = ops.make_kv8_workspace(B, G, 1, Dh, S, DEV)
+        ops.kv8_append(k.to(torch.bfloat16).to(DEV), v.to(torch.bfloat16).to(DEV), cache, torch.zeros(B, dtype=torch.int32, device=DEV), ws)
+        kk, vv = (x.double().cpu() for x in ops.kv8_load(cache, 0, S))
+        lens = torch.tensor([S, 130], dtype=torch.int32)
+        got = ops.flash_decode_kv8(q.to(DEV), cache, lens.to(DEV), ws, scale=1.0).double().cpu()
+        want = ref.attend(q, kk, vv, lens.tolist(), 1.0)
+        # (scores to 2^-22 of `base` and more: weights to 450 * 2^-22 = 2^-13)
+        assert bool(((got - want).abs() <= want.abs() * 2.0 ** -8 + 2.0 ** -12 * float(vv.abs().max())).all()), slope
