@@ -320,9 +320,10 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
   const int blk = start / BLOCK + j;
   const long long blk0 = (long long)blk * BLOCK;
   if (blk0 >= end_ll) return;
-  const int lo = (int)max((long long)start, blk0), hi = (int)min((long long)end, blk0 + BLOCK);
+  const long long lo = max((long long)start, blk0);   // position of this tile's first new token (behind 2^31 for a length near it)
+  const int from = (int)(lo - start);                 // and its place among the call's
   // (queries of tokens beyond the cache are rotated too: their range is not cut at the capacity)
-  const int nq = (int)(min(end_ll, blk0 + BLOCK) - lo), n = max(0, hi - lo);
+  const int nq = (int)(min(end_ll, blk0 + BLOCK) - lo), n = (int)max(0ll, min((long long)end, blk0 + BLOCK) - lo);
   const int R = a.rot.R, half = R >> 1, inter = a.rot.interleaved;
   // pair p of a token sits in slot (p % 8) * units + p / 8: the lanes of a warp, a unit of eight pairs each, read neighbours
   const int units = (half + 7) / 8, slots = 8 * units;
@@ -333,7 +334,7 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
 #pragma unroll
     for (int i = 0; i < 8; ++i) kreg[i] = vreg[i] = 0u;
     if (t < n) {
-      const size_t off = (size_t)b * a.kv_batch + (size_t)(lo - start + t) * a.kv_token + (size_t)hk * DH;
+      const size_t off = (size_t)b * a.kv_batch + (size_t)(from + t) * a.kv_token + (size_t)hk * DH;
       fsvd_rope::load_pairs<FORM>(a.k + off, u, R, inter, kreg);
       fsvd_rope::load_pairs<FORM>(a.v + off, u, R, inter, vreg);
     }
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
       if (p >= half) continue;
       const bool step = nq > 8 && k < 8;
       double c, s;
-      fsvd_rope::angle(step ? k : nq <= 8 ? lo + k : lo + 8 * (k - 8), a.rot.inv_freq[p], step ? 1.0f : a.rot.scale, c, s);
+      fsvd_rope::angle((double)(step ? k : nq <= 8 ? lo + k : lo + 8 * (k - 8)), a.rot.inv_freq[p], step ? 1.0f : a.rot.scale, c, s);
       steps[i] = make_double2(c, s);
     }
     __syncthreads();
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
       s[i] = (float)cs.y;
     }
   }
-  const size_t tok = (size_t)(lo - start + t);
+  const size_t tok = (size_t)(from + t);
   const __nv_bfloat16* src = a.q + (size_t)b * a.q_batch + tok * a.q_token;
   __nv_bfloat16* dst = a.q_out + ((size_t)b * a.L + tok) * a.H * DH;
   auto turn_heads = [&](auto many, int h) {

@@ -22,8 +22,8 @@ struct Rotary {
 
 // Sine and cosine of position * f, f in radians per position.  The angle is formed and reduced in 64 bits: in 32, a
 // position of 10^5 leaves the fastest pair 0.004 radians off.
-__device__ __forceinline__ void angle(int position, double f, float scale, double& c, double& s) {
-  const double turns = (double)position * (f * 0.15915494309189533577);   // 1 / (2 pi)
+__device__ __forceinline__ void angle(double position, double f, float scale, double& c, double& s) {
+  const double turns = position * (f * 0.15915494309189533577);   // 1 / (2 pi)
   sincospi(2.0 * (turns - rint(turns)), &s, &c);
   c *= (double)scale;
   s *= (double)scale;

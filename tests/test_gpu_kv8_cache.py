@@ -159,3 +159,23 @@ def test_a_dropped_token_is_reported():
     assert torch.equal(cache.layers8[1].k.view(torch.uint8)[0], before[1][0])
     cache.clear_status()
     assert cache.status() == 0
+
+
+def test_queries_behind_the_largest_position_are_rotated():
+    """A length next to 2^31: the tokens are dropped, their queries turn by the positions that they would have had.
+
+    Half a bf16 step, and angles of 2^31 radians to 2^-20 (a 64-bit angle has 2^-21 there)."""
+    from flashsvd_b200 import kv8, ops
+    from tests import kv8_reference as ref
+
+    rot = kv8.rotary(Dh, device=DEV)
+    for L in (3, 40):
+        cache = kv8.KV8Cache.empty(2, 24, Hk, Dh, block=16, device=DEV)
+        ws = ops.make_kv8_workspace(2, H, Hk, Dh, 24, DEV)
+        q, k, v = _qkv(2, L, L)
+        starts = torch.tensor([2 ** 31 - 1, 2 ** 31 - 20], dtype=torch.int32, device=DEV)
+        got = ops.kv8_append(k, v, cache, starts, ws, q=q, rotary=rot).double().cpu()
+        pos = starts.cpu().long()[:, None] + torch.arange(L)
+        want = ref.rotate(q.cpu(), pos, rot.inv_freq.cpu())
+        assert bool(((got - want).abs() <= want.abs() * 2.0 ** -8 + 2.0 ** -19 * float(q.abs().max())).all())
+        assert ws.raw_status() != 0 and not bool(cache.k.view(torch.uint8).any())
