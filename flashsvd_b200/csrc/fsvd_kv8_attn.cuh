@@ -190,10 +190,10 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// x 2^-up, for an `up` whose power alone may leave the 32-bit range
+// x 2^-up, for a whole `up` whose power alone may leave the 32-bit range
 __device__ __forceinline__ float lowered(float x, float up) {
-  const float f = ex2(-0.5f * up);
-  return x * f * f;
+  const float half = truncf(0.5f * up);
+  return x * ex2(-half) * ex2(half - up);
 }
 // Whether any thread of a softmax group says so.
 __device__ __forceinline__ bool group_any(bool x, int group) {

@@ -308,7 +308,8 @@ class SVD_LlamaAttention(_WithWorkspace):
     def forward(self, hidden_states: torch.Tensor, attention_mask=None, position_ids=None, past_key_values=None,
                 cache_position: Optional[torch.Tensor] = None, position_embeddings=None, **kwargs):
         """Returns (attn_output[B, L, d], None) like the transformers attention protocol.
-        ``past_key_values`` is a ``runtime.FlashSVDV15DenseKVCache``, or a ``runtime.FlashSVDV15KV8Cache``."""
+        ``past_key_values`` is a ``runtime.FlashSVDV15DenseKVCache``, or a ``runtime.FlashSVDV15KV8Cache``.  Attention is causal
+        over what the cache holds; ``attention_mask`` is not read (no padded batches)."""
         x, cache = hidden_states, past_key_values
         if cache is None:
             raise ValueError("SVD_LlamaAttention needs past_key_values (a FlashSVDV15DenseKVCache)")

@@ -873,7 +873,8 @@ def generate_text(model: Any, tokenizer: Any, *, prompt: str, max_new_tokens: in
     Generation stops after an end-of-sequence token, like the reference loop.
 
     With ``uniforms`` (float32 [max_new_tokens] in [0, 1)), ``top_k`` or ``min_p`` the tokens are drawn by ``ops.sample``
-    on the device (from ``uniforms``, else from torch's CUDA generator) and the host reads none of them before the end."""
+    on the device (from ``uniforms``, else from torch's CUDA generator) and the host reads none of them before the end: all
+    ``max_new_tokens`` steps are made, and what follows an end-of-sequence token is cut off the result."""
     from .engine import DecodeEngine, engine_for_model, has_lowrank_modules
 
     if not isinstance(model, DecodeEngine):
