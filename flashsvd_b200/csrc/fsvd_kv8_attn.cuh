@@ -56,12 +56,12 @@ struct Args {
 
 template <int DH, int GP>
 struct Shape {
-  // Heads are shared out to groups of four softmax warps, four heads each: with 8 heads in one group a tile took 1.4 times as
-  // long as its bytes.
+  // Heads are shared out to groups of four softmax warps, four heads each: with 8 heads in one group (and weights of four
+  // numbers) a tile took 1.4 times as long as its bytes.
   static constexpr int kGroups = GP > 4 ? GP / 4 : 1, kHeads = GP / kGroups;
   static constexpr int kThreads = kSoft * kGroups + 64;
   // CTAs of an SM, and tiles that a CTA has under way.  32 sequences x 32 heads of 128 x 2048 tokens: two CTAs of three tiles
-  // 83 us, three of two 94; heads of 64, 128 ragged sequences: three CTAs of four tiles 41 us, two of six 48.
+  // 84 us, three of two 94; heads of 64, 128 ragged sequences: three CTAs of four tiles 44 us, two of six 50.
   static constexpr int kCtas = GP > 8 ? 1 : DH == 64 && GP <= 4 ? 3 : 2;
   static constexpr int kStages = GP > 8 ? 5 * (128 / DH) : DH == 128 ? 3 : GP <= 4 ? 4 : 6;
   static constexpr int kNq = kParts * GP < 16 ? 16 : kParts * GP;       // columns of S

@@ -392,7 +392,8 @@ int fsvd_kv8_append(const fsvd_kv8* cache, const void* k, const void* v, long lo
 int fsvd_kv8_load(const fsvd_kv8* cache, int start, int length, const int* cache_seqlens, int seqlen_add, void* k_out,
                   void* v_out, void* stream);
 /* As fsvd_flash_decode over an 8-bit cache: q and out [B, H, Dh] bf16, H / Hk any whole number up to
- * 16; a sequence of length 0 gives zeros. */
+ * 16; a sequence of length 0 gives zeros.  Scales from 2^-100 to 2^120 (fsvd_kv8_append writes 2^-60 to
+ * 2^120).  Softmax weights have 24 bits down to 2^-16 of the largest and reach to 2^-39 of it. */
 int fsvd_flash_decode_kv8(const fsvd_kv8* cache, const void* q, const int* cache_seqlens, int seqlen_add, void* out, int H,
                           float scale, void* ws, size_t ws_bytes, void* stream);
 
