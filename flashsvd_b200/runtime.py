@@ -506,6 +506,8 @@ class FlashSVDV15KV8Cache(_CacheBase):
         return self._max_cache_len
 
     def get_mask_sizes(self, cache_position, layer_idx: int = 0):
+        if self._seen and self._seen[int(layer_idx or 0)] is None:   # (nothing to wait for: a mask may be longer than the sequence)
+            return self._max_cache_len, 0
         q_len = int(cache_position.shape[0]) if torch.is_tensor(cache_position) else int(cache_position)
         return q_len + self.get_seq_length(), 0
 
