@@ -483,12 +483,12 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
     N x[E], sum = zero;
 #pragma unroll
     for (int e = 0; e < E; ++e) sum += x[e] = f(s.total[tid * E + e], tid * E + e);
-    const N inc = warp_scan(sum, lane);
+    const N inc = warp_scan(sum, lane), left = __shfl_up_sync(0xffffffffu, inc, 1);
     if (lane == 31) scan[warp] = inc;
     __syncthreads();
     const N upto = warp_scan(scan[lane], lane), all = __shfl_sync(0xffffffffu, upto, kWarps - 1);
     N run = __shfl_sync(0xffffffffu, upto, max(warp - 1, 0));
-    run = (warp ? run : zero) + (inc - sum);
+    run = (warp ? run : zero) + (lane ? left : zero);   // (not inc - sum: a bin that nobody counted stands for more than all others)
     // (a sum that was formed in another order may end a rounding short of the place)
     if constexpr (std::is_integral_v<N>) want = all > 0 ? min(want, all - 1) : want;
     else want = fmin(want, all);

@@ -79,3 +79,37 @@ def test_a_border_far_down_in_the_tail(B, V, octaves):
         want = 5 if place < 1.0 + 5 * w else 6 + math.floor((place - 1.0) / w) - 5
         assert abs(int(tokens[b]) - want) <= 1, (int(tokens[b]), want)
         assert abs(float(probs[b]) - (w if want != 5 else 1.0) / z) <= 2.0 ** -24 * (w if want != 5 else 1.0)
+
+
+@pytest.mark.parametrize("B,n1,n2", [(1, 100000, 900000), (40, 70000, 200000), (130, 30000, 50000)])
+@pytest.mark.parametrize("first", [31.02, 31.5, 31.97, 28.3])
+def test_a_border_behind_the_last_counted_octave(B, n1, n2, first):
+    """One likely token, n1 at 2^-first of its weight and n2 at 2^-34, among which the top-p ends: what lies in front of them
+    counts in full.
+
+    The likely token's weight is one exactly; 10^6 tail weights, each good to 2^-39 of itself and 2^-34 of itself in the
+    histogram, move the number kept by less than 10^6 2^-34 2^3 (a weight of the first group is at most 2^6 of the second
+    group's, and the roundings of equal weights add up): 2^-8, and sums of 64-bit numbers by 2^-50 of the mass, 2^-16 of a
+    weight.  One either way."""
+    import math
+
+    from flashsvd_b200 import ops
+
+    V = 1 + n1 + n2
+    x = torch.empty(V)
+    x[0], x[1:1 + n1], x[1 + n1:] = 0.0, -first * math.log(2.0), -34.0 * math.log(2.0)
+    w1, w2 = math.exp(float(x[1].double())), math.exp(float(x[-1].double()))
+    total = 1.0 + n1 * w1 + n2 * w2
+    p = float(torch.tensor(1.0 - 0.5 * n2 * w2 / total, dtype=torch.float32))
+    kept = math.floor((p * total - 1.0 - n1 * w1) / w2) + 1
+    assert 100 < kept < n2 - 100
+    z = 1.0 + n1 * w1 + kept * w2
+    u = torch.tensor([1.0 - 2.0 ** -24 * (1 + b % 2) for b in range(B)])
+    tokens, probs = ops.sample(x[None].expand(B, V).contiguous().to(DEV), u.to(DEV), top_p=p)
+    for b in range(B):
+        place = float(u[b].double()) * z - 1.0
+        want = 0 if place < 0 else 1 + math.floor(place / w1) if place < n1 * w1 else 1 + n1 + math.floor((place - n1 * w1) / w2)
+        assert abs(int(tokens[b]) - want) <= 1, (int(tokens[b]), want)
+    # the share of the likely token tells what is kept: z within one tail weight, rounded once
+    tokens, probs = ops.sample(x[None].expand(B, V).contiguous().to(DEV), torch.zeros(B, device=DEV), top_p=p)
+    assert bool((tokens == 0).all()) and bool(((probs.double() - 1.0 / z).abs() <= 2.0 ** -24).all())
