@@ -137,10 +137,10 @@ def load() -> C.CDLL:
     lib.fsvd_tp_decode_layer.argtypes = [
         C.POINTER(FsvdDims), C.POINTER(FsvdLayer), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     fp, ll = C.c_float, C.c_longlong
-    lib.fsvd_rope_qk.argtypes = [vp, ll, vp, ll, vp, vp, ip, ip, fp, vp, vp] + [ip] * 5 + [vp]
+    lib.fsvd_rope_qk.argtypes = [vp, ll, vp, ll, vp, vp, ip, ip, C.c_double, vp, vp] + [ip] * 5 + [vp]
     lib.fsvd_kv8_workspace_bytes.argtypes = [ip] * 5
     lib.fsvd_kv8_workspace_bytes.restype = sz
-    lib.fsvd_kv8_append.argtypes = [C.POINTER(FsvdKv8), vp, vp, ll, ll, vp, vp, vp, ll, ll, vp, vp, ip, ip, fp, ip, ip, vp, sz, vp]
+    lib.fsvd_kv8_append.argtypes = [C.POINTER(FsvdKv8), vp, vp, ll, ll, vp, vp, vp, ll, ll, vp, vp, ip, ip, C.c_double, ip, ip, vp, sz, vp]
     lib.fsvd_kv8_load.argtypes = [C.POINTER(FsvdKv8), ip, ip, vp, ip, vp, vp, vp]
     lib.fsvd_flash_decode_kv8.argtypes = [C.POINTER(FsvdKv8), vp, vp, ip, vp, ip, fp, vp, sz, vp]
     lib.fsvd_sample.argtypes = [vp, ll, ip, vp, vp, vp, vp, vp, fp, ip, fp, fp, vp, vp, ip, ip, vp]

@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kAppendThreads<DH, BLOCK>, kAppendCtas<DH, BLO
       if (p >= half) continue;
       const bool step = nq > 8 && k < 8;
       double c, s;
-      fsvd_rope::angle((double)(step ? k : nq <= 8 ? lo + k : lo + 8 * (k - 8)), a.rot.inv_freq[p], step ? 1.0f : a.rot.scale, c, s);
+      fsvd_rope::angle((double)(step ? k : nq <= 8 ? lo + k : lo + 8 * (k - 8)), a.rot.inv_freq[p], step ? 1.0 : a.rot.scale, c, s);
       steps[i] = make_double2(c, s);
     }
     __syncthreads();
@@ -774,7 +774,7 @@ using namespace fsvd_kv8_impl;
 extern "C" {
 
 int fsvd_rope_qk(const void* q, long long q_stride, const void* k, long long k_stride, const int* positions,
-                 const double* inv_freq, int rotary_dim, int interleaved, float rope_scale, void* q_out, void* k_out, int T,
+                 const double* inv_freq, int rotary_dim, int interleaved, double rope_scale, void* q_out, void* k_out, int T,
                  int H, int Hk, int Dh, int dtype, void* stream) {
   if (!q || !positions || !inv_freq || !q_out || (k != nullptr) != (k_out != nullptr)) return fail(FSVD_ERR_ARG, "null argument");
   if (dtype != FSVD_DTYPE_BF16 && dtype != FSVD_DTYPE_F32) return fail(FSVD_ERR_ARG, "bad dtype %d", dtype);
@@ -805,7 +805,7 @@ size_t fsvd_kv8_workspace_bytes(int B, int H, int Hk, int Dh, int S_max) {
 int fsvd_kv8_append(const fsvd_kv8* cache, const void* k, const void* v, long long kv_batch_stride, long long kv_token_stride,
                     const int* cache_seqlens, const int* new_lens, const void* q, long long q_batch_stride,
                     long long q_token_stride, void* q_out, const double* inv_freq, int rotary_dim, int interleaved,
-                    float rope_scale, int H, int L, void* ws, size_t ws_bytes, void* stream) {
+                    double rope_scale, int H, int L, void* ws, size_t ws_bytes, void* stream) {
   if (int e = check_cache(cache)) return e;
   if (!k || !v || !cache_seqlens || (q != nullptr) != (q_out != nullptr)) return fail(FSVD_ERR_ARG, "null argument");
   if (q && !inv_freq) return fail(FSVD_ERR_ARG, "queries are passed to be rotated: inv_freq is missing");

@@ -17,16 +17,16 @@ enum Form { kSingle, kVectors, kTogether };
 struct Rotary {
   const double* inv_freq;   // [R / 2], radians per position
   int R, interleaved;
-  float scale;
+  double scale;
 };
 
 // Sine and cosine of position * f, f in radians per position.  The angle is formed and reduced in 64 bits: in 32, a
 // position of 10^5 leaves the fastest pair 0.004 radians off.
-__device__ __forceinline__ void angle(double position, double f, float scale, double& c, double& s) {
+__device__ __forceinline__ void angle(double position, double f, double scale, double& c, double& s) {
   const double turns = position * (f * 0.15915494309189533577);   // 1 / (2 pi)
   sincospi(2.0 * (turns - rint(turns)), &s, &c);
-  c *= (double)scale;
-  s *= (double)scale;
+  c *= scale;
+  s *= scale;
 }
 
 // Offsets of the two numbers of pair p within the row.

@@ -354,7 +354,7 @@ int fsvd_tp_decode_layer(const fsvd_dims* dims, const fsvd_layer* layer, const v
  * q_out / k_out [T, H|Hk, Dh] (contiguous) may be the inputs when those are contiguous.  k and k_out
  * may both be NULL.  dtype bf16 or f32, Dh a multiple of 16 up to 256. */
 int fsvd_rope_qk(const void* q, long long q_stride, const void* k, long long k_stride, const int* positions,
-                 const double* inv_freq, int rotary_dim, int interleaved, float rope_scale, void* q_out, void* k_out,
+                 const double* inv_freq, int rotary_dim, int interleaved, double rope_scale, void* q_out, void* k_out,
                  int T, int H, int Hk, int Dh, int dtype, void* stream);
 
 /* 8-bit cache: k8 / v8 [B, Hk, S_max, Dh] e4m3 codes, k_scale / v_scale [B, Hk, ceil(S_max / block)]
@@ -386,7 +386,7 @@ size_t fsvd_kv8_workspace_bytes(int B, int H, int Hk, int Dh, int S_max);
 int fsvd_kv8_append(const fsvd_kv8* cache, const void* k, const void* v, long long kv_batch_stride, long long kv_token_stride,
                     const int* cache_seqlens, const int* new_lens, const void* q, long long q_batch_stride,
                     long long q_token_stride, void* q_out, const double* inv_freq, int rotary_dim, int interleaved,
-                    float rope_scale, int H, int L, void* ws, size_t ws_bytes, void* stream);
+                    double rope_scale, int H, int L, void* ws, size_t ws_bytes, void* stream);
 /* Positions [start, start + length) as bf16 numbers, k_out / v_out [B, Hk, length, Dh].  With
  * cache_seqlens, rows from cache_seqlens[b] + seqlen_add on are zeros. */
 int fsvd_kv8_load(const fsvd_kv8* cache, int start, int length, const int* cache_seqlens, int seqlen_add, void* k_out,

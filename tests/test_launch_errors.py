@@ -37,9 +37,9 @@ cache = C.byref(Kv8(p, p, p, p, 1, 2, 512, 128, 64))
 def sample(V, dtype, B):
     return lib.fsvd_sample(p, ll(V), dtype, p, None, None, None, None, f(1), 0, f(1), f(0), p, p, B, V, None)
 calls = {
-    "rope": lambda: lib.fsvd_rope_qk(p, ll(128), p, ll(128), p, p, 64, 0, f(1), p, p, 4, 2, 2, 64, 0, None),
-    "append": lambda: lib.fsvd_kv8_append(cache, p, p, ll(16384), ll(256), p, None, p, ll(16384), ll(256), p, p, 128, 0, f(1), 2, 64, p, size, None),
-    "step": lambda: lib.fsvd_kv8_append(cache, p, p, ll(256), ll(256), p, None, None, ll(0), ll(0), None, None, 0, 0, f(1), 0, 1, p, size, None),
+    "rope": lambda: lib.fsvd_rope_qk(p, ll(128), p, ll(128), p, p, 64, 0, C.c_double(1), p, p, 4, 2, 2, 64, 0, None),
+    "append": lambda: lib.fsvd_kv8_append(cache, p, p, ll(16384), ll(256), p, None, p, ll(16384), ll(256), p, p, 128, 0, C.c_double(1), 2, 64, p, size, None),
+    "step": lambda: lib.fsvd_kv8_append(cache, p, p, ll(256), ll(256), p, None, None, ll(0), ll(0), None, None, 0, 0, C.c_double(1), 0, 1, p, size, None),
     "load": lambda: lib.fsvd_kv8_load(cache, 0, 8, None, 0, p, p, None),
     "attend": lambda: lib.fsvd_flash_decode_kv8(cache, p, p, 0, p, 2, f(0), p, size, None),
     "sample": lambda: sample(1000, 1, 2),
