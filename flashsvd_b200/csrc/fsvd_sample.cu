@@ -204,7 +204,8 @@ __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const Args a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid < kPer) s.table[tid] = exp2((double)tid / kPer);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const float temp = fminf(a.temperature ? a.temperature[b] : a.T_all, kHuge);
+  float temp = fminf(a.temperature ? a.temperature[b] : a.T_all, kHuge);
+  if (temp > 0.0f) temp = fmaxf(temp, 0x1p-64f);   // (`wide` makes a zero +-2^-127, which has to stay nothing beside it)
   int k = a.top_k ? a.top_k[b] : a.k_all;
   const float p = a.top_p ? a.top_p[b] : a.p_all, mp = fminf(a.min_p ? a.min_p[b] : a.m_all, 1.0f);
   if (k <= 0 || k > V) k = V;

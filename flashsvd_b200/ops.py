@@ -546,7 +546,8 @@ def sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     Weights are exp((logit - max) / temperature).  In descending order of the logits (lower index first among equals)
     the first ``top_k`` stay (0: all), of those the ones whose preceding mass is at most ``top_p`` of it (1: all), of
     those the ones with weight >= ``min_p`` (0: all).  The token is the first one in index order whose running mass
-    exceeds uniforms[b] of the kept mass; probs is its share.  temperature <= 0 takes the largest logit.  Each setting
+    exceeds uniforms[b] of the kept mass; probs is its share.  temperature <= 0 takes the largest logit (a positive one
+    below 2^-64 counts as 2^-64).  Each setting
     is a number or a tensor with one value per row (float32; top_k int32)."""
     index = _device_of("logits", logits, 2, "[B, V]")
     B, V = logits.shape

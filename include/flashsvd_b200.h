@@ -403,7 +403,8 @@ int fsvd_flash_decode_kv8(const fsvd_kv8* cache, const void* q, const int* cache
  * mass is at most top_p times the mass of all of them (>= 1: all), of those the ones with weight >=
  * min_p (<= 0: all); at least one.  The token is the first kept one in index order whose running mass
  * exceeds uniforms[b] times the kept mass; probs (may be NULL) gets its share of that mass.  A
- * temperature <= 0 (or NaN) takes the largest logit, an infinite one counts as the largest finite number.
+ * temperature <= 0 (or NaN) takes the largest logit, one below 2^-64 counts as 2^-64, an infinite one
+ * as the largest finite number.
  * NaN counts as -infinity; a row without anything above -infinity gives token 0 with share 0; where +infinity
  * is the largest, the elements that are infinite share everything.  temperature, top_k, top_p, min_p: one
  * value per row in device memory, or NULL and the value for all rows.  Weights are 64-bit numbers, their

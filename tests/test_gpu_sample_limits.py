@@ -113,3 +113,20 @@ def test_a_border_behind_the_last_counted_octave(B, n1, n2, first):
     # the share of the likely token tells what is kept: z within one tail weight, rounded once
     tokens, probs = ops.sample(x[None].expand(B, V).contiguous().to(DEV), torch.zeros(B, device=DEV), top_p=p)
     assert bool((tokens == 0).all()) and bool(((probs.double() - 1.0 / z).abs() <= 2.0 ** -24).all())
+
+
+def test_temperatures_next_to_zero():
+    """Positive ones below 2^-64 count as 2^-64: the largest logits share everything, zeros among them."""
+    from flashsvd_b200 import ops
+
+    V = 1000
+    x = -torch.rand(4, V, generator=torch.Generator().manual_seed(1)) - 0.5
+    x[0, 17], x[1, 3], x[1, 900], x[2, 5], x[3] = 0.0, -0.0, 0.0, 2.0, 0.0
+    u = torch.full((4,), 0.75)
+    for T in (1e-45, 1e-42, 1e-39, 1e-37, 1e-31, 1e-20):
+        for T_all in (T, torch.full((4,), T, device=DEV)):
+            out, share = torch.full((4,), -7, dtype=torch.int32, device=DEV), torch.full((4,), -7.0, device=DEV)
+            ops.sample(x.to(DEV), u.to(DEV), temperature=T_all, out=out, probs_out=share)
+            assert out.tolist() == [17, 900, 5, 750] and share.tolist()[:3] == [1.0, 0.5, 1.0]
+            ops.sample(x.to(DEV), u.to(DEV), temperature=T_all, top_p=0.5, top_k=9, min_p=0.5, out=out, probs_out=share)
+            assert out.tolist()[:3] == [17, 900, 5]
